@@ -26,6 +26,19 @@ _i = C.c_int
 _f = C.c_float
 _sz = C.c_size_t
 
+_i64 = C.c_int64
+
+
+class CrossAttention(C.Structure):
+    """aria_hip_cross_attn of include/aria_hip.h: one cross attention over ragged encoder states."""
+    _fields_ = ([(n, _P) for n in ("q", "k", "v", "out", "kv_len", "mask")] +
+                [(n, _i) for n in ("type", "out_f32", "B", "H", "Hkv", "Nq", "Nk", "D")] + [("scale", _f)] +
+                [(n, _i64) for n in ("q_batch", "q_head", "q_token", "k_batch", "k_head", "k_token", "v_batch", "v_head",
+                                     "v_token", "o_batch", "o_head", "o_token", "mask_stride")])
+
+
+_X = C.POINTER(CrossAttention)
+
 # name -> (restype, argtypes); every symbol declared in include/aria_gpu.h and include/aria_hip.h
 SIGNATURES = {
     # include/aria_gpu.h
@@ -105,6 +118,14 @@ SIGNATURES = {
     "aria_hip_qkv_prep_dev": (_i, [_P, _i, _i, _i, _i, _i, _P, _P, _P, _P, _P, _i, _f, _P]),
     "aria_hip_flash_attention_dev": (_i, [_P, _P, _P, _P, _i, _i, _i, _i, _i, _i, _P]),
     "aria_hip_attention_f16": (_i, [_P, _P, _P, _P, _i, _i, _i, _i, _i]),
+    "aria_hip_cross_attention_ws_bytes": (_sz, [_X]),
+    "aria_hip_cross_attention_dev": (_i, [_X, _P, _P]),
+    "aria_hip_mx4_quant_dev": (_i, [_P, _P, _P, _i, _i, _i, _i64, _P]),
+    "aria_hip_mx4_dequant_dev": (_i, [_P, _i, _P, _P, _i, _i, _P]),
+    "aria_hip_gemm_mx4_dev": (_i, [_P, _i, _P, _P, _P, _P, _P, _i, _i, _i, _P]),
+    "aria_hip_mx4_ws_bytes": (_sz, [_i, _i]),
+    "aria_hip_linear_mx4_dev": (_i, [_P, _i, _P, _i, _i64, _P, _P, _P, _i, _i, _i, _P, _P]),
+    "aria_hip_glu_mx4_dev": (_i, [_P, _i, _P, _i, _i64, _P, _P, _P, _i, _i, _i, _P, _P]),
     # include/aria_dit.h
     "aria_hip_dit_block_create": (_P, [_P, _i, _i, _i, _i, _i, _i, _i]),
     "aria_hip_dit_block_free": (None, [_P]),
@@ -142,6 +163,11 @@ SIGNATURES = {
     "aria_hip_q4_quant": (_i, [_P, _P, _P, _i, _i]),
     "aria_hip_q8_dequant": (_i, [_P, _P, _P, _i, _i]),
     "aria_hip_q4_dequant": (_i, [_P, _P, _P, _i, _i]),
+    "aria_hip_mx4_quant": (_i, [_P, _P, _P, _i, _i]),
+    "aria_hip_mx4_dequant": (_i, [_P, _P, _P, _i, _i]),
+    "aria_hip_linear_mx4": (_i, [_P, _P, _P, _P, _P, _i, _i, _i]),
+    "aria_hip_glu_mx4": (_i, [_P, _P, _P, _P, _P, _i, _i, _i]),
+    "aria_hip_cross_attention_f16": (_i, [_P, _P, _P, _P, _P, _P, _i, _i, _i, _i, _i, _i]),
     "aria_hip_layernorm": (_i, [_P, _P, _P, _P, _i, _i, _f]),
     "aria_hip_rmsnorm_adaln": (_i, [_P, _P, _P, _P, _P, _i, _i, _i, _f]),
     "aria_hip_ln_mod_gelu_res": (_i, [_P, _P, _P, _P, _P, _P, _i, _i, _i, _f]),

@@ -250,7 +250,7 @@ void aria_cuda_sync(void) {
 /* host-wrapper scratch: device staging buffers for one synchronous call     */
 /* ------------------------------------------------------------------------- */
 
-#define STAGE_MAX 8
+#define STAGE_MAX 12
 typedef struct {
     void *p[STAGE_MAX];
     int n;
@@ -567,6 +567,102 @@ int aria_hip_linear_q8a8_dev(float *dy, const void *dx, int x_f16, const int8_t 
     return aria_hip_gemm_i8_dev(dy, 0, xq, sx, dq, dscale, db, M, K, N, stream);
 }
 
+/* MXFP4 (k_mx4.hip, k_mx4_gemm.hip). Arguments are checked before the device is looked for. */
+#define MX4_TYPE(t) ((t) == 0 || (t) == 1 || (t) == 2)
+#define MX4_KMAX (1 << 30)
+static size_t mx4_blocks(int K) { return ((size_t)K + 31) / 32; }
+static uintptr_t mx4_el_mask(int type) { return type == 0 ? 3u : 1u; }
+
+int aria_hip_mx4_quant_dev(uint8_t *dq, uint8_t *dscale, const void *dx, int xtype, int rows, int K, int64_t ldx,
+                           void *stream) {
+    REQ(rows >= 0 && K > 0 && K <= MX4_KMAX && MX4_TYPE(xtype) && ldx >= K);
+    REQ(rows == 0 || (dq && dscale && dx));
+    REQ(((uintptr_t)dq & 15u) == 0 && ((uintptr_t)dx & mx4_el_mask(xtype)) == 0);
+    ENSURE();
+    KCK(aria_k_mx4_quant(dq, dscale, dx, xtype, rows, K, (long)ldx, pick(stream)), "k_mx4_quant");
+    return 0;
+}
+int aria_hip_mx4_dequant_dev(void *dy, int ytype, const uint8_t *dq, const uint8_t *dscale, int rows, int K,
+                             void *stream) {
+    REQ(rows >= 0 && K > 0 && K <= MX4_KMAX && MX4_TYPE(ytype));
+    REQ(rows == 0 || (dy && dq && dscale));
+    REQ(((uintptr_t)dq & 15u) == 0 && ((uintptr_t)dy & mx4_el_mask(ytype)) == 0);
+    ENSURE();
+    KCK(aria_k_mx4_dequant(dy, ytype, dq, dscale, rows, K, pick(stream)), "k_mx4_dequant");
+    return 0;
+}
+static int gemm_mx4(void *dy, int ytype, const uint8_t *dxq, const uint8_t *dxs, const uint8_t *dq,
+                    const uint8_t *dscale, const float *db, int M, int K, int N, int glu, void *stream) {
+    REQ(M >= 0 && K > 0 && K <= MX4_KMAX && N >= 0 && N <= (1 << 30) && MX4_TYPE(ytype));
+    REQ(M == 0 || N == 0 || (dy && dxq && dxs && dq && dscale));
+    REQ((((uintptr_t)dxq | (uintptr_t)dq) & 15u) == 0 && ((uintptr_t)dy & mx4_el_mask(ytype)) == 0);
+    REQ(((uintptr_t)db & 3u) == 0);
+    ENSURE();
+    KCK(aria_k_mx4_gemm(dy, ytype, dxq, dxs, dq, dscale, db, M, K, N, glu, pick(stream)), "k_mx4_gemm");
+    return 0;
+}
+int aria_hip_gemm_mx4_dev(void *dy, int ytype, const uint8_t *dxq, const uint8_t *dxs, const uint8_t *dq,
+                          const uint8_t *dscale, const float *db, int M, int K, int N, void *stream) {
+    return gemm_mx4(dy, ytype, dxq, dxs, dq, dscale, db, M, K, N, 0, stream);
+}
+static size_t mx4_ws_scale(int M, int K) { return ((size_t)M * mx4_blocks(K) * 16 + 255) & ~(size_t)255; }
+size_t aria_hip_mx4_ws_bytes(int M, int K) {
+    if (M <= 0 || K <= 0) return 0;
+    return mx4_ws_scale(M, K) + (size_t)M * mx4_blocks(K);
+}
+static int linear_mx4(void *dy, int ytype, const void *dx, int xtype, int64_t ldx, const uint8_t *dq,
+                      const uint8_t *dscale, const float *db, int M, int K, int N, int glu, void *dws, void *stream) {
+    REQ(M >= 0 && K > 0 && K <= MX4_KMAX && N >= 0 && N <= (1 << 30) && MX4_TYPE(ytype));
+    REQ(MX4_TYPE(xtype) && ldx >= K);
+    REQ(M == 0 || N == 0 || (dy && dx && dq && dscale && dws));
+    REQ(((uintptr_t)dq & 15u) == 0 && ((uintptr_t)dws & 255u) == 0 && ((uintptr_t)db & 3u) == 0);
+    REQ(((uintptr_t)dy & mx4_el_mask(ytype)) == 0 && ((uintptr_t)dx & mx4_el_mask(xtype)) == 0);
+    if (M == 0 || N == 0) return 0;
+    ENSURE();
+    uint8_t *xq = (uint8_t *)dws, *xs = xq + mx4_ws_scale(M, K);
+    KCK(aria_k_mx4_quant(xq, xs, dx, xtype, M, K, (long)ldx, pick(stream)), "k_mx4_quant");
+    KCK(aria_k_mx4_gemm(dy, ytype, xq, xs, dq, dscale, db, M, K, N, glu, pick(stream)), "k_mx4_gemm");
+    return 0;
+}
+int aria_hip_linear_mx4_dev(void *dy, int ytype, const void *dx, int xtype, int64_t ldx, const uint8_t *dq,
+                            const uint8_t *dscale, const float *db, int M, int K, int N, void *dws, void *stream) {
+    return linear_mx4(dy, ytype, dx, xtype, ldx, dq, dscale, db, M, K, N, 0, dws, stream);
+}
+int aria_hip_glu_mx4_dev(void *dy, int ytype, const void *dx, int xtype, int64_t ldx, const uint8_t *dq,
+                         const uint8_t *dscale, const float *db, int M, int K, int inner, void *dws, void *stream) {
+    return linear_mx4(dy, ytype, dx, xtype, ldx, dq, dscale, db, M, K, inner, 1, dws, stream);
+}
+
+/* cross attention over ragged encoder states (k_xattn.hip) */
+static int xattn_check(const aria_hip_cross_attn *a) {
+    REQ(a && (a->type == 1 || a->type == 2));
+    REQ(a->B >= 0 && a->H > 0 && a->Hkv > 0 && a->H % a->Hkv == 0 && a->Nq >= 0 && a->Nk >= 0);
+    REQ(a->D >= 8 && a->D <= 128 && a->D % 8 == 0);
+    REQ((int64_t)a->Nq * (a->H / a->Hkv) <= (1 << 30) && a->Nk <= (1 << 30));
+    REQ((int64_t)a->B * a->H <= (1 << 24));
+    REQ(a->B == 0 || a->Nq == 0 || (a->q && a->out && (a->Nk == 0 || (a->k && a->v))));
+    REQ((((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->out) & 15u) == 0);
+    REQ(((uintptr_t)a->kv_len & 3u) == 0);
+    const int64_t st = a->q_batch | a->q_head | a->q_token | a->k_batch | a->k_head | a->k_token | a->v_batch |
+                       a->v_head | a->v_token | a->o_batch | a->o_head | a->o_token;
+    REQ(st >= 0 && st % 8 == 0);
+    REQ(!a->mask || a->mask_stride >= 0);
+    return 0;
+}
+size_t aria_hip_cross_attention_ws_bytes(const aria_hip_cross_attn *a) {
+    if (xattn_check(a) || a->B == 0 || a->Nq == 0) return 0;
+    return aria_k_xattn_ws_bytes(a);
+}
+int aria_hip_cross_attention_dev(const aria_hip_cross_attn *a, void *dws, void *stream) {
+    const int r = xattn_check(a);
+    if (r) return r;
+    if (a->B == 0 || a->Nq == 0) return 0;
+    REQ(((uintptr_t)dws & 255u) == 0 && (dws || aria_k_xattn_ws_bytes(a) == 0));
+    ENSURE();
+    KCK(aria_k_xattn_run(a, dws, pick(stream)), "k_xattn");
+    return 0;
+}
+
 /* ------------------------------------------------------------------------- */
 /* host-pointer forms (aria_hip.h) - one synchronous staged call each        */
 /* ------------------------------------------------------------------------- */
@@ -681,6 +777,91 @@ int aria_hip_q4_dequant(float *W, const uint8_t *q, const float *scale, int N, i
     float *dW = st_alloc(&st_, FB((size_t)N * K));
     if (!st_.err) st_kernel(&st_, aria_k_q4_dequant(dW, dq, ds, N, K, g_stream), "k_q4_dequant");
     st_out(&st_, W, dW, FB((size_t)N * K));
+    HOST_END();
+}
+
+int aria_hip_mx4_quant(uint8_t *q, uint8_t *scale, const float *x, int rows, int K) {
+    REQ(rows >= 0 && K > 0 && K <= MX4_KMAX && q && scale && x);
+    if (rows == 0) return 0;
+    HOST_BEGIN();
+    const size_t nb = (size_t)rows * mx4_blocks(K);
+    float *dx = st_in(&st_, x, FB((size_t)rows * K));
+    uint8_t *dq = st_alloc(&st_, nb * 16), *ds = st_alloc(&st_, nb);
+    if (!st_.err) st_kernel(&st_, aria_k_mx4_quant(dq, ds, dx, 0, rows, K, K, g_stream), "k_mx4_quant");
+    st_out(&st_, q, dq, nb * 16);
+    st_out(&st_, scale, ds, nb);
+    HOST_END();
+}
+int aria_hip_mx4_dequant(float *y, const uint8_t *q, const uint8_t *scale, int rows, int K) {
+    REQ(rows >= 0 && K > 0 && K <= MX4_KMAX && y && q && scale);
+    if (rows == 0) return 0;
+    HOST_BEGIN();
+    const size_t nb = (size_t)rows * mx4_blocks(K);
+    uint8_t *dq = st_in(&st_, q, nb * 16), *ds = st_in(&st_, scale, nb);
+    float *dy = st_alloc(&st_, FB((size_t)rows * K));
+    if (!st_.err) st_kernel(&st_, aria_k_mx4_dequant(dy, 0, dq, ds, rows, K, g_stream), "k_mx4_dequant");
+    st_out(&st_, y, dy, FB((size_t)rows * K));
+    HOST_END();
+}
+static int host_linear_mx4(float *y, const float *x, const uint8_t *q, const uint8_t *scale, const float *b, int M,
+                           int K, int N, int glu) {
+    REQ(M >= 0 && K > 0 && K <= MX4_KMAX && N >= 0 && N <= (1 << 30) && y && x && q && scale);
+    if (M == 0 || N == 0) return 0;
+    HOST_BEGIN();
+    const size_t rows = (size_t)N << glu, nb = rows * mx4_blocks(K);
+    float *dx = st_in(&st_, x, FB((size_t)M * K));
+    uint8_t *dq = st_in(&st_, q, nb * 16), *ds = st_in(&st_, scale, nb);
+    float *db = st_in(&st_, b, FB(rows));
+    float *dy = st_alloc(&st_, FB((size_t)M * N));
+    void *ws = st_alloc(&st_, aria_hip_mx4_ws_bytes(M, K));
+    if (!st_.err) st_.err = linear_mx4(dy, 0, dx, 0, K, dq, ds, db, M, K, N, glu, ws, g_stream);
+    st_out(&st_, y, dy, FB((size_t)M * N));
+    HOST_END();
+}
+int aria_hip_linear_mx4(float *y, const float *x, const uint8_t *q, const uint8_t *scale, const float *b, int M,
+                        int K, int N) {
+    return host_linear_mx4(y, x, q, scale, b, M, K, N, 0);
+}
+int aria_hip_glu_mx4(float *y, const float *x, const uint8_t *q, const uint8_t *scale, const float *b, int M, int K,
+                     int inner) {
+    return host_linear_mx4(y, x, q, scale, b, M, K, inner, 1);
+}
+int aria_hip_cross_attention_f16(float *out, const float *q, const float *k, const float *v, const int32_t *kv_len,
+                                 const uint8_t *mask, int B, int H, int Hkv, int Nq, int Nk, int D) {
+    aria_hip_cross_attn a = {0};
+    a.type = 1; a.out_f32 = 1;
+    a.B = B; a.H = H; a.Hkv = Hkv; a.Nq = Nq; a.Nk = Nk; a.D = D;
+    REQ(B >= 0 && Nq >= 0 && Nk >= 0 && H > 0 && Hkv > 0 && D > 0);
+    REQ(out && q && (Nk == 0 || (k && v)));
+    if (B == 0 || Nq == 0) return 0;
+    const size_t nq = (size_t)B * H * Nq * D, nk = (size_t)B * Hkv * Nk * D;
+    a.scale = 1.0f / sqrtf((float)D);
+    a.q_token = a.k_token = a.v_token = D;
+    a.q_head = (int64_t)Nq * D; a.q_batch = a.q_head * H;
+    a.k_head = a.v_head = (int64_t)Nk * D; a.k_batch = a.v_batch = a.k_head * Hkv;
+    a.o_head = D; a.o_token = (int64_t)H * D; a.o_batch = a.o_token * Nq;
+    a.mask_stride = Nk;
+    /* everything but the pointers, before any device work */
+    a.q = a.k = a.v = a.out = (void *)16;
+    const int r = xattn_check(&a);
+    if (r) return r;
+    HOST_BEGIN();
+    const float *src[3] = {q, k, v};
+    uint16_t *dst[3] = {NULL, NULL, NULL};
+    for (int i = 0; i < 3; i++) {
+        const size_t n = i ? nk : nq;
+        float *d32 = st_in(&st_, n ? src[i] : NULL, FB(n));
+        dst[i] = st_alloc(&st_, n * 2);
+        if (!st_.err && n) st_kernel(&st_, aria_k_f32_to_f16(dst[i], d32, n, g_stream), "k_f2h");
+    }
+    a.kv_len = st_in(&st_, kv_len, (size_t)B * sizeof(int32_t));
+    a.mask = st_in(&st_, Nk ? mask : NULL, (size_t)B * Nk);
+    float *dout = st_alloc(&st_, FB(nq));
+    a.q = dst[0]; a.k = dst[1]; a.v = dst[2]; a.out = dout;
+    const size_t wb = aria_k_xattn_ws_bytes(&a);
+    void *ws = wb ? st_alloc(&st_, wb) : NULL;
+    if (!st_.err) st_kernel(&st_, aria_k_xattn_run(&a, ws, g_stream), "k_xattn");
+    st_out(&st_, out, dout, FB(nq));
     HOST_END();
 }
 

@@ -13,6 +13,8 @@
 #include <stdint.h>
 #include <hip/hip_runtime_api.h>
 
+#include "aria_hip.h"
+
 #ifdef __cplusplus
 extern "C" {
 #endif
@@ -244,6 +246,24 @@ hipError_t aria_k_dec_split(void *xs, const float *seq, int Lt, int Lout, hipStr
 hipError_t aria_k_dec_split_w(void *ws, const float *W, hipStream_t s);
 hipError_t aria_k_dec_map(float *audio, const void *xs, const void *ws, const float *b, int M, int form,
                           hipStream_t s);
+
+/* MXFP4 (k_mx4.hip, k_mx4_gemm.hip). Element types 0 fp32, 1 fp16, 2 bf16. Packed rows: 16 bytes of
+ * codes and one scale byte per block of 32 along K.
+ * aria_k_mx4_quant: x [rows, K] with rows ld elements apart; aria_k_mx4_dequant: y [rows, K].
+ * aria_k_mx4_gemm: y [M, N] = x w^T (+ bias) on packed rows; glu: w holds 2N rows, value rows first,
+ * y = v * silu(g). */
+hipError_t aria_k_mx4_quant(uint8_t *q, uint8_t *scale, const void *x, int xtype, int rows, int K, long ld,
+                            hipStream_t s);
+hipError_t aria_k_mx4_dequant(void *y, int ytype, const uint8_t *q, const uint8_t *scale, int rows, int K,
+                              hipStream_t s);
+hipError_t aria_k_mx4_gemm(void *y, int ytype, const uint8_t *xq, const uint8_t *xs, const uint8_t *wq,
+                           const uint8_t *ws, const float *bias, int M, int K, int N, int glu, hipStream_t s);
+
+/* Cross attention over ragged encoder states (k_xattn.hip): the public description as the kernels
+ * take it; ws holds aria_k_xattn_ws_bytes bytes. */
+typedef aria_hip_cross_attn aria_k_xattn;
+size_t aria_k_xattn_ws_bytes(const aria_k_xattn *a);
+hipError_t aria_k_xattn_run(const aria_k_xattn *a, void *ws, hipStream_t s);
 
 #ifdef __cplusplus
 }

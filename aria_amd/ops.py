@@ -296,3 +296,76 @@ def q4_dequant(q, s, K):
     W = np.empty((N, K), np.float32)
     check(lib().aria_hip_q4_dequant(_p(W), _p(q), _p(s), N, K), "aria_hip_q4_dequant")
     return W
+
+
+# ---- MXFP4 and cross attention over ragged states (include/aria_hip.h; no counterpart in the reference) ----
+
+def mx4_quant(x):
+    """x [rows, K] -> codes u8 [rows, 16 * ceil(K/32)] and scale bytes u8 [rows, ceil(K/32)]."""
+    x = _f32(x)
+    rows, K = x.shape
+    nb = (K + 31) // 32
+    q = np.empty((rows, 16 * nb), np.uint8); s = np.empty((rows, nb), np.uint8)
+    check(lib().aria_hip_mx4_quant(_p(q), _p(s), _p(x), rows, K), "aria_hip_mx4_quant")
+    return q, s
+
+
+def _mx4(q, s, K):
+    q = np.ascontiguousarray(q, np.uint8); s = np.ascontiguousarray(s, np.uint8)
+    nb = (K + 31) // 32
+    if q.ndim != 2 or q.shape[1] != 16 * nb or s.shape != (q.shape[0], nb):
+        raise ValueError(f"MXFP4 rows of {K} values are codes [rows, {16 * nb}] and scales [rows, {nb}]: "
+                         f"got {q.shape} and {s.shape}")
+    return q, s
+
+
+def mx4_dequant(q, s, K):
+    q, s = _mx4(q, s, K)
+    y = np.empty((q.shape[0], K), np.float32)
+    check(lib().aria_hip_mx4_dequant(_p(y), _p(q), _p(s), q.shape[0], K), "aria_hip_mx4_dequant")
+    return y
+
+
+def linear_mx4(x, q, s, b=None):
+    """y = Q(x) W^T + b: x [M, K] quantised to MXFP4 in the call, W packed [N rows]."""
+    x = _f32(x); b = _f32(b)
+    M, K = x.shape
+    q, s = _mx4(q, s, K)
+    y = np.empty((M, q.shape[0]), np.float32)
+    check(lib().aria_hip_linear_mx4(_p(y), _p(x), _p(q), _p(s), _p(b), M, K, q.shape[0]), "aria_hip_linear_mx4")
+    return y
+
+
+def glu_mx4(x, q, s, b=None):
+    """v * silu(g) with [v | g] = Q(x) W^T + b, W packed [2 * inner rows]."""
+    x = _f32(x); b = _f32(b)
+    M, K = x.shape
+    q, s = _mx4(q, s, K)
+    inner = q.shape[0] // 2
+    if q.shape[0] != 2 * inner:
+        raise ValueError("a gated projection has an even number of weight rows")
+    y = np.empty((M, inner), np.float32)
+    check(lib().aria_hip_glu_mx4(_p(y), _p(x), _p(q), _p(s), _p(b), M, K, inner), "aria_hip_glu_mx4")
+    return y
+
+
+def cross_attention(q, k, v, kv_len=None, mask=None):
+    """q [B, H, Nq, D], k / v [B, Hkv, Nk, D] (rounded to fp16), kv_len [B], mask [B, Nk] (nonzero =
+    attend) -> [B, Nq, H * D]; a row without a valid key is zero."""
+    q = _f32(q); k = _f32(k); v = _f32(v)
+    B, H, Nq, D = q.shape
+    Hkv, Nk = k.shape[1:3]
+    if k.shape != (B, Hkv, Nk, D) or v.shape != k.shape:
+        raise ValueError(f"k and v are [{B}, Hkv, Nk, {D}]: got {k.shape} and {v.shape}")
+    if kv_len is not None:
+        kv_len = np.ascontiguousarray(kv_len, np.int32)
+        if kv_len.shape != (B,):
+            raise ValueError(f"kv_len holds one length per sequence: got {kv_len.shape}")
+    if mask is not None:
+        mask = np.ascontiguousarray(np.asarray(mask) != 0, np.uint8)
+        if mask.shape != (B, Nk):
+            raise ValueError(f"mask is [{B}, {Nk}]: got {mask.shape}")
+    out = np.empty((B, Nq, H * D), np.float32)
+    check(lib().aria_hip_cross_attention_f16(_p(out), _p(q), _p(k), _p(v), _p(kv_len), _p(mask), B, H, Hkv, Nq, Nk, D),
+          "aria_hip_cross_attention_f16")
+    return out

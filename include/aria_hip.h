@@ -220,6 +220,76 @@ int aria_hip_flash_attention_dev(const uint16_t *dq, const uint16_t *dk, const u
 int aria_hip_attention_f16(float *out, const float *q, const float *k, const float *v, int B, int H,
                            int Nq, int Nk, int D);
 
+/* ---- cross attention to an encoder's states of another length ----
+ * o[b,t,h,:] = sum_j p_j v[b,j,h / (H/Hkv),:], p = softmax over the valid keys j of
+ * scale * q[b,t,h,:] . k[b,j,h / (H/Hkv),:]. Key j of sequence b is valid when j < kv_len[b] (kv_len
+ * NULL: Nk; values are taken as clamped to 0..Nk) and mask[b * mask_stride + j] != 0 (mask NULL:
+ * all). A row with no valid key (Nk = 0 included) is written as zeros. Keys and values that are
+ * not valid may hold anything (Inf and NaN included): they do not reach the result, but all Nk
+ * rows must be readable memory. type: 1 = fp16, 2 = bf16 (aria_dtype's values) for q, k, v and
+ * out; out_f32 != 0 writes fp32. D: a multiple of 8 up to 128. H a multiple of Hkv.
+ * Strides count elements and are multiples of 8, not negative, pointers are 16-byte aligned (for
+ * an fp32 out too); batch / head / token strides of q, k and v may be 0 (broadcast). Probabilities
+ * are rounded to the type before they multiply v; sums and softmax statistics are fp32.
+ * dws: aria_hip_cross_attention_ws_bytes(a) bytes (0: may be NULL), 256-byte aligned, not shared
+ * by calls that may run at the same time. No counterpart in the reference, whose attention takes
+ * one length (src/aria_ops.h:135). */
+typedef struct {
+    const void *q, *k, *v;
+    void *out;
+    const int32_t *kv_len;   /* [B] or NULL */
+    const uint8_t *mask;     /* rows of Nk bytes, mask_stride apart, or NULL */
+    int type, out_f32;
+    int B, H, Hkv, Nq, Nk, D;
+    float scale;
+    int64_t q_batch, q_head, q_token, k_batch, k_head, k_token, v_batch, v_head, v_token;
+    int64_t o_batch, o_head, o_token, mask_stride;
+} aria_hip_cross_attn;
+size_t aria_hip_cross_attention_ws_bytes(const aria_hip_cross_attn *a);
+int aria_hip_cross_attention_dev(const aria_hip_cross_attn *a, void *dws, void *stream);
+/* Host form: q fp32 [B*H, Nq, D] and k/v [B*Hkv, Nk, D] are rounded to fp16 on the device, scale is
+ * 1/sqrt(D); kv_len [B] and mask [B, Nk] may be NULL; out fp32 [B, Nq, H*D]. */
+int aria_hip_cross_attention_f16(float *out, const float *q, const float *k, const float *v, const int32_t *kv_len,
+                                 const uint8_t *mask, int B, int H, int Hkv, int Nq, int Nk, int D);
+
+/* ---- MXFP4: microscaled 4-bit floating point (no counterpart in the reference) ----
+ * Blocks of 32 values along K share a power of two 2^(byte - 127); a value is a 4-bit code: sign
+ * and magnitude 0, 0.5, 1, 1.5, 2, 3, 4 or 6 (e2m1). A packed row is ceil(K/32) blocks of 16
+ * bytes (the even element in the low nibble, codes past K zero) in dq [rows, 16 * ceil(K/32)]
+ * and one byte per block in dscale [rows, ceil(K/32)]; dq is 16-byte aligned.
+ * Quantisation: byte = floor(log2 max|x|) - 2 + 127 (at least 0; 0 for a block of zeros), codes
+ * x / 2^(byte - 127) to nearest, ties to the even code, saturating at 6, the sign of zero kept. A
+ * block that holds an Inf or a NaN gets byte 255 and codes 0: it stands for NaN.
+ * Element types of activations and outputs are aria_dtype's values: 0 fp32, 1 fp16, 2 bf16;
+ * ldx: elements between rows of x (at least K). K at most 2^30. */
+int aria_hip_mx4_quant_dev(uint8_t *dq, uint8_t *dscale, const void *dx, int xtype, int rows, int K, int64_t ldx,
+                           void *stream);
+/* y [rows, K] from packed rows, rounded to ytype (fp32 holds every value) */
+int aria_hip_mx4_dequant_dev(void *dy, int ytype, const uint8_t *dq, const uint8_t *dscale, int rows, int K,
+                             void *stream);
+/* dy[m,n] = sum_k x[m,k] w[n,k] (+ db[n]; db NULL = none) on packed activations [M, K] and weights
+ * [N, K]: block-scaled MFMA, fp32 sums, rounded once to ytype. */
+int aria_hip_gemm_mx4_dev(void *dy, int ytype, const uint8_t *dxq, const uint8_t *dxs, const uint8_t *dq,
+                          const uint8_t *dscale, const float *db, int M, int K, int N, void *stream);
+/* The same with the activations quantised in the call. dws: caller workspace of
+ * aria_hip_mx4_ws_bytes(M, K) bytes, 256-byte aligned, not shared by calls that may run at the
+ * same time. */
+size_t aria_hip_mx4_ws_bytes(int M, int K);
+int aria_hip_linear_mx4_dev(void *dy, int ytype, const void *dx, int xtype, int64_t ldx, const uint8_t *dq,
+                            const uint8_t *dscale, const float *db, int M, int K, int N, void *dws, void *stream);
+/* Gated feed-forward up-projection, one pass: dq / dscale / db hold 2 * inner rows [value | gate]
+ * (the order of aria_hip_glu_combine_dev), dy[m,i] = v * silu(g) with v = x . w[i] + db[i] and
+ * g = x . w[inner + i] + db[inner + i] in fp32; neither projection is stored. */
+int aria_hip_glu_mx4_dev(void *dy, int ytype, const void *dx, int xtype, int64_t ldx, const uint8_t *dq,
+                         const uint8_t *dscale, const float *db, int M, int K, int inner, void *dws, void *stream);
+/* Host forms (fp32): q [rows, 16 * ceil(K/32)], scale [rows, ceil(K/32)]. */
+int aria_hip_mx4_quant(uint8_t *q, uint8_t *scale, const float *x, int rows, int K);
+int aria_hip_mx4_dequant(float *y, const uint8_t *q, const uint8_t *scale, int rows, int K);
+int aria_hip_linear_mx4(float *y, const float *x, const uint8_t *q, const uint8_t *scale, const float *b, int M,
+                        int K, int N);
+int aria_hip_glu_mx4(float *y, const float *x, const uint8_t *q, const uint8_t *scale, const float *b, int M, int K,
+                     int inner);
+
 /* Host-pointer forms with the reference's signatures (src/aria_quant.h:43-45, 64-65):
  * allocate, copy in, run, copy out, free; synchronous. Return 0 or an error. */
 int aria_hip_q8_quant(int8_t *q, float *scale, const float *W, int N, int K);
