@@ -191,4 +191,19 @@ __device__ __forceinline__ void f4set(float4 &v, int i, float x) {
     if (i == 0) v.x = x; else if (i == 1) v.y = x; else if (i == 2) v.z = x; else v.w = x;
 }
 
+/* s_waitcnt vmcnt(n) with the other counters left alone (gfx9 encoding) */
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+    static_assert(N >= 0 && N < 64, "vmcnt");
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (0x7 << 4) | (0xF << 8));
+}
+
+/* One LDS DMA instruction: every lane moves 16 B from global address g to LDS byte address
+ * m0 + 16 * lane (m0 wave-uniform). Issued as inline assembly, so the compiler neither waits
+ * for it nor reorders memory accesses across it: the kernel waits on vmcnt itself. */
+__device__ __forceinline__ void dma16(const void *g, uint32_t m0) {
+    const uint32_t m = __builtin_amdgcn_readfirstlane(m0);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(m), "v"(g) : "memory");
+}
+
 #endif /* ARIA_DEV_H */

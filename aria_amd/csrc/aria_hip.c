@@ -638,8 +638,8 @@ static int xattn_check(const aria_hip_cross_attn *a) {
     REQ(a && (a->type == 1 || a->type == 2));
     REQ(a->B >= 0 && a->H > 0 && a->Hkv > 0 && a->H % a->Hkv == 0 && a->Nq >= 0 && a->Nk >= 0);
     REQ(a->D >= 8 && a->D <= 128 && a->D % 8 == 0);
-    REQ((int64_t)a->Nq * (a->H / a->Hkv) <= (1 << 30) && a->Nk <= (1 << 30));
-    REQ((int64_t)a->B * a->H <= (1 << 24));
+    REQ(a->Nk <= (1 << 30) && (int64_t)a->B * a->H <= (1 << 20));
+    REQ((int64_t)a->B * a->H * a->Nq <= (1 << 30));
     REQ(a->B == 0 || a->Nq == 0 || (a->q && a->out && (a->Nk == 0 || (a->k && a->v))));
     REQ((((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->out) & 15u) == 0);
     REQ(((uintptr_t)a->kv_len & 3u) == 0);

@@ -3,61 +3,432 @@
  * sequence (gfx950): o = sum_j p_j v_j, p = softmax over the valid keys of scale * q . k_j, where key
  * j of sequence b is valid when j < kv_len[b] and mask[b, j] != 0. A row without a valid key is zero.
  * H query heads share Hkv key/value heads (H / Hkv consecutive query heads to each).
+ *
+ * One pass over the keys: each wave keeps 32 rows' running maximum, sum and fp32 output while key
+ * tiles go by; scores never leave registers. The rows of one key/value head are (token, query head of
+ * its group) pairs, so grouped heads and single tokens fill the 32 columns of an MFMA together.
+ *
+ * S^T = K Q^T and O^T = V^T P^T with v_mfma_f32_32x32x16: the accumulator of lane l (row l % 32, keys
+ * 8 (r / 4) + 4 (l / 32) + r % 4) is the second product's B operand once rounded to 16 bits; V's
+ * operand comes from key-major LDS by the transpose read in the same key order. Lanes l and l ^ 32
+ * share a row, so a maximum needs one exchange.
+ *
+ * K and V tiles arrive by LDS DMA, two stages. Slots of keys that are not valid, and of dims past D, are
+ * filled from 16 bytes of zeros: whatever lies in masked places (NaN, Inf, memory behind the last
+ * state) never enters LDS. Scores of such keys are set to -inf before the maximum.
+ *
+ * The maximum is a lazy reference: it moves only when a tile exceeds it by 2^8, which leaves O / l
+ * unchanged. It starts finite (below any score of 16-bit operands that a softmax can tell apart), so
+ * a slice whose keys all score -inf has weight zero instead of NaN. P is rounded to the type of V; the
+ * row sum adds the rounded values, so the weights still sum to one.
  */
 #include "aria_dev.h"
 #include "aria_hip_kernels.h"
 
-/* One wave per query row: scores of 64 keys by lane, running maximum and sum, output dims by lane. */
-template <typename T>
-__global__ __launch_bounds__(64) void k_xattn_row(aria_k_xattn a) {
-    __shared__ float P[64];
-    const int lane = threadIdx.x;
-    const long long w = blockIdx.x;            /* (b * H + h) * Nq + t */
-    const int t = (int)(w % a.Nq), h = (int)(w / a.Nq % a.H), b = (int)(w / a.Nq / a.H), hk = h / (a.H / a.Hkv);
-    const T *q = (const T *)a.q + b * a.q_batch + h * a.q_head + t * a.q_token;
-    const T *k = (const T *)a.k + b * a.k_batch + hk * a.k_head;
-    const T *v = (const T *)a.v + b * a.v_batch + hk * a.v_head;
-    const int n = a.kv_len ? min(max(a.kv_len[b], 0), a.Nk) : a.Nk;
-    float m = -INFINITY, l = 0.0f, o0 = 0.0f, o1 = 0.0f;
-    for (int j0 = 0; j0 < n; j0 += 64) {
-        const int j = j0 + lane;
-        const bool ok = j < n && (!a.mask || a.mask[b * a.mask_stride + j] != 0);
-        float s = 0.0f;
-        if (ok)
-            for (int d = 0; d < a.D; d++) s = __builtin_fmaf((float)q[d], (float)k[j * a.k_token + d], s);
-        s = ok ? s * a.scale : -INFINITY;
-        const float mn = fmaxf(m, grp_max<64>(s));
-        const float ref = mn == -INFINITY ? 0.0f : mn;
-        const float p = ok ? expf(s - ref) : 0.0f, al = expf(m - ref);
-        l = l * al + grp_sum<64>(p);
-        o0 *= al; o1 *= al; m = mn;
-        P[lane] = p;
-        __syncthreads();
-        for (int i = 0; i < 64 && j0 + i < n; i++) {
-            if (P[i] == 0.0f) continue;
-            const T *vj = v + (j0 + i) * a.v_token;
-            if (lane < a.D) o0 = __builtin_fmaf(P[i], (float)vj[lane], o0);
-            if (64 + lane < a.D) o1 = __builtin_fmaf(P[i], (float)vj[64 + lane], o1);
-        }
-        __syncthreads();
+typedef float xa_f32x16_t __attribute__((ext_vector_type(16)));
+typedef short xa_i16x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) xa_i16x4_t xa_lds_i16x4_t;
+
+#define XA_SLACK 8.0f      /* log2 units that the reference may lag the maximum */
+#define XA_MIN (-3e38f)    /* the reference before any key */
+
+/* 16-byte source of slots that hold no valid key or no dim */
+__device__ const uint4 xa_zero = {0, 0, 0, 0};
+
+template <typename T> struct Xa;
+template <> struct Xa<_Float16> {
+    typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+    typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+    static __device__ __forceinline__ xa_f32x16_t mfma(v8 a, v8 b, xa_f32x16_t c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
     }
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    const long long ob = b * a.o_batch + h * a.o_head + t * a.o_token;
-    if (a.out_f32) {
-        if (lane < a.D) ((float *)a.out)[ob + lane] = o0 * inv;
-        if (64 + lane < a.D) ((float *)a.out)[ob + 64 + lane] = o1 * inv;
-    } else {
-        if (lane < a.D) ((T *)a.out)[ob + lane] = (T)(o0 * inv);
-        if (64 + lane < a.D) ((T *)a.out)[ob + 64 + lane] = (T)(o1 * inv);
+    static __device__ __forceinline__ float dot2(v2 a, v2 b, float c) { return __builtin_amdgcn_fdot2(a, b, c, false); }
+};
+template <> struct Xa<__bf16> {
+    typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+    typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+    static __device__ __forceinline__ xa_f32x16_t mfma(v8 a, v8 b, xa_f32x16_t c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ float dot2(v2 a, v2 b, float c) { return __builtin_amdgcn_fdot2_f32_bf16(a, b, c, false); }
+};
+
+__device__ __forceinline__ float xa_max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
+struct XaArgs {
+    aria_k_xattn a;
+    int G, R;            /* query heads per key head; rows per (batch, key head) */
+    int nrb, T;          /* row blocks per (batch, key head); workgroups per split */
+    int ns;              /* splits of the keys across workgroups */
+    float scale_log2;
+    float *part;         /* ns > 1: per (tile, split) 32 x DP sums, 32 references, 32 row sums */
+};
+
+/* floats of one partial result */
+__host__ __device__ constexpr int xa_part(int DP) { return 32 * DP + 64; }
+
+/* QW waves of 32 rows share every tile (KS = 1), or KS waves take the tiles in turn, each on LDS
+ * stages of its own and without barriers, and join their results at the end (QW = 1). */
+template <typename T, int DP, int KT, int QW, int KS>
+__global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
+    static_assert((QW == 1 || KS == 1) && (DP == 64 || DP == 128) && (KT == 64 || KT == 32), "");
+    constexpr int NW = QW * KS;
+    constexpr int CPR = DP / 8;                     /* 16-byte chunks per key row */
+    constexpr int SLOTS = KT * CPR;                 /* per tile and operand */
+    constexpr int ND = SLOTS / 64 / QW;             /* DMA instructions per wave, tile and operand */
+    constexpr int TB = SLOTS * 16;                  /* bytes of a tile */
+    constexpr int ES = DP + 4;                      /* floats per staged output row */
+    constexpr int KB = KT / 32, DT = DP / 32, DS = DP / 16;
+    constexpr int STAGE = 2 * TB * KS;              /* K and V of every slice */
+    constexpr int EPI = NW * 32 * ES * 4 + KS * 64 * 4;
+    __shared__ __attribute__((aligned(16))) uint8_t smem[2 * STAGE > EPI ? 2 * STAGE : EPI];
+    typedef typename Xa<T>::v8 v8;
+    typedef typename Xa<T>::v2 v2;
+    const aria_k_xattn &a = x.a;
+
+    const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
+    const int wid = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int qw = KS == 1 ? wid : 0, ks = KS == 1 ? 0 : wid;
+
+    /* row blocks of one key head run on one XCD, whose L2 then holds its K and V; batches alternate
+     * fastest so that unequal lengths spread over the XCDs */
+    const int wg = xcd_tile(blockIdx.x, x.T * x.ns);
+    if (wg >= x.T * x.ns) return;
+    const int split = wg % x.ns, t = wg / x.ns;
+    const int rb = t % x.nrb, bh = t / x.nrb, b = bh % a.B, hk = bh / a.B;
+    const int n = a.kv_len ? min(max(a.kv_len[b], 0), a.Nk) : a.Nk;
+    const uint8_t *mask = a.mask ? a.mask + b * a.mask_stride : nullptr;
+    const int row = rb * 32 * QW + qw * 32 + l32;   /* this lane's row; rows past R repeat the last */
+    const int rr = min(row, x.R - 1), tok = rr / x.G, hd = hk * x.G + rr % x.G;
+
+    v8 qf[DS];
+    {
+        const T *q = (const T *)a.q + b * a.q_batch + hd * a.q_head + tok * a.q_token;
+#pragma unroll
+        for (int i = 0; i < DS; i++) {
+            const int d = 16 * i + 8 * g;
+            uint4 u = make_uint4(0, 0, 0, 0);
+            if (d < a.D) u = *reinterpret_cast<const uint4 *>(q + d);
+            qf[i] = __builtin_bit_cast(v8, u);
+        }
+    }
+
+    /* this workgroup's tiles, and this slice's share of them: [t0, t1) */
+    const int nt = (n + KT - 1) / KT, per = (nt + x.ns - 1) / x.ns;
+    const int w0 = min(split * per, nt), w1 = min(w0 + per, nt);
+    const int sp = (w1 - w0 + KS - 1) / KS;
+    const int t0 = min(w0 + ks * sp, w1), t1 = min(t0 + sp, w1);
+
+    /* DMA sources of key 0 of the slice, one per instruction: slot p holds chunk cp of key row r, and
+     * receives the chunk that the swizzle puts there */
+    const T *kp[ND], *vp[ND];
+    int krow[ND];
+    bool kd[ND], vd[ND];
+    {
+        const T *Kh = (const T *)a.k + b * a.k_batch + hk * a.k_head + (long long)t0 * KT * a.k_token;
+        const T *Vh = (const T *)a.v + b * a.v_batch + hk * a.v_head + (long long)t0 * KT * a.v_token;
+#pragma unroll
+        for (int i = 0; i < ND; i++) {
+            const int p = 64 * (QW * i + qw) + lane, r = p / CPR, cp = p % CPR;
+            const int ck = DP == 64 ? cp ^ ((r >> 1) & 7) : cp ^ (r & 15);
+            const int cv = DP == 64 ? cp ^ (((r >> 1) & 1) << 2) : cp ^ ((r & 3) << 2);
+            krow[i] = r;
+            kp[i] = Kh + r * a.k_token + 8 * ck;
+            vp[i] = Vh + r * a.v_token + 8 * cv;
+            kd[i] = 8 * ck < a.D;
+            vd[i] = 8 * cv < a.D;
+        }
+    }
+    const long long kstep = KT * a.k_token, vstep = KT * a.v_token;
+    auto dma = [&](int buf, uint64_t bits) __attribute__((always_inline)) {
+        const uint32_t S = (uint32_t)(uintptr_t)smem + buf * STAGE + ks * 2 * TB;
+#pragma unroll
+        for (int i = 0; i < ND; i++) {
+            const bool ok = (bits >> krow[i]) & 1;
+            const void *k = ok && kd[i] ? (const void *)kp[i] : (const void *)&xa_zero;
+            const void *v = ok && vd[i] ? (const void *)vp[i] : (const void *)&xa_zero;
+            dma16(k, S + 1024 * (QW * i + qw));
+            dma16(v, S + TB + 1024 * (QW * i + qw));
+            kp[i] += kstep;
+            vp[i] += vstep;
+        }
+    };
+    /* the valid keys of tile i (bit j: key KT i + j) where no mask says otherwise */
+    auto in_len = [&](int i) __attribute__((always_inline)) -> uint64_t {
+        const int left = n - i * KT;
+        const uint64_t all = KT == 64 ? ~0ull : 0xFFFFFFFFull;
+        return left >= KT ? all : left <= 0 ? 0ull : (1ull << left) - 1;
+    };
+    auto mask_byte = [&](int i) __attribute__((always_inline)) -> int {
+        const int j = i * KT + (lane & (KT - 1));
+        return mask && i < t1 && j < n ? mask[j] : 1;
+    };
+    auto to_bits = [&](int i, int byte) __attribute__((always_inline)) -> uint64_t {
+        return i < t1 ? in_len(i) & __ballot(byte != 0) : 0ull;
+    };
+
+    xa_f32x16_t o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
+    float l = 0.0f, ref = XA_MIN;
+    const v2 one2 = {(T)1.0f, (T)1.0f};
+
+    /* byte offsets of the fragment reads */
+    int koff[DS], voff[DT];
+#pragma unroll
+    for (int i = 0; i < DS; i++) {
+        const int c = 2 * i + g;
+        koff[i] = (l32 * CPR + (DP == 64 ? c ^ ((l32 >> 1) & 7) : c ^ (l32 & 15))) * 16;
+    }
+    {
+        const int v = (lane & 15) >> 2, w = lane & 3, Gq = lane >> 4, key = 4 * (Gq >> 1) + v;
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            const int dd = 32 * d + 16 * (Gq & 1) + 4 * w, c = dd >> 3;
+            voff[d] = (key * CPR + (DP == 64 ? c ^ (((key >> 1) & 1) << 2) : c ^ ((key & 3) << 2))) * 16 + (dd & 7) * 2;
+        }
+    }
+
+    auto tile = [&](int buf, uint64_t bits) __attribute__((always_inline)) {
+        const uint8_t *K = smem + buf * STAGE + ks * 2 * TB, *V = K + TB;
+        xa_f32x16_t s[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[kb][r] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < DS; i++)
+#pragma unroll
+            for (int kb = 0; kb < KB; kb++)
+                s[kb] = Xa<T>::mfma(*reinterpret_cast<const v8 *>(K + koff[i] + kb * 32 * CPR * 16), qf[i], s[kb]);
+        if (bits != (KT == 64 ? ~0ull : 0xFFFFFFFFull)) {
+            const float ninf = -INFINITY;
+#pragma unroll
+            for (int kb = 0; kb < KB; kb++) {
+                const unsigned w = (unsigned)(bits >> (32 * kb));
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int k0 = 8 * (r >> 2) + (r & 3);   /* lanes 0..31; lanes 32..63 hold key k0 + 4 */
+                    const unsigned lo = 0u - ((w >> k0) & 1u), hi = 0u - ((w >> (k0 + 4)) & 1u);
+                    const uint64_t m = ((uint64_t)hi << 32) | lo;
+                    asm("v_cndmask_b32 %0, %1, %2, %3" : "=v"(s[kb][r]) : "v"(ninf), "v"(s[kb][r]), "s"(m));
+                }
+            }
+        }
+        float mt = s[0][0];
+#pragma unroll
+        for (int i = 1; i + 1 < 16 * KB; i += 2) mt = xa_max3(mt, s[i >> 4][i & 15], s[(i + 1) >> 4][(i + 1) & 15]);
+        mt = fmaxf(mt, s[KB - 1][15]);
+        mt = fmaxf(mt, xor32_f32(mt, lane)) * x.scale_log2;
+        if (__ballot(mt > ref + XA_SLACK)) {
+            asm volatile("" ::: "memory");   /* a branch, not 16 DT predicated multiplies */
+            const float m2 = fmaxf(ref, mt), al = __builtin_amdgcn_exp2f(ref - m2);
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) o[d][r] *= al;
+            l *= al;
+            ref = m2;
+        }
+#pragma unroll
+        for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int s16 = 2 * kb + h;      /* keys 16 s16 .. 16 s16 + 15 */
+                v8 vf[DT];
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    const uint8_t *p = V + voff[d] + 16 * s16 * CPR * 16;
+                    const xa_i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((xa_lds_i16x4_t *)p);
+                    const xa_i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((xa_lds_i16x4_t *)(p + 8 * CPR * 16));
+                    vf[d] = __builtin_bit_cast(v8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                }
+                v8 p;
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    p[i] = (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * h + i], x.scale_log2, -ref));
+#pragma unroll
+                for (int d = 0; d < DT; d++) o[d] = Xa<T>::mfma(vf[d], p, o[d]);
+#pragma unroll
+                for (int i = 0; i < 4; i++) l = Xa<T>::dot2(v2{p[2 * i], p[2 * i + 1]}, one2, l);
+            }
+    };
+    /* this wave's transfers have landed and its fragment reads have returned: without the latter a read
+     * still in flight would race with the next transfer into its stage. The compiler does not know of
+     * the transfers, so this is also its fence */
+    auto drain = []() __attribute__((always_inline)) { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); };
+    auto meet = [&]() __attribute__((always_inline)) {
+        if constexpr (KS == 1) __syncthreads();
+    };
+
+    uint64_t cur = to_bits(t0, mask_byte(t0)), nxt = to_bits(t0 + 1, mask_byte(t0 + 1));
+    if (t0 < t1) dma(0, cur);
+    drain();
+    meet();
+    for (int i = t0; i < t1; i++) {
+        const int buf = (i - t0) & 1;
+        const int byte = mask_byte(i + 2);
+        if (i + 1 < t1) dma(buf ^ 1, nxt);
+        if (cur) tile(buf, cur);
+        drain();
+        meet();
+        cur = nxt;
+        nxt = to_bits(i + 2, byte);
+    }
+
+    /* join: lanes l and l ^ 32 hold half of a row's sum each */
+    l += xor32_f32(l, lane);
+    float *E = (float *)smem + wid * 32 * ES;
+    float *ML = (float *)smem + NW * 32 * ES;       /* KS x (32 references, 32 sums) */
+    if (KS > 1) __syncthreads();                     /* slices still reading their stages */
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            *reinterpret_cast<float4 *>(E + l32 * ES + 32 * d + 8 * r + 4 * g) =
+                make_float4(o[d][4 * r], o[d][4 * r + 1], o[d][4 * r + 2], o[d][4 * r + 3]);
+    if (KS > 1 && g == 0) { ML[ks * 64 + l32] = ref; ML[ks * 64 + 32 + l32] = l; }
+    __syncthreads();
+
+    /* a group of CPR lanes finishes one row, 8 dims per lane; the NW waves take rows in turn
+     * (KS > 1: all of them the workgroup's one block of 32) */
+    constexpr int RPW = 64 / CPR;                    /* rows per wave at once */
+    const int c8 = 8 * (lane % CPR);
+#pragma unroll 1
+    for (int i = KS == 1 ? 0 : wid; i < 32 / RPW; i += KS) {
+        const int q = i * RPW + lane / CPR;          /* row within the block */
+        float v[8], rs, rm;
+        if constexpr (KS == 1) {
+            const float *e = E + q * ES + c8;
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = e[j];
+            rs = __shfl(l, q, 64);
+            rm = __shfl(ref, q, 64);
+        } else {
+            rm = XA_MIN;
+#pragma unroll
+            for (int w = 0; w < KS; w++) rm = fmaxf(rm, ML[w * 64 + q]);
+            rs = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < KS; w++) {
+                const float f = __builtin_amdgcn_exp2f(ML[w * 64 + q] - rm);
+                rs = __builtin_fmaf(f, ML[w * 64 + 32 + q], rs);
+                const float *e = (const float *)smem + (w * 32 + q) * ES + c8;
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] = __builtin_fmaf(f, e[j], v[j]);
+            }
+        }
+        const int orow = rb * 32 * QW + qw * 32 + q;
+        if (orow >= x.R || c8 >= a.D) continue;
+        if (x.ns > 1) {
+            float *P = x.part + (size_t)(t * x.ns + split) * xa_part(DP);
+            *reinterpret_cast<float4 *>(P + q * DP + c8) = make_float4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<float4 *>(P + q * DP + c8 + 4) = make_float4(v[4], v[5], v[6], v[7]);
+            if (c8 == 0) { P[32 * DP + q] = rm; P[32 * DP + 32 + q] = rs; }
+            continue;
+        }
+        const float inv = rs > 0.0f ? 1.0f / rs : 0.0f;
+        const long long at = b * a.o_batch + (hk * x.G + orow % x.G) * a.o_head + (orow / x.G) * a.o_token + c8;
+        if (a.out_f32) {
+            float *y = (float *)a.out + at;
+            *reinterpret_cast<float4 *>(y) = make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+            *reinterpret_cast<float4 *>(y + 4) = make_float4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
+        } else {
+            v8 y;
+#pragma unroll
+            for (int j = 0; j < 8; j++) y[j] = (T)(v[j] * inv);
+            *reinterpret_cast<v8 *>((T *)a.out + at) = y;
+        }
     }
 }
 
-extern "C" size_t aria_k_xattn_ws_bytes(const aria_k_xattn *a) { return 0; }
+/* Joins the ns partial results of each block of 32 rows: a lane per 8 dims of a row. */
+template <typename T>
+__global__ __launch_bounds__(256) void k_xattn_join(XaArgs x, int DP) {
+    const aria_k_xattn &a = x.a;
+    const int cpr = DP / 8, t = blockIdx.x, rb = t % x.nrb, bh = t / x.nrb, b = bh % a.B, hk = bh / a.B;
+    for (int i = threadIdx.x; i < 32 * cpr; i += 256) {
+        const int q = i / cpr, c8 = 8 * (i % cpr), row = rb * 32 + q;
+        if (row >= x.R || c8 >= a.D) continue;
+        const float *P = x.part + (size_t)t * x.ns * xa_part(DP);
+        float m = XA_MIN, rs = 0.0f, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        for (int s = 0; s < x.ns; s++) m = fmaxf(m, P[(size_t)s * xa_part(DP) + 32 * DP + q]);
+        for (int s = 0; s < x.ns; s++) {
+            const float *p = P + (size_t)s * xa_part(DP);
+            const float f = __builtin_amdgcn_exp2f(p[32 * DP + q] - m);
+            rs = __builtin_fmaf(f, p[32 * DP + 32 + q], rs);
+            const float4 u = *reinterpret_cast<const float4 *>(p + q * DP + c8), w = *reinterpret_cast<const float4 *>(p + q * DP + c8 + 4);
+            const float e[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = __builtin_fmaf(f, e[j], v[j]);
+        }
+        const float inv = rs > 0.0f ? 1.0f / rs : 0.0f;
+        const long long at = b * a.o_batch + (hk * x.G + row % x.G) * a.o_head + (row / x.G) * a.o_token + c8;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            if (a.out_f32) ((float *)a.out)[at + j] = v[j] * inv;
+            else ((T *)a.out)[at + j] = (T)(v[j] * inv);
+        }
+    }
+}
+
+/* how a call runs: few = KS waves per 32 rows, else QW = 4 blocks of 32 rows; ns splits of the keys */
+struct XaPlan { bool few; int DP, nrb, T, ns; };
+static XaPlan xa_plan(const aria_k_xattn *a) {
+    XaPlan p;
+    const long long R = (long long)a->Nq * (a->H / a->Hkv), bh = (long long)a->B * a->Hkv;
+    p.DP = a->D <= 64 ? 64 : 128;
+    p.few = bh * ((R + 127) / 128) < 256;
+    p.nrb = (int)(p.few ? (R + 31) / 32 : (R + 127) / 128);
+    p.T = (int)(bh * p.nrb);
+    p.ns = 1;
+    if (p.few) {
+        /* at least 512 keys to a workgroup, and about three workgroups to a CU */
+        const int most = a->Nk / 512;
+        while (p.ns < most && (long long)p.T * p.ns < 768) p.ns++;
+    }
+    return p;
+}
+
+extern "C" size_t aria_k_xattn_ws_bytes(const aria_k_xattn *a) {
+    const XaPlan p = xa_plan(a);
+    return p.ns > 1 ? (size_t)p.T * p.ns * xa_part(p.DP) * sizeof(float) : 0;
+}
+
+template <typename T>
+static hipError_t xa_launch(const XaPlan &p, const XaArgs &x, hipStream_t s) {
+    const int n = p.T * p.ns;
+    const dim3 grid((unsigned)((n + 7) / 8 * 8));
+    if (p.few) {
+        if (p.DP == 64) hipLaunchKernelGGL((k_xattn<T, 64, 64, 1, 4>), grid, dim3(256), 0, s, x);
+        else hipLaunchKernelGGL((k_xattn<T, 128, 32, 1, 4>), grid, dim3(256), 0, s, x);
+        if (p.ns > 1) hipLaunchKernelGGL(k_xattn_join<T>, dim3(p.T), dim3(256), 0, s, x, p.DP);
+    } else {
+        if (p.DP == 64) hipLaunchKernelGGL((k_xattn<T, 64, 64, 4, 1>), grid, dim3(256), 0, s, x);
+        else hipLaunchKernelGGL((k_xattn<T, 128, 64, 4, 1>), grid, dim3(256), 0, s, x);
+    }
+    return hipGetLastError();
+}
 
 extern "C" hipError_t aria_k_xattn_run(const aria_k_xattn *a, void *ws, hipStream_t s) {
     if (a->B <= 0 || a->Nq <= 0) return hipSuccess;
-    const dim3 grid((unsigned)((long long)a->B * a->H * a->Nq));
-    if (a->type == 1) hipLaunchKernelGGL(k_xattn_row<_Float16>, grid, dim3(64), 0, s, *a);
-    else hipLaunchKernelGGL(k_xattn_row<__bf16>, grid, dim3(64), 0, s, *a);
-    return hipGetLastError();
+    const XaPlan p = xa_plan(a);
+    XaArgs x;
+    x.a = *a;
+    x.G = a->H / a->Hkv;
+    x.R = a->Nq * x.G;
+    x.nrb = p.nrb;
+    x.T = p.T;
+    x.ns = p.ns;
+    x.scale_log2 = a->scale * ARIA_LOG2E;
+    x.part = (float *)ws;
+    return a->type == 1 ? xa_launch<_Float16>(p, x, s) : xa_launch<__bf16>(p, x, s);
 }

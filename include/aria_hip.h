@@ -227,7 +227,8 @@ int aria_hip_attention_f16(float *out, const float *q, const float *k, const flo
  * all). A row with no valid key (Nk = 0 included) is written as zeros. Keys and values that are
  * not valid may hold anything (Inf and NaN included): they do not reach the result, but all Nk
  * rows must be readable memory. type: 1 = fp16, 2 = bf16 (aria_dtype's values) for q, k, v and
- * out; out_f32 != 0 writes fp32. D: a multiple of 8 up to 128. H a multiple of Hkv.
+ * out; out_f32 != 0 writes fp32. D: a multiple of 8 up to 128. H a multiple of Hkv. B * H at most
+ * 2^20, B * H * Nq and Nk at most 2^30.
  * Strides count elements and are multiples of 8, not negative, pointers are 16-byte aligned (for
  * an fp32 out too); batch / head / token strides of q, k and v may be 0 (broadcast). Probabilities
  * are rounded to the type before they multiply v; sums and softmax statistics are fp32.
