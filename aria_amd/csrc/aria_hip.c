@@ -569,7 +569,8 @@ int aria_hip_linear_q8a8_dev(float *dy, const void *dx, int x_f16, const int8_t 
 
 /* MXFP4 (k_mx4.hip, k_mx4_gemm.hip). Arguments are checked before the device is looked for. */
 #define MX4_TYPE(t) ((t) == 0 || (t) == 1 || (t) == 2)
-#define MX4_KMAX (1 << 30)
+#define MX4_KMAX (1 << 24)   /* lane offsets within a tile's 256 rows are 32 bits wide */
+#define MX4_NMAX (1 << 26)
 static size_t mx4_blocks(int K) { return ((size_t)K + 31) / 32; }
 static uintptr_t mx4_el_mask(int type) { return type == 0 ? 3u : 1u; }
 
@@ -593,7 +594,7 @@ int aria_hip_mx4_dequant_dev(void *dy, int ytype, const uint8_t *dq, const uint8
 }
 static int gemm_mx4(void *dy, int ytype, const uint8_t *dxq, const uint8_t *dxs, const uint8_t *dq,
                     const uint8_t *dscale, const float *db, int M, int K, int N, int glu, void *stream) {
-    REQ(M >= 0 && K > 0 && K <= MX4_KMAX && N >= 0 && N <= (1 << 30) && MX4_TYPE(ytype));
+    REQ(M >= 0 && K > 0 && K <= MX4_KMAX && N >= 0 && N <= MX4_NMAX && MX4_TYPE(ytype));
     REQ(M == 0 || N == 0 || (dy && dxq && dxs && dq && dscale));
     REQ((((uintptr_t)dxq | (uintptr_t)dq) & 15u) == 0 && ((uintptr_t)dy & mx4_el_mask(ytype)) == 0);
     REQ(((uintptr_t)db & 3u) == 0);
@@ -612,13 +613,17 @@ size_t aria_hip_mx4_ws_bytes(int M, int K) {
 }
 static int linear_mx4(void *dy, int ytype, const void *dx, int xtype, int64_t ldx, const uint8_t *dq,
                       const uint8_t *dscale, const float *db, int M, int K, int N, int glu, void *dws, void *stream) {
-    REQ(M >= 0 && K > 0 && K <= MX4_KMAX && N >= 0 && N <= (1 << 30) && MX4_TYPE(ytype));
+    REQ(M >= 0 && K > 0 && K <= MX4_KMAX && N >= 0 && N <= MX4_NMAX && MX4_TYPE(ytype));
     REQ(MX4_TYPE(xtype) && ldx >= K);
     REQ(M == 0 || N == 0 || (dy && dx && dq && dscale && dws));
     REQ(((uintptr_t)dq & 15u) == 0 && ((uintptr_t)dws & 255u) == 0 && ((uintptr_t)db & 3u) == 0);
     REQ(((uintptr_t)dy & mx4_el_mask(ytype)) == 0 && ((uintptr_t)dx & mx4_el_mask(xtype)) == 0);
     if (M == 0 || N == 0) return 0;
     ENSURE();
+    if (M <= ARIA_MX4_ROWS) {
+        KCK(aria_k_mx4_rows(dy, ytype, dx, xtype, (long)ldx, dq, dscale, db, M, K, N, glu, pick(stream)), "k_mx4_rows");
+        return 0;
+    }
     uint8_t *xq = (uint8_t *)dws, *xs = xq + mx4_ws_scale(M, K);
     KCK(aria_k_mx4_quant(xq, xs, dx, xtype, M, K, (long)ldx, pick(stream)), "k_mx4_quant");
     KCK(aria_k_mx4_gemm(dy, ytype, xq, xs, dq, dscale, db, M, K, N, glu, pick(stream)), "k_mx4_gemm");
@@ -805,7 +810,7 @@ int aria_hip_mx4_dequant(float *y, const uint8_t *q, const uint8_t *scale, int r
 }
 static int host_linear_mx4(float *y, const float *x, const uint8_t *q, const uint8_t *scale, const float *b, int M,
                            int K, int N, int glu) {
-    REQ(M >= 0 && K > 0 && K <= MX4_KMAX && N >= 0 && N <= (1 << 30) && y && x && q && scale);
+    REQ(M >= 0 && K > 0 && K <= MX4_KMAX && N >= 0 && N <= MX4_NMAX && y && x && q && scale);
     if (M == 0 || N == 0) return 0;
     HOST_BEGIN();
     const size_t rows = (size_t)N << glu, nb = rows * mx4_blocks(K);

@@ -258,6 +258,10 @@ hipError_t aria_k_mx4_dequant(void *y, int ytype, const uint8_t *q, const uint8_
                               hipStream_t s);
 hipError_t aria_k_mx4_gemm(void *y, int ytype, const uint8_t *xq, const uint8_t *xs, const uint8_t *wq,
                            const uint8_t *ws, const float *bias, int M, int K, int N, int glu, hipStream_t s);
+/* the same on unpacked activations of at most ARIA_MX4_ROWS rows, in one launch */
+#define ARIA_MX4_ROWS 16
+hipError_t aria_k_mx4_rows(void *y, int ytype, const void *x, int xtype, long ldx, const uint8_t *wq,
+                           const uint8_t *ws, const float *bias, int M, int K, int N, int glu, hipStream_t s);
 
 /* Cross attention over ragged encoder states (k_xattn.hip): the public description as the kernels
  * take it; ws holds aria_k_xattn_ws_bytes bytes. */

@@ -7,7 +7,8 @@
  * v_mfma_scale_f32_32x32x64_f8f6f4 takes one block of 32 codes (16 bytes) and one scale byte per
  * lane and operand, so a packed row is the operand as it lies in memory: no unpacking at all. Weights
  * are the A operand and activations the B operand: a lane's accumulators are then 4 consecutive
- * columns n of one row m.
+ * columns n of one row m. Sums over K do not depend on which block a lane half takes, so half h takes
+ * blocks 4h .. 4h + 3 of each 8-block chunk: its four scale bytes are one dword, picked by op_sel.
  */
 #include "mx4_dev.h"
 
@@ -18,60 +19,356 @@ struct MxArgs {
     int M, N;          /* N: output columns (GLU: inner) */
     int nb;            /* blocks of 32 along K */
     int ytype;
-    int tn, T;         /* tiles along N, tiles in all */
+    int tm, tn, T;     /* tiles along M and N, tiles in all */
+    int vec;           /* rows of y are 16-byte aligned */
 };
 
-__device__ __forceinline__ float mx_glu(float v, float g) { return v * silu_f(g); }
+/* the scale dword of blocks b .. b + 3 of a row; absent blocks read as byte 0. A row's scales start at any byte */
+__device__ __forceinline__ unsigned mx_scale4(const uint8_t *row, int b, int nb) {
+    unsigned w = 0;
+    if (b + 4 <= nb) {
+        __builtin_memcpy(&w, row + b, 4);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (b + i < nb) w |= (unsigned)row[b + i] << (8 * i);
+    }
+    return w;
+}
 
-/* One wave per 32 x 32 outputs (GLU: two accumulators). */
-template <bool GLU>
-__global__ __launch_bounds__(64) void k_mx4_tile(MxArgs a) {
-    const int t = blockIdx.x, lane = threadIdx.x, l32 = lane & 31, h = lane >> 5;
-    const int m0 = (t / a.tn) * 32, n0 = (t % a.tn) * 32;
-    const int m = min(m0 + l32, a.M - 1), n = min(n0 + l32, a.N - 1);
-    const uint4 *xr = (const uint4 *)a.xq + (size_t)m * a.nb;
-    const uint8_t *xsr = a.xs + (size_t)m * a.nb;
-    mx_f32x16_t acc[GLU ? 2 : 1];
+/* eight results of one row, from column n on */
+__device__ __forceinline__ void mx_store8(const MxArgs &a, int m, int n, const float (&v)[8]) {
+    const size_t at = (size_t)m * a.N + n;
+    if (a.vec && n + 8 <= a.N) {
+        if (a.ytype == MX_F32) {
+            float *y = (float *)a.y + at;
+            *reinterpret_cast<float4 *>(y) = make_float4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<float4 *>(y + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        } else if (a.ytype == MX_F16) {
+            typedef _Float16 v8_t __attribute__((ext_vector_type(8)));
+            v8_t o;
 #pragma unroll
-    for (int g = 0; g < (GLU ? 2 : 1); g++)
+            for (int i = 0; i < 8; i++) o[i] = (_Float16)v[i];
+            *reinterpret_cast<v8_t *>((_Float16 *)a.y + at) = o;
+        } else {
+            typedef __bf16 v8_t __attribute__((ext_vector_type(8)));
+            v8_t o;
 #pragma unroll
-        for (int r = 0; r < 16; r++) acc[g][r] = 0.0f;
-    for (int b = 0; b < a.nb; b += 2) {
-        const bool in = b + h < a.nb;          /* an absent block: codes zero, scale one */
-        const uint4 z = make_uint4(0, 0, 0, 0);
-        const uint4 xv = in ? xr[b + h] : z;
-        const int xsc = in ? xsr[b + h] : 127;
+            for (int i = 0; i < 8; i++) o[i] = (__bf16)v[i];
+            *reinterpret_cast<v8_t *>((__bf16 *)a.y + at) = o;
+        }
+    } else {
 #pragma unroll
-        for (int g = 0; g < (GLU ? 2 : 1); g++) {
-            const size_t wr = (size_t)(n + g * a.N) * a.nb + b + h;
-            const uint4 wv = in ? ((const uint4 *)a.wq)[wr] : z;
-            const int wsc = in ? a.ws[wr] : 127;
-            acc[g] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_op(wv), mx_op(xv), acc[g], 4, 4, 0, wsc, 0, xsc);
+        for (int i = 0; i < 8; i++)
+            if (n + i < a.N) mx_store(a.y, a.ytype, at + i, v[i]);
+    }
+}
+
+/* LDS DMA with a scalar base and a 32-bit lane offset */
+__device__ __forceinline__ void dma16_s(const void *base, unsigned off, uint32_t m0) {
+    const uint32_t m = __builtin_amdgcn_readfirstlane(m0);
+    const uint64_t u = (uint64_t)base;
+    const uint64_t b = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(u >> 32)) << 32) |
+                       (uint32_t)__builtin_amdgcn_readfirstlane((int)u);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(m), "v"(off), "s"(b) : "memory");
+}
+
+/*
+ * WK groups of WM x WN waves; a group's waves share LDS stages and take every WK-th part of K; a wave owns
+ * FM x FN blocks of 32 x 32 outputs (GLU: the first half of its FN are value rows, the second half
+ * the gate rows of the same columns). Chunks of 256 K (128 bytes of every row) move to LDS by DMA, two
+ * stages; chunk c of a row sits at c ^ ((row >> 1) & 7), so that fragment reads (32 rows x 16 bytes
+ * per lane half) are free of bank conflicts. Scales go straight to registers.
+ * One barrier a chunk (none where a group is one wave): it follows the wait for this wave's transfers and fragment reads, so
+ * behind it the chunk is whole and the other stage is free.
+ */
+template <int FM, int FN, int WM, int WN, int WK, bool GLU>
+__global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
+    constexpr int NW = WM * WN * WK, GW = WM * WN;
+    constexpr int BM = 32 * FM * WM, BN = 32 * FN * WN;          /* rows of x and of w per tile */
+    constexpr int OW = GLU ? 16 * FN : 32 * FN;                  /* columns of y per wave */
+    constexpr int NR = BM + BN, STAGE = NR * 128;
+    constexpr int ND = NR / 8 / GW;                              /* DMA instructions per wave and chunk */
+    static_assert(NR % (8 * GW) == 0 && (!GLU || FN % 2 == 0), "");
+    constexpr int ES = 32 * FN + 4;                              /* floats per staged row */
+    constexpr int EPI = NW * 32 * ES * 4;
+    __shared__ __attribute__((aligned(16))) uint8_t smem[2 * WK * STAGE > EPI ? 2 * WK * STAGE : EPI];
+    const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
+    const int wid = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int wk = wid / GW, gw = wid % GW, wm = gw / WN, wn = gw % WN;
+
+    /* tiles in bands of 4 tile rows, columns fastest after them: the tiles that run side by side on an XCD then
+     * share few panels of both operands */
+    const int t = xcd_tile(blockIdx.x, a.T);
+    if (t >= a.T) return;
+    const int band = t / (4 * a.tn), gm = min(4, a.tm - 4 * band), r = t - band * 4 * a.tn;
+    const int m0 = (4 * band + r % gm) * BM, n0 = (r / gm) * (OW * WN);
+
+    /* w rows of the LDS tile lie behind its x rows; GLU: wave by wave, value rows before gate rows. The column of
+     * w row i, counted from n0, and whether it is a gate row */
+    auto is_gate = [&](int i) __attribute__((always_inline)) { return GLU && i % (32 * FN) >= OW; };
+    auto w_col = [&](int i) __attribute__((always_inline)) {
+        const int c = GLU ? i / (32 * FN) * OW + i % OW : i;
+        return min(c, a.N - 1 - n0);
+    };
+    /* lane offsets of the DMA slots: slot lane of instruction i fills 16 bytes of LDS row 8 (GW i + gw) + lane / 8 */
+    unsigned off[ND];
+    const size_t rb = (size_t)a.nb * 16;
+    auto source = [&](int i, int c) __attribute__((always_inline)) -> unsigned {
+        const int row = 8 * (GW * i + gw) + (lane >> 3);
+        if (8 * (GW * i + gw) < BM) return (unsigned)((min(m0 + row, a.M - 1) - m0) * rb) + 16 * c;
+        return (unsigned)(w_col(row - BM) * rb) + 16 * c;
+    };
+#pragma unroll
+    for (int i = 0; i < ND; i++) {
+        const int row = 8 * (GW * i + gw) + (lane >> 3);
+        off[i] = source(i, (lane & 7) ^ ((row >> 1) & 7));
+    }
+    const uint8_t *xb = a.xq + (size_t)m0 * rb, *wb = a.wq + (size_t)n0 * rb, *gb = wb + (size_t)a.N * rb;
+    const int nc = (a.nb + 7) / 8, per = (nc + WK - 1) / WK;
+    const int c0 = min(wk * per, nc), c1 = min(c0 + per, nc);
+    const uint32_t sb = (uint32_t)(uintptr_t)smem + wk * 2 * STAGE;
+
+    const uint8_t *xsr[FM], *wsr[FN];
+#pragma unroll
+    for (int i = 0; i < FM; i++) xsr[i] = a.xs + (size_t)min(m0 + (wm * FM + i) * 32 + l32, a.M - 1) * a.nb;
+#pragma unroll
+    for (int j = 0; j < FN; j++) {
+        const int i = (wn * FN + j) * 32 + l32;
+        wsr[j] = a.ws + ((size_t)(n0 + w_col(i)) + (is_gate(i) ? a.N : 0)) * a.nb;
+    }
+    unsigned xs[2][FM], ws[2][FN];
+
+    auto issue = [&](int buf, int c) __attribute__((always_inline)) {
+        const size_t ck = (size_t)c * 128;
+        const int left = a.nb - 8 * c;
+#pragma unroll
+        for (int i = 0; i < ND; i++) {
+            const int row0 = 8 * (GW * i + gw);
+            unsigned o = off[i];
+            if (left < 8) {          /* the last chunk: slots of absent blocks take the chunk's first (their scales are 0) */
+                const int row = row0 + (lane >> 3), k = (lane & 7) ^ ((row >> 1) & 7);
+                if (k >= left) o -= 16 * k;
+            }
+            dma16_s((row0 < BM ? xb : is_gate(row0 - BM) ? gb : wb) + ck, o, sb + buf * STAGE + row0 * 128);
+        }
+    };
+    auto scales = [&](unsigned (&x)[FM], unsigned (&w)[FN], int c) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < FM; i++) x[i] = mx_scale4(xsr[i], 8 * c + 4 * h, a.nb);
+#pragma unroll
+        for (int j = 0; j < FN; j++) w[j] = mx_scale4(wsr[j], 8 * c + 4 * h, a.nb);
+    };
+
+    mx_f32x16_t acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; i++)
+#pragma unroll
+        for (int j = 0; j < FN; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[i][j][e] = 0.0f;
+
+    auto compute = [&](int buf, const unsigned (&x)[FM], const unsigned (&w)[FN]) __attribute__((always_inline)) {
+        const uint8_t *S = smem + wk * 2 * STAGE + buf * STAGE;
+        auto frag = [&](int row, int k) __attribute__((always_inline)) {
+            return *reinterpret_cast<const uint4 *>(S + row * 128 + ((k ^ ((row >> 1) & 7)) << 4));
+        };
+#define MX_STEP(J)                                                                                            \
+        {                                                                                                     \
+            uint4 xf[FM], wf[FN];                                                                             \
+            _Pragma("unroll") for (int i = 0; i < FM; i++) xf[i] = frag((wm * FM + i) * 32 + l32, 4 * h + J); \
+            _Pragma("unroll") for (int j = 0; j < FN; j++) wf[j] = frag(BM + (wn * FN + j) * 32 + l32, 4 * h + J); \
+            _Pragma("unroll") for (int i = 0; i < FM; i++)                                                    \
+                _Pragma("unroll") for (int j = 0; j < FN; j++)                                                \
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_op(wf[j]), mx_op(xf[i]), acc[i][j], 4, 4, \
+                                                                               J, (int)w[j], J, (int)x[i]);   \
+        }
+        MX_STEP(0) MX_STEP(1) MX_STEP(2) MX_STEP(3)
+#undef MX_STEP
+    };
+    /* this wave's transfers have landed and its fragment reads have returned; then the group's */
+    auto turn = [&]() __attribute__((always_inline)) {
+        if constexpr (GW == 1) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    };
+
+    /* every group takes the same number of turns (the barrier is the workgroup's) */
+    const int turns = GW == 1 ? c1 - c0 : per;
+    if (c0 < c1) { issue(0, c0); scales(xs[0], ws[0], c0); }
+    for (int i = 0; i < turns; i += 2) {
+        turn();
+        if (c0 + i + 1 < c1) { issue(1, c0 + i + 1); scales(xs[1], ws[1], c0 + i + 1); }
+        if (c0 + i < c1) compute(0, xs[0], ws[0]);
+        if (i + 1 >= turns) break;
+        turn();
+        if (c0 + i + 2 < c1) { issue(0, c0 + i + 2); scales(xs[0], ws[0], c0 + i + 2); }
+        if (c0 + i + 1 < c1) compute(1, xs[1], ws[1]);
+    }
+
+    /* epilogue, 32 rows of every wave at a time: staged in LDS, the groups' parts added in order, whole row
+     * segments stored */
+    float *E = (float *)smem + wid * 32 * ES;
+    constexpr int LPR = OW / 8;                                  /* lanes per row, 8 columns each */
+    constexpr int RPI = 64 / LPR;                                /* rows per wave at once */
+#pragma unroll
+    for (int i = 0; i < FM; i++) {
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < FN; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                *reinterpret_cast<float4 *>(E + l32 * ES + 32 * j + 8 * e + 4 * h) =
+                    make_float4(acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]);
+        __syncthreads();
+        const int n = n0 + wn * OW + 8 * (lane % LPR);
+        float b[8], bg[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            b[e] = a.bias && n + e < a.N ? a.bias[n + e] : 0.0f;
+            if constexpr (GLU) bg[e] = a.bias && n + e < a.N ? a.bias[a.N + n + e] : 0.0f;
+        }
+        for (int q = wk * RPI + lane / LPR; q < 32; q += WK * RPI) {
+            const int m = m0 + (wm * FM + i) * 32 + q;
+            float v[8], g[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) { v[e] = 0.0f; g[e] = 0.0f; }
+#pragma unroll
+            for (int k = 0; k < WK; k++) {
+                const float *p = (const float *)smem + (k * GW + gw) * 32 * ES + q * ES + 8 * (lane % LPR);
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    v[e] += p[e];
+                    if constexpr (GLU) g[e] += p[OW + e];
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                v[e] += b[e];
+                if constexpr (GLU) v[e] *= silu_f(g[e] + bg[e]);
+            }
+            if (m < a.M && n < a.N) mx_store8(a, m, n, v);
         }
     }
-    if (m0 + l32 >= a.M) return;
+}
+
+/*
+ * Up to 16 rows: quantised by the wave that multiplies them, in the same launch. A workgroup owns 16
+ * weight rows (GLU: 16 value and 16 gate rows), its NW waves take K in turn, and the 16 x 16 sums meet in LDS.
+ * v_mfma_scale_f32_16x16x128: lane l holds block l / 16 of four, of row l % 16, so a lane reads 32
+ * activations, finds their maximum and packs its own operand: no lane exchange. Every workgroup
+ * quantises all of x, which is little beside the latency of a second launch.
+ */
+template <int XT, bool GLU, int NW>
+__global__ __launch_bounds__(64 * NW) void k_mx4_rows(MxArgs a, const void *x, long ldx, int K, int xvec) {
+    constexpr int F = GLU ? 2 : 1;
+    __shared__ __attribute__((aligned(16))) float E[NW][F][16][20];
+    const int lane = threadIdx.x & 63, l16 = lane & 15, kg = lane >> 4;
+    const int wid = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int n0 = blockIdx.x * 16, n = min(n0 + l16, a.N - 1), steps = (a.nb + 3) / 4;
+    mx_f32x4_t acc[F];
 #pragma unroll
-    for (int r = 0; r < 16; r++) {
-        const int c = n0 + 8 * (r >> 2) + 4 * h + (r & 3);
-        if (c >= a.N) continue;
-        float v = acc[0][r];
-        if (a.bias) v += a.bias[c];
+    for (int f = 0; f < F; f++) acc[f] = mx_f32x4_t{0, 0, 0, 0};
+    const bool row = l16 < a.M;
+    for (int s = wid; s < steps; s += NW) {
+        const int b = 4 * s + kg;
+        const bool in = b < a.nb;
+        uint4 w[F];
+        int sc[F];
+#pragma unroll
+        for (int f = 0; f < F; f++) {
+            const size_t at = (size_t)(n + f * a.N) * a.nb + b;
+            w[f] = in ? ((const uint4 *)a.wq)[at] : make_uint4(0, 0, 0, 0);
+            sc[f] = in ? a.ws[at] : 127;
+        }
+        uint4 u = make_uint4(0, 0, 0, 0);
+        unsigned byte = 127;
+        if (in && row) {
+            float v[4][8];
+            unsigned m = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) mx_load8<XT>(x, (size_t)l16 * ldx + 32 * b + 8 * i, K - 32 * b - 8 * i, xvec, v[i]);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) m = max(m, mx_abs_bits(v[i][e]));
+            byte = mx_scale_byte(m);
+            u = make_uint4(mx_pack8(v[0], byte), mx_pack8(v[1], byte), mx_pack8(v[2], byte), mx_pack8(v[3], byte));
+        }
+#pragma unroll
+        for (int f = 0; f < F; f++)
+            acc[f] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_op(w[f]), mx_op(u), acc[f], 4, 4, 0, sc[f], 0, (int)byte);
+    }
+#pragma unroll
+    for (int f = 0; f < F; f++)
+        *reinterpret_cast<mx_f32x4_t *>(&E[wid][f][l16][4 * kg]) = acc[f];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 256; i += 64 * NW) {
+        const int m = i >> 4, c = i & 15;
+        if (m >= a.M || n0 + c >= a.N) continue;
+        float v = 0.0f, g = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            v += E[w][0][m][c];
+            if constexpr (GLU) g += E[w][F - 1][m][c];
+        }
+        if (a.bias) v += a.bias[n0 + c];
         if constexpr (GLU) {
-            float g = acc[1][r];
-            if (a.bias) g += a.bias[a.N + c];
-            v = mx_glu(v, g);
+            if (a.bias) g += a.bias[a.N + n0 + c];
+            v *= silu_f(g);
         }
-        mx_store(a.y, a.ytype, (size_t)(m0 + l32) * a.N + c, v);
+        mx_store(a.y, a.ytype, (size_t)m * a.N + n0 + c, v);
     }
+}
+
+template <int FM, int FN, int WM, int WN, int WK, bool GLU>
+static hipError_t launch(MxArgs a, hipStream_t s) {
+    constexpr int OW = (GLU ? 16 : 32) * FN * WN;
+    a.tm = (a.M + 32 * FM * WM - 1) / (32 * FM * WM);
+    a.tn = (a.N + OW - 1) / OW;
+    a.T = a.tm * a.tn;
+    hipLaunchKernelGGL((k_mx4_gemm<FM, FN, WM, WN, WK, GLU>), dim3((unsigned)((a.T + 7) / 8 * 8)), dim3(64 * WM * WN * WK), 0, s, a);
+    return hipGetLastError();
+}
+
+template <bool GLU>
+static hipError_t pick(const MxArgs &a, hipStream_t s) {
+    const long cols = GLU ? 2L * a.N : a.N;
+    auto tiles = [&](int bm, int bn) { return (long)((a.M + bm - 1) / bm) * ((cols + bn - 1) / bn); };
+    if (tiles(256, 256) >= 200) return launch<4, 2, 2, 4, 1, GLU>(a, s);
+    if (tiles(128, 128) >= 200) return launch<2, 2, 2, 2, 1, GLU>(a, s);
+    if constexpr (GLU) return launch<2, 2, 1, 1, 4, GLU>(a, s);
+    if (tiles(64, 64) >= 200) return launch<2, 2, 1, 1, 4, GLU>(a, s);
+    return launch<1, 1, 1, 1, 8, GLU && false>(a, s);
 }
 
 extern "C" hipError_t aria_k_mx4_gemm(void *y, int ytype, const uint8_t *xq, const uint8_t *xs, const uint8_t *wq,
                                       const uint8_t *ws, const float *bias, int M, int K, int N, int glu, hipStream_t s) {
     if (M <= 0 || N <= 0) return hipSuccess;
-    MxArgs a = {y, xq, xs, wq, ws, bias, M, N, (K + 31) / 32, ytype, 0, 0};
-    a.tn = (N + 31) / 32;
-    a.T = a.tn * ((M + 31) / 32);
-    if (glu) hipLaunchKernelGGL(k_mx4_tile<true>, dim3(a.T), dim3(64), 0, s, a);
-    else hipLaunchKernelGGL(k_mx4_tile<false>, dim3(a.T), dim3(64), 0, s, a);
+    MxArgs a = {y, xq, xs, wq, ws, bias, M, N, (K + 31) / 32, ytype, 0, 0, 0, 0};
+    a.vec = N % 8 == 0 && ((uintptr_t)y & 15u) == 0;
+    return glu ? pick<true>(a, s) : pick<false>(a, s);
+}
+
+template <int XT, bool GLU>
+static void launch_rows(const MxArgs &a, const void *x, long ldx, int K, hipStream_t s) {
+    const int xvec = ldx % 8 == 0 && ((uintptr_t)x & 15u) == 0;
+    const dim3 grid((unsigned)((a.N + 15) / 16));
+    if (a.nb > 64) hipLaunchKernelGGL((k_mx4_rows<XT, GLU, 8>), grid, dim3(512), 0, s, a, x, ldx, K, xvec);
+    else hipLaunchKernelGGL((k_mx4_rows<XT, GLU, 4>), grid, dim3(256), 0, s, a, x, ldx, K, xvec);
+}
+
+extern "C" hipError_t aria_k_mx4_rows(void *y, int ytype, const void *x, int xtype, long ldx, const uint8_t *wq,
+                                      const uint8_t *ws, const float *bias, int M, int K, int N, int glu, hipStream_t s) {
+    if (M <= 0 || N <= 0) return hipSuccess;
+    const MxArgs a = {y, nullptr, nullptr, wq, ws, bias, M, N, (K + 31) / 32, ytype, 0, 0, 0, 0};
+    if (glu) {
+        if (xtype == MX_F32) launch_rows<MX_F32, true>(a, x, ldx, K, s);
+        else if (xtype == MX_F16) launch_rows<MX_F16, true>(a, x, ldx, K, s);
+        else launch_rows<MX_BF16, true>(a, x, ldx, K, s);
+    } else {
+        if (xtype == MX_F32) launch_rows<MX_F32, false>(a, x, ldx, K, s);
+        else if (xtype == MX_F16) launch_rows<MX_F16, false>(a, x, ldx, K, s);
+        else launch_rows<MX_BF16, false>(a, x, ldx, K, s);
+    }
     return hipGetLastError();
 }
