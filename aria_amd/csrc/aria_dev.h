@@ -13,6 +13,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #define ARIA_WAVE 64
 
 /* ---- wave64 reductions over groups of G lanes (G = 4, 8, 16, 32 or 64) ----
@@ -204,6 +206,17 @@ __device__ __forceinline__ void wait_vm() {
 __device__ __forceinline__ void dma16(const void *g, uint32_t m0) {
     const uint32_t m = __builtin_amdgcn_readfirstlane(m0);
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(m), "v"(g) : "memory");
+}
+
+template <int I>
+using IC = std::integral_constant<int, I>;
+/* f(IC<0>{}), ..., f(IC<N-1>{}) */
+template <int N, int I = 0, class Fn>
+__device__ __forceinline__ void static_for(Fn &&f) {
+    if constexpr (I < N) {
+        f(IC<I>{});
+        static_for<N, I + 1>(f);
+    }
 }
 
 #endif /* ARIA_DEV_H */

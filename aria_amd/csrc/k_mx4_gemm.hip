@@ -23,16 +23,18 @@ struct MxArgs {
     int vec;           /* rows of y are 16-byte aligned */
 };
 
-/* the scale dword of blocks b .. b + 3 of a row; absent blocks read as byte 0. A row's scales start at any byte */
-__device__ __forceinline__ unsigned mx_scale4(const uint8_t *row, int b, int nb) {
+/* the scale dword of blocks b .. b + 3 of a row, all of them there: a row's scales start at any byte */
+__device__ __forceinline__ unsigned mx_scale4(const uint8_t *row, int b) {
+    unsigned w;
+    __builtin_memcpy(&w, row + b, 4);
+    return w;
+}
+/* the same where the row may end: absent blocks read as byte 0 */
+__device__ __forceinline__ unsigned mx_scale4_end(const uint8_t *row, int b, int nb) {
     unsigned w = 0;
-    if (b + 4 <= nb) {
-        __builtin_memcpy(&w, row + b, 4);
-    } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (b + i < nb) w |= (unsigned)row[b + i] << (8 * i);
-    }
+    for (int i = 0; i < 4; i++)
+        if (b + i < nb) w |= (unsigned)row[b + i] << (8 * i);
     return w;
 }
 
@@ -89,7 +91,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
     constexpr int OW = GLU ? 16 * FN : 32 * FN;                  /* columns of y per wave */
     constexpr int NR = BM + BN, STAGE = NR * 128;
     constexpr int ND = NR / 8 / GW;                              /* DMA instructions per wave and chunk */
-    static_assert(NR % (8 * GW) == 0 && (!GLU || FN % 2 == 0), "");
+    constexpr int NDX = BM / 8 / GW;                             /* the first of them move x */
+    static_assert(BM % (8 * GW) == 0 && BN % (8 * GW) == 0 && (!GLU || FN % 2 == 0), "");
     constexpr int ES = 32 * FN + 4;                              /* floats per staged row */
     constexpr int EPI = NW * 32 * ES * 4;
     __shared__ __attribute__((aligned(16))) uint8_t smem[2 * WK * STAGE > EPI ? 2 * WK * STAGE : EPI];
@@ -116,7 +119,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
     const size_t rb = (size_t)a.nb * 16;
     auto source = [&](int i, int c) __attribute__((always_inline)) -> unsigned {
         const int row = 8 * (GW * i + gw) + (lane >> 3);
-        if (8 * (GW * i + gw) < BM) return (unsigned)((min(m0 + row, a.M - 1) - m0) * rb) + 16 * c;
+        if (i < NDX) return (unsigned)((min(m0 + row, a.M - 1) - m0) * rb) + 16 * c;
         return (unsigned)(w_col(row - BM) * rb) + 16 * c;
     };
 #pragma unroll
@@ -124,9 +127,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
         const int row = 8 * (GW * i + gw) + (lane >> 3);
         off[i] = source(i, (lane & 7) ^ ((row >> 1) & 7));
     }
-    const uint8_t *xb = a.xq + (size_t)m0 * rb, *wb = a.wq + (size_t)n0 * rb, *gb = wb + (size_t)a.N * rb;
-    const int nc = (a.nb + 7) / 8, per = (nc + WK - 1) / WK;
-    const int c0 = min(wk * per, nc), c1 = min(c0 + per, nc);
+    const uint8_t *xb = a.xq + (size_t)m0 * rb, *wb = a.wq + (size_t)n0 * rb;
+    const size_t gate = (size_t)a.N * rb;                        /* from a value row to its gate row */
     const uint32_t sb = (uint32_t)(uintptr_t)smem + wk * 2 * STAGE;
 
     const uint8_t *xsr[FM], *wsr[FN];
@@ -137,54 +139,66 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
         const int i = (wn * FN + j) * 32 + l32;
         wsr[j] = a.ws + ((size_t)(n0 + w_col(i)) + (is_gate(i) ? a.N : 0)) * a.nb;
     }
-    unsigned xs[2][FM], ws[2][FN];
 
-    auto issue = [&](int buf, int c) __attribute__((always_inline)) {
-        const size_t ck = (size_t)c * 128;
-        const int left = a.nb - 8 * c;
-#pragma unroll
-        for (int i = 0; i < ND; i++) {
+    /* chunk c to stage buf. In the row's last, short chunk the slots of absent blocks take the chunk's first
+     * block instead: their scales are 0, and 2^-127 times 2^-127 leaves nothing of any code */
+    auto issue = [&](int buf, int c, bool whole) __attribute__((always_inline)) {
+        static_for<ND>([&](auto I) __attribute__((always_inline)) {
+            constexpr int i = decltype(I)::value;
             const int row0 = 8 * (GW * i + gw);
             unsigned o = off[i];
-            if (left < 8) {          /* the last chunk: slots of absent blocks take the chunk's first (their scales are 0) */
+            if (!whole) {
                 const int row = row0 + (lane >> 3), k = (lane & 7) ^ ((row >> 1) & 7);
-                if (k >= left) o -= 16 * k;
+                if (k >= a.nb - 8 * c) o -= 16 * k;
             }
-            dma16_s((row0 < BM ? xb : is_gate(row0 - BM) ? gb : wb) + ck, o, sb + buf * STAGE + row0 * 128);
-        }
+            const size_t at = (size_t)c * 128;
+            const uint8_t *p;
+            if constexpr (i < NDX) p = xb + at;
+            else p = wb + at + (is_gate(row0 - BM) ? gate : (size_t)0);
+            dma16_s(p, o, sb + buf * STAGE + row0 * 128);
+        });
     };
     auto scales = [&](unsigned (&x)[FM], unsigned (&w)[FN], int c) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < FM; i++) x[i] = mx_scale4(xsr[i], 8 * c + 4 * h, a.nb);
-#pragma unroll
-        for (int j = 0; j < FN; j++) w[j] = mx_scale4(wsr[j], 8 * c + 4 * h, a.nb);
+        static_for<FM>([&](auto I) __attribute__((always_inline)) { x[I] = mx_scale4(xsr[I], 8 * c + 4 * h); });
+        static_for<FN>([&](auto J) __attribute__((always_inline)) { w[J] = mx_scale4(wsr[J], 8 * c + 4 * h); });
     };
 
     mx_f32x16_t acc[FM][FN];
-#pragma unroll
-    for (int i = 0; i < FM; i++)
-#pragma unroll
-        for (int j = 0; j < FN; j++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) acc[i][j][e] = 0.0f;
+    static_for<FM * FN>([&](auto I) __attribute__((always_inline)) {
+        acc[I / FN][I % FN] = mx_f32x16_t{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+    });
 
+    /* four MFMA steps; the fragments of step J + 1 are read while step J multiplies. Each step is a scheduling
+     * region in which the reads are spread over the MFMAs */
     auto compute = [&](int buf, const unsigned (&x)[FM], const unsigned (&w)[FN]) __attribute__((always_inline)) {
         const uint8_t *S = smem + wk * 2 * STAGE + buf * STAGE;
+        uint4 xf[2][FM], wf[2][FN];
         auto frag = [&](int row, int k) __attribute__((always_inline)) {
             return *reinterpret_cast<const uint4 *>(S + row * 128 + ((k ^ ((row >> 1) & 7)) << 4));
         };
-#define MX_STEP(J)                                                                                            \
-        {                                                                                                     \
-            uint4 xf[FM], wf[FN];                                                                             \
-            _Pragma("unroll") for (int i = 0; i < FM; i++) xf[i] = frag((wm * FM + i) * 32 + l32, 4 * h + J); \
-            _Pragma("unroll") for (int j = 0; j < FN; j++) wf[j] = frag(BM + (wn * FN + j) * 32 + l32, 4 * h + J); \
-            _Pragma("unroll") for (int i = 0; i < FM; i++)                                                    \
-                _Pragma("unroll") for (int j = 0; j < FN; j++)                                                \
-                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_op(wf[j]), mx_op(xf[i]), acc[i][j], 4, 4, \
-                                                                               J, (int)w[j], J, (int)x[i]);   \
-        }
-        MX_STEP(0) MX_STEP(1) MX_STEP(2) MX_STEP(3)
-#undef MX_STEP
+        auto read = [&](auto J) __attribute__((always_inline)) {
+            constexpr int j = decltype(J)::value, p = j & 1;
+            static_for<FM>([&](auto I) __attribute__((always_inline)) { xf[p][I] = frag((wm * FM + I) * 32 + l32, 4 * h + j); });
+            static_for<FN>([&](auto I) __attribute__((always_inline)) { wf[p][I] = frag(BM + (wn * FN + I) * 32 + l32, 4 * h + j); });
+        };
+        read(IC<0>{});
+        __builtin_amdgcn_sched_barrier(0);
+        static_for<4>([&](auto J) __attribute__((always_inline)) {
+            constexpr int j = decltype(J)::value, p = j & 1;
+            if constexpr (j < 3) read(IC<j + 1>{});
+            static_for<FM * FN>([&](auto I) __attribute__((always_inline)) {
+                constexpr int m = decltype(I)::value / FN, n = decltype(I)::value % FN;
+                acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_op(wf[p][n]), mx_op(xf[p][m]), acc[m][n], 4, 4,
+                                                                           j, (int)w[n], j, (int)x[m]);
+            });
+            static_for<FM * FN>([&](auto I) __attribute__((always_inline)) {
+                constexpr int i = decltype(I)::value, nr = FM + FN, nm = FM * FN;
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                constexpr int d = nr * (i + 1) / nm - nr * i / nm;
+                if constexpr (j < 3 && d > 0) __builtin_amdgcn_sched_group_barrier(0x100, d, 0);
+            });
+            __builtin_amdgcn_sched_barrier(0);
+        });
     };
     /* this wave's transfers have landed and its fragment reads have returned; then the group's */
     auto turn = [&]() __attribute__((always_inline)) {
@@ -192,17 +206,40 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     };
 
-    /* every group takes the same number of turns (the barrier is the workgroup's) */
-    const int turns = GW == 1 ? c1 - c0 : per;
-    if (c0 < c1) { issue(0, c0); scales(xs[0], ws[0], c0); }
-    for (int i = 0; i < turns; i += 2) {
+    /* the scale loads are behind the wait of turn(): this use tells the compiler so, which else would wait for
+     * them, and with them for every later transfer, at the first MFMA */
+    auto arrived = [&](unsigned (&x)[FM], unsigned (&w)[FN]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < FM; i++) asm volatile("" : "+v"(x[i]));
+#pragma unroll
+        for (int j = 0; j < FN; j++) asm volatile("" : "+v"(w[j]));
+    };
+
+    /* the whole chunks of this group, then, by the last group, a short one. Groups of several waves come alone
+     * (WK = 1), so every wave takes the same number of turns */
+    static_assert(GW == 1 || WK == 1, "");
+    const int nc = a.nb / 8, per = (nc + WK - 1) / WK;
+    const int c0 = min(wk * per, nc), c1 = min(c0 + per, nc);
+    unsigned xsA[FM], wsA[FN], xsB[FM], wsB[FN];
+    if (c0 < c1) { issue(0, c0, true); scales(xsA, wsA, c0); }
+    for (int c = c0; c < c1; c += 2) {
         turn();
-        if (c0 + i + 1 < c1) { issue(1, c0 + i + 1); scales(xs[1], ws[1], c0 + i + 1); }
-        if (c0 + i < c1) compute(0, xs[0], ws[0]);
-        if (i + 1 >= turns) break;
+        arrived(xsA, wsA);
+        if (c + 1 < c1) { issue(1, c + 1, true); scales(xsB, wsB, c + 1); }
+        compute(0, xsA, wsA);
+        if (c + 1 >= c1) break;
         turn();
-        if (c0 + i + 2 < c1) { issue(0, c0 + i + 2); scales(xs[0], ws[0], c0 + i + 2); }
-        if (c0 + i + 1 < c1) compute(1, xs[1], ws[1]);
+        arrived(xsB, wsB);
+        if (c + 2 < c1) { issue(0, c + 2, true); scales(xsA, wsA, c + 2); }
+        compute(1, xsB, wsB);
+    }
+    if ((a.nb & 7) && wk == WK - 1) {
+        turn();
+        issue(0, nc, false);
+        static_for<FM>([&](auto I) __attribute__((always_inline)) { xsA[I] = mx_scale4_end(xsr[I], 8 * nc + 4 * h, a.nb); });
+        static_for<FN>([&](auto J) __attribute__((always_inline)) { wsA[J] = mx_scale4_end(wsr[J], 8 * nc + 4 * h, a.nb); });
+        turn();
+        compute(0, xsA, wsA);
     }
 
     /* epilogue, 32 rows of every wave at a time: staged in LDS, the groups' parts added in order, whole row
@@ -210,35 +247,38 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
     float *E = (float *)smem + wid * 32 * ES;
     constexpr int LPR = OW / 8;                                  /* lanes per row, 8 columns each */
     constexpr int RPI = 64 / LPR;                                /* rows per wave at once */
+    const int c8 = 8 * (lane % LPR), n = n0 + wn * OW + c8;
+    float b[8], bg[8];
 #pragma unroll
-    for (int i = 0; i < FM; i++) {
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < FN; j++)
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                *reinterpret_cast<float4 *>(E + l32 * ES + 32 * j + 8 * e + 4 * h) =
-                    make_float4(acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]);
-        __syncthreads();
-        const int n = n0 + wn * OW + 8 * (lane % LPR);
-        float b[8], bg[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            b[e] = a.bias && n + e < a.N ? a.bias[n + e] : 0.0f;
-            if constexpr (GLU) bg[e] = a.bias && n + e < a.N ? a.bias[a.N + n + e] : 0.0f;
-        }
+    for (int e = 0; e < 8; e++) {
+        b[e] = a.bias && n + e < a.N ? a.bias[n + e] : 0.0f;
+        bg[e] = GLU && a.bias && n + e < a.N ? a.bias[a.N + n + e] : 0.0f;
+    }
+    __syncthreads();                                             /* stages still being read */
+    static_for<FM>([&](auto I) __attribute__((always_inline)) {
+        constexpr int i = decltype(I)::value;
+        if constexpr (i > 0 && WK > 1) __syncthreads();          /* parts still being read */
+        static_for<4 * FN>([&](auto JE) __attribute__((always_inline)) {
+            constexpr int j = decltype(JE)::value / 4, e = decltype(JE)::value % 4;
+            *reinterpret_cast<float4 *>(E + l32 * ES + 32 * j + 8 * e + 4 * h) =
+                make_float4(acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]);
+        });
+        if constexpr (WK > 1) __syncthreads();
         for (int q = wk * RPI + lane / LPR; q < 32; q += WK * RPI) {
             const int m = m0 + (wm * FM + i) * 32 + q;
             float v[8], g[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) { v[e] = 0.0f; g[e] = 0.0f; }
-#pragma unroll
             for (int k = 0; k < WK; k++) {
-                const float *p = (const float *)smem + (k * GW + gw) * 32 * ES + q * ES + 8 * (lane % LPR);
+                const float4 *p = (const float4 *)((const float *)smem + (k * GW + gw) * 32 * ES + q * ES + c8);
+                const float4 v0 = p[0], v1 = p[1];
+                const float w[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    v[e] += p[e];
-                    if constexpr (GLU) g[e] += p[OW + e];
+                for (int e = 0; e < 8; e++) v[e] = k ? v[e] + w[e] : w[e];
+                if constexpr (GLU) {
+                    const float4 g0 = p[OW / 4], g1 = p[OW / 4 + 1];
+                    const float u[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
+#pragma unroll
+                    for (int e = 0; e < 8; e++) g[e] = k ? g[e] + u[e] : u[e];
                 }
             }
 #pragma unroll
@@ -248,7 +288,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
             }
             if (m < a.M && n < a.N) mx_store8(a, m, n, v);
         }
-    }
+    });
 }
 
 /*

@@ -13,17 +13,6 @@
 #include <cstring>
 #include <type_traits>
 
-template <int I>
-using IC = std::integral_constant<int, I>;
-/* f(IC<0>{}), ..., f(IC<N-1>{}) */
-template <int N, int I = 0, class Fn>
-__device__ __forceinline__ void static_for(Fn &&f) {
-    if constexpr (I < N) {
-        f(IC<I>{});
-        static_for<N, I + 1>(f);
-    }
-}
-
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef float float2_t __attribute__((ext_vector_type(2)));
