@@ -23,19 +23,13 @@ struct MxArgs {
     int vec;           /* rows of y are 16-byte aligned */
 };
 
-/* the scale dword of blocks b .. b + 3 of a row, all of them there: a row's scales start at any byte */
-__device__ __forceinline__ unsigned mx_scale4(const uint8_t *row, int b) {
-    unsigned w;
-    __builtin_memcpy(&w, row + b, 4);
-    return w;
-}
-/* the same where the row may end: absent blocks read as byte 0 */
-__device__ __forceinline__ unsigned mx_scale4_end(const uint8_t *row, int b, int nb) {
-    unsigned w = 0;
+/* the scale bytes of a row's last blocks, b to b + 15; absent ones read as 0 */
+__device__ __forceinline__ uint4 mx_scale_end(const uint8_t *row, int b, int nb) {
+    unsigned w[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-        if (b + i < nb) w |= (unsigned)row[b + i] << (8 * i);
-    return w;
+    for (int i = 0; i < 16; i++)
+        if (b + i < nb) w[i >> 2] |= (unsigned)row[b + i] << (8 * (i & 3));
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 /* eight results of one row, from column n on */
@@ -66,13 +60,24 @@ __device__ __forceinline__ void mx_store8(const MxArgs &a, int m, int n, const f
     }
 }
 
+/* v, as a value that the compiler knows nothing of: what is computed from it is not kept in registers from further up */
+__device__ __forceinline__ int fresh(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+/* the same for a value that is one for the wave, which stays in a scalar register */
+__device__ __forceinline__ uint32_t fresh_s(uint32_t v) {
+    v = __builtin_amdgcn_readfirstlane(v);
+    asm volatile("" : "+s"(v));
+    return v;
+}
 /* LDS DMA with a scalar base and a 32-bit lane offset */
 __device__ __forceinline__ void dma16_s(const void *base, unsigned off, uint32_t m0) {
-    const uint32_t m = __builtin_amdgcn_readfirstlane(m0);
     const uint64_t u = (uint64_t)base;
     const uint64_t b = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(u >> 32)) << 32) |
                        (uint32_t)__builtin_amdgcn_readfirstlane((int)u);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(m), "v"(off), "s"(b) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(m0), "v"(off), "s"(b) : "memory");
 }
 
 /*
@@ -95,7 +100,12 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
     static_assert(BM % (8 * GW) == 0 && BN % (8 * GW) == 0 && (!GLU || FN % 2 == 0), "");
     constexpr int ES = 32 * FN + 4;                              /* floats per staged row */
     constexpr int EPI = NW * 32 * ES * 4;
-    __shared__ __attribute__((aligned(16))) uint8_t smem[2 * WK * STAGE > EPI ? 2 * WK * STAGE : EPI];
+    constexpr bool SHARED = GW > 1;                              /* scales go through LDS */
+    constexpr int SCALES = SHARED ? NR * 16 : 0;                 /* scale bytes of two chunks */
+    constexpr int NS = NR / (64 * GW);                           /* scale rows per lane */
+    static_assert(NR % (64 * GW) == 0 && (!SHARED || WK == 1), "");
+    constexpr int GROUP = 2 * STAGE + 2 * SCALES;                /* LDS of one K group */
+    __shared__ __attribute__((aligned(16))) uint8_t smem[WK * GROUP > EPI ? WK * GROUP : EPI];
     const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
     const int wid = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int wk = wid / GW, gw = wid % GW, wm = gw / WN, wn = gw % WN;
@@ -129,38 +139,62 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
     }
     const uint8_t *xb = a.xq + (size_t)m0 * rb, *wb = a.wq + (size_t)n0 * rb;
     const size_t gate = (size_t)a.N * rb;                        /* from a value row to its gate row */
-    const uint32_t sb = (uint32_t)(uintptr_t)smem + wk * 2 * STAGE;
+    const uint32_t sb = (uint32_t)(uintptr_t)smem + wk * GROUP;
 
+    /* SHARED: scales of two chunks at a time: 16 bytes of a row per lane (a load of one dword per fragment row and lane half would keep the
+     * address unit busy for longer than the multiplications take), through registers to LDS */
+    const uint8_t *srow[NS];
+#pragma unroll
+    for (int i = 0; i < NS; i++) {
+        const int row = 64 * (GW * i + gw) + lane;
+        srow[i] = row < BM ? a.xs + (size_t)min(m0 + row, a.M - 1) * a.nb
+                           : a.ws + ((size_t)(n0 + w_col(row - BM)) + (is_gate(row - BM) ? a.N : 0)) * a.nb;
+    }
+    uint4 sreg[NS];
+    auto load_scales = [&](int c) __attribute__((always_inline)) {   /* a row's scales start at any byte */
+#pragma unroll
+        for (int i = 0; i < NS; i++) __builtin_memcpy(&sreg[i], srow[i] + 8 * c, 16);
+    };
+    auto put_scales = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NS; i++)
+            *reinterpret_cast<uint4 *>(smem + wk * GROUP + 2 * STAGE + buf * SCALES + (64 * (GW * i + gw) + lane) * 16) = sreg[i];
+    };
+
+    /* a one-wave group takes its few scales straight to registers, a dword per fragment row and lane half */
     const uint8_t *xsr[FM], *wsr[FN];
 #pragma unroll
-    for (int i = 0; i < FM; i++) xsr[i] = a.xs + (size_t)min(m0 + (wm * FM + i) * 32 + l32, a.M - 1) * a.nb;
+    for (int i = 0; i < FM; i++) xsr[i] = a.xs + (size_t)min(m0 + (wm * FM + i) * 32 + l32, a.M - 1) * a.nb + 4 * h;
 #pragma unroll
     for (int j = 0; j < FN; j++) {
         const int i = (wn * FN + j) * 32 + l32;
-        wsr[j] = a.ws + ((size_t)(n0 + w_col(i)) + (is_gate(i) ? a.N : 0)) * a.nb;
+        wsr[j] = a.ws + ((size_t)(n0 + w_col(i)) + (is_gate(i) ? a.N : 0)) * a.nb + 4 * h;
     }
+    auto scales = [&](unsigned (&x)[FM], unsigned (&w)[FN], int c) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < FM; i++) __builtin_memcpy(&x[i], xsr[i] + 8 * c, 4);
+#pragma unroll
+        for (int j = 0; j < FN; j++) __builtin_memcpy(&w[j], wsr[j] + 8 * c, 4);
+    };
 
-    /* chunk c to stage buf. In the row's last, short chunk the slots of absent blocks take the chunk's first
+    /* chunk c to stage buf. In a row's last, short chunk (END) the slots of absent blocks take the chunk's first
      * block instead: their scales are 0, and 2^-127 times 2^-127 leaves nothing of any code */
-    auto issue = [&](int buf, int c, bool whole) __attribute__((always_inline)) {
+    const uint32_t mb = fresh_s(sb + gw * 1024);
+    auto issue = [&](auto END, int buf, int c) __attribute__((always_inline)) {
         static_for<ND>([&](auto I) __attribute__((always_inline)) {
             constexpr int i = decltype(I)::value;
             const int row0 = 8 * (GW * i + gw);
             unsigned o = off[i];
-            if (!whole) {
-                const int row = row0 + (lane >> 3), k = (lane & 7) ^ ((row >> 1) & 7);
+            if constexpr (decltype(END)::value != 0) {
+                const int ln = fresh(lane), row = row0 + (ln >> 3), k = (ln & 7) ^ ((row >> 1) & 7);
                 if (k >= a.nb - 8 * c) o -= 16 * k;
             }
             const size_t at = (size_t)c * 128;
             const uint8_t *p;
             if constexpr (i < NDX) p = xb + at;
             else p = wb + at + (is_gate(row0 - BM) ? gate : (size_t)0);
-            dma16_s(p, o, sb + buf * STAGE + row0 * 128);
+            dma16_s(p, o, mb + buf * STAGE + i * (1024 * GW));
         });
-    };
-    auto scales = [&](unsigned (&x)[FM], unsigned (&w)[FN], int c) __attribute__((always_inline)) {
-        static_for<FM>([&](auto I) __attribute__((always_inline)) { x[I] = mx_scale4(xsr[I], 8 * c + 4 * h); });
-        static_for<FN>([&](auto J) __attribute__((always_inline)) { w[J] = mx_scale4(wsr[J], 8 * c + 4 * h); });
     };
 
     mx_f32x16_t acc[FM][FN];
@@ -170,16 +204,28 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
 
     /* four MFMA steps; the fragments of step J + 1 are read while step J multiplies. Each step is a scheduling
      * region in which the reads are spread over the MFMAs */
+    uint32_t fx[4], fw[4];                                       /* where step j's first fragments lie in a stage */
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const uint32_t at = l32 * 128 + (((4 * h + j) ^ ((l32 >> 1) & 7)) << 4);
+        fx[j] = at + wm * FM * 4096;
+        fw[j] = at + (BM / 32 + wn * FN) * 4096;
+    }
+    const uint32_t cx = (wm * FM * 32 + l32) * 16 + 4 * h, cw = cx + (BM + (wn * FN - wm * FM) * 32) * 16;
+    auto shared_scales = [&](unsigned (&x)[FM], unsigned (&w)[FN], int buf, int sbuf) __attribute__((always_inline)) {
+        const uint8_t *C = smem + wk * GROUP + 2 * STAGE + sbuf * SCALES + buf * 8;
+#pragma unroll
+        for (int i = 0; i < FM; i++) x[i] = *reinterpret_cast<const unsigned *>(C + cx + i * 512);
+#pragma unroll
+        for (int j = 0; j < FN; j++) w[j] = *reinterpret_cast<const unsigned *>(C + cw + j * 512);
+    };
     auto compute = [&](int buf, const unsigned (&x)[FM], const unsigned (&w)[FN]) __attribute__((always_inline)) {
-        const uint8_t *S = smem + wk * 2 * STAGE + buf * STAGE;
+        const uint8_t *S = smem + wk * GROUP + buf * STAGE;
         uint4 xf[2][FM], wf[2][FN];
-        auto frag = [&](int row, int k) __attribute__((always_inline)) {
-            return *reinterpret_cast<const uint4 *>(S + row * 128 + ((k ^ ((row >> 1) & 7)) << 4));
-        };
         auto read = [&](auto J) __attribute__((always_inline)) {
             constexpr int j = decltype(J)::value, p = j & 1;
-            static_for<FM>([&](auto I) __attribute__((always_inline)) { xf[p][I] = frag((wm * FM + I) * 32 + l32, 4 * h + j); });
-            static_for<FN>([&](auto I) __attribute__((always_inline)) { wf[p][I] = frag(BM + (wn * FN + I) * 32 + l32, 4 * h + j); });
+            static_for<FM>([&](auto I) __attribute__((always_inline)) { xf[p][I] = *reinterpret_cast<const uint4 *>(S + fx[j] + I * 4096); });
+            static_for<FN>([&](auto I) __attribute__((always_inline)) { wf[p][I] = *reinterpret_cast<const uint4 *>(S + fw[j] + I * 4096); });
         };
         read(IC<0>{});
         __builtin_amdgcn_sched_barrier(0);
@@ -194,9 +240,12 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
             static_for<FM * FN>([&](auto I) __attribute__((always_inline)) {
                 constexpr int i = decltype(I)::value, nr = FM + FN, nm = FM * FN;
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                constexpr int d = nr * (i + 1) / nm - nr * i / nm;
+                constexpr int d = nr < nm ? (i < nr) : (nr * (i + 1) / nm - nr * i / nm);   /* early in the step */
                 if constexpr (j < 3 && d > 0) __builtin_amdgcn_sched_group_barrier(0x100, d, 0);
             });
+            /* holds the step's MFMAs here: nothing else keeps them from sinking below the reads of all later steps */
+#pragma unroll
+            for (int i = 0; i < FM * FN; i++) asm volatile("" : "+v"(acc[i / FN][i % FN]));
             __builtin_amdgcn_sched_barrier(0);
         });
     };
@@ -206,48 +255,108 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     };
 
-    /* the scale loads are behind the wait of turn(): this use tells the compiler so, which else would wait for
-     * them, and with them for every later transfer, at the first MFMA */
-    auto arrived = [&](unsigned (&x)[FM], unsigned (&w)[FN]) __attribute__((always_inline)) {
+    /* Scale loads are behind the wait of turn(): arrived() is a use that tells the compiler so, which else would wait for
+     * them, and with them for every later transfer, where they are used */
+    unsigned xa[FM], wa[FN];
+    if constexpr (SHARED) {
+        /* Whole pairs of chunks. Behind a pair's first turn() its scales are in LDS and those of the next pair are
+         * requested; they are stored behind its second turn(), when no wave reads the pair before any more */
+        auto arrived = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < FM; i++) asm volatile("" : "+v"(x[i]));
+            for (int i = 0; i < NS; i++)
+                asm volatile("" : "+v"(sreg[i].x), "+v"(sreg[i].y), "+v"(sreg[i].z), "+v"(sreg[i].w));
+        };
+        const int np = a.nb / 16;
+        int sbuf = 0;
+        if (np) {
+            load_scales(0);
+            issue(IC<0>{}, 0, 0);
+            put_scales(0);
+        }
+        for (int p = 0; p < np; p++) {
+            turn();
+            issue(IC<0>{}, 1, 2 * p + 1);
+            const bool more = p + 1 < np;
+            if (more) load_scales(2 * p + 2);
+            shared_scales(xa, wa, 0, sbuf);
+            compute(0, xa, wa);
+            turn();
+            if (more) {
+                arrived();
+                issue(IC<0>{}, 0, 2 * p + 2);
+                put_scales(sbuf ^ 1);
+            }
+            shared_scales(xa, wa, 1, sbuf);
+            compute(1, xa, wa);
+            sbuf ^= 1;
+        }
+        const int left = a.nb - 16 * np;                         /* blocks of up to two chunks */
+        if (left) {
 #pragma unroll
-        for (int j = 0; j < FN; j++) asm volatile("" : "+v"(w[j]));
-    };
-
-    /* the whole chunks of this group, then, by the last group, a short one. Groups of several waves come alone
-     * (WK = 1), so every wave takes the same number of turns */
-    static_assert(GW == 1 || WK == 1, "");
-    const int nc = a.nb / 8, per = (nc + WK - 1) / WK;
-    const int c0 = min(wk * per, nc), c1 = min(c0 + per, nc);
-    unsigned xsA[FM], wsA[FN], xsB[FM], wsB[FN];
-    if (c0 < c1) { issue(0, c0, true); scales(xsA, wsA, c0); }
-    for (int c = c0; c < c1; c += 2) {
-        turn();
-        arrived(xsA, wsA);
-        if (c + 1 < c1) { issue(1, c + 1, true); scales(xsB, wsB, c + 1); }
-        compute(0, xsA, wsA);
-        if (c + 1 >= c1) break;
-        turn();
-        arrived(xsB, wsB);
-        if (c + 2 < c1) { issue(0, c + 2, true); scales(xsA, wsA, c + 2); }
-        compute(1, xsB, wsB);
-    }
-    if ((a.nb & 7) && wk == WK - 1) {
-        turn();
-        issue(0, nc, false);
-        static_for<FM>([&](auto I) __attribute__((always_inline)) { xsA[I] = mx_scale4_end(xsr[I], 8 * nc + 4 * h, a.nb); });
-        static_for<FN>([&](auto J) __attribute__((always_inline)) { wsA[J] = mx_scale4_end(wsr[J], 8 * nc + 4 * h, a.nb); });
-        turn();
-        compute(0, xsA, wsA);
+            for (int i = 0; i < NS; i++) sreg[i] = mx_scale_end(srow[i], 16 * np, a.nb);
+            turn();                                              /* the last pair is still being read */
+            put_scales(0);
+            issue(IC<1>{}, 0, 2 * np);
+            if (left > 8) issue(IC<1>{}, 1, 2 * np + 1);
+            turn();
+            shared_scales(xa, wa, 0, 0);
+            compute(0, xa, wa);
+            if (left > 8) {
+                shared_scales(xa, wa, 1, 0);
+                compute(1, xa, wa);
+            }
+        }
+    } else {
+        /* the whole chunks [c0, c1) of this wave, then, by the last wave, a short one */
+        auto arrived = [](unsigned (&x)[FM], unsigned (&w)[FN]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < FM; i++) asm volatile("" : "+v"(x[i]));
+#pragma unroll
+            for (int j = 0; j < FN; j++) asm volatile("" : "+v"(w[j]));
+        };
+        unsigned xb_[FM], wb_[FN];
+        const int nc = a.nb / 8, per = (nc + WK - 1) / WK;
+        const int c0 = min(wk * per, nc), c1 = min(c0 + per, nc);
+        if (c0 < c1) {
+            issue(IC<0>{}, 0, c0);
+            scales(xa, wa, c0);
+        }
+        for (int c = c0; c < c1; c += 2) {
+            turn();
+            arrived(xa, wa);
+            if (c + 1 < c1) {
+                issue(IC<0>{}, 1, c + 1);
+                scales(xb_, wb_, c + 1);
+            }
+            compute(0, xa, wa);
+            if (c + 1 >= c1) break;
+            turn();
+            arrived(xb_, wb_);
+            if (c + 2 < c1) {
+                issue(IC<0>{}, 0, c + 2);
+                scales(xa, wa, c + 2);
+            }
+            compute(1, xb_, wb_);
+        }
+        if ((a.nb & 7) && wk == WK - 1) {
+            turn();
+            issue(IC<1>{}, 0, nc);
+#pragma unroll
+            for (int i = 0; i < FM; i++) xa[i] = mx_scale_end(xsr[i] - 4 * h, 8 * nc + 4 * h, a.nb).x;
+#pragma unroll
+            for (int j = 0; j < FN; j++) wa[j] = mx_scale_end(wsr[j] - 4 * h, 8 * nc + 4 * h, a.nb).x;
+            turn();
+            compute(0, xa, wa);
+        }
     }
 
     /* epilogue, 32 rows of every wave at a time: staged in LDS, the groups' parts added in order, whole row
      * segments stored */
+    const int el = fresh(lane), el32 = el & 31, eh = el >> 5;
     float *E = (float *)smem + wid * 32 * ES;
     constexpr int LPR = OW / 8;                                  /* lanes per row, 8 columns each */
     constexpr int RPI = 64 / LPR;                                /* rows per wave at once */
-    const int c8 = 8 * (lane % LPR), n = n0 + wn * OW + c8;
+    const int c8 = 8 * (el % LPR), n = n0 + wn * OW + c8;
     float b[8], bg[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
@@ -260,11 +369,11 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
         if constexpr (i > 0 && WK > 1) __syncthreads();          /* parts still being read */
         static_for<4 * FN>([&](auto JE) __attribute__((always_inline)) {
             constexpr int j = decltype(JE)::value / 4, e = decltype(JE)::value % 4;
-            *reinterpret_cast<float4 *>(E + l32 * ES + 32 * j + 8 * e + 4 * h) =
+            *reinterpret_cast<float4 *>(E + el32 * ES + 32 * j + 8 * e + 4 * eh) =
                 make_float4(acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]);
         });
         if constexpr (WK > 1) __syncthreads();
-        for (int q = wk * RPI + lane / LPR; q < 32; q += WK * RPI) {
+        for (int q = wk * RPI + el / LPR; q < 32; q += WK * RPI) {
             const int m = m0 + (wm * FM + i) * 32 + q;
             float v[8], g[8];
 #pragma unroll

@@ -15,7 +15,7 @@
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
 typedef float mx_f32x4_t __attribute__((ext_vector_type(4)));
 typedef float mx_f32x16_t __attribute__((ext_vector_type(16)));
-typedef float mx_f32x2_t __attribute__((ext_vector_type(2)));
+typedef unsigned mx_u32x4_t __attribute__((ext_vector_type(4)));
 
 /* element types of activations and outputs: the values of aria_dtype */
 enum { MX_F32 = 0, MX_F16 = 1, MX_BF16 = 2 };
