@@ -435,7 +435,7 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_rows(MxArgs a, const void *x, l
             float v[4][8];
             unsigned m = 0;
 #pragma unroll
-            for (int i = 0; i < 4; i++) mx_load8<XT>(x, (size_t)l16 * ldx + 32 * b + 8 * i, K - 32 * b - 8 * i, xvec, v[i]);
+            for (int i = 0; i < 4; i++) mx_load<XT, 8>(x, (size_t)l16 * ldx + 32 * b + 8 * i, K - 32 * b - 8 * i, xvec, v[i]);
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll

@@ -63,11 +63,13 @@ struct XaArgs {
     aria_k_xattn a;
     int G, R;            /* query heads per key head; rows per (batch, key head) */
     int nrb, T;          /* row blocks per (batch, key head); workgroups per split */
-    int ns;              /* splits of the keys across workgroups */
+    int ns, per;         /* splits of the keys across workgroups, key tiles to each */
     float scale_log2;
     float *part;         /* ns > 1: per (tile, split) 32 x DP sums, 32 references, 32 row sums */
 };
 
+/* keys of a tile where KS waves take tiles in turn */
+__host__ __device__ constexpr int xa_tile(int DP) { return DP == 64 ? 64 : 32; }
 /* floats of one partial result */
 __host__ __device__ constexpr int xa_part(int DP) { return 32 * DP + 64; }
 
@@ -117,9 +119,11 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
         }
     }
 
-    /* this workgroup's tiles, and this slice's share of them: [t0, t1) */
-    const int nt = (n + KT - 1) / KT, per = (nt + x.ns - 1) / x.ns;
-    const int w0 = min(split * per, nt), w1 = min(w0 + per, nt);
+    /* this workgroup's tiles, and this slice's share of them: [t0, t1). Every split has as many tiles, and a short
+     * sequence fewer splits, so that workgroups are equally long */
+    const int nt = (n + KT - 1) / KT;
+    const int w0 = x.ns > 1 ? split * x.per : 0, w1 = x.ns > 1 ? min(w0 + x.per, nt) : nt;
+    if (split > 0 && w0 >= nt) return;      /* uniform per workgroup, before any barrier */
     const int sp = (w1 - w0 + KS - 1) / KS;
     const int t0 = min(w0 + ks * sp, w1), t1 = min(t0 + sp, w1);
 
@@ -350,18 +354,27 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
     }
 }
 
-/* Joins the ns partial results of each block of 32 rows: a lane per 8 dims of a row. */
-template <typename T>
-__global__ __launch_bounds__(256) void k_xattn_join(XaArgs x, int DP) {
+/* Joins the partial results of one row: a group of DP / 8 lanes per 8 dims, the wave's 64 / (DP / 8) groups take the
+ * splits in turn and add up through lane exchanges */
+template <typename T, int DP>
+__global__ __launch_bounds__(64) void k_xattn_join(XaArgs x) {
+    constexpr int CPR = DP / 8, NG = 64 / CPR;
     const aria_k_xattn &a = x.a;
-    const int cpr = DP / 8, t = blockIdx.x, rb = t % x.nrb, bh = t / x.nrb, b = bh % a.B, hk = bh / a.B;
-    for (int i = threadIdx.x; i < 32 * cpr; i += 256) {
-        const int q = i / cpr, c8 = 8 * (i % cpr), row = rb * 32 + q;
-        if (row >= x.R || c8 >= a.D) continue;
-        const float *P = x.part + (size_t)t * x.ns * xa_part(DP);
-        float m = XA_MIN, rs = 0.0f, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        for (int s = 0; s < x.ns; s++) m = fmaxf(m, P[(size_t)s * xa_part(DP) + 32 * DP + q]);
-        for (int s = 0; s < x.ns; s++) {
+    const int rows = min(32, x.R);                             /* one row block where R is smaller */
+    const int t = blockIdx.x / rows, q = blockIdx.x % rows;
+    const int rb = t % x.nrb, bh = t / x.nrb, b = bh % a.B, hk = bh / a.B, row = rb * 32 + q;
+    if (row >= x.R) return;
+    const int lane = threadIdx.x, grp = lane / CPR, c8 = 8 * (lane % CPR);
+    const float *P = x.part + (size_t)t * x.ns * xa_part(DP);
+    const int n = a.kv_len ? min(max(a.kv_len[b], 0), a.Nk) : a.Nk;
+    const int ns = max(1, (n + x.per * xa_tile(DP) - 1) / (x.per * xa_tile(DP)));   /* the splits that hold keys */
+    float m = XA_MIN;
+    for (int s = lane; s < ns; s += 64) m = fmaxf(m, P[(size_t)s * xa_part(DP) + 32 * DP + q]);
+    m = grp_max<64>(m);
+    float rs = 0.0f, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (c8 < a.D)
+#pragma unroll 4
+        for (int s = grp; s < ns; s += NG) {
             const float *p = P + (size_t)s * xa_part(DP);
             const float f = __builtin_amdgcn_exp2f(p[32 * DP + q] - m);
             rs = __builtin_fmaf(f, p[32 * DP + 32 + q], rs);
@@ -370,18 +383,24 @@ __global__ __launch_bounds__(256) void k_xattn_join(XaArgs x, int DP) {
 #pragma unroll
             for (int j = 0; j < 8; j++) v[j] = __builtin_fmaf(f, e[j], v[j]);
         }
-        const float inv = rs > 0.0f ? 1.0f / rs : 0.0f;
-        const long long at = b * a.o_batch + (hk * x.G + row % x.G) * a.o_head + (row / x.G) * a.o_token + c8;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            if (a.out_f32) ((float *)a.out)[at + j] = v[j] * inv;
-            else ((T *)a.out)[at + j] = (T)(v[j] * inv);
-        }
+    for (int k = CPR; k < 64; k *= 2) {
+        rs += __shfl_xor(rs, k, 64);
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] += __shfl_xor(v[j], k, 64);
+    }
+    if (grp != 0 || c8 >= a.D) return;
+    const float inv = rs > 0.0f ? 1.0f / rs : 0.0f;
+    const long long at = b * a.o_batch + (hk * x.G + row % x.G) * a.o_head + (row / x.G) * a.o_token + c8;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        if (a.out_f32) ((float *)a.out)[at + j] = v[j] * inv;
+        else ((T *)a.out)[at + j] = (T)(v[j] * inv);
     }
 }
 
 /* how a call runs: few = KS waves per 32 rows, else QW = 4 blocks of 32 rows; ns splits of the keys */
-struct XaPlan { bool few; int DP, nrb, T, ns; };
+struct XaPlan { bool few; int DP, nrb, T, ns, per; };
 static XaPlan xa_plan(const aria_k_xattn *a) {
     XaPlan p;
     const long long R = (long long)a->Nq * (a->H / a->Hkv), bh = (long long)a->B * a->Hkv;
@@ -395,6 +414,7 @@ static XaPlan xa_plan(const aria_k_xattn *a) {
         const int most = a->Nk / 512;
         while (p.ns < most && (long long)p.T * p.ns < 768) p.ns++;
     }
+    p.per = ((a->Nk + xa_tile(p.DP) - 1) / xa_tile(p.DP) + p.ns - 1) / p.ns;
     return p;
 }
 
@@ -410,7 +430,11 @@ static hipError_t xa_launch(const XaPlan &p, const XaArgs &x, hipStream_t s) {
     if (p.few) {
         if (p.DP == 64) hipLaunchKernelGGL((k_xattn<T, 64, 64, 1, 4>), grid, dim3(256), 0, s, x);
         else hipLaunchKernelGGL((k_xattn<T, 128, 32, 1, 4>), grid, dim3(256), 0, s, x);
-        if (p.ns > 1) hipLaunchKernelGGL(k_xattn_join<T>, dim3(p.T), dim3(256), 0, s, x, p.DP);
+        if (p.ns > 1) {
+            const dim3 rows((unsigned)p.T * (unsigned)(x.R < 32 ? x.R : 32));
+            if (p.DP == 64) hipLaunchKernelGGL((k_xattn_join<T, 64>), rows, dim3(64), 0, s, x);
+            else hipLaunchKernelGGL((k_xattn_join<T, 128>), rows, dim3(64), 0, s, x);
+        }
     } else {
         if (p.DP == 64) hipLaunchKernelGGL((k_xattn<T, 64, 64, 4, 1>), grid, dim3(256), 0, s, x);
         else hipLaunchKernelGGL((k_xattn<T, 128, 64, 4, 1>), grid, dim3(256), 0, s, x);
@@ -428,6 +452,7 @@ extern "C" hipError_t aria_k_xattn_run(const aria_k_xattn *a, void *ws, hipStrea
     x.nrb = p.nrb;
     x.T = p.T;
     x.ns = p.ns;
+    x.per = p.per;
     x.scale_log2 = a->scale * ARIA_LOG2E;
     x.part = (float *)ws;
     return a->type == 1 ? xa_launch<_Float16>(p, x, s) : xa_launch<__bf16>(p, x, s);

@@ -26,24 +26,31 @@ template <> struct MxT<MX_F16> { using type = _Float16; };
 template <> struct MxT<MX_BF16> { using type = __bf16; };
 template <int T> using mx_t = typename MxT<T>::type;
 
-/* elements off .. off + 7 of x as fp32; those past n (counted from off) read as zero. vec: x + off
- * is 16-byte aligned */
-template <int T>
-__device__ __forceinline__ void mx_load8(const void *x, size_t off, int n, bool vec, float (&f)[8]) {
+/* elements off .. off + V - 1 of x as fp32; those past n (counted from off) read as zero. vec: x + off is 16-byte
+ * aligned (else aligned to an element) */
+template <int T, int V>
+__device__ __forceinline__ void mx_load(const void *x, size_t off, int n, bool vec, float (&f)[V]) {
+    typedef mx_t<T> v_t __attribute__((ext_vector_type(V)));
     const mx_t<T> *p = (const mx_t<T> *)x + off;
-    if (vec && n >= 8) {
-        typedef mx_t<T> v8_t __attribute__((ext_vector_type(8)));
-        if constexpr (T == MX_F32) {
-            const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
-            f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+    if (n >= V) {
+        v_t v;
+        if (vec) {
+            if constexpr (sizeof v == 32) {    /* eight fp32 */
+                typedef mx_t<T> h_t __attribute__((ext_vector_type(V / 2)));
+                const h_t a = *reinterpret_cast<const h_t *>(p), b = *reinterpret_cast<const h_t *>(p + V / 2);
+                __builtin_memcpy(&v, &a, 16);
+                __builtin_memcpy((char *)&v + 16, &b, 16);
+            } else {
+                v = *reinterpret_cast<const v_t *>(p);
+            }
         } else {
-            const v8_t v = *reinterpret_cast<const v8_t *>(p);
-#pragma unroll
-            for (int i = 0; i < 8; i++) f[i] = (float)v[i];
+            __builtin_memcpy(&v, p, sizeof v);
         }
+#pragma unroll
+        for (int i = 0; i < V; i++) f[i] = (float)v[i];
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) f[i] = i < n ? (float)p[i] : 0.0f;
+        for (int i = 0; i < V; i++) f[i] = i < n ? (float)p[i] : 0.0f;
     }
 }
 
@@ -55,6 +62,15 @@ __device__ __forceinline__ unsigned mx_abs_bits(float v) { return __builtin_bit_
 __device__ __forceinline__ unsigned mx_scale_byte(unsigned amax_bits) {
     const unsigned e = amax_bits >> 23;
     return e == 255u ? 255u : max(e, 2u) - 2u;
+}
+
+/* four values over 2^(byte - 127) -> 16 bits of codes; the rule of mx_pack8 */
+__device__ __forceinline__ unsigned mx_pack4(const float (&f)[4], unsigned byte) {
+    const float r = __builtin_bit_cast(float, (254u - min(byte, 253u)) << 23);
+    unsigned w = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[0] * r, f[1] * r, 1.0f, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[2] * r, f[3] * r, 1.0f, 1);
+    return byte == 255u ? 0u : w;
 }
 
 /* eight values over 2^(byte - 127) -> eight codes, ties to even, saturating at 6. The scaling is a
