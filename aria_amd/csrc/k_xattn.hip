@@ -73,12 +73,16 @@ __host__ __device__ constexpr int xa_tile(int DP) { return DP == 64 ? 64 : 32; }
 /* floats of one partial result */
 __host__ __device__ constexpr int xa_part(int DP) { return 32 * DP + 64; }
 
-/* QW waves of 32 rows share every tile (KS = 1), or KS waves take the tiles in turn, each on LDS
- * stages of its own and without barriers, and join their results at the end (QW = 1). */
+/* QW waves of 32 rows share every tile (KS = 1), or KS waves take the tiles in turn, each in LDS of its own and without
+ * barriers, and join their results at the end (QW = 1). The former hold two stages, the next tile moving
+ * under the current one's products. The latter are bound by the keys' bytes and hold one: two workgroups then
+ * fit a CU, and one wave's transfer runs beside another's products (cross_one's shape, 16 x 4 key heads x
+ * up to 8192 keys of 128: 56 us with two stages and one workgroup, 44 with one and two, the join included). */
 template <typename T, int DP, int KT, int QW, int KS>
 __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
     static_assert((QW == 1 || KS == 1) && (DP == 64 || DP == 128) && (KT == 64 || KT == 32), "");
     constexpr int NW = QW * KS;
+    constexpr int NST = KS == 1 ? 2 : 1;            /* LDS stages */
     constexpr int CPR = DP / 8;                     /* 16-byte chunks per key row */
     constexpr int SLOTS = KT * CPR;                 /* per tile and operand */
     constexpr int ND = SLOTS / 64 / QW;             /* DMA instructions per wave, tile and operand */
@@ -87,7 +91,7 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
     constexpr int KB = KT / 32, DT = DP / 32, DS = DP / 16;
     constexpr int STAGE = 2 * TB * KS;              /* K and V of every slice */
     constexpr int EPI = NW * 32 * ES * 4 + KS * 64 * 4;
-    __shared__ __attribute__((aligned(16))) uint8_t smem[2 * STAGE > EPI ? 2 * STAGE : EPI];
+    __shared__ __attribute__((aligned(16))) uint8_t smem[NST * STAGE > EPI ? NST * STAGE : EPI];
     typedef typename Xa<T>::v8 v8;
     typedef typename Xa<T>::v2 v2;
     const aria_k_xattn &a = x.a;
@@ -271,19 +275,35 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
         if constexpr (KS == 1) __syncthreads();
     };
 
-    uint64_t cur = to_bits(t0, mask_byte(t0)), nxt = to_bits(t0 + 1, mask_byte(t0 + 1));
-    if (t0 < t1) dma(0, cur);
-    drain();
-    meet();
-    for (int i = t0; i < t1; i++) {
-        const int buf = (i - t0) & 1;
-        const int byte = mask_byte(i + 2);
-        if (i + 1 < t1) dma(buf ^ 1, nxt);
-        if (cur) tile(buf, cur);
+    uint64_t cur = to_bits(t0, mask_byte(t0));
+    if constexpr (NST == 2) {
+        uint64_t nxt = to_bits(t0 + 1, mask_byte(t0 + 1));
+        if (t0 < t1) dma(0, cur);
         drain();
+        /* the rows are here: this use tells the compiler, which else would wait for them, and with them for the next
+         * tile's transfer, at every tile's first product */
+#pragma unroll
+        for (int i = 0; i < DS; i++) asm volatile("" : "+v"(qf[i]));
         meet();
-        cur = nxt;
-        nxt = to_bits(i + 2, byte);
+        for (int i = t0; i < t1; i++) {
+            const int buf = (i - t0) & 1;
+            const int byte = mask_byte(i + 2);
+            if (i + 1 < t1) dma(buf ^ 1, nxt);
+            if (cur) tile(buf, cur);
+            drain();
+            meet();
+            cur = nxt;
+            nxt = to_bits(i + 2, byte);
+        }
+    } else {
+        for (int i = t0; i < t1; i++) {
+            const int byte = mask_byte(i + 1);
+            dma(0, cur);
+            drain();
+            if (cur) tile(0, cur);
+            drain();
+            cur = to_bits(i + 1, byte);
+        }
     }
 
     /* join: lanes l and l ^ 32 hold half of a row's sum each */
@@ -410,9 +430,9 @@ static XaPlan xa_plan(const aria_k_xattn *a) {
     p.T = (int)(bh * p.nrb);
     p.ns = 1;
     if (p.few) {
-        /* at least 512 keys to a workgroup, and about three workgroups to a CU */
-        const int most = a->Nk / 512;
-        while (p.ns < most && (long long)p.T * p.ns < 768) p.ns++;
+        /* at least 256 keys to a workgroup, and up to four workgroups to a CU */
+        const int most = a->Nk / 256;
+        while (p.ns < most && (long long)p.T * p.ns < 1024) p.ns++;
     }
     p.per = ((a->Nk + xa_tile(p.DP) - 1) / xa_tile(p.DP) + p.ns - 1) / p.ns;
     return p;
