@@ -208,6 +208,15 @@ __device__ __forceinline__ void dma16(const void *g, uint32_t m0) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(m), "v"(g) : "memory");
 }
 
+/* the same from a scalar base and an unsigned 32-bit lane offset */
+__device__ __forceinline__ void dma16_s(const void *base, unsigned off, uint32_t m0) {
+    const uint32_t m = __builtin_amdgcn_readfirstlane(m0);
+    const uint64_t u = (uint64_t)base;
+    const uint64_t b = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(u >> 32)) << 32) |
+                       (uint32_t)__builtin_amdgcn_readfirstlane((int)u);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(m), "v"(off), "s"(b) : "memory");
+}
+
 template <int I>
 using IC = std::integral_constant<int, I>;
 /* f(IC<0>{}), ..., f(IC<N-1>{}) */

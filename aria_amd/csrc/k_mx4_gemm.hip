@@ -72,14 +72,6 @@ __device__ __forceinline__ uint32_t fresh_s(uint32_t v) {
     asm volatile("" : "+s"(v));
     return v;
 }
-/* LDS DMA with a scalar base and a 32-bit lane offset */
-__device__ __forceinline__ void dma16_s(const void *base, unsigned off, uint32_t m0) {
-    const uint64_t u = (uint64_t)base;
-    const uint64_t b = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(u >> 32)) << 32) |
-                       (uint32_t)__builtin_amdgcn_readfirstlane((int)u);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(m0), "v"(off), "s"(b) : "memory");
-}
-
 /*
  * WK groups of WM x WN waves; a group's waves share LDS stages and take every WK-th part of K; a wave owns
  * FM x FN blocks of 32 x 32 outputs (GLU: the first half of its FN are value rows, the second half
@@ -89,7 +81,7 @@ __device__ __forceinline__ void dma16_s(const void *base, unsigned off, uint32_t
  * One barrier a chunk (none where a group is one wave): it follows the wait for this wave's transfers and fragment reads, so
  * behind it the chunk is whole and the other stage is free.
  */
-template <int FM, int FN, int WM, int WN, int WK, bool GLU>
+template <int FM, int FN, int WM, int WN, int WK, int NST, bool GLU>
 __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
     constexpr int NW = WM * WN * WK, GW = WM * WN;
     constexpr int BM = 32 * FM * WM, BN = 32 * FN * WN;          /* rows of x and of w per tile */
@@ -104,7 +96,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
     constexpr int SCALES = SHARED ? NR * 16 : 0;                 /* scale bytes of two chunks */
     constexpr int NS = NR / (64 * GW);                           /* scale rows per lane */
     static_assert(NR % (64 * GW) == 0 && (!SHARED || WK == 1), "");
-    constexpr int GROUP = 2 * STAGE + 2 * SCALES;                /* LDS of one K group */
+    constexpr int GROUP = NST * STAGE + 2 * SCALES;              /* LDS of one K group */
+    static_assert(NST == 2 || (NST == 1 && !SHARED), "");
     __shared__ __attribute__((aligned(16))) uint8_t smem[WK * GROUP > EPI ? WK * GROUP : EPI];
     const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
     const int wid = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -314,29 +307,40 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
 #pragma unroll
             for (int j = 0; j < FN; j++) asm volatile("" : "+v"(w[j]));
         };
-        unsigned xb_[FM], wb_[FN];
         const int nc = a.nb / 8, per = (nc + WK - 1) / WK;
         const int c0 = min(wk * per, nc), c1 = min(c0 + per, nc);
-        if (c0 < c1) {
-            issue(IC<0>{}, 0, c0);
-            scales(xa, wa, c0);
-        }
-        for (int c = c0; c < c1; c += 2) {
-            turn();
-            arrived(xa, wa);
-            if (c + 1 < c1) {
-                issue(IC<0>{}, 1, c + 1);
-                scales(xb_, wb_, c + 1);
+        if constexpr (NST == 1) {
+            for (int c = c0; c < c1; c++) {
+                if (c > c0) turn();                              /* the stage is still being read */
+                issue(IC<0>{}, 0, c);
+                scales(xa, wa, c);
+                turn();
+                arrived(xa, wa);
+                compute(0, xa, wa);
             }
-            compute(0, xa, wa);
-            if (c + 1 >= c1) break;
-            turn();
-            arrived(xb_, wb_);
-            if (c + 2 < c1) {
-                issue(IC<0>{}, 0, c + 2);
-                scales(xa, wa, c + 2);
+        } else {
+            unsigned xb_[FM], wb_[FN];
+            if (c0 < c1) {
+                issue(IC<0>{}, 0, c0);
+                scales(xa, wa, c0);
             }
-            compute(1, xb_, wb_);
+            for (int c = c0; c < c1; c += 2) {
+                turn();
+                arrived(xa, wa);
+                if (c + 1 < c1) {
+                    issue(IC<0>{}, 1, c + 1);
+                    scales(xb_, wb_, c + 1);
+                }
+                compute(0, xa, wa);
+                if (c + 1 >= c1) break;
+                turn();
+                arrived(xb_, wb_);
+                if (c + 2 < c1) {
+                    issue(IC<0>{}, 0, c + 2);
+                    scales(xa, wa, c + 2);
+                }
+                compute(1, xb_, wb_);
+            }
         }
         if ((a.nb & 7) && wk == WK - 1) {
             turn();
@@ -469,25 +473,41 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_rows(MxArgs a, const void *x, l
     }
 }
 
-template <int FM, int FN, int WM, int WN, int WK, bool GLU>
+template <int FM, int FN, int WM, int WN, int WK, int NST, bool GLU>
 static hipError_t launch(MxArgs a, hipStream_t s) {
     constexpr int OW = (GLU ? 16 : 32) * FN * WN;
     a.tm = (a.M + 32 * FM * WM - 1) / (32 * FM * WM);
     a.tn = (a.N + OW - 1) / OW;
     a.T = a.tm * a.tn;
-    hipLaunchKernelGGL((k_mx4_gemm<FM, FN, WM, WN, WK, GLU>), dim3((unsigned)((a.T + 7) / 8 * 8)), dim3(64 * WM * WN * WK), 0, s, a);
+    hipLaunchKernelGGL((k_mx4_gemm<FM, FN, WM, WN, WK, NST, GLU>), dim3((unsigned)((a.T + 7) / 8 * 8)), dim3(64 * WM * WN * WK), 0, s, a);
     return hipGetLastError();
 }
 
+#ifdef MX_EXP
+static int mx_cfg() { const char *e = getenv("MXCFG"); return e ? atoi(e) : 0; }
+#endif
 template <bool GLU>
 static hipError_t pick(const MxArgs &a, hipStream_t s) {
     const long cols = GLU ? 2L * a.N : a.N;
+#ifdef MX_EXP
+    switch (mx_cfg()) {
+    case 1: return launch<4, 2, 2, 4, 1, 2, GLU>(a, s);
+    case 2: return launch<2, 2, 2, 2, 1, 2, GLU>(a, s);
+    case 3: return launch<2, 2, 1, 1, 4, 2, GLU>(a, s);
+    case 4: return launch<2, 2, 1, 1, 4, 1, GLU>(a, s);
+    case 5: return launch<2, 2, 1, 1, 8, 1, GLU>(a, s);
+    case 6: if constexpr (!GLU) return launch<1, 1, 1, 1, 8, 2, GLU>(a, s); else return launch<1, 2, 1, 1, 8, 1, GLU>(a, s);
+    case 7: if constexpr (!GLU) return launch<1, 1, 1, 1, 8, 1, GLU>(a, s); else return launch<1, 2, 1, 1, 4, 1, GLU>(a, s);
+    case 8: if constexpr (!GLU) return launch<2, 1, 1, 1, 8, 1, GLU>(a, s); else return launch<1, 2, 1, 1, 4, 2, GLU>(a, s);
+    case 9: if constexpr (!GLU) return launch<1, 1, 1, 1, 4, 1, GLU>(a, s); else return launch<1, 2, 1, 1, 2, 2, GLU>(a, s);
+    }
+#endif
     auto tiles = [&](int bm, int bn) { return (long)((a.M + bm - 1) / bm) * ((cols + bn - 1) / bn); };
-    if (tiles(256, 256) >= 200) return launch<4, 2, 2, 4, 1, GLU>(a, s);
-    if (tiles(128, 128) >= 200) return launch<2, 2, 2, 2, 1, GLU>(a, s);
-    if constexpr (GLU) return launch<2, 2, 1, 1, 4, GLU>(a, s);
-    if (tiles(64, 64) >= 200) return launch<2, 2, 1, 1, 4, GLU>(a, s);
-    return launch<1, 1, 1, 1, 8, GLU && false>(a, s);
+    if (tiles(256, 256) >= 200) return launch<4, 2, 2, 4, 1, 2, GLU>(a, s);
+    if (tiles(128, 128) >= 200) return launch<2, 2, 2, 2, 1, 2, GLU>(a, s);
+    if constexpr (GLU) return launch<2, 2, 1, 1, 4, 2, GLU>(a, s);
+    if (tiles(64, 64) >= 200) return launch<2, 2, 1, 1, 4, 2, GLU>(a, s);
+    return launch<1, 1, 1, 1, 8, 2, GLU && false>(a, s);
 }
 
 extern "C" hipError_t aria_k_mx4_gemm(void *y, int ytype, const uint8_t *xq, const uint8_t *xs, const uint8_t *wq,

@@ -64,6 +64,7 @@ struct XaArgs {
     int G, R;            /* query heads per key head; rows per (batch, key head) */
     int nrb, T;          /* row blocks per (batch, key head); workgroups per split */
     int ns, per;         /* splits of the keys across workgroups, key tiles to each */
+    int plain;           /* every chunk holds dims, and lane offsets within a tile fit 32 bits */
     float scale_log2;
     float *part;         /* ns > 1: per (tile, split) 32 x DP sums, 32 references, 32 row sums */
 };
@@ -84,6 +85,7 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
     constexpr int NW = QW * KS;
     constexpr int NST = KS == 1 ? 2 : 1;            /* LDS stages */
     constexpr int CPR = DP / 8;                     /* 16-byte chunks per key row */
+    constexpr uint64_t ALL = KT == 64 ? ~0ull : 0xFFFFFFFFull;   /* every key of a tile */
     constexpr int SLOTS = KT * CPR;                 /* per tile and operand */
     constexpr int ND = SLOTS / 64 / QW;             /* DMA instructions per wave, tile and operand */
     constexpr int TB = SLOTS * 16;                  /* bytes of a tile */
@@ -131,45 +133,49 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
     const int sp = (w1 - w0 + KS - 1) / KS;
     const int t0 = min(w0 + ks * sp, w1), t1 = min(t0 + sp, w1);
 
-    /* DMA sources of key 0 of the slice, one per instruction: slot p holds chunk cp of key row r, and
-     * receives the chunk that the swizzle puts there */
-    const T *kp[ND], *vp[ND];
-    int krow[ND];
-    bool kd[ND], vd[ND];
-    {
-        const T *Kh = (const T *)a.k + b * a.k_batch + hk * a.k_head + (long long)t0 * KT * a.k_token;
-        const T *Vh = (const T *)a.v + b * a.v_batch + hk * a.v_head + (long long)t0 * KT * a.v_token;
+    /* DMA sources: slot p of the tile holds chunk cp of key row r, and receives the chunk that the swizzle puts there.
+     * Scalar bases move from tile to tile; a lane's offset within a tile stays */
+    const char *kb = (const char *)((const T *)a.k + b * a.k_batch + hk * a.k_head + (long long)t0 * KT * a.k_token);
+    const char *vb = (const char *)((const T *)a.v + b * a.v_batch + hk * a.v_head + (long long)t0 * KT * a.v_token);
+    const long long kstep = KT * a.k_token * 2, vstep = KT * a.v_token * 2;
+    auto slot = [&](int i, int &r, int &ck, int &cv) __attribute__((always_inline)) {
+        const int p = 64 * (QW * i + qw) + lane, cp = p % CPR;
+        r = p / CPR;
+        ck = DP == 64 ? cp ^ ((r >> 1) & 7) : cp ^ (r & 15);
+        cv = DP == 64 ? cp ^ (((r >> 1) & 1) << 2) : cp ^ ((r & 3) << 2);
+    };
+    unsigned koff_g[ND], voff_g[ND];
 #pragma unroll
-        for (int i = 0; i < ND; i++) {
-            const int p = 64 * (QW * i + qw) + lane, r = p / CPR, cp = p % CPR;
-            const int ck = DP == 64 ? cp ^ ((r >> 1) & 7) : cp ^ (r & 15);
-            const int cv = DP == 64 ? cp ^ (((r >> 1) & 1) << 2) : cp ^ ((r & 3) << 2);
-            krow[i] = r;
-            kp[i] = Kh + r * a.k_token + 8 * ck;
-            vp[i] = Vh + r * a.v_token + 8 * cv;
-            kd[i] = 8 * ck < a.D;
-            vd[i] = 8 * cv < a.D;
-        }
+    for (int i = 0; i < ND; i++) {
+        int r, ck, cv;
+        slot(i, r, ck, cv);
+        koff_g[i] = (unsigned)(r * a.k_token + 8 * ck) * 2;
+        voff_g[i] = (unsigned)(r * a.v_token + 8 * cv) * 2;
     }
-    const long long kstep = KT * a.k_token, vstep = KT * a.v_token;
     auto dma = [&](int buf, uint64_t bits) __attribute__((always_inline)) {
-        const uint32_t S = (uint32_t)(uintptr_t)smem + buf * STAGE + ks * 2 * TB;
+        const uint32_t S = (uint32_t)(uintptr_t)smem + buf * STAGE + ks * 2 * TB + 1024 * qw;
+        if (x.plain && bits == ALL) {
 #pragma unroll
-        for (int i = 0; i < ND; i++) {
-            const bool ok = (bits >> krow[i]) & 1;
-            const void *k = ok && kd[i] ? (const void *)kp[i] : (const void *)&xa_zero;
-            const void *v = ok && vd[i] ? (const void *)vp[i] : (const void *)&xa_zero;
-            dma16(k, S + 1024 * (QW * i + qw));
-            dma16(v, S + TB + 1024 * (QW * i + qw));
-            kp[i] += kstep;
-            vp[i] += vstep;
+            for (int i = 0; i < ND; i++) {
+                dma16_s(kb, koff_g[i], S + 1024 * QW * i);
+                dma16_s(vb, voff_g[i], S + TB + 1024 * QW * i);
+            }
+        } else {
+            for (int i = 0; i < ND; i++) {
+                int r, ck, cv;
+                slot(i, r, ck, cv);
+                const bool ok = (bits >> r) & 1;
+                dma16(ok && 8 * ck < a.D ? kb + (r * a.k_token + 8 * ck) * 2 : (const char *)&xa_zero, S + 1024 * QW * i);
+                dma16(ok && 8 * cv < a.D ? vb + (r * a.v_token + 8 * cv) * 2 : (const char *)&xa_zero, S + TB + 1024 * QW * i);
+            }
         }
+        kb += kstep;
+        vb += vstep;
     };
     /* the valid keys of tile i (bit j: key KT i + j) where no mask says otherwise */
     auto in_len = [&](int i) __attribute__((always_inline)) -> uint64_t {
         const int left = n - i * KT;
-        const uint64_t all = KT == 64 ? ~0ull : 0xFFFFFFFFull;
-        return left >= KT ? all : left <= 0 ? 0ull : (1ull << left) - 1;
+        return left >= KT ? ALL : left <= 0 ? 0ull : (1ull << left) - 1;
     };
     auto mask_byte = [&](int i) __attribute__((always_inline)) -> int {
         const int j = i * KT + (lane & (KT - 1));
@@ -215,7 +221,7 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
 #pragma unroll
             for (int kb = 0; kb < KB; kb++)
                 s[kb] = Xa<T>::mfma(*reinterpret_cast<const v8 *>(K + koff[i] + kb * 32 * CPR * 16), qf[i], s[kb]);
-        if (bits != (KT == 64 ? ~0ull : 0xFFFFFFFFull)) {
+        if (bits != ALL) {
             const float ninf = -INFINITY;
 #pragma unroll
             for (int kb = 0; kb < KB; kb++) {
@@ -285,8 +291,9 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
 #pragma unroll
         for (int i = 0; i < DS; i++) asm volatile("" : "+v"(qf[i]));
         meet();
-        for (int i = t0; i < t1; i++) {
-            const int buf = (i - t0) & 1;
+        /* one tile from stage BUF; a compile-time stage keeps every LDS offset an immediate */
+        auto turn = [&](auto BUF, int i) __attribute__((always_inline)) {
+            constexpr int buf = decltype(BUF)::value;
             const int byte = mask_byte(i + 2);
             if (i + 1 < t1) dma(buf ^ 1, nxt);
             if (cur) tile(buf, cur);
@@ -294,6 +301,11 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
             meet();
             cur = nxt;
             nxt = to_bits(i + 2, byte);
+        };
+        for (int i = t0; i < t1; i += 2) {
+            turn(IC<0>{}, i);
+            if (i + 1 >= t1) break;
+            turn(IC<1>{}, i + 1);
         }
     } else {
         for (int i = t0; i < t1; i++) {
@@ -419,17 +431,20 @@ __global__ __launch_bounds__(64) void k_xattn_join(XaArgs x) {
     }
 }
 
-/* how a call runs: few = KS waves per 32 rows, else QW = 4 blocks of 32 rows; ns splits of the keys */
-struct XaPlan { bool few; int DP, nrb, T, ns, per; };
+/* How a call runs: KS waves per 32 rows (qw 1) where blocks of 128 rows would leave CUs idle, else qw blocks of 32 rows a
+ * workgroup: 4, or, where four rounds of 256 rows fill the CUs, 8 (4 x 16 heads x 4096 rows x 2048 keys of 64: 166 us with 4, 158
+ * with 8; of 128, where 8 waves' registers fill the CU: 164 and 168). ns splits of the keys. */
+struct XaPlan { int qw, DP, nrb, T, ns, per; };
 static XaPlan xa_plan(const aria_k_xattn *a) {
     XaPlan p;
     const long long R = (long long)a->Nq * (a->H / a->Hkv), bh = (long long)a->B * a->Hkv;
+    auto tiles = [&](int qw) { return bh * ((R + 32 * qw - 1) / (32 * qw)); };
     p.DP = a->D <= 64 ? 64 : 128;
-    p.few = bh * ((R + 127) / 128) < 256;
-    p.nrb = (int)(p.few ? (R + 31) / 32 : (R + 127) / 128);
-    p.T = (int)(bh * p.nrb);
+    p.qw = p.DP == 64 && tiles(8) >= 1024 ? 8 : tiles(4) >= 256 ? 4 : 1;
+    p.T = (int)tiles(p.qw);
+    p.nrb = (int)(p.T / bh);
     p.ns = 1;
-    if (p.few) {
+    if (p.qw == 1) {
         /* at least 256 keys to a workgroup, and up to four workgroups to a CU */
         const int most = a->Nk / 256;
         while (p.ns < most && (long long)p.T * p.ns < 1024) p.ns++;
@@ -447,7 +462,7 @@ template <typename T>
 static hipError_t xa_launch(const XaPlan &p, const XaArgs &x, hipStream_t s) {
     const int n = p.T * p.ns;
     const dim3 grid((unsigned)((n + 7) / 8 * 8));
-    if (p.few) {
+    if (p.qw == 1) {
         if (p.DP == 64) hipLaunchKernelGGL((k_xattn<T, 64, 64, 1, 4>), grid, dim3(256), 0, s, x);
         else hipLaunchKernelGGL((k_xattn<T, 128, 32, 1, 4>), grid, dim3(256), 0, s, x);
         if (p.ns > 1) {
@@ -455,6 +470,8 @@ static hipError_t xa_launch(const XaPlan &p, const XaArgs &x, hipStream_t s) {
             if (p.DP == 64) hipLaunchKernelGGL((k_xattn_join<T, 64>), rows, dim3(64), 0, s, x);
             else hipLaunchKernelGGL((k_xattn_join<T, 128>), rows, dim3(64), 0, s, x);
         }
+    } else if (p.qw == 8) {
+        hipLaunchKernelGGL((k_xattn<T, 64, 64, 8, 1>), grid, dim3(512), 0, s, x);
     } else {
         if (p.DP == 64) hipLaunchKernelGGL((k_xattn<T, 64, 64, 4, 1>), grid, dim3(256), 0, s, x);
         else hipLaunchKernelGGL((k_xattn<T, 128, 64, 4, 1>), grid, dim3(256), 0, s, x);
@@ -473,6 +490,7 @@ extern "C" hipError_t aria_k_xattn_run(const aria_k_xattn *a, void *ws, hipStrea
     x.T = p.T;
     x.ns = p.ns;
     x.per = p.per;
+    x.plain = a->D == p.DP && a->k_token < (1 << 24) && a->v_token < (1 << 24);   /* 64 keys x 2 bytes x 2^24 = 2^31 */
     x.scale_log2 = a->scale * ARIA_LOG2E;
     x.part = (float *)ws;
     return a->type == 1 ? xa_launch<_Float16>(p, x, s) : xa_launch<__bf16>(p, x, s);
