@@ -32,14 +32,13 @@ __device__ __forceinline__ uint4 mx_scale_end(const uint8_t *row, int b, int nb)
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-/* eight results of one row, from column n on */
-__device__ __forceinline__ void mx_store8(const MxArgs &a, int m, int n, const float (&v)[8]) {
+/* V results of one row from column n on: four fp32 or eight 16-bit values */
+template <int V>
+__device__ __forceinline__ void mx_store_row(const MxArgs &a, int m, int n, const float (&v)[V]) {
     const size_t at = (size_t)m * a.N + n;
-    if (a.vec && n + 8 <= a.N) {
-        if (a.ytype == MX_F32) {
-            float *y = (float *)a.y + at;
-            *reinterpret_cast<float4 *>(y) = make_float4(v[0], v[1], v[2], v[3]);
-            *reinterpret_cast<float4 *>(y + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    if (a.vec && n + V <= a.N) {
+        if constexpr (V == 4) {
+            *reinterpret_cast<float4 *>((float *)a.y + at) = make_float4(v[0], v[1], v[2], v[3]);
         } else if (a.ytype == MX_F16) {
             typedef _Float16 v8_t __attribute__((ext_vector_type(8)));
             v8_t o;
@@ -55,7 +54,7 @@ __device__ __forceinline__ void mx_store8(const MxArgs &a, int m, int n, const f
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++)
+        for (int i = 0; i < V; i++)
             if (n + i < a.N) mx_store(a.y, a.ytype, at + i, v[i]);
     }
 }
@@ -81,7 +80,7 @@ __device__ __forceinline__ uint32_t fresh_s(uint32_t v) {
  * One barrier a chunk (none where a group is one wave): it follows the wait for this wave's transfers and fragment reads, so
  * behind it the chunk is whole and the other stage is free.
  */
-template <int FM, int FN, int WM, int WN, int WK, int NST, bool GLU>
+template <int FM, int FN, int WM, int WN, int WK, bool GLU>
 __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
     constexpr int NW = WM * WN * WK, GW = WM * WN;
     constexpr int BM = 32 * FM * WM, BN = 32 * FN * WN;          /* rows of x and of w per tile */
@@ -94,10 +93,10 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
     constexpr int EPI = NW * 32 * ES * 4;
     constexpr bool SHARED = GW > 1;                              /* scales go through LDS */
     constexpr int SCALES = SHARED ? NR * 16 : 0;                 /* scale bytes of two chunks */
-    constexpr int NS = NR / (64 * GW);                           /* scale rows per lane */
-    static_assert(NR % (64 * GW) == 0 && (!SHARED || WK == 1), "");
+    constexpr int NS = SHARED ? NR / (64 * GW) : 1;              /* scale rows per lane */
+    static_assert(!SHARED || (NR % (64 * GW) == 0 && WK == 1), "");
+    constexpr int NST = SHARED ? 2 : 1;                          /* stages */
     constexpr int GROUP = NST * STAGE + 2 * SCALES;              /* LDS of one K group */
-    static_assert(NST == 2 || (NST == 1 && !SHARED), "");
     __shared__ __attribute__((aligned(16))) uint8_t smem[WK * GROUP > EPI ? WK * GROUP : EPI];
     const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
     const int wid = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -309,38 +308,13 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
         };
         const int nc = a.nb / 8, per = (nc + WK - 1) / WK;
         const int c0 = min(wk * per, nc), c1 = min(c0 + per, nc);
-        if constexpr (NST == 1) {
-            for (int c = c0; c < c1; c++) {
-                if (c > c0) turn();                              /* the stage is still being read */
-                issue(IC<0>{}, 0, c);
-                scales(xa, wa, c);
-                turn();
-                arrived(xa, wa);
-                compute(0, xa, wa);
-            }
-        } else {
-            unsigned xb_[FM], wb_[FN];
-            if (c0 < c1) {
-                issue(IC<0>{}, 0, c0);
-                scales(xa, wa, c0);
-            }
-            for (int c = c0; c < c1; c += 2) {
-                turn();
-                arrived(xa, wa);
-                if (c + 1 < c1) {
-                    issue(IC<0>{}, 1, c + 1);
-                    scales(xb_, wb_, c + 1);
-                }
-                compute(0, xa, wa);
-                if (c + 1 >= c1) break;
-                turn();
-                arrived(xb_, wb_);
-                if (c + 2 < c1) {
-                    issue(IC<0>{}, 0, c + 2);
-                    scales(xa, wa, c + 2);
-                }
-                compute(1, xb_, wb_);
-            }
+        for (int c = c0; c < c1; c++) {
+            if (c > c0) turn();                                  /* the stage is still being read */
+            issue(IC<0>{}, 0, c);
+            scales(xa, wa, c);
+            turn();
+            arrived(xa, wa);
+            compute(0, xa, wa);
         }
         if ((a.nb & 7) && wk == WK - 1) {
             turn();
@@ -358,15 +332,6 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
      * segments stored */
     const int el = fresh(lane), el32 = el & 31, eh = el >> 5;
     float *E = (float *)smem + wid * 32 * ES;
-    constexpr int LPR = OW / 8;                                  /* lanes per row, 8 columns each */
-    constexpr int RPI = 64 / LPR;                                /* rows per wave at once */
-    const int c8 = 8 * (el % LPR), n = n0 + wn * OW + c8;
-    float b[8], bg[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-        b[e] = a.bias && n + e < a.N ? a.bias[n + e] : 0.0f;
-        bg[e] = GLU && a.bias && n + e < a.N ? a.bias[a.N + n + e] : 0.0f;
-    }
     __syncthreads();                                             /* stages still being read */
     static_for<FM>([&](auto I) __attribute__((always_inline)) {
         constexpr int i = decltype(I)::value;
@@ -377,30 +342,48 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
                 make_float4(acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]);
         });
         if constexpr (WK > 1) __syncthreads();
-        for (int q = wk * RPI + el / LPR; q < 32; q += WK * RPI) {
-            const int m = m0 + (wm * FM + i) * 32 + q;
-            float v[8], g[8];
+        /* 16 bytes of a row per lane: V columns */
+        auto rows = [&](auto VV) __attribute__((always_inline)) {
+            constexpr int V = decltype(VV)::value, LPR = OW / V, RPI = 64 / LPR;   /* lanes per row, rows per wave at once */
+            const int cv = V * (el % LPR), n = n0 + wn * OW + cv;
+            float b[V], bg[V];
 #pragma unroll
-            for (int k = 0; k < WK; k++) {
-                const float4 *p = (const float4 *)((const float *)smem + (k * GW + gw) * 32 * ES + q * ES + c8);
-                const float4 v0 = p[0], v1 = p[1];
-                const float w[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+            for (int e = 0; e < V; e++) {
+                b[e] = a.bias && n + e < a.N ? a.bias[n + e] : 0.0f;
+                bg[e] = GLU && a.bias && n + e < a.N ? a.bias[a.N + n + e] : 0.0f;
+            }
 #pragma unroll
-                for (int e = 0; e < 8; e++) v[e] = k ? v[e] + w[e] : w[e];
-                if constexpr (GLU) {
-                    const float4 g0 = p[OW / 4], g1 = p[OW / 4 + 1];
-                    const float u[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
+            for (int q0 = 0; q0 < 32; q0 += WK * RPI) {
+                const int q = q0 + wk * RPI + el / LPR, m = m0 + (wm * FM + i) * 32 + q;
+                if (WK * RPI > 32 && q >= 32) break;
+                float v[V], g[V];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) g[e] = k ? g[e] + u[e] : u[e];
+                for (int k = 0; k < WK; k++) {
+                    const float *p = (const float *)smem + (k * GW + gw) * 32 * ES + q * ES + cv;
+#pragma unroll
+                    for (int e4 = 0; e4 < V; e4 += 4) {
+                        const float4 u = *reinterpret_cast<const float4 *>(p + e4);
+                        const float w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                        for (int e = 0; e < 4; e++) v[e4 + e] = k ? v[e4 + e] + w[e] : w[e];
+                        if constexpr (GLU) {
+                            const float4 t4 = *reinterpret_cast<const float4 *>(p + OW + e4);
+                            const float z[4] = {t4.x, t4.y, t4.z, t4.w};
+#pragma unroll
+                            for (int e = 0; e < 4; e++) g[e4 + e] = k ? g[e4 + e] + z[e] : z[e];
+                        }
+                    }
                 }
-            }
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                v[e] += b[e];
-                if constexpr (GLU) v[e] *= silu_f(g[e] + bg[e]);
+                for (int e = 0; e < V; e++) {
+                    v[e] += b[e];
+                    if constexpr (GLU) v[e] *= silu_f(g[e] + bg[e]);
+                }
+                if (m < a.M && n < a.N) mx_store_row<V>(a, m, n, v);
             }
-            if (m < a.M && n < a.N) mx_store8(a, m, n, v);
-        }
+        };
+        if (a.ytype == MX_F32) rows(IC<4>{});
+        else rows(IC<8>{});
     });
 }
 
@@ -473,48 +456,43 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_rows(MxArgs a, const void *x, l
     }
 }
 
-template <int FM, int FN, int WM, int WN, int WK, int NST, bool GLU>
+template <int FM, int FN, int WM, int WN, int WK, bool GLU>
 static hipError_t launch(MxArgs a, hipStream_t s) {
     constexpr int OW = (GLU ? 16 : 32) * FN * WN;
     a.tm = (a.M + 32 * FM * WM - 1) / (32 * FM * WM);
     a.tn = (a.N + OW - 1) / OW;
     a.T = a.tm * a.tn;
-    hipLaunchKernelGGL((k_mx4_gemm<FM, FN, WM, WN, WK, NST, GLU>), dim3((unsigned)((a.T + 7) / 8 * 8)), dim3(64 * WM * WN * WK), 0, s, a);
+    hipLaunchKernelGGL((k_mx4_gemm<FM, FN, WM, WN, WK, GLU>), dim3((unsigned)((a.T + 7) / 8 * 8)), dim3(64 * WM * WN * WK), 0, s, a);
     return hipGetLastError();
 }
 
-#ifdef MX_EXP
-static int mx_cfg() { const char *e = getenv("MXCFG"); return e ? atoi(e) : 0; }
-#endif
+/* Which tile: the least estimated time, in us, over one launch. A configuration takes at least the latency of one tile, and where
+ * there are many tiles the time that all CUs need for them; both grow with the chunks of K, the large tiles' also
+ * with the bytes of output. Fitted to M = 17 .. 8192, N = 1024 .. 8192, K = 256 .. 8192 (within 20 % there, mostly 10 %). 256 x 256
+ * tiles come in rounds of one per CU. 64 x 64 and 32 x 32 tiles split K over four one-wave groups: at M = 344, K = 1024,
+ * N = 4096 32 x 32 take 6.8 us, 64 x 64 6.4, 128 x 128 7.4, 256 x 256 13.8; at M = 172, K = 4096, N = 1024 5.1, 7.8, 15.0, 30.8; at
+ * M = N = 8192, K = 4096 256 x 256 155 and 128 x 128 186. */
 template <bool GLU>
 static hipError_t pick(const MxArgs &a, hipStream_t s) {
-    const long cols = GLU ? 2L * a.N : a.N;
-#ifdef MX_EXP
-    switch (mx_cfg()) {
-    case 1: return launch<4, 2, 2, 4, 1, 2, GLU>(a, s);
-    case 2: return launch<2, 2, 2, 2, 1, 2, GLU>(a, s);
-    case 3: return launch<2, 2, 1, 1, 4, 2, GLU>(a, s);
-    case 4: return launch<2, 2, 1, 1, 4, 1, GLU>(a, s);
-    case 5: return launch<2, 2, 1, 1, 8, 1, GLU>(a, s);
-    case 6: if constexpr (!GLU) return launch<1, 1, 1, 1, 8, 2, GLU>(a, s); else return launch<1, 2, 1, 1, 8, 1, GLU>(a, s);
-    case 7: if constexpr (!GLU) return launch<1, 1, 1, 1, 8, 1, GLU>(a, s); else return launch<1, 2, 1, 1, 4, 1, GLU>(a, s);
-    case 8: if constexpr (!GLU) return launch<2, 1, 1, 1, 8, 1, GLU>(a, s); else return launch<1, 2, 1, 1, 4, 2, GLU>(a, s);
-    case 9: if constexpr (!GLU) return launch<1, 1, 1, 1, 4, 1, GLU>(a, s); else return launch<1, 2, 1, 1, 2, 2, GLU>(a, s);
-    }
-#endif
-    auto tiles = [&](int bm, int bn) { return (long)((a.M + bm - 1) / bm) * ((cols + bn - 1) / bn); };
-    if (tiles(256, 256) >= 200) return launch<4, 2, 2, 4, 1, 2, GLU>(a, s);
-    if (tiles(128, 128) >= 200) return launch<2, 2, 2, 2, 1, 2, GLU>(a, s);
-    if constexpr (GLU) return launch<2, 2, 1, 1, 4, 2, GLU>(a, s);
-    if (tiles(64, 64) >= 200) return launch<2, 2, 1, 1, 4, 2, GLU>(a, s);
-    return launch<1, 1, 1, 1, 8, 2, GLU && false>(a, s);
+    const double nc = (a.nb + 7) / 8, es = a.ytype == MX_F32 ? 4 : 2;
+    auto tiles = [&](int bm, int cols) { return (double)((a.M + bm - 1) / bm) * (double)((a.N + cols - 1) / cols); };
+    auto most = [](double x, double y) { return x > y ? x : y; };
+    constexpr int H = GLU ? 2 : 1;                               /* weight rows per column */
+    const double kb2 = 128 * (128 / H) * es / 1024, t2 = tiles(128, 128 / H), t1 = tiles(256, 256 / H);
+    const double c9 = GLU ? most(4.4 + 0.2 * nc, 3 + tiles(32, 32) * 0.0012 * nc) : most(4.4 + 0.04 * nc, 3 + tiles(32, 32) * (0.001 + 0.00043 * nc));
+    const double c4 = most(4.0 + 0.25 * nc, 2.7 + tiles(64, 64 / H) * (0.004 + 0.00138 * nc));
+    const double c2 = most(4.4 + 0.66 * nc, 3 + t2 * (0.0053 + 0.00025 * kb2 + 0.0018 * nc));
+    const double c1 = 3 + (double)((long)(t1 + 255) / 256) * (2.7 + 0.0234 * 4 * kb2 + 2.2 * nc);
+    if (c9 <= c4 && c9 <= c2 && c9 <= c1) return launch<1, H, 1, 1, 4, GLU>(a, s);
+    if (c4 <= c2 && c4 <= c1) return launch<2, 2, 1, 1, 4, GLU>(a, s);
+    return c2 <= c1 ? launch<2, 2, 2, 2, 1, GLU>(a, s) : launch<4, 2, 2, 4, 1, GLU>(a, s);
 }
 
 extern "C" hipError_t aria_k_mx4_gemm(void *y, int ytype, const uint8_t *xq, const uint8_t *xs, const uint8_t *wq,
                                       const uint8_t *ws, const float *bias, int M, int K, int N, int glu, hipStream_t s) {
     if (M <= 0 || N <= 0) return hipSuccess;
     MxArgs a = {y, xq, xs, wq, ws, bias, M, N, (K + 31) / 32, ytype, 0, 0, 0, 0};
-    a.vec = N % 8 == 0 && ((uintptr_t)y & 15u) == 0;
+    a.vec = N % (ytype == MX_F32 ? 4 : 8) == 0 && ((uintptr_t)y & 15u) == 0;
     return glu ? pick<true>(a, s) : pick<false>(a, s);
 }
 

@@ -192,6 +192,17 @@ def test_linear(hip, M, K, N, xt, yt, bias):
     assert (np.abs(got - y) <= linear_tol(y, terms, K, yt)).all(), np.abs(got - y).max()
 
 
+LARGE = [(900, 480, 1501), (900, 1000, 1500), (1500, 1024, 2050), (2592, 1056, 3500), (2700, 1111, 4090)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N", LARGE)
+@pytest.mark.parametrize("xt,yt,bias", [("f32", "f32", True), ("bf16", "f16", False)])
+def test_linear_large(hip, M, K, N, xt, yt, bias):
+    """Tiles of 64, 128 and 256 rows, whole and cut at every edge, K in whole chunks and not."""
+    test_linear(hip, M, K, N, xt, yt, bias)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("M", [1, 5, 60, 300])
 @pytest.mark.parametrize("pad", [8, 3])
@@ -228,6 +239,13 @@ def test_glu(hip, M, K, N, xt, yt, bias):
     tol += HALF_STEP[yt] * np.abs(y) * 1.001 + SUB[yt]
     got = run_linear(hip, "aria_hip_glu_mx4_dev", x, xt, K, q, s, b, M, K, N, yt)
     assert (np.abs(got - y) <= tol).all(), np.abs(got - y).max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N", [(260, 1000, 2050), (520, 700, 1030), (1300, 416, 2050), (2700, 416, 4090)])
+@pytest.mark.parametrize("xt,yt,bias", [("f32", "f32", True), ("f16", "bf16", False)])
+def test_glu_large(hip, M, K, N, xt, yt, bias):
+    test_glu(hip, M, K, N, xt, yt, bias)
 
 
 @pytest.mark.gpu
