@@ -189,6 +189,29 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
         });
     };
 
+    /* the biases of this lane's columns of the epilogue, whose loads end under the first chunk's transfer */
+    float bias[8], gbias[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) { bias[e] = 0.0f; gbias[e] = 0.0f; }
+    if (a.bias) {
+        const int V = a.ytype == MX_F32 ? 4 : 8, n = n0 + wn * OW + V * (lane % (OW / V));
+        if (n + V <= a.N) {
+            __builtin_memcpy(bias, a.bias + n, 16);
+            if (V == 8) __builtin_memcpy(bias + 4, a.bias + n + 4, 16);
+            if constexpr (GLU) {
+                __builtin_memcpy(gbias, a.bias + a.N + n, 16);
+                if (V == 8) __builtin_memcpy(gbias + 4, a.bias + a.N + n + 4, 16);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (e < V && n + e < a.N) {
+                    bias[e] = a.bias[n + e];
+                    if constexpr (GLU) gbias[e] = a.bias[a.N + n + e];
+                }
+        }
+    }
+
     mx_f32x16_t acc[FM][FN];
     static_for<FM * FN>([&](auto I) __attribute__((always_inline)) {
         acc[I / FN][I % FN] = mx_f32x16_t{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
@@ -346,12 +369,6 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
         auto rows = [&](auto VV) __attribute__((always_inline)) {
             constexpr int V = decltype(VV)::value, LPR = OW / V, RPI = 64 / LPR;   /* lanes per row, rows per wave at once */
             const int cv = V * (el % LPR), n = n0 + wn * OW + cv;
-            float b[V], bg[V];
-#pragma unroll
-            for (int e = 0; e < V; e++) {
-                b[e] = a.bias && n + e < a.N ? a.bias[n + e] : 0.0f;
-                bg[e] = GLU && a.bias && n + e < a.N ? a.bias[a.N + n + e] : 0.0f;
-            }
 #pragma unroll
             for (int q0 = 0; q0 < 32; q0 += WK * RPI) {
                 const int q = q0 + wk * RPI + el / LPR, m = m0 + (wm * FM + i) * 32 + q;
@@ -376,8 +393,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
                 }
 #pragma unroll
                 for (int e = 0; e < V; e++) {
-                    v[e] += b[e];
-                    if constexpr (GLU) v[e] *= silu_f(g[e] + bg[e]);
+                    v[e] += bias[e];
+                    if constexpr (GLU) v[e] *= silu_f(g[e] + gbias[e]);
                 }
                 if (m < a.M && n < a.N) mx_store_row<V>(a, m, n, v);
             }
