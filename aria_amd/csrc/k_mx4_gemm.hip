@@ -72,15 +72,19 @@ __device__ __forceinline__ uint32_t fresh_s(uint32_t v) {
     return v;
 }
 /*
- * WK groups of WM x WN waves; a group's waves share LDS stages and take every WK-th part of K; a wave owns
+ * WK groups of WM x WN waves; a group's waves share LDS stages and take one of WK parts of K; a wave owns
  * FM x FN blocks of 32 x 32 outputs (GLU: the first half of its FN are value rows, the second half
- * the gate rows of the same columns). Chunks of 256 K (128 bytes of every row) move to LDS by DMA, two
- * stages; chunk c of a row sits at c ^ ((row >> 1) & 7), so that fragment reads (32 rows x 16 bytes
- * per lane half) are free of bank conflicts. Scales go straight to registers.
- * One barrier a chunk (none where a group is one wave): it follows the wait for this wave's transfers and fragment reads, so
- * behind it the chunk is whole and the other stage is free.
+ * the gate rows of the same columns). Chunks of 256 K (128 bytes of every row) move to LDS by DMA, NST stages;
+ * chunk c of a row sits at c ^ ((row >> 1) & 7), so that fragment reads (32 rows x 16 bytes per lane half) are
+ * free of bank conflicts. With two stages the next chunk moves under the current one's products; with one, the CU's other
+ * workgroups fill the wait.
+ * Barriers (none where a group is one wave) follow the wait for this wave's transfers and fragment reads, so behind one the
+ * chunk is whole and, with two stages, the other stage free.
+ * What bounds it: at 8192 x 4096 x 8192 the matrix pipes' power (the fp4 MFMA from registers reaches 6.6 - 6.9
+ * PFLOP/s on random codes, 8.9 on zeros; the chunk loop 4.4, the launch with its prologue and output 3.4);
+ * at a few rounds of tiles the latency of a tile's first chunk and of its output.
  */
-template <int FM, int FN, int WM, int WN, int WK, bool GLU>
+template <int FM, int FN, int WM, int WN, int WK, int NST, bool GLU>
 __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
     constexpr int NW = WM * WN * WK, GW = WM * WN;
     constexpr int BM = 32 * FM * WM, BN = 32 * FN * WN;          /* rows of x and of w per tile */
@@ -94,8 +98,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
     constexpr bool SHARED = GW > 1;                              /* scales go through LDS */
     constexpr int SCALES = SHARED ? NR * 16 : 0;                 /* scale bytes of two chunks */
     constexpr int NS = SHARED ? NR / (64 * GW) : 1;              /* scale rows per lane */
-    static_assert(!SHARED || (NR % (64 * GW) == 0 && WK == 1), "");
-    constexpr int NST = SHARED ? 2 : 1;                          /* stages */
+    static_assert(SHARED ? NR % (64 * GW) == 0 && WK == 1 : NST == 1, "");
     constexpr int GROUP = NST * STAGE + 2 * SCALES;              /* LDS of one K group */
     __shared__ __attribute__((aligned(16))) uint8_t smem[WK * GROUP > EPI ? WK * GROUP : EPI];
     const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
@@ -150,7 +153,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
     auto put_scales = [&](int buf) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < NS; i++)
-            *reinterpret_cast<uint4 *>(smem + wk * GROUP + 2 * STAGE + buf * SCALES + (64 * (GW * i + gw) + lane) * 16) = sreg[i];
+            *reinterpret_cast<uint4 *>(smem + wk * GROUP + NST * STAGE + buf * SCALES + (64 * (GW * i + gw) + lane) * 16) = sreg[i];
     };
 
     /* a one-wave group takes its few scales straight to registers, a dword per fragment row and lane half */
@@ -228,7 +231,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
     }
     const uint32_t cx = (wm * FM * 32 + l32) * 16 + 4 * h, cw = cx + (BM + (wn * FN - wm * FM) * 32) * 16;
     auto shared_scales = [&](unsigned (&x)[FM], unsigned (&w)[FN], int buf, int sbuf) __attribute__((always_inline)) {
-        const uint8_t *C = smem + wk * GROUP + 2 * STAGE + sbuf * SCALES + buf * 8;
+        const uint8_t *C = smem + wk * GROUP + NST * STAGE + sbuf * SCALES + buf * 8;
 #pragma unroll
         for (int i = 0; i < FM; i++) x[i] = *reinterpret_cast<const unsigned *>(C + cx + i * 512);
 #pragma unroll
@@ -283,6 +286,21 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
         };
         const int np = a.nb / 16;
         int sbuf = 0;
+        if constexpr (NST == 1) {
+            if (np) load_scales(0);
+            for (int c = 0; c < 2 * np; c++) {
+                if (c > 0) turn();                               /* the stage is still being read */
+                issue(IC<0>{}, 0, c);
+                if ((c & 1) == 0) {
+                    if (c > 0) arrived();
+                    put_scales((c >> 1) & 1);
+                    if (c + 2 < 2 * np) load_scales(c + 2);
+                }
+                turn();
+                shared_scales(xa, wa, c & 1, (c >> 1) & 1);
+                compute(0, xa, wa);
+            }
+        } else {
         if (np) {
             load_scales(0);
             issue(IC<0>{}, 0, 0);
@@ -305,6 +323,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
             compute(1, xa, wa);
             sbuf ^= 1;
         }
+        }
         const int left = a.nb - 16 * np;                         /* blocks of up to two chunks */
         if (left) {
 #pragma unroll
@@ -312,13 +331,18 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
             turn();                                              /* the last pair is still being read */
             put_scales(0);
             issue(IC<1>{}, 0, 2 * np);
-            if (left > 8) issue(IC<1>{}, 1, 2 * np + 1);
+            if (NST == 2 && left > 8) issue(IC<1>{}, 1, 2 * np + 1);
             turn();
             shared_scales(xa, wa, 0, 0);
             compute(0, xa, wa);
             if (left > 8) {
+                if constexpr (NST == 1) {
+                    turn();
+                    issue(IC<1>{}, 0, 2 * np + 1);
+                    turn();
+                }
                 shared_scales(xa, wa, 1, 0);
-                compute(1, xa, wa);
+                compute(NST - 1, xa, wa);
             }
         }
     } else {
@@ -473,36 +497,51 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_rows(MxArgs a, const void *x, l
     }
 }
 
-template <int FM, int FN, int WM, int WN, int WK, bool GLU>
+template <int FM, int FN, int WM, int WN, int WK, int NST, bool GLU>
 static hipError_t launch(MxArgs a, hipStream_t s) {
     constexpr int OW = (GLU ? 16 : 32) * FN * WN;
     a.tm = (a.M + 32 * FM * WM - 1) / (32 * FM * WM);
     a.tn = (a.N + OW - 1) / OW;
     a.T = a.tm * a.tn;
-    hipLaunchKernelGGL((k_mx4_gemm<FM, FN, WM, WN, WK, GLU>), dim3((unsigned)((a.T + 7) / 8 * 8)), dim3(64 * WM * WN * WK), 0, s, a);
+    hipLaunchKernelGGL((k_mx4_gemm<FM, FN, WM, WN, WK, NST, GLU>), dim3((unsigned)((a.T + 7) / 8 * 8)), dim3(64 * WM * WN * WK), 0, s, a);
     return hipGetLastError();
 }
 
 /* Which tile: the least estimated time, in us, over one launch. A configuration takes at least the latency of one tile, and where
  * there are many tiles the time that all CUs need for them; both grow with the chunks of K, the large tiles' also
- * with the bytes of output. Fitted to M = 17 .. 8192, N = 1024 .. 8192, K = 256 .. 8192 (within 20 % there, mostly 10 %). 256 x 256
- * tiles come in rounds of one per CU. 64 x 64 and 32 x 32 tiles split K over four one-wave groups: at M = 344, K = 1024,
- * N = 4096 32 x 32 take 6.8 us, 64 x 64 6.4, 128 x 128 7.4, 256 x 256 13.8; at M = 172, K = 4096, N = 1024 5.1, 7.8, 15.0, 30.8; at
- * M = N = 8192, K = 4096 256 x 256 155 and 128 x 128 186. */
+ * with the bytes of output. Fitted to M = 17 .. 8192, N = 1024 .. 8192, K = 256 .. 8192 (within 25 % there, mostly 10 %).
+ *  t32, t64: 32 x 32 (GLU: 32 x 64) and 64 x 64, K split over four one-wave groups, several workgroups to a CU;
+ *  t128a, t128b: 128 x 128 in one stage, three workgroups to a CU, and in two stages, two to a CU, for long K and few tiles;
+ *  t256: 256 x 256 in rounds of one to a CU.
+ * Measured, in that order, us: M 344, K 1024, N 4096 6.8, 6.4, 7.5, 7.4, 13.8; M 172, K 4096, N 1024 5.1, 7.8, 18.7, 15.0, 30.8;
+ * M 2592, K 1024, N 4096 29.2, 23.5, 13.4, 15.4, 16.2; M 2592, K 4096, N 1024 25.0, 17.7, 20.5, 16.9, 31.9; M 8192, K 4096, N 8192
+ * 512, 299, 181, 189, 164. */
 template <bool GLU>
 static hipError_t pick(const MxArgs &a, hipStream_t s) {
+    constexpr int H = GLU ? 2 : 1;                               /* weight rows per column */
     const double nc = (a.nb + 7) / 8, es = a.ytype == MX_F32 ? 4 : 2;
     auto tiles = [&](int bm, int cols) { return (double)((a.M + bm - 1) / bm) * (double)((a.N + cols - 1) / cols); };
     auto most = [](double x, double y) { return x > y ? x : y; };
-    constexpr int H = GLU ? 2 : 1;                               /* weight rows per column */
-    const double kb2 = 128 * (128 / H) * es / 1024, t2 = tiles(128, 128 / H), t1 = tiles(256, 256 / H);
-    const double c9 = GLU ? most(4.4 + 0.2 * nc, 3 + tiles(32, 32) * 0.0012 * nc) : most(4.4 + 0.04 * nc, 3 + tiles(32, 32) * (0.001 + 0.00043 * nc));
-    const double c4 = most(4.0 + 0.25 * nc, 2.7 + tiles(64, 64 / H) * (0.004 + 0.00138 * nc));
-    const double c2 = most(4.4 + 0.66 * nc, 3 + t2 * (0.0053 + 0.00025 * kb2 + 0.0018 * nc));
-    const double c1 = 3 + (double)((long)(t1 + 255) / 256) * (2.7 + 0.0234 * 4 * kb2 + 2.2 * nc);
-    if (c9 <= c4 && c9 <= c2 && c9 <= c1) return launch<1, H, 1, 1, 4, GLU>(a, s);
-    if (c4 <= c2 && c4 <= c1) return launch<2, 2, 1, 1, 4, GLU>(a, s);
-    return c2 <= c1 ? launch<2, 2, 2, 2, 1, GLU>(a, s) : launch<4, 2, 2, 4, 1, GLU>(a, s);
+    const double kb = 128 * (128 / H) * es / 1024;               /* output of a 128 x 128 tile */
+    const double n128 = tiles(128, 128 / H), rounds = (double)((long)(tiles(256, 256 / H) + 255) / 256);
+    const double t32 = GLU ? most(4.4 + 0.2 * nc, 3 + tiles(32, 32) * (0.0021 + 0.00057 * nc))
+                           : most(4.4 + 0.04 * nc, 3 + tiles(32, 32) * (0.001 + 0.00043 * nc));
+    const double t64 = most(4.0 + 0.25 * nc, 2.7 + tiles(64, 64 / H) * (0.004 + 0.00138 * nc));
+    const double t128a = most(3.7 + 1.05 * nc, 3 + n128 * (0.0015 + 0.00015 * kb + 0.0023 * nc));
+    const double t128b = most(4.4 + 0.66 * nc, 3 + n128 * (0.0035 + 0.00025 * kb + 0.002 * nc));
+    const double t256 = 3 + rounds * ((nc < 2 ? 5.7 : 2.7) + 0.0234 * 4 * kb + 2.2 * nc);
+    double t = t32;
+    int which = 0;
+    const double other[4] = {t64, t128a, t128b, t256};
+    for (int i = 0; i < 4; i++)
+        if (other[i] < t) { t = other[i]; which = i + 1; }
+    switch (which) {
+    case 0: return launch<1, H, 1, 1, 4, 1, GLU>(a, s);
+    case 1: return launch<2, 2, 1, 1, 4, 1, GLU>(a, s);
+    case 2: return launch<2, 2, 2, 2, 1, 1, GLU>(a, s);
+    case 3: return launch<2, 2, 2, 2, 1, 2, GLU>(a, s);
+    default: return launch<4, 2, 2, 4, 1, 2, GLU>(a, s);
+    }
 }
 
 extern "C" hipError_t aria_k_mx4_gemm(void *y, int ytype, const uint8_t *xq, const uint8_t *xs, const uint8_t *wq,

@@ -192,7 +192,8 @@ def test_linear(hip, M, K, N, xt, yt, bias):
     assert (np.abs(got - y) <= linear_tol(y, terms, K, yt)).all(), np.abs(got - y).max()
 
 
-LARGE = [(900, 480, 1501), (900, 1000, 1500), (1500, 1024, 2050), (2592, 1056, 3500), (2700, 1111, 4090)]
+LARGE = [(900, 480, 1501), (900, 1000, 1500), (1500, 1024, 2050), (2592, 1056, 3500), (2700, 1111, 4090),
+         (1000, 2500, 2100), (4090, 2111, 4095)]
 
 
 @pytest.mark.gpu
@@ -242,7 +243,8 @@ def test_glu(hip, M, K, N, xt, yt, bias):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("M,K,N", [(260, 1000, 2050), (520, 700, 1030), (1300, 416, 2050), (2700, 416, 4090)])
+@pytest.mark.parametrize("M,K,N", [(260, 1000, 2050), (520, 700, 1030), (1300, 416, 2050), (2700, 416, 4090), (1000, 2500, 2100),
+                                   (4090, 2111, 2047)])
 @pytest.mark.parametrize("xt,yt,bias", [("f32", "f32", True), ("f16", "bf16", False)])
 def test_glu_large(hip, M, K, N, xt, yt, bias):
     test_glu(hip, M, K, N, xt, yt, bias)
