@@ -620,7 +620,7 @@ static int linear_mx4(void *dy, int ytype, const void *dx, int xtype, int64_t ld
     REQ(((uintptr_t)dy & mx4_el_mask(ytype)) == 0 && ((uintptr_t)dx & mx4_el_mask(xtype)) == 0);
     if (M == 0 || N == 0) return 0;
     ENSURE();
-    if (M <= ARIA_MX4_ROWS) {
+    if (aria_k_mx4_rows_fit(xtype, M, K, N)) {
         KCK(aria_k_mx4_rows(dy, ytype, dx, xtype, (long)ldx, dq, dscale, db, M, K, N, glu, pick(stream)), "k_mx4_rows");
         return 0;
     }

@@ -258,8 +258,8 @@ hipError_t aria_k_mx4_dequant(void *y, int ytype, const uint8_t *q, const uint8_
                               hipStream_t s);
 hipError_t aria_k_mx4_gemm(void *y, int ytype, const uint8_t *xq, const uint8_t *xs, const uint8_t *wq,
                            const uint8_t *ws, const float *bias, int M, int K, int N, int glu, hipStream_t s);
-/* the same on unpacked activations of at most ARIA_MX4_ROWS rows, in one launch */
-#define ARIA_MX4_ROWS 16
+/* the same on unpacked activations in one launch, for the few rows where that is faster (aria_k_mx4_rows_fit) */
+int aria_k_mx4_rows_fit(int xtype, int M, int K, int N);
 hipError_t aria_k_mx4_rows(void *y, int ytype, const void *x, int xtype, long ldx, const uint8_t *wq,
                            const uint8_t *ws, const float *bias, int M, int K, int N, int glu, hipStream_t s);
 

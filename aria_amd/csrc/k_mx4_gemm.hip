@@ -428,52 +428,90 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
     });
 }
 
+/* 32 values of a row, kept as loaded until they are quantised */
+template <int T>
+struct MxRaw {
+    typedef mx_t<T> v_t __attribute__((ext_vector_type(16 / sizeof(mx_t<T>))));
+    static constexpr int V = 16 / (int)sizeof(mx_t<T>), NV = 32 / V;
+    v_t v[NV];
+    /* whole blocks on 16-byte addresses */
+    __device__ __forceinline__ void load(const mx_t<T> *p) {
+#pragma unroll
+        for (int i = 0; i < NV; i++) v[i] = reinterpret_cast<const v_t *>(p)[i];
+    }
+    /* any address; values past the first n are zero */
+    __device__ __forceinline__ void load_some(const mx_t<T> *p, int n) {
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            if (V * (i + 1) <= n) {
+                __builtin_memcpy(&v[i], p + V * i, 16);
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; e++) v[i][e] = V * i + e < n ? p[V * i + e] : (mx_t<T>)0.0f;
+            }
+        }
+    }
+    __device__ __forceinline__ uint4 pack(unsigned &byte) const {
+        unsigned m = 0, w[4];
+#pragma unroll
+        for (int i = 0; i < 32; i++) m = max(m, mx_abs_bits((float)v[i / V][i % V]));
+        byte = mx_scale_byte(m);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) f[e] = (float)v[(8 * i + e) / V][(8 * i + e) % V];
+            w[i] = mx_pack8(f, byte);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+
 /*
- * Up to 16 rows: quantised by the wave that multiplies them, in the same launch. A workgroup owns 16
- * weight rows (GLU: 16 value and 16 gate rows), its NW waves take K in turn, and the 16 x 16 sums meet in LDS.
- * v_mfma_scale_f32_16x16x128: lane l holds block l / 16 of four, of row l % 16, so a lane reads 32
- * activations, finds their maximum and packs its own operand: no lane exchange. Every workgroup
- * quantises all of x, which is little beside the latency of a second launch.
+ * Few rows: quantised by the wave that multiplies them, in the same launch. A workgroup owns 16 rows and 16 weight rows (GLU: 16
+ * value and 16 gate rows), its NW waves take K in turn, and the 16 x 16 sums meet in LDS. v_mfma_scale_f32_16x16x128:
+ * lane l holds block l / 16 of four, of row l % 16, so a lane reads 32 activations, finds their maximum and packs
+ * its own operand: no lane exchange. Every workgroup quantises its rows again, which is little beside the latency
+ * of a second launch. What bounds it is latency: WHOLE (whole blocks, 16-byte rows) loads two steps ahead of their use.
  */
-template <int XT, bool GLU, int NW>
-__global__ __launch_bounds__(64 * NW) void k_mx4_rows(MxArgs a, const void *x, long ldx, int K, int xvec) {
-    constexpr int F = GLU ? 2 : 1;
+template <int XT, bool GLU, int NW, bool WHOLE>
+__global__ __launch_bounds__(64 * NW) void k_mx4_rows(MxArgs a, const void *x, long ldx, int K) {
+    constexpr int F = GLU ? 2 : 1, U = 2;
     __shared__ __attribute__((aligned(16))) float E[NW][F][16][20];
     const int lane = threadIdx.x & 63, l16 = lane & 15, kg = lane >> 4;
     const int wid = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int n0 = blockIdx.x * 16, n = min(n0 + l16, a.N - 1), steps = (a.nb + 3) / 4;
+    const int n0 = blockIdx.x * 16, n = min(n0 + l16, a.N - 1), steps = (a.nb + 3) / 4, m0 = blockIdx.y * 16;
     mx_f32x4_t acc[F];
 #pragma unroll
     for (int f = 0; f < F; f++) acc[f] = mx_f32x4_t{0, 0, 0, 0};
-    const bool row = l16 < a.M;
-    for (int s = wid; s < steps; s += NW) {
-        const int b = 4 * s + kg;
-        const bool in = b < a.nb;
-        uint4 w[F];
-        int sc[F];
+    const mx_t<XT> *xr = (const mx_t<XT> *)x + (size_t)min(m0 + l16, a.M - 1) * ldx;   /* rows past M: not stored */
+    for (int s0 = wid; s0 < steps; s0 += U * NW) {
+        MxRaw<XT> raw[U];
+        uint4 w[U][F];
+        int sc[U][F];
+        /* an absent block loads the row's last; its codes are taken as zero, its scales as one */
 #pragma unroll
-        for (int f = 0; f < F; f++) {
-            const size_t at = (size_t)(n + f * a.N) * a.nb + b;
-            w[f] = in ? ((const uint4 *)a.wq)[at] : make_uint4(0, 0, 0, 0);
-            sc[f] = in ? a.ws[at] : 127;
-        }
-        uint4 u = make_uint4(0, 0, 0, 0);
-        unsigned byte = 127;
-        if (in && row) {
-            float v[4][8];
-            unsigned m = 0;
+        for (int u = 0; u < U; u++) {
+            const int b = 4 * (s0 + u * NW) + kg, bc = min(b, a.nb - 1);
 #pragma unroll
-            for (int i = 0; i < 4; i++) mx_load<XT, 8>(x, (size_t)l16 * ldx + 32 * b + 8 * i, K - 32 * b - 8 * i, xvec, v[i]);
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int e = 0; e < 8; e++) m = max(m, mx_abs_bits(v[i][e]));
-            byte = mx_scale_byte(m);
-            u = make_uint4(mx_pack8(v[0], byte), mx_pack8(v[1], byte), mx_pack8(v[2], byte), mx_pack8(v[3], byte));
+            for (int f = 0; f < F; f++) {
+                const size_t at = (size_t)(n + f * a.N) * a.nb + bc;
+                w[u][f] = ((const uint4 *)a.wq)[at];
+                sc[u][f] = b < a.nb ? a.ws[at] : 127;
+            }
+            if constexpr (WHOLE) raw[u].load(xr + 32 * bc);
+            else raw[u].load_some(xr + 32 * bc, K - 32 * bc);
         }
 #pragma unroll
-        for (int f = 0; f < F; f++)
-            acc[f] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_op(w[f]), mx_op(u), acc[f], 4, 4, 0, sc[f], 0, (int)byte);
+        for (int u = 0; u < U; u++) {
+            const bool in = 4 * (s0 + u * NW) + kg < a.nb;
+            unsigned byte;
+            uint4 q = raw[u].pack(byte);
+            if (!in) { q = make_uint4(0, 0, 0, 0); byte = 127; }
+#pragma unroll
+            for (int f = 0; f < F; f++)
+                acc[f] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_op(w[u][f]), mx_op(q), acc[f], 4, 4, 0, sc[u][f], 0, (int)byte);
+        }
     }
 #pragma unroll
     for (int f = 0; f < F; f++)
@@ -481,7 +519,7 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_rows(MxArgs a, const void *x, l
     __syncthreads();
     for (int i = threadIdx.x; i < 256; i += 64 * NW) {
         const int m = i >> 4, c = i & 15;
-        if (m >= a.M || n0 + c >= a.N) continue;
+        if (m0 + m >= a.M || n0 + c >= a.N) continue;
         float v = 0.0f, g = 0.0f;
 #pragma unroll
         for (int w = 0; w < NW; w++) {
@@ -493,7 +531,7 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_rows(MxArgs a, const void *x, l
             if (a.bias) g += a.bias[a.N + n0 + c];
             v *= silu_f(g);
         }
-        mx_store(a.y, a.ytype, (size_t)m * a.N + n0 + c, v);
+        mx_store(a.y, a.ytype, (size_t)(m0 + m) * a.N + n0 + c, v);
     }
 }
 
@@ -554,10 +592,23 @@ extern "C" hipError_t aria_k_mx4_gemm(void *y, int ytype, const uint8_t *xq, con
 
 template <int XT, bool GLU>
 static void launch_rows(const MxArgs &a, const void *x, long ldx, int K, hipStream_t s) {
-    const int xvec = ldx % 8 == 0 && ((uintptr_t)x & 15u) == 0;
-    const dim3 grid((unsigned)((a.N + 15) / 16));
-    if (a.nb > 64) hipLaunchKernelGGL((k_mx4_rows<XT, GLU, 8>), grid, dim3(512), 0, s, a, x, ldx, K, xvec);
-    else hipLaunchKernelGGL((k_mx4_rows<XT, GLU, 4>), grid, dim3(256), 0, s, a, x, ldx, K, xvec);
+    const bool whole = K % 32 == 0 && ldx * sizeof(mx_t<XT>) % 16 == 0 && ((uintptr_t)x & 15u) == 0;
+    const dim3 grid((unsigned)((a.N + 15) / 16), (unsigned)((a.M + 15) / 16));
+    if (a.nb > 32) {   /* K past 1024 keeps eight waves busy for two steps */
+        if (whole) hipLaunchKernelGGL((k_mx4_rows<XT, GLU, 8, true>), grid, dim3(512), 0, s, a, x, ldx, K);
+        else hipLaunchKernelGGL((k_mx4_rows<XT, GLU, 8, false>), grid, dim3(512), 0, s, a, x, ldx, K);
+    } else {
+        if (whole) hipLaunchKernelGGL((k_mx4_rows<XT, GLU, 4, true>), grid, dim3(256), 0, s, a, x, ldx, K);
+        else hipLaunchKernelGGL((k_mx4_rows<XT, GLU, 4, false>), grid, dim3(256), 0, s, a, x, ldx, K);
+    }
+}
+
+/* Whether one launch of k_mx4_rows beats quantisation and product: x's bytes per workgroup bound its latency (16 fp32 rows of 4096:
+ * 11.4 us against 7.5 in two launches; fp16 7.7; one row 6.0; 16 fp16 rows of 1024: 4.2), and beyond 16 rows every
+ * 16 columns quantise them again (N 4096, K 1024: 32 rows 5.0 against 7.5, 64 rows 7.7). */
+extern "C" int aria_k_mx4_rows_fit(int xtype, int M, int K, int N) {
+    const long bytes = (long)(M < 16 ? M : 16) * K * (xtype == MX_F32 ? 4 : 2);
+    return bytes <= 96 * 1024 && (M <= 16 || (K <= 1024 && ((M + 15L) / 16) * ((N + 15L) / 16) <= 640));
 }
 
 extern "C" hipError_t aria_k_mx4_rows(void *y, int ytype, const void *x, int xtype, long ldx, const uint8_t *wq,
