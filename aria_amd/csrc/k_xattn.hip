@@ -74,16 +74,19 @@ __host__ __device__ constexpr int xa_tile(int DP) { return DP == 64 ? 64 : 32; }
 /* floats of one partial result */
 __host__ __device__ constexpr int xa_part(int DP) { return 32 * DP + 64; }
 
-/* QW waves of 32 rows share every tile (KS = 1), or KS waves take the tiles in turn, each in LDS of its own and without
- * barriers, and join their results at the end (QW = 1). The former hold two stages, the next tile moving
- * under the current one's products. The latter are bound by the keys' bytes and hold one: two workgroups then
- * fit a CU, and one wave's transfer runs beside another's products (cross_one's shape, 16 x 4 key heads x
- * up to 8192 keys of 128: 56 us with two stages and one workgroup, 44 with one and two, the join included). */
+/* KS slices of the keys, each of QW waves of 32 rows that share its tiles; the slices' results are joined at the end. With
+ * QW > 1 there are two stages, the next tile moving under the current one's products. With QW = 1 a wave works by itself,
+ * without barriers, is bound by the keys' bytes, and has one stage: two workgroups then fit a CU, and one wave's
+ * transfer runs beside another's products (16 x 4 key heads x up to 8192 keys of 128: 56 us with two stages and
+ * one workgroup, 44 with one and two, the join included).
+ * What bounds it: with many rows the VALU, 71 % busy beside the MFMAs' 45 % at 4 x 16 x 4096 rows x 2048 keys of 64 (0.87
+ * PFLOP/s; an exponential, a fused multiply-add, half a maximum, half a conversion and half a dot product per score);
+ * with a single row the keys' bytes (4.5 TB/s); at a few tiles a wave the latency of one tile, about 1 us. */
 template <typename T, int DP, int KT, int QW, int KS>
 __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
-    static_assert((QW == 1 || KS == 1) && (DP == 64 || DP == 128) && (KT == 64 || KT == 32), "");
+    static_assert( (DP == 64 || DP == 128) && (KT == 64 || KT == 32), "");
     constexpr int NW = QW * KS;
-    constexpr int NST = KS == 1 ? 2 : 1;            /* LDS stages */
+    constexpr int NST = QW > 1 ? 2 : 1;             /* LDS stages */
     constexpr int CPR = DP / 8;                     /* 16-byte chunks per key row */
     constexpr uint64_t ALL = KT == 64 ? ~0ull : 0xFFFFFFFFull;   /* every key of a tile */
     constexpr int SLOTS = KT * CPR;                 /* per tile and operand */
@@ -92,7 +95,7 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
     constexpr int ES = DP + 4;                      /* floats per staged output row */
     constexpr int KB = KT / 32, DT = DP / 32, DS = DP / 16;
     constexpr int STAGE = 2 * TB * KS;              /* K and V of every slice */
-    constexpr int EPI = NW * 32 * ES * 4 + KS * 64 * 4;
+    constexpr int EPI = NW * 32 * ES * 4 + NW * 64 * 4;
     __shared__ __attribute__((aligned(16))) uint8_t smem[NST * STAGE > EPI ? NST * STAGE : EPI];
     typedef typename Xa<T>::v8 v8;
     typedef typename Xa<T>::v2 v2;
@@ -100,7 +103,7 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
 
     const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
     const int wid = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int qw = KS == 1 ? wid : 0, ks = KS == 1 ? 0 : wid;
+    const int qw = wid % QW, ks = wid / QW;
 
     /* row blocks of one key head run on one XCD, whose L2 then holds its K and V; batches alternate
      * fastest so that unequal lengths spread over the XCDs */
@@ -278,7 +281,7 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
      * the transfers, so this is also its fence */
     auto drain = []() __attribute__((always_inline)) { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); };
     auto meet = [&]() __attribute__((always_inline)) {
-        if constexpr (KS == 1) __syncthreads();
+        if constexpr (QW > 1) __syncthreads();
     };
 
     uint64_t cur = to_bits(t0, mask_byte(t0));
@@ -302,9 +305,9 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
             cur = nxt;
             nxt = to_bits(i + 2, byte);
         };
-        for (int i = t0; i < t1; i += 2) {
+        for (int i = t0; i < t0 + sp; i += 2) {     /* every slice meets as often; its tiles end at t1 */
             turn(IC<0>{}, i);
-            if (i + 1 >= t1) break;
+            if (i + 1 >= t0 + sp) break;
             turn(IC<1>{}, i + 1);
         }
     } else {
@@ -321,23 +324,22 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
     /* join: lanes l and l ^ 32 hold half of a row's sum each */
     l += xor32_f32(l, lane);
     float *E = (float *)smem + wid * 32 * ES;
-    float *ML = (float *)smem + NW * 32 * ES;       /* KS x (32 references, 32 sums) */
-    if (KS > 1) __syncthreads();                     /* slices still reading their stages */
+    float *ML = (float *)smem + NW * 32 * ES;       /* per wave 32 references, 32 sums */
+    if (QW == 1) __syncthreads();                    /* slices still reading their stages */
 #pragma unroll
     for (int d = 0; d < DT; d++)
 #pragma unroll
         for (int r = 0; r < 4; r++)
             *reinterpret_cast<float4 *>(E + l32 * ES + 32 * d + 8 * r + 4 * g) =
                 make_float4(o[d][4 * r], o[d][4 * r + 1], o[d][4 * r + 2], o[d][4 * r + 3]);
-    if (KS > 1 && g == 0) { ML[ks * 64 + l32] = ref; ML[ks * 64 + 32 + l32] = l; }
+    if (KS > 1 && g == 0) { ML[wid * 64 + l32] = ref; ML[wid * 64 + 32 + l32] = l; }
     __syncthreads();
 
-    /* a group of CPR lanes finishes one row, 8 dims per lane; the NW waves take rows in turn
-     * (KS > 1: all of them the workgroup's one block of 32) */
+    /* a group of CPR lanes finishes one row, 8 dims per lane; the KS waves of a block of rows take them in turn */
     constexpr int RPW = 64 / CPR;                    /* rows per wave at once */
     const int c8 = 8 * (lane % CPR);
 #pragma unroll 1
-    for (int i = KS == 1 ? 0 : wid; i < 32 / RPW; i += KS) {
+    for (int i = ks; i < 32 / RPW; i += KS) {
         const int q = i * RPW + lane / CPR;          /* row within the block */
         float v[8], rs, rm;
         if constexpr (KS == 1) {
@@ -349,15 +351,15 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
         } else {
             rm = XA_MIN;
 #pragma unroll
-            for (int w = 0; w < KS; w++) rm = fmaxf(rm, ML[w * 64 + q]);
+            for (int w = 0; w < KS; w++) rm = fmaxf(rm, ML[(w * QW + qw) * 64 + q]);
             rs = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; j++) v[j] = 0.0f;
 #pragma unroll
             for (int w = 0; w < KS; w++) {
-                const float f = __builtin_amdgcn_exp2f(ML[w * 64 + q] - rm);
-                rs = __builtin_fmaf(f, ML[w * 64 + 32 + q], rs);
-                const float *e = (const float *)smem + (w * 32 + q) * ES + c8;
+                const float f = __builtin_amdgcn_exp2f(ML[(w * QW + qw) * 64 + q] - rm);
+                rs = __builtin_fmaf(f, ML[(w * QW + qw) * 64 + 32 + q], rs);
+                const float *e = (const float *)smem + ((w * QW + qw) * 32 + q) * ES + c8;
 #pragma unroll
                 for (int j = 0; j < 8; j++) v[j] = __builtin_fmaf(f, e[j], v[j]);
             }
@@ -431,16 +433,22 @@ __global__ __launch_bounds__(64) void k_xattn_join(XaArgs x) {
     }
 }
 
-/* How a call runs: KS waves per 32 rows (qw 1) where blocks of 128 rows would leave CUs idle, else qw blocks of 32 rows a
- * workgroup: 4, or, where four rounds of 256 rows fill the CUs, 8 (4 x 16 heads x 4096 rows x 2048 keys of 64: 166 us with 4, 158
- * with 8; of 128, where 8 waves' registers fill the CU: 164 and 168). ns splits of the keys. */
-struct XaPlan { int qw, DP, nrb, T, ns, per; };
+/* How a call runs: qw blocks of 32 rows and ks slices of the keys to a workgroup, ns splits of the keys across workgroups.
+ *  qw 1, ks 4: up to 32 rows a key head, and where blocks of 128 rows would leave CUs idle, which every block of 32 rows then has to fill by reading the keys
+ *    for itself (16 heads x 172 rows x 257 keys of 64: 6.2 us, 8.5 with qw 4; x 710 rows x 1024 keys: 25.2 and 14.5);
+ *  qw 4, ks 2: up to a workgroup per CU, and up to 700 of them over long keys of 64 (2 x 16 x 710 rows x 257 keys: 8.9 us, 9.5 with
+ *    one slice; 2 x 16 x 1296 x 1296: 29.1 and 31.4, of 128 54.2 and 49.4);
+ *  qw 4, ks 1; and qw 8 where four rounds of 256 rows fill the CUs (4 x 16 x 4096 x 2048 of 64: 166 us with 4, 158 with 8; of 128,
+ *    where 8 waves' registers fill the CU: 164 and 168). */
+struct XaPlan { int qw, ks, DP, nrb, T, ns, per; };
 static XaPlan xa_plan(const aria_k_xattn *a) {
     XaPlan p;
     const long long R = (long long)a->Nq * (a->H / a->Hkv), bh = (long long)a->B * a->Hkv;
     auto tiles = [&](int qw) { return bh * ((R + 32 * qw - 1) / (32 * qw)); };
     p.DP = a->D <= 64 ? 64 : 128;
-    p.qw = p.DP == 64 && tiles(8) >= 1024 ? 8 : tiles(4) >= 256 ? 4 : 1;
+    const long long w4 = tiles(4);
+    p.qw = R <= 32 || w4 < 64 || (w4 < 128 && a->Nk <= 512) ? 1 : p.DP == 64 && tiles(8) >= 1024 ? 8 : 4;
+    p.ks = p.qw == 1 ? 4 : p.qw == 4 && (w4 < 300 || (w4 < 700 && p.DP == 64 && a->Nk >= 1024)) ? 2 : 1;
     p.T = (int)tiles(p.qw);
     p.nrb = (int)(p.T / bh);
     p.ns = 1;
@@ -472,6 +480,9 @@ static hipError_t xa_launch(const XaPlan &p, const XaArgs &x, hipStream_t s) {
         }
     } else if (p.qw == 8) {
         hipLaunchKernelGGL((k_xattn<T, 64, 64, 8, 1>), grid, dim3(512), 0, s, x);
+    } else if (p.ks == 2) {
+        if (p.DP == 64) hipLaunchKernelGGL((k_xattn<T, 64, 64, 4, 2>), grid, dim3(512), 0, s, x);
+        else hipLaunchKernelGGL((k_xattn<T, 128, 64, 4, 2>), grid, dim3(512), 0, s, x);
     } else {
         if (p.DP == 64) hipLaunchKernelGGL((k_xattn<T, 64, 64, 4, 1>), grid, dim3(256), 0, s, x);
         else hipLaunchKernelGGL((k_xattn<T, 128, 64, 4, 1>), grid, dim3(256), 0, s, x);

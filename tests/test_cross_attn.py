@@ -147,6 +147,19 @@ def test_full(hip, t, B, H, Hkv, Nq, Nk, D):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("B,H,Hkv,Nq,Nk,D", [(2, 4, 4, 2000, 130, 64), (1, 16, 8, 1100, 600, 64), (3, 16, 16, 1000, 300, 64),
+                                             (2, 8, 8, 1025, 1090, 128), (3, 16, 16, 1000, 200, 72), (8, 16, 16, 2050, 100, 64),
+                                             (1, 8, 2, 700, 1100, 128)])
+def test_many_rows(hip, t, B, H, Hkv, Nq, Nk, D):
+    """Enough rows for every form of workgroup: two slices of the keys, one, and eight waves; ragged and masked."""
+    check(hip, t, B, H, Hkv, Nq, Nk, D, seed=Nq + Nk)
+    lens = [Nk - 1, Nk // 3, 0, Nk, 1, 64, 65, 70][:B]
+    mask = (rng(Nq).random((B, Nk)) < 0.6).astype(np.uint8)
+    check(hip, t, B, H, Hkv, Nq, Nk, D, seed=Nq, kv_len=lens, mask=mask, layout="tokens")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", ["f16", "bf16"])
 @pytest.mark.parametrize("Nq,Nk,D", [(1, 200, 64), (40, 200, 128), (150, 500, 64), (3, 3000, 128)])
 def test_lengths_and_masks(hip, t, Nq, Nk, D):
     """Every length from none over one tile's corners to all; a mask beside it; all masked away."""
