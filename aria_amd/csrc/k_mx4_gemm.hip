@@ -71,6 +71,7 @@ __device__ __forceinline__ uint32_t fresh_s(uint32_t v) {
     asm volatile("" : "+s"(v));
     return v;
 }
+
 /*
  * WK groups of WM x WN waves; a group's waves share LDS stages and take one of WK parts of K; a wave owns
  * FM x FN blocks of 32 x 32 outputs (GLU: the first half of its FN are value rows, the second half
@@ -136,8 +137,9 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
     const size_t gate = (size_t)a.N * rb;                        /* from a value row to its gate row */
     const uint32_t sb = (uint32_t)(uintptr_t)smem + wk * GROUP;
 
-    /* SHARED: scales of two chunks at a time: 16 bytes of a row per lane (a load of one dword per fragment row and lane half would keep the
-     * address unit busy for longer than the multiplications take), through registers to LDS */
+    /* SHARED: scales of two chunks at a time, 16 bytes of a row per lane, through registers to LDS. (A dword per fragment row
+     * and lane half, straight to registers, kept the address unit busy for longer than the products took: 200 us
+     * against 155 at 8192 x 4096 x 8192) */
     const uint8_t *srow[NS];
 #pragma unroll
     for (int i = 0; i < NS; i++) {
@@ -277,8 +279,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
      * them, and with them for every later transfer, where they are used */
     unsigned xa[FM], wa[FN];
     if constexpr (SHARED) {
-        /* Whole pairs of chunks. Behind a pair's first turn() its scales are in LDS and those of the next pair are
-         * requested; they are stored behind its second turn(), when no wave reads the pair before any more */
+        /* Whole pairs of chunks. Behind the turn() before a pair's first product its scales are in LDS and those of the next
+         * pair are requested; they are stored behind a later turn(), into the half that no wave reads any more */
         auto arrived = [&]() __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < NS; i++)
@@ -301,28 +303,28 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
                 compute(0, xa, wa);
             }
         } else {
-        if (np) {
-            load_scales(0);
-            issue(IC<0>{}, 0, 0);
-            put_scales(0);
-        }
-        for (int p = 0; p < np; p++) {
-            turn();
-            issue(IC<0>{}, 1, 2 * p + 1);
-            const bool more = p + 1 < np;
-            if (more) load_scales(2 * p + 2);
-            shared_scales(xa, wa, 0, sbuf);
-            compute(0, xa, wa);
-            turn();
-            if (more) {
-                arrived();
-                issue(IC<0>{}, 0, 2 * p + 2);
-                put_scales(sbuf ^ 1);
+            if (np) {
+                load_scales(0);
+                issue(IC<0>{}, 0, 0);
+                put_scales(0);
             }
-            shared_scales(xa, wa, 1, sbuf);
-            compute(1, xa, wa);
-            sbuf ^= 1;
-        }
+            for (int p = 0; p < np; p++) {
+                turn();
+                issue(IC<0>{}, 1, 2 * p + 1);
+                const bool more = p + 1 < np;
+                if (more) load_scales(2 * p + 2);
+                shared_scales(xa, wa, 0, sbuf);
+                compute(0, xa, wa);
+                turn();
+                if (more) {
+                    arrived();
+                    issue(IC<0>{}, 0, 2 * p + 2);
+                    put_scales(sbuf ^ 1);
+                }
+                shared_scales(xa, wa, 1, sbuf);
+                compute(1, xa, wa);
+                sbuf ^= 1;
+            }
         }
         const int left = a.nb - 16 * np;                         /* blocks of up to two chunks */
         if (left) {

@@ -228,9 +228,10 @@ int aria_hip_attention_f16(float *out, const float *q, const float *k, const flo
  * not valid may hold anything (Inf and NaN included): they do not reach the result, but all Nk
  * rows must be readable memory. type: 1 = fp16, 2 = bf16 (aria_dtype's values) for q, k, v and
  * out; out_f32 != 0 writes fp32. D: a multiple of 8 up to 128. H a multiple of Hkv. B * H at most
- * 2^20, B * H * Nq and Nk at most 2^30.
+ * 2^20, B * H * Nq and Nk at most 2^30. scale: positive and finite.
  * Strides count elements and are multiples of 8, not negative, pointers are 16-byte aligned (for
- * an fp32 out too); batch / head / token strides of q, k and v may be 0 (broadcast). Probabilities
+ * an fp32 out too); batch / head / token strides of q, k and v may be 0 (broadcast); rows of out lie
+ * apart from each other and from every input. Probabilities
  * are rounded to the type before they multiply v; sums and softmax statistics are fp32.
  * dws: aria_hip_cross_attention_ws_bytes(a) bytes (0: may be NULL), 256-byte aligned, not shared
  * by calls that may run at the same time. No counterpart in the reference, whose attention takes
@@ -262,7 +263,8 @@ int aria_hip_cross_attention_f16(float *out, const float *q, const float *k, con
  * x / 2^(byte - 127) to nearest, ties to the even code, saturating at 6, the sign of zero kept. A
  * block that holds an Inf or a NaN gets byte 255 and codes 0: it stands for NaN.
  * Element types of activations and outputs are aria_dtype's values: 0 fp32, 1 fp16, 2 bf16;
- * ldx: elements between rows of x (at least K). K at most 2^24, N (inner) at most 2^26. */
+ * ldx: elements between rows of x (at least K). K at most 2^24, N (inner) at most 2^26. Outputs and
+ * workspaces overlap no input. */
 int aria_hip_mx4_quant_dev(uint8_t *dq, uint8_t *dscale, const void *dx, int xtype, int rows, int K, int64_t ldx,
                            void *stream);
 /* y [rows, K] from packed rows, rounded to ytype (fp32 holds every value) */

@@ -46,7 +46,8 @@ def test_refusals():
     for kw in (dict(type=0), dict(type=3), dict(D=4), dict(D=12), dict(D=136), dict(D=0), dict(H=3), dict(Hkv=0), dict(H=0),
                dict(Nq=-1), dict(Nk=-1), dict(B=-1), dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(q=p + 2),
                dict(out=p + 8), dict(kv_len=p + 2), dict(k_token=60), dict(v_batch=-8), dict(o_token=12), dict(q_head=4),
-               dict(Nq=1 << 30), dict(mask=p, mask_stride=-1)):
+               dict(Nq=1 << 30), dict(mask=p, mask_stride=-1), dict(scale=0.0), dict(scale=-0.1), dict(scale=float("nan")),
+               dict(scale=float("inf"))):
         rc, ws = call(**kw)
         assert rc == -1 and ws == 0, kw
         assert "invalid argument" in aria_amd.last_error()
