@@ -15,7 +15,9 @@
  *
  * K and V tiles arrive by LDS DMA, two stages. Slots of keys that are not valid, and of dims past D, are
  * filled from 16 bytes of zeros: whatever lies in masked places (NaN, Inf, memory behind the last
- * state) never enters LDS. Scores of such keys are set to -inf before the maximum.
+ * state) never enters LDS. In a tile that has such keys one more product per 32 keys, of -inf at theirs and a column of ones,
+ * adds -inf to their scores (0 before): 2 MFMAs in place of 32 selects on the busier VALU (4 x 16 x 4096 rows x up to
+ * 2048 masked keys of 64: 109 us, 118 with selects).
  *
  * The maximum is a lazy reference: it moves only when a tile exceeds it by 2^8, which leaves O / l
  * unchanged. It starts finite (below any score of 16-bit operands that a softmax can tell apart), so
@@ -39,6 +41,11 @@ template <typename T> struct Xa;
 template <> struct Xa<_Float16> {
     typedef _Float16 v8 __attribute__((ext_vector_type(8)));
     typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+    static constexpr unsigned ONE = 0x3C00u, NINF = 0xFC00u;
+    static __device__ __forceinline__ xa_f32x16_t mfma8(uint2 a, uint2 b, xa_f32x16_t c) {
+        typedef _Float16 v4 __attribute__((ext_vector_type(4)));
+        return __builtin_amdgcn_mfma_f32_32x32x8f16(__builtin_bit_cast(v4, a), __builtin_bit_cast(v4, b), c, 0, 0, 0);
+    }
     static __device__ __forceinline__ xa_f32x16_t mfma(v8 a, v8 b, xa_f32x16_t c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
     }
@@ -47,6 +54,10 @@ template <> struct Xa<_Float16> {
 template <> struct Xa<__bf16> {
     typedef __bf16 v8 __attribute__((ext_vector_type(8)));
     typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+    static constexpr unsigned ONE = 0x3F80u, NINF = 0xFF80u;
+    static __device__ __forceinline__ xa_f32x16_t mfma8(uint2 a, uint2 b, xa_f32x16_t c) {
+        return __builtin_amdgcn_mfma_f32_32x32x8bf16_1k(__builtin_bit_cast(xa_i16x4_t, a), __builtin_bit_cast(xa_i16x4_t, b), c, 0, 0, 0);
+    }
     static __device__ __forceinline__ xa_f32x16_t mfma(v8 a, v8 b, xa_f32x16_t c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
     }
@@ -212,6 +223,7 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
         }
     }
 
+    const unsigned ninf = g ? 0u : Xa<T>::NINF;     /* element 0 of lanes 0 .. 31, whose keys are their numbers */
     auto tile = [&](int buf, uint64_t bits) __attribute__((always_inline)) {
         const uint8_t *K = smem + buf * STAGE + ks * 2 * TB, *V = K + TB;
         xa_f32x16_t s[KB];
@@ -224,25 +236,19 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
 #pragma unroll
             for (int kb = 0; kb < KB; kb++)
                 s[kb] = Xa<T>::mfma(*reinterpret_cast<const v8 *>(K + koff[i] + kb * 32 * CPR * 16), qf[i], s[kb]);
-        if (bits != ALL) {
-            const float ninf = -INFINITY;
+        if (bits != ALL) {   /* one more product adds -inf (a 16-bit value) times 1 to the scores of the other keys */
 #pragma unroll
             for (int kb = 0; kb < KB; kb++) {
-                const unsigned w = (unsigned)(bits >> (32 * kb));
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const int k0 = 8 * (r >> 2) + (r & 3);   /* lanes 0..31; lanes 32..63 hold key k0 + 4 */
-                    const unsigned lo = 0u - ((w >> k0) & 1u), hi = 0u - ((w >> (k0 + 4)) & 1u);
-                    const uint64_t m = ((uint64_t)hi << 32) | lo;
-                    asm("v_cndmask_b32 %0, %1, %2, %3" : "=v"(s[kb][r]) : "v"(ninf), "v"(s[kb][r]), "s"(m));
-                }
+                const unsigned w = ~(unsigned)(bits >> (32 * kb)) >> l32;
+                s[kb] = Xa<T>::mfma8(make_uint2(0u - (w & 1u) & ninf, 0), make_uint2(Xa<T>::ONE, 0), s[kb]);
             }
         }
         float mt = s[0][0];
 #pragma unroll
         for (int i = 1; i + 1 < 16 * KB; i += 2) mt = xa_max3(mt, s[i >> 4][i & 15], s[(i + 1) >> 4][(i + 1) & 15]);
-        mt = fmaxf(mt, s[KB - 1][15]);
-        mt = fmaxf(mt, xor32_f32(mt, lane)) * x.scale_log2;
+        mt = xa_max3(mt, s[KB - 1][15], s[KB - 1][15]);
+        const float mo = xor32_f32(mt, lane);
+        mt = xa_max3(mt, mo, mo) * x.scale_log2;
         if (__ballot(mt > ref + XA_SLACK)) {
             asm volatile("" ::: "memory");   /* a branch, not 16 DT predicated multiplies */
             const float m2 = fmaxf(ref, mt), al = __builtin_amdgcn_exp2f(ref - m2);
