@@ -32,25 +32,27 @@ __device__ __forceinline__ uint4 mx_scale_end(const uint8_t *row, int b, int nb)
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-/* V results of one row from column n on: four fp32 or eight 16-bit values */
+/* V results of one row from column n on: four fp32 or eight 16-bit values. Non-temporal: they are not read here, and in
+ * the L2s they would take the operands' place (2592 x 1024 x 4096 to fp32 18.3 us, 15.1 so; 8192 x 1024 x 8192 108 and 82) */
 template <int V>
 __device__ __forceinline__ void mx_store_row(const MxArgs &a, int m, int n, const float (&v)[V]) {
     const size_t at = (size_t)m * a.N + n;
     if (a.vec && n + V <= a.N) {
         if constexpr (V == 4) {
-            *reinterpret_cast<float4 *>((float *)a.y + at) = make_float4(v[0], v[1], v[2], v[3]);
+            typedef float v4_t __attribute__((ext_vector_type(4)));
+            __builtin_nontemporal_store(v4_t{v[0], v[1], v[2], v[3]}, reinterpret_cast<v4_t *>((float *)a.y + at));
         } else if (a.ytype == MX_F16) {
             typedef _Float16 v8_t __attribute__((ext_vector_type(8)));
             v8_t o;
 #pragma unroll
             for (int i = 0; i < 8; i++) o[i] = (_Float16)v[i];
-            *reinterpret_cast<v8_t *>((_Float16 *)a.y + at) = o;
+            __builtin_nontemporal_store(o, reinterpret_cast<v8_t *>((_Float16 *)a.y + at));
         } else {
             typedef __bf16 v8_t __attribute__((ext_vector_type(8)));
             v8_t o;
 #pragma unroll
             for (int i = 0; i < 8; i++) o[i] = (__bf16)v[i];
-            *reinterpret_cast<v8_t *>((__bf16 *)a.y + at) = o;
+            __builtin_nontemporal_store(o, reinterpret_cast<v8_t *>((__bf16 *)a.y + at));
         }
     } else {
 #pragma unroll
@@ -553,9 +555,9 @@ static hipError_t launch(MxArgs a, hipStream_t s) {
  *  t32, t64: 32 x 32 (GLU: 32 x 64) and 64 x 64, K split over four one-wave groups, several workgroups to a CU;
  *  t128a, t128b: 128 x 128 in one stage, three workgroups to a CU, and in two stages, two to a CU, for long K and few tiles;
  *  t256: 256 x 256 in rounds of one to a CU.
- * Measured, in that order, us: M 344, K 1024, N 4096 6.8, 6.4, 7.5, 7.4, 13.8; M 172, K 4096, N 1024 5.1, 7.8, 18.7, 15.0, 30.8;
- * M 2592, K 1024, N 4096 29.2, 23.5, 13.4, 15.4, 16.2; M 2592, K 4096, N 1024 25.0, 17.7, 20.5, 16.9, 31.9; M 8192, K 4096, N 8192
- * 512, 299, 181, 189, 164. */
+ * Measured, in that order, us: M 344, K 1024, N 4096 6.5, 6.2, 7.3, 7.1, 13.2; M 172, K 4096, N 1024 4.9, 7.5, 15.7, 14.7, 29.8;
+ * M 2592, K 1024, N 4096 26.3, 23.4, 12.1, 14.5, 14.1; M 2592, K 4096, N 1024 23.7, 17.3, 20.0, 16.4, 31.7; M 8192, K 4096, N 8192
+ * 503, 288, 170, 182, 153. */
 template <bool GLU>
 static hipError_t pick(const MxArgs &a, hipStream_t s) {
     constexpr int H = GLU ? 2 : 1;                               /* weight rows per column */
@@ -564,12 +566,15 @@ static hipError_t pick(const MxArgs &a, hipStream_t s) {
     auto most = [](double x, double y) { return x > y ? x : y; };
     const double kb = 128 * (128 / H) * es / 1024;               /* output of a 128 x 128 tile */
     const double n128 = tiles(128, 128 / H), rounds = (double)((long)(tiles(256, 256 / H) + 255) / 256);
-    const double t32 = GLU ? most(4.4 + 0.2 * nc, 3 + tiles(32, 32) * (0.0021 + 0.00057 * nc))
+    const double t32 = GLU ? most(4.4 + 0.2 * nc, 3 + tiles(32, 32) * (0.0006 + 0.00083 * nc))
                            : most(4.4 + 0.04 * nc, 3 + tiles(32, 32) * (0.001 + 0.00043 * nc));
     const double t64 = most(4.0 + 0.25 * nc, 2.7 + tiles(64, 64 / H) * (0.004 + 0.00138 * nc));
-    const double t128a = most(3.7 + 1.05 * nc, 3 + n128 * (0.0015 + 0.00015 * kb + 0.0023 * nc));
-    const double t128b = most(4.4 + 0.66 * nc, 3 + n128 * (0.0035 + 0.00025 * kb + 0.002 * nc));
-    const double t256 = 3 + rounds * ((nc < 2 ? 5.7 : 2.7) + 0.0234 * 4 * kb + 2.2 * nc);
+    auto half = [&](double at_once) {                            /* past one round, the last one counts half of what it is short of */
+        return n128 <= at_once ? n128 : (n128 + at_once * (double)(long)((n128 + at_once - 1) / at_once)) / 2;
+    };
+    const double t128a = most(3.7 + 1.05 * nc, 3 + half(768) * (0.002 + 0.000075 * kb + 0.0023 * nc));
+    const double t128b = most(4.4 + 0.66 * nc, 3 + half(512) * (0.0024 + 0.000075 * kb + 0.0025 * nc));
+    const double t256 = 3 + rounds * ((nc < 2 ? 2.4 : -0.6) + 0.16 * kb + 2.02 * nc);
     double t = t32;
     int which = 0;
     const double other[4] = {t64, t128a, t128b, t256};

@@ -90,7 +90,7 @@ __host__ __device__ constexpr int xa_part(int DP) { return 32 * DP + 64; }
  * without barriers, is bound by the keys' bytes, and has one stage: two workgroups then fit a CU, and one wave's
  * transfer runs beside another's products (16 x 4 key heads x up to 8192 keys of 128: 56 us with two stages and
  * one workgroup, 44 with one and two, the join included).
- * What bounds it: with many rows the VALU, 71 % busy beside the MFMAs' 45 % at 4 x 16 x 4096 rows x 2048 keys of 64 (0.87
+ * What bounds it: with many rows the VALU, 71 % busy beside the MFMAs' 45 % at 4 x 16 x 4096 rows x 2048 keys of 64 (0.88
  * PFLOP/s; an exponential, a fused multiply-add, half a maximum, half a conversion and half a dot product per score);
  * with a single row the keys' bytes (4.5 TB/s); at a few tiles a wave the latency of one tile, about 1 us. */
 template <typename T, int DP, int KT, int QW, int KS>
@@ -381,15 +381,17 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
         }
         const float inv = rs > 0.0f ? 1.0f / rs : 0.0f;
         const long long at = b * a.o_batch + (hk * x.G + orow % x.G) * a.o_head + (orow / x.G) * a.o_token + c8;
+        /* non-temporal: the L2s keep keys and values (2 x 16 x 1296 rows x up to 257 keys 12.2 us, 11.9 so) */
         if (a.out_f32) {
-            float *y = (float *)a.out + at;
-            *reinterpret_cast<float4 *>(y) = make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-            *reinterpret_cast<float4 *>(y + 4) = make_float4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
+            typedef float f4_t __attribute__((ext_vector_type(4)));
+            f4_t *y = reinterpret_cast<f4_t *>((float *)a.out + at);
+            __builtin_nontemporal_store(f4_t{v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv}, y);
+            __builtin_nontemporal_store(f4_t{v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv}, y + 1);
         } else {
             v8 y;
 #pragma unroll
             for (int j = 0; j < 8; j++) y[j] = (T)(v[j] * inv);
-            *reinterpret_cast<v8 *>((T *)a.out + at) = y;
+            __builtin_nontemporal_store(y, reinterpret_cast<v8 *>((T *)a.out + at));
         }
     }
 }
