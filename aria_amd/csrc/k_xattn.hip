@@ -13,7 +13,7 @@
  * operand comes from key-major LDS by the transpose read in the same key order. Lanes l and l ^ 32
  * share a row, so a maximum needs one exchange.
  *
- * K and V tiles arrive by LDS DMA, two stages. Slots of keys that are not valid, and of dims past D, are
+ * K and V tiles arrive by LDS DMA. Slots of keys that are not valid, and of dims past D, are
  * filled from 16 bytes of zeros: whatever lies in masked places (NaN, Inf, memory behind the last
  * state) never enters LDS. In a tile that has such keys one more product per 32 keys, of -inf at theirs and a column of ones,
  * adds -inf to their scores (0 before): 2 MFMAs in place of 32 selects on the busier VALU (4 x 16 x 4096 rows x up to
@@ -26,6 +26,8 @@
  */
 #include "aria_dev.h"
 #include "aria_hip_kernels.h"
+
+#include <algorithm>
 
 typedef float xa_f32x16_t __attribute__((ext_vector_type(16)));
 typedef short xa_i16x4_t __attribute__((ext_vector_type(4)));
@@ -87,12 +89,12 @@ __host__ __device__ constexpr int xa_part(int DP) { return 32 * DP + 64; }
 
 /* KS slices of the keys, each of QW waves of 32 rows that share its tiles; the slices' results are joined at the end. With
  * QW > 1 there are two stages, the next tile moving under the current one's products. With QW = 1 a wave works by itself,
- * without barriers, is bound by the keys' bytes, and has one stage: two workgroups then fit a CU, and one wave's
- * transfer runs beside another's products (16 x 4 key heads x up to 8192 keys of 128: 56 us with two stages and
- * one workgroup, 44 with one and two, the join included).
+ * without barriers, is bound by the keys' bytes, and has one stage, so that two workgroups fit a CU (16 x 4 key heads x up to
+ * 8192 keys of 128: 56 us with two stages and one workgroup, 45 with one and two, the join included); the next tile's keys
+ * then move while this one's values are added, its values while the scores are made (45 to 42).
  * What bounds it: with many rows the VALU, 71 % busy beside the MFMAs' 45 % at 4 x 16 x 4096 rows x 2048 keys of 64 (0.88
  * PFLOP/s; an exponential, a fused multiply-add, half a maximum, half a conversion and half a dot product per score);
- * with a single row the keys' bytes (4.5 TB/s); at a few tiles a wave the latency of one tile, about 1 us. */
+ * with a single row the keys' bytes (4.9 TB/s without the join); at a few tiles a wave the latency of one tile, about 1 us. */
 template <typename T, int DP, int KT, int QW, int KS>
 __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
     static_assert( (DP == 64 || DP == 128) && (KT == 64 || KT == 32), "");
@@ -166,25 +168,27 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
         koff_g[i] = (unsigned)(r * a.k_token + 8 * ck) * 2;
         voff_g[i] = (unsigned)(r * a.v_token + 8 * cv) * 2;
     }
-    auto dma = [&](int buf, uint64_t bits) __attribute__((always_inline)) {
-        const uint32_t S = (uint32_t)(uintptr_t)smem + buf * STAGE + ks * 2 * TB + 1024 * qw;
+    auto dma_one = [&](auto IS_V, int buf, uint64_t bits) __attribute__((always_inline)) {
+        constexpr bool is_v = decltype(IS_V)::value != 0;
+        const uint32_t S = (uint32_t)(uintptr_t)smem + buf * STAGE + ks * 2 * TB + (is_v ? TB : 0) + 1024 * qw;
+        const char *&base = is_v ? vb : kb;
         if (x.plain && bits == ALL) {
 #pragma unroll
-            for (int i = 0; i < ND; i++) {
-                dma16_s(kb, koff_g[i], S + 1024 * QW * i);
-                dma16_s(vb, voff_g[i], S + TB + 1024 * QW * i);
-            }
+            for (int i = 0; i < ND; i++) dma16_s(base, is_v ? voff_g[i] : koff_g[i], S + 1024 * QW * i);
         } else {
             for (int i = 0; i < ND; i++) {
                 int r, ck, cv;
                 slot(i, r, ck, cv);
-                const bool ok = (bits >> r) & 1;
-                dma16(ok && 8 * ck < a.D ? kb + (r * a.k_token + 8 * ck) * 2 : (const char *)&xa_zero, S + 1024 * QW * i);
-                dma16(ok && 8 * cv < a.D ? vb + (r * a.v_token + 8 * cv) * 2 : (const char *)&xa_zero, S + TB + 1024 * QW * i);
+                const int c = is_v ? cv : ck;
+                const bool ok = ((bits >> r) & 1) && 8 * c < a.D;
+                dma16(ok ? base + (r * (is_v ? a.v_token : a.k_token) + 8 * c) * 2 : (const char *)&xa_zero, S + 1024 * QW * i);
             }
         }
-        kb += kstep;
-        vb += vstep;
+        base += is_v ? vstep : kstep;
+    };
+    auto dma = [&](int buf, uint64_t bits) __attribute__((always_inline)) {
+        dma_one(IC<0>{}, buf, bits);
+        dma_one(IC<1>{}, buf, bits);
     };
     /* the valid keys of tile i (bit j: key KT i + j) where no mask says otherwise */
     auto in_len = [&](int i) __attribute__((always_inline)) -> uint64_t {
@@ -224,9 +228,8 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
     }
 
     const unsigned ninf = g ? 0u : Xa<T>::NINF;     /* element 0 of lanes 0 .. 31, whose keys are their numbers */
-    auto tile = [&](int buf, uint64_t bits) __attribute__((always_inline)) {
-        const uint8_t *K = smem + buf * STAGE + ks * 2 * TB, *V = K + TB;
-        xa_f32x16_t s[KB];
+    auto scores = [&](int buf, uint64_t bits, xa_f32x16_t (&s)[KB]) __attribute__((always_inline)) {
+        const uint8_t *K = smem + buf * STAGE + ks * 2 * TB;
 #pragma unroll
         for (int kb = 0; kb < KB; kb++)
 #pragma unroll
@@ -243,6 +246,8 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
                 s[kb] = Xa<T>::mfma8(make_uint2(0u - (w & 1u) & ninf, 0), make_uint2(Xa<T>::ONE, 0), s[kb]);
             }
         }
+    };
+    auto move_ref = [&](const xa_f32x16_t (&s)[KB]) __attribute__((always_inline)) {
         float mt = s[0][0];
 #pragma unroll
         for (int i = 1; i + 1 < 16 * KB; i += 2) mt = xa_max3(mt, s[i >> 4][i & 15], s[(i + 1) >> 4][(i + 1) & 15]);
@@ -259,6 +264,9 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
             l *= al;
             ref = m2;
         }
+    };
+    auto add = [&](int buf, const xa_f32x16_t (&s)[KB]) __attribute__((always_inline)) {
+        const uint8_t *V = smem + buf * STAGE + ks * 2 * TB + TB;
 #pragma unroll
         for (int kb = 0; kb < KB; kb++)
 #pragma unroll
@@ -305,7 +313,12 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
             constexpr int buf = decltype(BUF)::value;
             const int byte = mask_byte(i + 2);
             if (i + 1 < t1) dma(buf ^ 1, nxt);
-            if (cur) tile(buf, cur);
+            if (cur) {
+                xa_f32x16_t s[KB];
+                scores(buf, cur, s);
+                move_ref(s);
+                add(buf, s);
+            }
             drain();
             meet();
             cur = nxt;
@@ -317,13 +330,34 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
             turn(IC<1>{}, i + 1);
         }
     } else {
+        /* keys of tile i + 1 leave when the scores of tile i stand, its values when tile i is added: one of the two is
+         * always on its way. Newer transfers may be in flight behind the ones waited for */
+        auto behind = [](bool more) __attribute__((always_inline)) {
+            if (more) asm volatile("s_waitcnt vmcnt(%0)" : : "i"(ND) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        };
+        auto have_read = []() __attribute__((always_inline)) { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
+        int byte = mask_byte(t0 + 1);
+        if (t0 < t1) dma(0, cur);
+        behind(t0 < t1);
+#pragma unroll
+        for (int i = 0; i < DS; i++) asm volatile("" : "+v"(qf[i]));
         for (int i = t0; i < t1; i++) {
-            const int byte = mask_byte(i + 1);
-            dma(0, cur);
-            drain();
-            if (cur) tile(0, cur);
-            drain();
-            cur = to_bits(i + 1, byte);
+            const bool more = i + 1 < t1;
+            uint64_t nxt = in_len(i + 1);
+            if (mask) nxt &= __ballot(byte != 0);
+            behind(true);
+            xa_f32x16_t s[KB];
+            if (cur) scores(0, cur, s);
+            have_read();
+            if (more) dma_one(IC<0>{}, 0, nxt);
+            if (mask) byte = mask_byte(i + 2);
+            if (cur) move_ref(s);
+            behind(more);
+            if (cur) add(0, s);
+            have_read();
+            if (more) dma_one(IC<1>{}, 0, nxt);
+            cur = nxt;
         }
     }
 
@@ -461,9 +495,9 @@ static XaPlan xa_plan(const aria_k_xattn *a) {
     p.nrb = (int)(p.T / bh);
     p.ns = 1;
     if (p.qw == 1) {
-        /* at least 256 keys to a workgroup, and up to four workgroups to a CU */
-        const int most = a->Nk / 256;
-        while (p.ns < most && (long long)p.T * p.ns < 1024) p.ns++;
+        /* at least 256 keys to a workgroup, and as many workgroups as the CUs hold at once, two each (16 x 4 key heads x up
+         * to 8192 keys of 128: 39.4 us, 42 with twice as many, 47 with three quarters) */
+        p.ns = std::max(1, std::min(a->Nk / 256, 512 / p.T));
     }
     p.per = ((a->Nk + xa_tile(p.DP) - 1) / xa_tile(p.DP) + p.ns - 1) / p.ns;
     return p;
