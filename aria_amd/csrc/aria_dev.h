@@ -208,7 +208,13 @@ __device__ __forceinline__ void dma16(const void *g, uint32_t m0) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(m), "v"(g) : "memory");
 }
 
-/* the same from a scalar base and an unsigned 32-bit lane offset */
+/* the same with 4 B per lane, to m0 + 4 * lane */
+__device__ __forceinline__ void dma4(const void *g, uint32_t m0) {
+    const uint32_t m = __builtin_amdgcn_readfirstlane(m0);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(m), "v"(g) : "memory");
+}
+
+/* dma16 from a scalar base and an unsigned 32-bit lane offset */
 __device__ __forceinline__ void dma16_s(const void *base, unsigned off, uint32_t m0) {
     const uint32_t m = __builtin_amdgcn_readfirstlane(m0);
     const uint64_t u = (uint64_t)base;

@@ -103,7 +103,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
     constexpr int NS = SHARED ? NR / (64 * GW) : 1;              /* scale rows per lane */
     static_assert(SHARED ? NR % (64 * GW) == 0 && WK == 1 : NST == 1, "");
     constexpr int GROUP = NST * STAGE + 2 * SCALES;              /* LDS of one K group */
-    __shared__ __attribute__((aligned(16))) uint8_t smem[WK * GROUP > EPI ? WK * GROUP : EPI];
+    constexpr int BIAS = WK * GROUP > EPI ? WK * GROUP : EPI;    /* biases of the tile's w rows behind the rest */
+    __shared__ __attribute__((aligned(16))) uint8_t smem[BIAS + (SHARED ? 4 * BN : 0)];
     const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
     const int wid = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int wk = wid / GW, gw = wid % GW, wm = gw / WN, wn = gw % WN;
@@ -196,23 +197,29 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
         });
     };
 
-    /* the biases of this lane's columns of the epilogue, whose loads end under the first chunk's transfer */
+    /* The biases end under the first chunk's transfer. SHARED: those of the tile's w rows go to LDS as well, since loads to
+     * registers behind a branch are waited for where it ends, before any transfer has left */
     float bias[8], gbias[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) { bias[e] = 0.0f; gbias[e] = 0.0f; }
-    if (a.bias) {
-        const int V = a.ytype == MX_F32 ? 4 : 8, n = n0 + wn * OW + V * (lane % (OW / V));
-        if (n + V <= a.N) {
+    const int bv = a.ytype == MX_F32 ? 4 : 8, bc = bv * (lane % (OW / bv));   /* this lane's columns of the wave's */
+    if constexpr (SHARED) {
+        static_assert(BN % 64 == 0 && BN / 64 <= NW, "");
+        const int i = 64 * wid + lane;
+        if (a.bias && wid < BN / 64) dma4(a.bias + n0 + w_col(i) + (is_gate(i) ? a.N : 0), (uint32_t)(uintptr_t)smem + BIAS + 256 * wid);
+    } else if (a.bias) {
+        const int n = n0 + wn * OW + bc;
+        if (n + bv <= a.N) {
             __builtin_memcpy(bias, a.bias + n, 16);
-            if (V == 8) __builtin_memcpy(bias + 4, a.bias + n + 4, 16);
+            if (bv == 8) __builtin_memcpy(bias + 4, a.bias + n + 4, 16);
             if constexpr (GLU) {
                 __builtin_memcpy(gbias, a.bias + a.N + n, 16);
-                if (V == 8) __builtin_memcpy(gbias + 4, a.bias + a.N + n + 4, 16);
+                if (bv == 8) __builtin_memcpy(gbias + 4, a.bias + a.N + n + 4, 16);
             }
         } else {
 #pragma unroll
             for (int e = 0; e < 8; e++)
-                if (e < V && n + e < a.N) {
+                if (e < bv && n + e < a.N) {
                     bias[e] = a.bias[n + e];
                     if constexpr (GLU) gbias[e] = a.bias[a.N + n + e];
                 }
@@ -291,18 +298,26 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
         const int np = a.nb / 16;
         int sbuf = 0;
         if constexpr (NST == 1) {
-            if (np) load_scales(0);
-            for (int c = 0; c < 2 * np; c++) {
-                if (c > 0) turn();                               /* the stage is still being read */
-                issue(IC<0>{}, 0, c);
-                if ((c & 1) == 0) {
-                    if (c > 0) arrived();
-                    put_scales((c >> 1) & 1);
-                    if (c + 2 < 2 * np) load_scales(c + 2);
+            if (np) {
+                load_scales(0);
+                issue(IC<0>{}, 0, 0);
+                put_scales(0);
+                for (int p = 0;; p++) {
+                    turn();
+                    shared_scales(xa, wa, 0, p & 1);
+                    compute(0, xa, wa);
+                    turn();                                      /* the stage is still being read */
+                    issue(IC<0>{}, 0, 2 * p + 1);
+                    load_scales(2 * min(p + 1, np - 1));
+                    turn();
+                    arrived();
+                    shared_scales(xa, wa, 1, p & 1);
+                    compute(0, xa, wa);
+                    if (p + 1 == np) break;
+                    turn();
+                    issue(IC<0>{}, 0, 2 * p + 2);
+                    put_scales((p + 1) & 1);
                 }
-                turn();
-                shared_scales(xa, wa, c & 1, (c >> 1) & 1);
-                compute(0, xa, wa);
             }
         } else {
             if (np) {
@@ -314,12 +329,12 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
                 turn();
                 issue(IC<0>{}, 1, 2 * p + 1);
                 const bool more = p + 1 < np;
-                if (more) load_scales(2 * p + 2);
+                load_scales(2 * min(p + 1, np - 1));
                 shared_scales(xa, wa, 0, sbuf);
                 compute(0, xa, wa);
                 turn();
+                arrived();
                 if (more) {
-                    arrived();
                     issue(IC<0>{}, 0, 2 * p + 2);
                     put_scales(sbuf ^ 1);
                 }
@@ -383,6 +398,15 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
      * segments stored */
     const int el = fresh(lane), el32 = el & 31, eh = el >> 5;
     float *E = (float *)smem + wid * 32 * ES;
+    if constexpr (SHARED)
+        if (a.bias) {
+            const float *p = (const float *)(smem + BIAS) + wn * 32 * FN + bc;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                bias[e] = e < bv ? p[e] : 0.0f;
+                if constexpr (GLU) gbias[e] = e < bv ? p[OW + e] : 0.0f;
+            }
+        }
     __syncthreads();                                             /* stages still being read */
     static_for<FM>([&](auto I) __attribute__((always_inline)) {
         constexpr int i = decltype(I)::value;
