@@ -179,6 +179,22 @@ def test_lengths_and_masks(hip, t, Nq, Nk, D):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("D", [64, 72, 128])
+def test_few_rows_many_tiles(hip, t, D):
+    """Several tiles to each wave and split: lengths that end anywhere, with a mask and without, whole tiles of it gone."""
+    B, Nk = 24, 2500
+    r = rng(D)
+    lens = [int(n) for n in r.integers(0, Nk + 1, B)]
+    mask = (r.random((B, Nk)) < 0.8).astype(np.uint8)
+    mask[3, 256:900] = 0
+    mask[4, :2000] = 0
+    check(hip, t, B, 8, 4, 2, Nk, D, seed=D, kv_len=lens)
+    check(hip, t, B, 8, 4, 2, Nk, D, seed=D + 1, kv_len=lens, mask=mask, layout="tokens")
+    check(hip, t, B, 8, 4, 2, Nk, D, seed=D + 2, mask=mask, spread=3.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", ["f16", "bf16"])
 @pytest.mark.parametrize("Nq", [1, 70])
 def test_anything_in_masked_places(hip, t, Nq):
     """NaN and Inf in masked keys and values, and behind the lengths, change no bit of the result."""

@@ -251,6 +251,21 @@ def test_glu_large(hip, M, K, N, xt, yt, bias):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N", [(260, 1700, 2570), (1100, 300, 1550), (1500, 300, 3085), (1900, 1700, 3085)])
+@pytest.mark.parametrize("xt,yt", [("f32", "f32"), ("bf16", "bf16")])
+def test_linear_tiles(hip, M, K, N, xt, yt):
+    """Every tile over K of one pair of chunks, several pairs and none, with biases at a cut column edge."""
+    test_linear(hip, M, K, N, xt, yt, True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N", [(129, 300, 257), (129, 1700, 257), (200, 300, 2570), (2300, 300, 515), (900, 1700, 3085)])
+@pytest.mark.parametrize("xt,yt", [("f32", "f32"), ("f16", "f16")])
+def test_glu_tiles(hip, M, K, N, xt, yt):
+    test_glu(hip, M, K, N, xt, yt, True)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("M", [1, 9, 50, 400])
 def test_not_finite(hip, M):
     """A row with an Inf or NaN gives NaN in that row alone; a weight row with byte 255 in that column alone."""
