@@ -92,7 +92,7 @@ __host__ __device__ constexpr int xa_part(int DP) { return 32 * DP + 64; }
  * without barriers, is bound by the keys' bytes, and has one stage, so that two workgroups fit a CU (16 x 4 key heads x up to
  * 8192 keys of 128: 56 us with two stages and one workgroup, 45 with one and two, the join included); the next tile's keys
  * then move while this one's values are added, its values while the scores are made (45 to 42).
- * What bounds it: with many rows the VALU, 71 % busy beside the MFMAs' 45 % at 4 x 16 x 4096 rows x 2048 keys of 64 (0.88
+ * What bounds it: with many rows the VALU, 69 % busy beside the MFMAs' 46 % at 4 x 16 x 4096 rows x 2048 keys of 64 (0.88
  * PFLOP/s; an exponential, a fused multiply-add, half a maximum, half a conversion and half a dot product per score);
  * with a single row the keys' bytes (4.9 TB/s without the join); at a few tiles a wave the latency of one tile, about 1 us. */
 template <typename T, int DP, int KT, int QW, int KS>
@@ -477,8 +477,8 @@ __global__ __launch_bounds__(64) void k_xattn_join(XaArgs x) {
 }
 
 /* How a call runs: qw blocks of 32 rows and ks slices of the keys to a workgroup, ns splits of the keys across workgroups.
- *  qw 1, ks 4: up to 32 rows a key head, and where blocks of 128 rows would leave CUs idle, which every block of 32 rows then has to fill by reading the keys
- *    for itself (16 heads x 172 rows x 257 keys of 64: 6.2 us, 8.5 with qw 4; x 710 rows x 1024 keys: 25.2 and 14.5);
+ *  qw 1, ks 4: up to 32 rows a key head, and where blocks of 128 rows would leave CUs idle, which blocks of 32 rows then
+ *    fill, each reading the keys for itself (16 heads x 172 rows x 257 keys of 64: 6.2 us, 8.5 with qw 4; x 710 rows x 1024 keys: 25.2 and 14.5);
  *  qw 4, ks 2: up to a workgroup per CU, and up to 700 of them over long keys of 64 (2 x 16 x 710 rows x 257 keys: 8.9 us, 9.5 with
  *    one slice; 2 x 16 x 1296 x 1296: 29.1 and 31.4, of 128 54.2 and 49.4);
  *  qw 4, ks 1; and qw 8 where four rounds of 256 rows fill the CUs (4 x 16 x 4096 x 2048 of 64: 166 us with 4, 158 with 8; of 128,
