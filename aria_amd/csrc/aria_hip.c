@@ -571,12 +571,15 @@ int aria_hip_linear_q8a8_dev(float *dy, const void *dx, int x_f16, const int8_t 
 #define MX4_TYPE(t) ((t) == 0 || (t) == 1 || (t) == 2)
 #define MX4_KMAX (1 << 24)   /* lane offsets within a tile's 256 rows are 32 bits wide */
 #define MX4_NMAX (1 << 26)
+#define MX4_ROWS (1 << 30)   /* rows and rows + one launch's share of them (2^28) fit an int */
+/* the products: tiles of 32 rows and their edges are counted in 32 bits, a launch holds less than 2^32 threads */
+#define MX4_FITS(M, N) ((M) <= (1 << 28) && (int64_t)(M) * (N) <= ((int64_t)1 << 36))
 static size_t mx4_blocks(int K) { return ((size_t)K + 31) / 32; }
 static uintptr_t mx4_el_mask(int type) { return type == 0 ? 3u : 1u; }
 
 int aria_hip_mx4_quant_dev(uint8_t *dq, uint8_t *dscale, const void *dx, int xtype, int rows, int K, int64_t ldx,
                            void *stream) {
-    REQ(rows >= 0 && K > 0 && K <= MX4_KMAX && MX4_TYPE(xtype) && ldx >= K);
+    REQ(rows >= 0 && rows <= MX4_ROWS && K > 0 && K <= MX4_KMAX && MX4_TYPE(xtype) && ldx >= K);
     REQ(rows == 0 || (dq && dscale && dx));
     REQ(((uintptr_t)dq & 15u) == 0 && ((uintptr_t)dx & mx4_el_mask(xtype)) == 0);
     ENSURE();
@@ -585,7 +588,7 @@ int aria_hip_mx4_quant_dev(uint8_t *dq, uint8_t *dscale, const void *dx, int xty
 }
 int aria_hip_mx4_dequant_dev(void *dy, int ytype, const uint8_t *dq, const uint8_t *dscale, int rows, int K,
                              void *stream) {
-    REQ(rows >= 0 && K > 0 && K <= MX4_KMAX && MX4_TYPE(ytype));
+    REQ(rows >= 0 && rows <= MX4_ROWS && K > 0 && K <= MX4_KMAX && MX4_TYPE(ytype));
     REQ(rows == 0 || (dy && dq && dscale));
     REQ(((uintptr_t)dq & 15u) == 0 && ((uintptr_t)dy & mx4_el_mask(ytype)) == 0);
     ENSURE();
@@ -595,6 +598,7 @@ int aria_hip_mx4_dequant_dev(void *dy, int ytype, const uint8_t *dq, const uint8
 static int gemm_mx4(void *dy, int ytype, const uint8_t *dxq, const uint8_t *dxs, const uint8_t *dq,
                     const uint8_t *dscale, const float *db, int M, int K, int N, int glu, void *stream) {
     REQ(M >= 0 && K > 0 && K <= MX4_KMAX && N >= 0 && N <= MX4_NMAX && MX4_TYPE(ytype));
+    REQ(MX4_FITS(M, N));
     REQ(M == 0 || N == 0 || (dy && dxq && dxs && dq && dscale));
     REQ((((uintptr_t)dxq | (uintptr_t)dq) & 15u) == 0 && ((uintptr_t)dy & mx4_el_mask(ytype)) == 0);
     REQ(((uintptr_t)db & 3u) == 0);
@@ -614,6 +618,7 @@ size_t aria_hip_mx4_ws_bytes(int M, int K) {
 static int linear_mx4(void *dy, int ytype, const void *dx, int xtype, int64_t ldx, const uint8_t *dq,
                       const uint8_t *dscale, const float *db, int M, int K, int N, int glu, void *dws, void *stream) {
     REQ(M >= 0 && K > 0 && K <= MX4_KMAX && N >= 0 && N <= MX4_NMAX && MX4_TYPE(ytype));
+    REQ(MX4_FITS(M, N));
     REQ(MX4_TYPE(xtype) && ldx >= K);
     REQ(M == 0 || N == 0 || (dy && dx && dq && dscale && dws));
     REQ(((uintptr_t)dq & 15u) == 0 && ((uintptr_t)dws & 255u) == 0 && ((uintptr_t)db & 3u) == 0);
@@ -787,7 +792,7 @@ int aria_hip_q4_dequant(float *W, const uint8_t *q, const float *scale, int N, i
 }
 
 int aria_hip_mx4_quant(uint8_t *q, uint8_t *scale, const float *x, int rows, int K) {
-    REQ(rows >= 0 && K > 0 && K <= MX4_KMAX && q && scale && x);
+    REQ(rows >= 0 && rows <= MX4_ROWS && K > 0 && K <= MX4_KMAX && q && scale && x);
     if (rows == 0) return 0;
     HOST_BEGIN();
     const size_t nb = (size_t)rows * mx4_blocks(K);
@@ -799,7 +804,7 @@ int aria_hip_mx4_quant(uint8_t *q, uint8_t *scale, const float *x, int rows, int
     HOST_END();
 }
 int aria_hip_mx4_dequant(float *y, const uint8_t *q, const uint8_t *scale, int rows, int K) {
-    REQ(rows >= 0 && K > 0 && K <= MX4_KMAX && y && q && scale);
+    REQ(rows >= 0 && rows <= MX4_ROWS && K > 0 && K <= MX4_KMAX && y && q && scale);
     if (rows == 0) return 0;
     HOST_BEGIN();
     const size_t nb = (size_t)rows * mx4_blocks(K);
@@ -812,6 +817,7 @@ int aria_hip_mx4_dequant(float *y, const uint8_t *q, const uint8_t *scale, int r
 static int host_linear_mx4(float *y, const float *x, const uint8_t *q, const uint8_t *scale, const float *b, int M,
                            int K, int N, int glu) {
     REQ(M >= 0 && K > 0 && K <= MX4_KMAX && N >= 0 && N <= MX4_NMAX && y && x && q && scale);
+    REQ(MX4_FITS(M, N));
     if (M == 0 || N == 0) return 0;
     HOST_BEGIN();
     const size_t rows = (size_t)N << glu, nb = rows * mx4_blocks(K);

@@ -599,11 +599,13 @@ static hipError_t pick(const MxArgs &a, hipStream_t s) {
     const double t128a = most(3.7 + 1.05 * nc, 3 + half(768) * (0.002 + 0.000075 * kb + 0.0023 * nc));
     const double t128b = most(4.4 + 0.66 * nc, 3 + half(512) * (0.0024 + 0.000075 * kb + 0.0025 * nc));
     const double t256 = 3 + rounds * ((nc < 2 ? 2.4 : -0.6) + 0.16 * kb + 2.02 * nc);
-    double t = t32;
-    int which = 0;
-    const double other[4] = {t64, t128a, t128b, t256};
-    for (int i = 0; i < 4; i++)
-        if (other[i] < t) { t = other[i]; which = i + 1; }
+    /* A launch holds less than 2^32 threads: tiles of 256 threads are counted; of 256 x 256 there are never too many
+     * (M up to 2^28, M N up to 2^36) */
+    const double most_tiles = (double)((1l << 24) - 8);
+    const double us[5] = {t32, t64, t128a, t128b, t256}, count[5] = {tiles(32, 32), tiles(64, 64 / H), n128, n128, 0};
+    int which = 4;
+    for (int i = 3; i >= 0; i--)
+        if (us[i] <= us[which] && count[i] <= most_tiles) which = i;
     switch (which) {
     case 0: return launch<1, H, 1, 1, 4, 1, GLU>(a, s);
     case 1: return launch<2, 2, 1, 1, 4, 1, GLU>(a, s);

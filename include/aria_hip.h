@@ -263,8 +263,9 @@ int aria_hip_cross_attention_f16(float *out, const float *q, const float *k, con
  * x / 2^(byte - 127) to nearest, ties to the even code, saturating at 6, the sign of zero kept. A
  * block that holds an Inf or a NaN gets byte 255 and codes 0: it stands for NaN.
  * Element types of activations and outputs are aria_dtype's values: 0 fp32, 1 fp16, 2 bf16;
- * ldx: elements between rows of x (at least K). K at most 2^24, N (inner) at most 2^26. Outputs and
- * workspaces overlap no input. */
+ * ldx: elements between rows of x (at least K). K at most 2^24, rows at most 2^30; of the
+ * products M at most 2^28, N (inner) at most 2^26 and M * N at most 2^36. Outputs and workspaces
+ * overlap no input. */
 int aria_hip_mx4_quant_dev(uint8_t *dq, uint8_t *dscale, const void *dx, int xtype, int rows, int K, int64_t ldx,
                            void *stream);
 /* y [rows, K] from packed rows, rounded to ytype (fp32 holds every value) */
