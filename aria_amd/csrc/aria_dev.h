@@ -56,6 +56,14 @@ __device__ __forceinline__ float xor32_f32(float v, int lane) {
     return __builtin_bit_cast(float, lane < 32 ? r[1] : r[0]);
 }
 
+/* max(a, b, c) in one v_maximum3_f32; a NaN among them gives NaN. An operation that the compiler sees, not inline
+ * assembly: scores come straight from MFMAs, and it puts the wait states between an MFMA and the first VALU instruction that
+ * reads its result only for instructions of its own. (fmaxf would be followed by canonicalisations of what it cannot
+ * trace to an MFMA.) */
+__device__ __forceinline__ float max3_f32(float a, float b, float c) {
+    return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
+}
+
 struct OpSum {
     template <typename T> __device__ __forceinline__ T operator()(T a, T b) const { return a + b; }
 };

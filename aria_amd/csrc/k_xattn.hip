@@ -66,12 +66,6 @@ template <> struct Xa<__bf16> {
     static __device__ __forceinline__ float dot2(v2 a, v2 b, float c) { return __builtin_amdgcn_fdot2_f32_bf16(a, b, c, false); }
 };
 
-__device__ __forceinline__ float xa_max3(float a, float b, float c) {
-    float r;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
-}
-
 struct XaArgs {
     aria_k_xattn a;
     int G, R;            /* query heads per key head; rows per (batch, key head) */
@@ -251,10 +245,10 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
     auto move_ref = [&](const xa_f32x16_t (&s)[KB]) __attribute__((always_inline)) {
         float mt = s[0][0];
 #pragma unroll
-        for (int i = 1; i + 1 < 16 * KB; i += 2) mt = xa_max3(mt, s[i >> 4][i & 15], s[(i + 1) >> 4][(i + 1) & 15]);
-        mt = xa_max3(mt, s[KB - 1][15], s[KB - 1][15]);
+        for (int i = 1; i + 1 < 16 * KB; i += 2) mt = max3_f32(mt, s[i >> 4][i & 15], s[(i + 1) >> 4][(i + 1) & 15]);
+        mt = max3_f32(mt, s[KB - 1][15], s[KB - 1][15]);
         const float mo = xor32_f32(mt, lane);
-        mt = xa_max3(mt, mo, mo) * x.scale_log2;
+        mt = max3_f32(mt, mo, mo) * x.scale_log2;
         if (__ballot(mt > ref + XA_SLACK)) {
             asm volatile("" ::: "memory");   /* a branch, not 16 DT predicated multiplies */
             const float m2 = fmaxf(ref, mt), al = __builtin_amdgcn_exp2f(ref - m2);

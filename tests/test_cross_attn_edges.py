@@ -1,0 +1,32 @@
+"""Cross attention where values, scores or descriptions lie at an edge, against the definition in 64 bits
+(oracle/mx4.py). Refusals run on the CPU."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from conftest import randn, rng
+from oracle import mx4
+from test_cross_attn import cast, run, tolerance
+
+# every form of workgroup: four slices of one wave (split over workgroups too), four waves and two slices, four waves, eight
+FORMS = [(1, 8, 2, 3, 700, 64), (1, 4, 4, 5, 700, 128), (1, 16, 8, 1100, 600, 64), (2, 8, 8, 1025, 300, 128), (3, 16, 16, 1000, 300, 64),
+         (3, 16, 16, 1000, 200, 72), (8, 16, 16, 2050, 100, 64)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("B,H,Hkv,Nq,Nk,D", FORMS)
+def test_masked_keys_above_low_scores(hip, t, B, H, Hkv, Nq, Nk, D):
+    """Every valid score is -60 or less, a masked key's products alone would be 0: a maximum that saw those would leave no
+    weight in 16 bits."""
+    print(f"[gpu] low scores {t} {B} {H}/{Hkv} {Nq} {Nk} {D}", flush=True)
+    r = rng(Nq + Nk)
+    q, qv = cast(1.0 + 0.05 * randn(r, (B, H, Nq, D)), t)
+    k, kv = cast(-90.0 / np.sqrt(D) + 0.05 * randn(r, (B, Hkv, Nk, D)), t)
+    v, vv = cast(randn(r, (B, Hkv, Nk, D)), t)
+    mask = (r.random((B, Nk)) < 0.4).astype(np.uint8)
+    got = run(hip, t, q, k, v, mask=mask)
+    want, mag = mx4.cross_attention(qv, kv, vv, mask=mask)
+    assert qv.min() > 0 and qv.min() * kv.max() * np.sqrt(D) < -60
+    assert (np.abs(got - want) <= tolerance(want, mag, qv, kv, vv, t, t, 1 / np.sqrt(D), Nk)).all(), np.abs(got - want).max()
