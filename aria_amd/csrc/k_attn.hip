@@ -195,13 +195,6 @@ __device__ __forceinline__ int v_off(int key, int d) {
  * the 8 B rows addressed by lanes 4v+w (v = 0..3): addressing key kb' + v at d0 + 4w
  * delivers V[kb'+0..3][d0 + (lane & 15)] to each lane (voff below). */
 
-/* max(a, b, c) in one v_max3_f32 */
-__device__ __forceinline__ float max3f(float a, float b, float c) {
-    float r;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
-}
-
 /* fp32 pair -> packed fp16, round to nearest even */
 __device__ __forceinline__ uint32_t pack2h_rn(float x, float y) {
     typedef float float2_v __attribute__((ext_vector_type(2)));
@@ -330,14 +323,14 @@ __global__ __launch_bounds__(64 * QW * KS) __attribute__((amdgpu_waves_per_eu(KS
                     if (kt0 + 32 * kb + 8 * (r >> 2) + 4 * g + (r & 3) >= a.Nk) sc[kb][r] = -INFINITY;
         }
         /* tile max over this lane's 32 keys and the partner lane's 32: a tree of 3-input
-         * maxima (15 v_max3_f32, depth 3; two-input fmaxf trees compile to twice as many ops) */
+         * maxima (15 v_maximum3_f32, depth 3; two-input fmaxf trees compile to twice as many ops) */
         float t1[11];
 #pragma unroll
-        for (int i = 0; i < 10; i++) t1[i] = max3f(sc[(3 * i) >> 4][(3 * i) & 15], sc[(3 * i + 1) >> 4][(3 * i + 1) & 15],
+        for (int i = 0; i < 10; i++) t1[i] = max3_f32(sc[(3 * i) >> 4][(3 * i) & 15], sc[(3 * i + 1) >> 4][(3 * i + 1) & 15],
                                                    sc[(3 * i + 2) >> 4][(3 * i + 2) & 15]);
         t1[10] = fmaxf(sc[1][14], sc[1][15]);
-        float mt = max3f(max3f(t1[0], t1[1], t1[2]), max3f(t1[3], t1[4], t1[5]), max3f(t1[6], t1[7], t1[8]));
-        mt = max3f(mt, t1[9], t1[10]);
+        float mt = max3_f32(max3_f32(t1[0], t1[1], t1[2]), max3_f32(t1[3], t1[4], t1[5]), max3_f32(t1[6], t1[7], t1[8]));
+        mt = max3_f32(mt, t1[9], t1[10]);
         mt = fmaxf(mt, xor32_f32(mt, lane)) * a.scale_log2;
         /* lazy rescale: the reference max only moves when the tile max exceeds it by more
          * than RESCALE_SLACK (probabilities stay <= 2^8, exact in fp16's range); the final

@@ -103,7 +103,7 @@ def test_the_reader():
 
 
 @pytest.mark.skipif(not shutil.which(os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")), reason="no hipcc")
-@pytest.mark.parametrize("kernel", ["k_xattn"])
+@pytest.mark.parametrize("kernel", ["k_xattn", "k_attn"])
 def test_inline_asm_behind_mfma(tmp_path, kernel):
     subprocess.run(["make", "-C", CSRC, f"OBJDIR={tmp_path}", f"{tmp_path}/{kernel}.s"], check=True, capture_output=True)
     with open(tmp_path / f"{kernel}.s") as f:
