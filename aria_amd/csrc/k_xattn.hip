@@ -19,10 +19,14 @@
  * adds -inf to their scores (0 before): 2 MFMAs in place of 32 selects on the busier VALU (4 x 16 x 4096 rows x up to
  * 2048 masked keys of 64: 109 us, 118 with selects).
  *
- * The maximum is a lazy reference: it moves only when a tile exceeds it by 2^8, which leaves O / l
- * unchanged. It starts finite (below any score of 16-bit operands that a softmax can tell apart), so
- * a slice whose keys all score -inf has weight zero instead of NaN. P is rounded to the type of V; the
- * row sum adds the rounded values, so the weights still sum to one.
+ * The weights are 2^(scale_log2 s - ref) with a lazy reference: it lies 7 below a tile's largest exponent where it moves,
+ * and moves when a tile exceeds that by 8, which leaves O / l unchanged. The largest weight of a row is thus between 2^7 and
+ * 2^15 (fp16 reaches 2^16), and in fp16 a weight vanishes only below 2^-32 of it. The reference starts finite (below any
+ * score of 16-bit operands that a softmax can tell apart), so a slice whose keys all score -inf has weight zero instead of NaN.
+ * P is rounded to the type of V: the second product takes 16-bit operands, and its weights in two parts would double the
+ * matrix work. That is half a step, 2^-11 or 2^-8, per weight at most (errors of an output against 64 bits 2.8e-4 in fp16
+ * and 2.3e-3 in bf16, 2.1e-4 and 1.7e-3 with fp32 weights; the output's own rounding is in both); the row sum adds the
+ * rounded values, so the weights still sum to one.
  */
 #include "aria_dev.h"
 #include "aria_hip_kernels.h"
@@ -33,7 +37,8 @@ typedef float xa_f32x16_t __attribute__((ext_vector_type(16)));
 typedef short xa_i16x4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) xa_i16x4_t xa_lds_i16x4_t;
 
-#define XA_SLACK 8.0f      /* log2 units that the reference may lag the maximum */
+#define XA_TOP 7.0f        /* log2 of the largest weight where the reference has just moved */
+#define XA_SLACK 8.0f      /* log2 units that the maximum may rise above that before the reference moves again */
 #define XA_MIN (-3e38f)    /* the reference before any key */
 
 /* 16-byte source of slots that hold no valid key or no dim */
@@ -249,9 +254,9 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
         mt = max3_f32(mt, s[KB - 1][15], s[KB - 1][15]);
         const float mo = xor32_f32(mt, lane);
         mt = max3_f32(mt, mo, mo) * x.scale_log2;
-        if (__ballot(mt > ref + XA_SLACK)) {
+        if (__ballot(mt > ref + (XA_TOP + XA_SLACK))) {
             asm volatile("" ::: "memory");   /* a branch, not 16 DT predicated multiplies */
-            const float m2 = fmaxf(ref, mt), al = __builtin_amdgcn_exp2f(ref - m2);
+            const float m2 = fmaxf(ref, mt - XA_TOP), al = __builtin_amdgcn_exp2f(ref - m2);
 #pragma unroll
             for (int d = 0; d < DT; d++)
 #pragma unroll

@@ -232,7 +232,8 @@ int aria_hip_attention_f16(float *out, const float *q, const float *k, const flo
  * Strides count elements and are multiples of 8, not negative, pointers are 16-byte aligned (for
  * an fp32 out too); batch / head / token strides of q, k and v may be 0 (broadcast); rows of out lie
  * apart from each other and from every input. Probabilities
- * are rounded to the type before they multiply v; sums and softmax statistics are fp32.
+ * are rounded to the type before they multiply v, whatever out's type; in fp16 one below 2^-32 of its
+ * row's largest may count as zero. Sums and softmax statistics are fp32.
  * dws: aria_hip_cross_attention_ws_bytes(a) bytes (0: may be NULL), 256-byte aligned, not shared
  * by calls that may run at the same time. No counterpart in the reference, whose attention takes
  * one length (src/aria_ops.h:135). */

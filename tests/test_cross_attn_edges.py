@@ -30,3 +30,25 @@ def test_masked_keys_above_low_scores(hip, t, B, H, Hkv, Nq, Nk, D):
     want, mag = mx4.cross_attention(qv, kv, vv, mask=mask)
     assert qv.min() > 0 and qv.min() * kv.max() * np.sqrt(D) < -60
     assert (np.abs(got - want) <= tolerance(want, mag, qv, kv, vv, t, t, 1 / np.sqrt(D), Nk)).all(), np.abs(got - want).max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,H,Hkv,Nq,Nk,D", FORMS)
+def test_many_small_weights(hip, B, H, Hkv, Nq, Nk, D):
+    """fp16: one key of weight 1 and value 0, all others of weight 2^-25.1 and large values, which make the whole
+    result. A weight is held to half a step of fp16's smallest numbers, 2^-25, against a largest weight of at least 2^6.5
+    (2^7 less the reference's rounding): 2^-31.5 of the largest."""
+    print(f"[gpu] small weights {B} {H}/{Hkv} {Nq} {Nk} {D}", flush=True)
+    r = rng(Nk)
+    q, qv = cast(np.ones((B, H, Nq, D), np.float32), "f16")
+    kf = np.full((B, Hkv, Nk, D), -17.4 / np.sqrt(D), np.float32)
+    kf[:, :, Nk // 2] = 0
+    vf = 2000.0 + 100 * randn(r, (B, Hkv, Nk, D))
+    vf[:, :, Nk // 2] = 0
+    (k, kv), (v, vv) = cast(kf, "f16"), cast(vf, "f16")
+    got = run(hip, "f16", q, k, v, out="f32")
+    want, mag = mx4.cross_attention(qv, kv, vv)
+    assert (np.abs(want) > 1e-3).all()
+    tol = Nk * 2.0 ** -31.5 * vv.max() + tolerance(want, mag, qv, kv, 0 * vv, "f16", "f32", 1 / np.sqrt(D), 0)
+    assert (tol < 0.1 * want).all()
+    assert (np.abs(got - want) <= tol).all(), (got.min(), want.min())
