@@ -21,8 +21,10 @@
  *
  * The weights are 2^(scale_log2 s - ref) with a lazy reference: it lies 7 below a tile's largest exponent where it moves,
  * and moves when a tile exceeds that by 8, which leaves O / l unchanged. The largest weight of a row is thus between 2^7 and
- * 2^15 (fp16 reaches 2^16), and in fp16 a weight vanishes only below 2^-32 of it. The reference starts finite (below any
- * score of 16-bit operands that a softmax can tell apart), so a slice whose keys all score -inf has weight zero instead of NaN.
+ * 2^15 (fp16 reaches 2^16), and in fp16 a weight vanishes only below 2^-32 of it. The reference starts at the lowest
+ * finite value, so a slice whose keys all score -inf has weight zero instead of NaN.
+ * Where fp32's steps at the reference are over 1 (2^24), what its rounding leaves out is kept beside it (lo, else 0), and the
+ * exponents of a tile are taken in two steps: without that the largest weight could be anything up to 2^(half a step).
  * P is rounded to the type of V: the second product takes 16-bit operands, and its weights in two parts would double the
  * matrix work. That is half a step, 2^-11 or 2^-8, per weight at most (errors of an output against 64 bits 2.8e-4 in fp16
  * and 2.3e-3 in bf16, 2.1e-4 and 1.7e-3 with fp32 weights; the output's own rounding is in both); the row sum adds the
@@ -39,7 +41,8 @@ typedef __attribute__((address_space(3))) xa_i16x4_t xa_lds_i16x4_t;
 
 #define XA_TOP 7.0f        /* log2 of the largest weight where the reference has just moved */
 #define XA_SLACK 8.0f      /* log2 units that the maximum may rise above that before the reference moves again */
-#define XA_MIN (-3e38f)    /* the reference before any key */
+#define XA_MIN (-3.40282347e38f)   /* the reference before any key */
+#define XA_FAR 16777216.0f /* from here on fp32's steps are over 1 */
 
 /* 16-byte source of slots that hold no valid key or no dim */
 __device__ const uint4 xa_zero = {0, 0, 0, 0};
@@ -78,13 +81,13 @@ struct XaArgs {
     int ns, per;         /* splits of the keys across workgroups, key tiles to each */
     int plain;           /* every chunk holds dims, and lane offsets within a tile fit 32 bits */
     float scale_log2;
-    float *part;         /* ns > 1: per (tile, split) 32 x DP sums, 32 references, 32 row sums */
+    float *part;         /* ns > 1: per (tile, split) 32 x DP sums, 32 references, 32 row sums, 32 remainders of the references */
 };
 
 /* keys of a tile where KS waves take tiles in turn */
 __host__ __device__ constexpr int xa_tile(int DP) { return DP == 64 ? 64 : 32; }
 /* floats of one partial result */
-__host__ __device__ constexpr int xa_part(int DP) { return 32 * DP + 64; }
+__host__ __device__ constexpr int xa_part(int DP) { return 32 * DP + 96; }
 
 /* KS slices of the keys, each of QW waves of 32 rows that share its tiles; the slices' results are joined at the end. With
  * QW > 1 there are two stages, the next tile moving under the current one's products. With QW = 1 a wave works by itself,
@@ -107,7 +110,7 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
     constexpr int ES = DP + 4;                      /* floats per staged output row */
     constexpr int KB = KT / 32, DT = DP / 32, DS = DP / 16;
     constexpr int STAGE = 2 * TB * KS;              /* K and V of every slice */
-    constexpr int EPI = NW * 32 * ES * 4 + NW * 64 * 4;
+    constexpr int EPI = NW * 32 * ES * 4 + NW * 96 * 4;
     __shared__ __attribute__((aligned(16))) uint8_t smem[NST * STAGE > EPI ? NST * STAGE : EPI];
     typedef typename Xa<T>::v8 v8;
     typedef typename Xa<T>::v2 v2;
@@ -208,7 +211,8 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
     for (int d = 0; d < DT; d++)
 #pragma unroll
         for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
-    float l = 0.0f, ref = XA_MIN;
+    float l = 0.0f, ref = XA_MIN, lo = 0.0f;
+    bool far = false;                               /* a row of the wave has a lo */
     const v2 one2 = {(T)1.0f, (T)1.0f};
 
     /* byte offsets of the fragment reads */
@@ -247,26 +251,38 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
             }
         }
     };
-    auto move_ref = [&](const xa_f32x16_t (&s)[KB]) __attribute__((always_inline)) {
+    /* behind it the exponent of a weight is s * scale_log2 - ref, or, where far, s - lo */
+    auto move_ref = [&](xa_f32x16_t (&s)[KB]) __attribute__((always_inline)) {
         float mt = s[0][0];
 #pragma unroll
         for (int i = 1; i + 1 < 16 * KB; i += 2) mt = max3_f32(mt, s[i >> 4][i & 15], s[(i + 1) >> 4][(i + 1) & 15]);
         mt = max3_f32(mt, s[KB - 1][15], s[KB - 1][15]);
         const float mo = xor32_f32(mt, lane);
-        mt = max3_f32(mt, mo, mo) * x.scale_log2;
-        if (__ballot(mt > ref + (XA_TOP + XA_SLACK))) {
+        mt = max3_f32(mt, mo, mo);
+        const float d = __builtin_fmaf(mt, x.scale_log2, -ref) - lo;
+        if (__ballot(d > XA_TOP + XA_SLACK)) {
             asm volatile("" ::: "memory");   /* a branch, not 16 DT predicated multiplies */
-            const float m2 = fmaxf(ref, mt - XA_TOP), al = __builtin_amdgcn_exp2f(ref - m2);
+            const bool up = d > XA_TOP;
+            const float r2 = up ? __builtin_fmaf(mt, x.scale_log2, -XA_TOP) : ref;
+            const float left = fabsf(r2) >= XA_FAR ? __builtin_fmaf(mt, x.scale_log2, -r2) - XA_TOP : 0.0f;
+            const float lo2 = up ? left : lo, al = __builtin_amdgcn_exp2f((ref - r2) + (lo - lo2));
 #pragma unroll
             for (int d = 0; d < DT; d++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) o[d][r] *= al;
             l *= al;
-            ref = m2;
+            ref = r2;
+            lo = lo2;
+            far = __ballot(lo != 0.0f) != 0;
+        }
+        if (__builtin_expect(far, 0)) {
+#pragma unroll
+            for (int i = 0; i < 16 * KB; i++) s[i >> 4][i & 15] = __builtin_fmaf(s[i >> 4][i & 15], x.scale_log2, -ref);
         }
     };
     auto add = [&](int buf, const xa_f32x16_t (&s)[KB]) __attribute__((always_inline)) {
         const uint8_t *V = smem + buf * STAGE + ks * 2 * TB + TB;
+        const float sc = far ? 1.0f : x.scale_log2, rr = far ? lo : ref;
 #pragma unroll
         for (int kb = 0; kb < KB; kb++)
 #pragma unroll
@@ -283,7 +299,7 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
                 v8 p;
 #pragma unroll
                 for (int i = 0; i < 8; i++)
-                    p[i] = (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * h + i], x.scale_log2, -ref));
+                    p[i] = (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * h + i], sc, -rr));
 #pragma unroll
                 for (int d = 0; d < DT; d++) o[d] = Xa<T>::mfma(vf[d], p, o[d]);
 #pragma unroll
@@ -364,7 +380,7 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
     /* join: lanes l and l ^ 32 hold half of a row's sum each */
     l += xor32_f32(l, lane);
     float *E = (float *)smem + wid * 32 * ES;
-    float *ML = (float *)smem + NW * 32 * ES;       /* per wave 32 references, 32 sums */
+    float *ML = (float *)smem + NW * 32 * ES;       /* per wave 32 references, 32 sums, 32 remainders of the references */
     if (QW == 1) __syncthreads();                    /* slices still reading their stages */
 #pragma unroll
     for (int d = 0; d < DT; d++)
@@ -372,7 +388,7 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
         for (int r = 0; r < 4; r++)
             *reinterpret_cast<float4 *>(E + l32 * ES + 32 * d + 8 * r + 4 * g) =
                 make_float4(o[d][4 * r], o[d][4 * r + 1], o[d][4 * r + 2], o[d][4 * r + 3]);
-    if (KS > 1 && g == 0) { ML[wid * 64 + l32] = ref; ML[wid * 64 + 32 + l32] = l; }
+    if (KS > 1 && g == 0) { ML[wid * 96 + l32] = ref; ML[wid * 96 + 32 + l32] = l; ML[wid * 96 + 64 + l32] = lo; }
     __syncthreads();
 
     /* a group of CPR lanes finishes one row, 8 dims per lane; the KS waves of a block of rows take them in turn */
@@ -381,24 +397,35 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
 #pragma unroll 1
     for (int i = ks; i < 32 / RPW; i += KS) {
         const int q = i * RPW + lane / CPR;          /* row within the block */
-        float v[8], rs, rm;
+        float v[8], rs, rm, rl;
         if constexpr (KS == 1) {
             const float *e = E + q * ES + c8;
 #pragma unroll
             for (int j = 0; j < 8; j++) v[j] = e[j];
             rs = __shfl(l, q, 64);
             rm = __shfl(ref, q, 64);
+            rl = __shfl(lo, q, 64);
         } else {
-            rm = XA_MIN;
+            float m[KS], c[KS];
 #pragma unroll
-            for (int w = 0; w < KS; w++) rm = fmaxf(rm, ML[(w * QW + qw) * 64 + q]);
+            for (int w = 0; w < KS; w++) {
+                m[w] = ML[(w * QW + qw) * 96 + q];
+                c[w] = ML[(w * QW + qw) * 96 + 64 + q];
+            }
+            rm = m[0];                               /* the largest reference, and of those that have it the largest remainder */
+            rl = c[0];
+#pragma unroll
+            for (int w = 1; w < KS; w++) {
+                rl = m[w] > rm ? c[w] : m[w] == rm ? fmaxf(rl, c[w]) : rl;
+                rm = fmaxf(rm, m[w]);
+            }
             rs = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; j++) v[j] = 0.0f;
 #pragma unroll
             for (int w = 0; w < KS; w++) {
-                const float f = __builtin_amdgcn_exp2f(ML[(w * QW + qw) * 64 + q] - rm);
-                rs = __builtin_fmaf(f, ML[(w * QW + qw) * 64 + 32 + q], rs);
+                const float f = __builtin_amdgcn_exp2f((m[w] - rm) + (c[w] - rl));
+                rs = __builtin_fmaf(f, ML[(w * QW + qw) * 96 + 32 + q], rs);
                 const float *e = (const float *)smem + ((w * QW + qw) * 32 + q) * ES + c8;
 #pragma unroll
                 for (int j = 0; j < 8; j++) v[j] = __builtin_fmaf(f, e[j], v[j]);
@@ -410,7 +437,7 @@ __global__ __launch_bounds__(64 * QW * KS) void k_xattn(XaArgs x) {
             float *P = x.part + (size_t)(t * x.ns + split) * xa_part(DP);
             *reinterpret_cast<float4 *>(P + q * DP + c8) = make_float4(v[0], v[1], v[2], v[3]);
             *reinterpret_cast<float4 *>(P + q * DP + c8 + 4) = make_float4(v[4], v[5], v[6], v[7]);
-            if (c8 == 0) { P[32 * DP + q] = rm; P[32 * DP + 32 + q] = rs; }
+            if (c8 == 0) { P[32 * DP + q] = rm; P[32 * DP + 32 + q] = rs; P[32 * DP + 64 + q] = rl; }
             continue;
         }
         const float inv = rs > 0.0f ? 1.0f / rs : 0.0f;
@@ -444,15 +471,21 @@ __global__ __launch_bounds__(64) void k_xattn_join(XaArgs x) {
     const float *P = x.part + (size_t)t * x.ns * xa_part(DP);
     const int n = a.kv_len ? min(max(a.kv_len[b], 0), a.Nk) : a.Nk;
     const int ns = max(1, (n + x.per * xa_tile(DP) - 1) / (x.per * xa_tile(DP)));   /* the splits that hold keys */
-    float m = XA_MIN;
-    for (int s = lane; s < ns; s += 64) m = fmaxf(m, P[(size_t)s * xa_part(DP) + 32 * DP + q]);
-    m = grp_max<64>(m);
+    float m = XA_MIN, ml = -INFINITY;                          /* the largest reference and its largest remainder */
+    for (int s = lane; s < ns; s += 64) {
+        const float *p = P + (size_t)s * xa_part(DP) + 32 * DP + q;
+        ml = p[0] > m ? p[64] : p[0] == m ? fmaxf(ml, p[64]) : ml;
+        m = fmaxf(m, p[0]);
+    }
+    const float ma = grp_max<64>(m);
+    ml = grp_max<64>(m == ma ? ml : -INFINITY);
+    m = ma;
     float rs = 0.0f, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (c8 < a.D)
 #pragma unroll 4
         for (int s = grp; s < ns; s += NG) {
             const float *p = P + (size_t)s * xa_part(DP);
-            const float f = __builtin_amdgcn_exp2f(p[32 * DP + q] - m);
+            const float f = __builtin_amdgcn_exp2f((p[32 * DP + q] - m) + (p[32 * DP + 64 + q] - ml));
             rs = __builtin_fmaf(f, p[32 * DP + 32 + q], rs);
             const float4 u = *reinterpret_cast<const float4 *>(p + q * DP + c8), w = *reinterpret_cast<const float4 *>(p + q * DP + c8 + 4);
             const float e[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};

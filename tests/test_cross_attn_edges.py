@@ -52,3 +52,39 @@ def test_many_small_weights(hip, B, H, Hkv, Nq, Nk, D):
     tol = Nk * 2.0 ** -31.5 * vv.max() + tolerance(want, mag, qv, kv, 0 * vv, "f16", "f32", 1 / np.sqrt(D), 0)
     assert (tol < 0.1 * want).all()
     assert (np.abs(got - want) <= tol).all(), (got.min(), want.min())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("B,H,Hkv,Nq,Nk,D", FORMS)
+def test_far_scores(hip, t, sign, B, H, Hkv, Nq, Nk, D):
+    """Scores so large that fp32's steps are 64: q and k are such that every score is exact, so a row's weights are those of
+    its largest keys alone, equal where they tie."""
+    print(f"[gpu] far scores {t} {sign} {B} {H}/{Hkv} {Nq} {Nk} {D}", flush=True)
+    r = rng(Nq + Nk)
+    q = np.zeros((B, H, Nq, D), np.float32)
+    k = np.zeros((B, Hkv, Nk, D), np.float32)
+    q[..., 0] = 32768
+    k[..., 0] = sign * 128 * r.integers(248, 256, (B, Hkv, Nk))   # scores just under 2^30 in size, whole multiples of 64, fp32's step
+    q[..., 1] = 8 * r.integers(0, 2, (B, H, Nq))                  # there; in half of the rows the largest are a few steps apart
+    k[..., 1] = 8 * r.integers(0, 4, (B, Hkv, Nk))
+    (q, qv), (k, kv), (v, vv) = cast(q, t), cast(k, t), cast(randn(r, (B, Hkv, Nk, D)), t)
+    got = run(hip, t, q, k, v, out="f32", scale=1.0)
+    want, mag = mx4.cross_attention(qv, kv, vv, scale=1.0)
+    # the weights are 1 / ties of each row, exact before the sum's rounding and the division
+    tol = (Nk + 8) * 2.0 ** -23 * (mag + np.abs(want))
+    assert (np.abs(got - want) <= tol).all(), np.abs(got - want).max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Nq", [1, 200])
+def test_lowest_scores(hip, Nq):
+    """bf16: every score -1.375 x 2^127, which in base 2 is just inside fp32: the mean of the values, not a row without weight."""
+    r = rng(Nq)
+    q, k = np.zeros((1, 2, Nq, 64), np.float32), np.zeros((1, 2, 300, 64), np.float32)
+    q[..., 3], k[..., 3] = -2.0 ** 63, 1.375 * 2.0 ** 64
+    (q, _), (k, _), (v, vv) = cast(q, "bf16"), cast(k, "bf16"), cast(randn(r, (1, 2, 300, 64)), "bf16")
+    got = run(hip, "bf16", q, k, v, out="f32", scale=1.0)
+    want = np.broadcast_to(vv.astype(np.float64).mean(2)[:, None], (1, Nq, 2, 64))
+    assert (np.abs(got - want) <= 308 * 2.0 ** -23 * np.abs(vv).max()).all()
