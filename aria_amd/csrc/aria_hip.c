@@ -644,12 +644,18 @@ int aria_hip_glu_mx4_dev(void *dy, int ytype, const void *dx, int xtype, int64_t
 }
 
 /* cross attention over ragged encoder states (k_xattn.hip) */
-static int xattn_check(const aria_hip_cross_attn *a) {
-    REQ(a && (a->type == 1 || a->type == 2));
+static int xattn_check_sizes(const aria_hip_cross_attn *a) {
+    REQ(a);
     REQ(a->B >= 0 && a->H > 0 && a->Hkv > 0 && a->H % a->Hkv == 0 && a->Nq >= 0 && a->Nk >= 0);
     REQ(a->D >= 8 && a->D <= 128 && a->D % 8 == 0);
     REQ(a->Nk <= (1 << 30) && (int64_t)a->B * a->H <= (1 << 20));
     REQ((int64_t)a->B * a->H * a->Nq <= (1 << 30));
+    return 0;
+}
+static int xattn_check(const aria_hip_cross_attn *a) {
+    const int r = xattn_check_sizes(a);
+    if (r) return r;
+    REQ(a->type == 1 || a->type == 2);
     REQ(a->B == 0 || a->Nq == 0 || (a->q && a->out && (a->Nk == 0 || (a->k && a->v))));
     REQ((((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->out) & 15u) == 0);
     REQ(((uintptr_t)a->kv_len & 3u) == 0);
@@ -661,7 +667,7 @@ static int xattn_check(const aria_hip_cross_attn *a) {
     return 0;
 }
 size_t aria_hip_cross_attention_ws_bytes(const aria_hip_cross_attn *a) {
-    if (xattn_check(a) || a->B == 0 || a->Nq == 0) return 0;
+    if (xattn_check_sizes(a) || a->B == 0 || a->Nq == 0) return 0;
     return aria_k_xattn_ws_bytes(a);
 }
 int aria_hip_cross_attention_dev(const aria_hip_cross_attn *a, void *dws, void *stream) {

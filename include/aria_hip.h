@@ -235,7 +235,8 @@ int aria_hip_attention_f16(float *out, const float *q, const float *k, const flo
  * are rounded to the type before they multiply v, whatever out's type; in fp16 one below 2^-32 of its
  * row's largest may count as zero. Sums and softmax statistics are fp32.
  * dws: aria_hip_cross_attention_ws_bytes(a) bytes (0: may be NULL), 256-byte aligned, not shared
- * by calls that may run at the same time. No counterpart in the reference, whose attention takes
+ * by calls that may run at the same time; the number goes by B, H, Hkv, Nq, Nk and D alone, so a
+ * program can ask for it before the rest of the description stands (0 for sizes that are refused). No counterpart in the reference, whose attention takes
  * one length (src/aria_ops.h:135). */
 typedef struct {
     const void *q, *k, *v;

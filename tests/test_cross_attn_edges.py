@@ -7,12 +7,32 @@ import pytest
 
 from conftest import randn, rng
 from oracle import mx4
-from test_cross_attn import cast, run, tolerance
+from test_cross_attn import cast, describe, run, tolerance
 
 # every form of workgroup: four slices of one wave (split over workgroups too), four waves and two slices, four waves, eight
 FORMS = [(1, 8, 2, 3, 700, 64), (1, 4, 4, 5, 700, 128), (1, 16, 8, 1100, 600, 64), (2, 8, 8, 1025, 300, 128), (3, 16, 16, 1000, 300, 64),
          (3, 16, 16, 1000, 200, 72), (8, 16, 16, 2050, 100, 64)]
 
+
+# ---- CPU ----
+
+def test_workspace_before_the_pointers():
+    """The workspace of a call goes by its sizes: a description without pointers, strides, type or scale gives the same
+    number, and not the 0 that says that there is none."""
+    import aria_amd
+    L = aria_amd.lib()
+    sizes = dict(B=16, H=16, Hkv=4, Nq=1, Nk=8192, D=128)
+    full = describe(aria_amd, "bf16", *sizes.values())
+    full.q = full.k = full.v = full.out = 4096
+    want = L.aria_hip_cross_attention_ws_bytes(full)
+    assert want > 0
+    assert L.aria_hip_cross_attention_ws_bytes(aria_amd.CrossAttention(**sizes)) == want
+    assert L.aria_hip_cross_attention_ws_bytes(aria_amd.CrossAttention(**{**sizes, "D": 12})) == 0
+    bare = aria_amd.CrossAttention(**sizes)
+    assert L.aria_hip_cross_attention_dev(bare, 4096, None) == -1       # still refused as a call
+
+
+# ---- GPU ----
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("t", ["f16", "bf16"])
