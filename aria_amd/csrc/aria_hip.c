@@ -663,7 +663,7 @@ static int xattn_check(const aria_hip_cross_attn *a) {
                        a->v_head | a->v_token | a->o_batch | a->o_head | a->o_token;
     REQ(st >= 0 && st % 8 == 0);
     REQ(!a->mask || a->mask_stride >= 0);
-    REQ(a->scale > 0.0f && a->scale < HUGE_VALF);
+    REQ(a->scale > 0.0f && a->scale <= 0x1p127f);   /* times log2 e still finite */
     return 0;
 }
 size_t aria_hip_cross_attention_ws_bytes(const aria_hip_cross_attn *a) {

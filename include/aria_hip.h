@@ -228,7 +228,7 @@ int aria_hip_attention_f16(float *out, const float *q, const float *k, const flo
  * not valid may hold anything (Inf and NaN included): they do not reach the result, but all Nk
  * rows must be readable memory. type: 1 = fp16, 2 = bf16 (aria_dtype's values) for q, k, v and
  * out; out_f32 != 0 writes fp32. D: a multiple of 8 up to 128. H a multiple of Hkv. B * H at most
- * 2^20, B * H * Nq and Nk at most 2^30. scale: positive and finite.
+ * 2^20, B * H * Nq and Nk at most 2^30. scale: positive, at most 2^127.
  * Strides count elements and are multiples of 8, not negative, pointers are 16-byte aligned (for
  * an fp32 out too); batch / head / token strides of q, k and v may be 0 (broadcast); rows of out lie
  * apart from each other and from every input. Probabilities

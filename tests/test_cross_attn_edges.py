@@ -32,6 +32,15 @@ def test_workspace_before_the_pointers():
     assert L.aria_hip_cross_attention_dev(bare, 4096, None) == -1       # still refused as a call
 
 
+@pytest.mark.parametrize("scale,taken", [(2.0 ** 127, True), (2.0 ** 127 * 1.0625, False), (3.4e38, False)])
+def test_largest_scale(scale, taken):
+    """Scores are taken times scale log2 e, which has to be finite itself: a score of 0 would be NaN. (No rows: a call that
+    is taken has nothing to do.)"""
+    import aria_amd
+    a = describe(aria_amd, "bf16", 1, 1, 1, 0, 8, 64, scale)
+    assert aria_amd.lib().aria_hip_cross_attention_dev(a, None, None) == (0 if taken else -1)
+
+
 # ---- GPU ----
 
 @pytest.mark.gpu
