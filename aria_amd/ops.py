@@ -319,6 +319,13 @@ def _mx4(q, s, K):
     return q, s
 
 
+def _bias(b, rows):
+    b = _f32(b)
+    if b is not None and b.shape != (rows,):
+        raise ValueError(f"the bias holds one value per weight row, [{rows}]: got {b.shape}")
+    return b
+
+
 def mx4_dequant(q, s, K):
     q, s = _mx4(q, s, K)
     y = np.empty((q.shape[0], K), np.float32)
@@ -328,9 +335,10 @@ def mx4_dequant(q, s, K):
 
 def linear_mx4(x, q, s, b=None):
     """y = Q(x) W^T + b: x [M, K] quantised to MXFP4 in the call, W packed [N rows]."""
-    x = _f32(x); b = _f32(b)
+    x = _f32(x)
     M, K = x.shape
     q, s = _mx4(q, s, K)
+    b = _bias(b, q.shape[0])
     y = np.empty((M, q.shape[0]), np.float32)
     check(lib().aria_hip_linear_mx4(_p(y), _p(x), _p(q), _p(s), _p(b), M, K, q.shape[0]), "aria_hip_linear_mx4")
     return y
@@ -338,9 +346,10 @@ def linear_mx4(x, q, s, b=None):
 
 def glu_mx4(x, q, s, b=None):
     """v * silu(g) with [v | g] = Q(x) W^T + b, W packed [2 * inner rows]."""
-    x = _f32(x); b = _f32(b)
+    x = _f32(x)
     M, K = x.shape
     q, s = _mx4(q, s, K)
+    b = _bias(b, q.shape[0])
     inner = q.shape[0] // 2
     if q.shape[0] != 2 * inner:
         raise ValueError("a gated projection has an even number of weight rows")

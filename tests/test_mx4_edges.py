@@ -1,6 +1,7 @@
 """MXFP4 at the edges of what its entry points take: row counts, packs, gates. Refusals run on the CPU."""
 from __future__ import annotations
 
+import numpy as np
 import pytest
 
 
@@ -36,3 +37,13 @@ def test_products_refused(M, N):
     assert L.aria_hip_gemm_mx4_dev(p, 1, p, p, p, p, None, M, 32, N, None) == -1 and "MX4_FITS" in aria_amd.last_error()
     for fn in (L.aria_hip_linear_mx4, L.aria_hip_glu_mx4):
         assert fn(p, p, p, p, None, M, 32, N) == -1 and "MX4_FITS" in aria_amd.last_error()
+
+
+@pytest.mark.parametrize("shape", [(3,), (5,), (1,), (0,), (4, 1), ()])
+def test_bias_of_another_size(shape):
+    """The numpy forms read one bias per weight row: another number of them is refused, not read past its end."""
+    from aria_amd import ops
+    x, q, s = np.zeros((2, 32), np.float32), np.zeros((4, 16), np.uint8), np.zeros((4, 1), np.uint8)
+    for fn in (ops.linear_mx4, ops.glu_mx4):
+        with pytest.raises(ValueError, match="bias"):
+            fn(x, q, s, np.zeros(shape, np.float32))
