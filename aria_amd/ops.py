@@ -367,7 +367,7 @@ def cross_attention(q, k, v, kv_len=None, mask=None):
     if k.shape != (B, Hkv, Nk, D) or v.shape != k.shape:
         raise ValueError(f"k and v are [{B}, Hkv, Nk, {D}]: got {k.shape} and {v.shape}")
     if kv_len is not None:
-        kv_len = np.ascontiguousarray(kv_len, np.int32)
+        kv_len = np.ascontiguousarray(np.clip(kv_len, 0, Nk), np.int32)   # in the type they come in: 2^32 is not 0
         if kv_len.shape != (B,):
             raise ValueError(f"kv_len holds one length per sequence: got {kv_len.shape}")
     if mask is not None:

@@ -41,6 +41,23 @@ def test_largest_scale(scale, taken):
     assert aria_amd.lib().aria_hip_cross_attention_dev(a, None, None) == (0 if taken else -1)
 
 
+@pytest.mark.parametrize("lens,want", [([2 ** 32, 2 ** 32 + 3], [5, 5]), ([-2 ** 40, 2], [0, 2]), ([3.0, 1e12], [3, 5])])
+def test_lengths_of_other_types(monkeypatch, lens, want):
+    """Lengths past 32 bits are clamped to 0..Nk like any other, not cut off to their low bits."""
+    import ctypes
+    from aria_amd import ops
+    seen = []
+
+    class Lib:
+        def aria_hip_cross_attention_f16(self, out, q, k, v, kv_len, mask, *sizes):
+            seen.extend(ctypes.cast(kv_len, ctypes.POINTER(ctypes.c_int32))[:2])
+            return 0
+    monkeypatch.setattr(ops, "lib", Lib)
+    z = np.zeros((2, 1, 5, 64), np.float32)
+    ops.cross_attention(z, z, z, kv_len=lens)
+    assert seen == want
+
+
 # ---- GPU ----
 
 @pytest.mark.gpu
