@@ -321,7 +321,7 @@ def _mx4(q, s, K):
 
 def _bias(b, rows):
     b = _f32(b)
-    if b is not None and b.shape != (rows,):
+    if b is not None and b.size != rows:
         raise ValueError(f"the bias holds one value per weight row, [{rows}]: got {b.shape}")
     return b
 

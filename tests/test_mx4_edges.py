@@ -39,7 +39,7 @@ def test_products_refused(M, N):
         assert fn(p, p, p, p, None, M, 32, N) == -1 and "MX4_FITS" in aria_amd.last_error()
 
 
-@pytest.mark.parametrize("shape", [(3,), (5,), (1,), (0,), (4, 1), ()])
+@pytest.mark.parametrize("shape", [(3,), (5,), (1,), (0,), (2, 4), ()])
 def test_bias_of_another_size(shape):
     """The numpy forms read one bias per weight row: another number of them is refused, not read past its end."""
     from aria_amd import ops
