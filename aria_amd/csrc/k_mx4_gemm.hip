@@ -446,7 +446,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
 #pragma unroll
                 for (int e = 0; e < V; e++) {
                     v[e] += bias[e];
-                    if constexpr (GLU) v[e] *= silu_f(g[e] + gbias[e]);
+                    if constexpr (GLU) v[e] *= mx_silu<V == 4>(g[e] + gbias[e]);   /* V = 4: fp32 out */
                 }
                 if (m < a.M && n < a.N) mx_store_row<V>(a, m, n, v);
             }
@@ -557,7 +557,7 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_rows(MxArgs a, const void *x, l
         if (a.bias) v += a.bias[n0 + c];
         if constexpr (GLU) {
             if (a.bias) g += a.bias[a.N + n0 + c];
-            v *= silu_f(g);
+            v *= a.ytype == MX_F32 ? mx_silu<true>(g) : mx_silu<false>(g);
         }
         mx_store(a.y, a.ytype, (size_t)(m0 + m) * a.N + n0 + c, v);
     }

@@ -4,6 +4,10 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
+from conftest import randn, rng
+from oracle import mx4
+from test_mx4 import run_linear
+
 
 # ---- CPU ----
 
@@ -47,3 +51,35 @@ def test_bias_of_another_size(shape):
     for fn in (ops.linear_mx4, ops.glu_mx4):
         with pytest.raises(ValueError, match="bias"):
             fn(x, q, s, np.zeros(shape, np.float32))
+
+
+# ---- GPU ----
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 40, 300, 1300])
+def test_gate_far_from_zero(hip, M):
+    """SiLU of gates from -85 to 85 in fp32. Products are zero, so the gates are the biases, exactly, and the values 1:
+    exp2 and rcp are a step (two half steps) each, the factor and the four products and sums half a step each: 9 half steps, whatever
+    the gate."""
+    r = rng(M)
+    K, N = 96, 2050
+    q, s = mx4.quant(randn(r, (2 * N, K)))
+    b = np.concatenate([np.ones(N), np.linspace(-85, 85, N)]).astype(np.float32)
+    got = run_linear(hip, "aria_hip_glu_mx4_dev", np.zeros((M, K), np.float32), "f32", K, q, s, b, M, K, N, "f32")
+    g = b[N:].astype(np.float64)
+    want = g / (1 + np.exp(-g))
+    assert (np.abs(got - want) <= 9.01 * 2.0 ** -24 * np.abs(want)).all(), (np.abs(got - want) / np.abs(want)).max() * 2 ** 24
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 200])
+def test_gate_limits(hip, M):
+    """Gates past e^-g's range: v g above, nothing below; an infinite gate gives v times infinity, or NaN as -Inf / Inf does."""
+    K = 32
+    gates = np.array([88.0, 104.5, 3e38, np.inf, -104.5, -3e38, -np.inf, np.nan, 0.0], np.float32)
+    N = len(gates)
+    q, s = mx4.quant(np.zeros((2 * N, K)))
+    b = np.concatenate([np.full(N, 0.5, np.float32), gates])
+    got = run_linear(hip, "aria_hip_glu_mx4_dev", np.zeros((M, K), np.float32), "f32", K, q, s, b, M, K, N, "f32")
+    want = np.array([44.0, 52.25, 1.5e38, np.inf, 0, 0, np.nan, np.nan, 0])
+    assert np.allclose(got, want[None], rtol=2.0 ** -21, atol=0, equal_nan=True)
