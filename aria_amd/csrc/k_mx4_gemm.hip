@@ -74,6 +74,14 @@ __device__ __forceinline__ uint32_t fresh_s(uint32_t v) {
     return v;
 }
 
+/* LDS written by some lanes of a wave stands for its other lanes behind this, and what was read before it has been: LDS is in
+ * order within a wave, so only the compiler has to keep the order, and no instruction comes of it */
+__device__ __forceinline__ void wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 /*
  * WK groups of WM x WN waves; a group's waves share LDS stages and take one of WK parts of K; a wave owns
  * FM x FN blocks of 32 x 32 outputs (GLU: the first half of its FN are value rows, the second half
@@ -410,13 +418,15 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mx4_gemm(MxArgs a) {
     __syncthreads();                                             /* stages still being read */
     static_for<FM>([&](auto I) __attribute__((always_inline)) {
         constexpr int i = decltype(I)::value;
-        if constexpr (i > 0 && WK > 1) __syncthreads();          /* parts still being read */
+        if constexpr (WK == 1) wave_order();                     /* a wave reads what it has written itself */
+        else if constexpr (i > 0) __syncthreads();               /* parts still being read */
         static_for<4 * FN>([&](auto JE) __attribute__((always_inline)) {
             constexpr int j = decltype(JE)::value / 4, e = decltype(JE)::value % 4;
             *reinterpret_cast<float4 *>(E + el32 * ES + 32 * j + 8 * e + 4 * eh) =
                 make_float4(acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]);
         });
-        if constexpr (WK > 1) __syncthreads();
+        if constexpr (WK == 1) wave_order();
+        else __syncthreads();
         /* 16 bytes of a row per lane: V columns */
         auto rows = [&](auto VV) __attribute__((always_inline)) {
             constexpr int V = decltype(VV)::value, LPR = OW / V, RPI = 64 / LPR;   /* lanes per row, rows per wave at once */

@@ -1,4 +1,6 @@
-"""CPU: no VALU instruction written as inline asm reads the result of a 32x32 16-bit MFMA before it stands. The compiler
+"""CPU: what the compiled kernels' assembly has to hold where no run would show its absence reliably.
+
+No VALU instruction written as inline asm reads the result of a 32x32 16-bit MFMA before it stands. The compiler
 puts the wait states that gfx950 asks for (12 behind an MFMA of eight passes) only in front of instructions of its
 own, so a kernel's inline asm has to stay clear of fresh accumulators. Read from the assembly that the Makefile's
 flags give, along every path of every kernel."""
@@ -102,12 +104,33 @@ def test_the_reader():
     assert [(r, d) for _, _, r, d in early_reads(parse(text)["k"])] == [(4, 2)]
 
 
-@pytest.mark.skipif(not shutil.which(os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")), reason="no hipcc")
-@pytest.mark.parametrize("kernel", ["k_xattn", "k_attn"])
-def test_inline_asm_behind_mfma(tmp_path, kernel):
+hipcc = pytest.mark.skipif(not shutil.which(os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")), reason="no hipcc")
+
+
+def assembly(tmp_path, kernel):
     subprocess.run(["make", "-C", CSRC, f"OBJDIR={tmp_path}", f"{tmp_path}/{kernel}.s"], check=True, capture_output=True)
     with open(tmp_path / f"{kernel}.s") as f:
-        kernels = parse(f.read())
+        return f.read()
+
+
+@hipcc
+@pytest.mark.parametrize("kernel", ["k_xattn", "k_attn"])
+def test_inline_asm_behind_mfma(tmp_path, kernel):
+    kernels = parse(assembly(tmp_path, kernel))
     assert any(op.startswith("v_mfma") for b in kernels.values() for _, ins in b for _, op, _, _ in ins)
     bad = {name: r[:3] for name, b in kernels.items() if (r := early_reads(b))}
     assert not bad, bad
+
+
+@hipcc
+def test_order_within_a_wave(tmp_path):
+    """The MXFP4 products of one K group stage their output in LDS wave by wave, without a workgroup's barrier: around each
+    of the FM blocks of rows the compiler is told of the order (its wave barrier, no instruction)."""
+    text = assembly(tmp_path, "k_mx4_gemm")
+    seen = 0
+    for body in re.split(r"(?m)^(?=_Z\w+:)", text)[1:]:
+        m = re.match(r"_Z10k_mx4_gemmILi(\d+)ELi\d+ELi\d+ELi\d+ELi(\d+)E", body)
+        if m and int(m[2]) == 1:
+            seen += 1
+            assert body.split(".end_amdhsa_kernel")[0].count("; wave barrier") >= 2 * int(m[1]), body[:60]
+    assert seen >= 6
