@@ -224,20 +224,22 @@ int aria_hip_attention_f16(float *out, const float *q, const float *k, const flo
  * o[b,t,h,:] = sum_j p_j v[b,j,h / (H/Hkv),:], p = softmax over the valid keys j of
  * scale * q[b,t,h,:] . k[b,j,h / (H/Hkv),:]. Key j of sequence b is valid when j < kv_len[b] (kv_len
  * NULL: Nk; values are taken as clamped to 0..Nk) and mask[b * mask_stride + j] != 0 (mask NULL:
- * all). A row with no valid key (Nk = 0 included) is written as zeros. Keys and values that are
- * not valid may hold anything (Inf and NaN included): they do not reach the result, but all Nk
- * rows must be readable memory. type: 1 = fp16, 2 = bf16 (aria_dtype's values) for q, k, v and
- * out; out_f32 != 0 writes fp32. D: a multiple of 8 up to 128. H a multiple of Hkv. B * H at most
- * 2^20, B * H * Nq and Nk at most 2^30. scale: positive, at most 2^127.
+ * all). A row with no valid key (Nk = 0 included), or of a finite query whose valid keys all score
+ * -Inf, is written as zeros. Keys and values that are not valid may hold anything (Inf and NaN
+ * included): they do not reach the result, but all Nk rows must be readable memory. type: 1 = fp16,
+ * 2 = bf16 (aria_dtype's values) for q, k, v and out; out_f32 != 0 writes fp32. D: a multiple of 8
+ * up to 128. H a multiple of Hkv. B * H at most 2^20, B * H * Nq and Nk at most 2^30. scale:
+ * positive, at most 2^127.
  * Strides count elements and are multiples of 8, not negative, pointers are 16-byte aligned (for
  * an fp32 out too); batch / head / token strides of q, k and v may be 0 (broadcast); rows of out lie
- * apart from each other and from every input. Probabilities
- * are rounded to the type before they multiply v, whatever out's type; in fp16 one below 2^-32 of its
- * row's largest may count as zero. Sums and softmax statistics are fp32.
+ * apart from each other and from every input.
+ * Probabilities are rounded to the type before they multiply v, whatever out's type; in fp16 one
+ * below 2^-32 of its row's largest may count as zero (an infinite value under one gives NaN). Sums
+ * and softmax statistics are fp32.
  * dws: aria_hip_cross_attention_ws_bytes(a) bytes (0: may be NULL), 256-byte aligned, not shared
  * by calls that may run at the same time; the number goes by B, H, Hkv, Nq, Nk and D alone, so a
- * program can ask for it before the rest of the description stands (0 for sizes that are refused). No counterpart in the reference, whose attention takes
- * one length (src/aria_ops.h:135). */
+ * program can ask for it before the rest of the description stands (0 for sizes that are refused).
+ * No counterpart in the reference, whose attention takes one length (src/aria_ops.h:135). */
 typedef struct {
     const void *q, *k, *v;
     void *out;

@@ -134,3 +134,74 @@ def test_lowest_scores(hip, Nq):
     got = run(hip, "bf16", q, k, v, out="f32", scale=1.0)
     want = np.broadcast_to(vv.astype(np.float64).mean(2)[:, None], (1, Nq, 2, 64))
     assert (np.abs(got - want) <= 308 * 2.0 ** -23 * np.abs(vv).max()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("B,H,Hkv,Nq,Nk,D", [(2, 4, 2, 1, 200, 64), (2, 4, 2, 3, 900, 128), (2, 4, 2, 300, 200, 64), (2, 8, 4, 1000, 300, 72)])
+def test_not_finite(hip, t, B, H, Hkv, Nq, Nk, D):
+    """Inf and NaN in queries, valid keys and values go where the definition takes them, and change no bit elsewhere."""
+    print(f"[gpu] not finite {t} {Nq} {Nk} {D}", flush=True)
+    r = rng(Nq + D)
+    G = H // Hkv
+    qf, kf, vf = randn(r, (B, H, Nq, D)), randn(r, (B, Hkv, Nk, D)), randn(r, (B, Hkv, Nk, D))
+    plain = run(hip, t, cast(qf, t)[0], cast(kf, t)[0], cast(vf, t)[0], out="f32")
+
+    def check(q, k, v, touched):
+        with np.errstate(invalid="ignore"):
+            (q, qv), (k, kv), (v, vv) = bits(q, t), bits(k, t), bits(v, t)
+            got = run(hip, t, q, k, v, out="f32")
+            want, mag = mx4.cross_attention(qv, kv, vv)
+        same = np.ones(got.shape, bool)
+        same[touched] = False
+        assert np.array_equal(got[same], plain[same])
+        assert np.array_equal(np.isnan(got), np.isnan(want))
+        assert np.array_equal(np.isposinf(got), np.isposinf(want)) and np.array_equal(np.isneginf(got), np.isneginf(want))
+        ok = np.isfinite(want)
+        clean = [np.where(np.isfinite(x), x, 0) for x in (qv, kv, vv)]
+        tol = tolerance(want, np.where(np.isfinite(mag), mag, 0), *clean, t, "f32", 1 / np.sqrt(D), Nk)
+        assert (np.abs(got[ok] - want[ok]) <= tol[ok]).all()
+
+    h, j, d = H - 1, Nk - 3, 5
+    for bad in (np.nan, np.inf, -np.inf):
+        q = qf.copy()
+        q[0, h, Nq // 2, d] = bad
+        check(q, kf, vf, np.s_[0, Nq // 2, h])              # one row, NaN: some of its scores are +Inf, or all NaN
+        k = kf.copy()
+        k[1, h // G, j, d] = bad                            # a key without weight, or of all rows' NaN, by the query's sign
+        check(qf, k, vf, np.s_[1, :, h // G * G:(h // G + 1) * G])
+        v = vf.copy()
+        v[1, h // G, j, d] = bad                            # that dim of those heads
+        check(qf, kf, v, np.s_[1, :, h // G * G:(h // G + 1) * G, d])
+
+
+def bits(x, t):
+    """cast(), with Inf and NaN kept"""
+    if t == "f16":
+        return cast(x, t)
+    u = np.where(np.isfinite(x), mx4.bf16_bits(np.where(np.isfinite(x), x, 0)),
+                 np.where(np.isnan(x), 0x7FC0, np.where(x > 0, 0x7F80, 0xFF80))).astype(np.uint16)
+    return u, mx4.bf16_value(u)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("B,H,Hkv,Nq,Nk,D", FORMS)
+def test_no_score_above_minus_infinity(hip, t, B, H, Hkv, Nq, Nk, D):
+    """A row whose valid keys all score -Inf is zero, like one without valid keys; its neighbours are as they would be."""
+    print(f"[gpu] all -inf {t} {Nq} {Nk} {D}", flush=True)
+    r = rng(Nq)
+    qf, kf, vf = np.abs(randn(r, (B, H, Nq, D))) + 0.25, randn(r, (B, Hkv, Nk, D)), randn(r, (B, Hkv, Nk, D))
+    kf[B - 1, :, :, 7] = -np.inf                            # the last sequence's keys
+    qf[0, 0, 0] = 0.5
+    (q, qv), (k, kv), (v, vv) = bits(qf, t), bits(kf, t), bits(vf, t)
+    got = run(hip, t, q, k, v)
+    assert (got[B - 1] == 0).all()
+    if B > 1:
+        want, mag = mx4.cross_attention(qv[:-1], kv[:-1], vv[:-1])
+        assert (np.abs(got[:-1] - want) <= tolerance(want, mag, qv[:-1], kv[:-1], vv, t, t, 1 / np.sqrt(D), Nk)).all()
+    kf[B - 1, :, Nk // 2] = 0.25                            # one key of a finite score: it alone counts
+    k, kv = bits(kf, t)
+    got = run(hip, t, q, k, v)
+    alone = np.repeat(vv[B - 1, :, Nk // 2], H // Hkv, 0)
+    assert np.array_equal(got[B - 1], np.broadcast_to(alone, got[B - 1].shape))
