@@ -121,6 +121,10 @@ def test_far_scores(hip, t, sign, B, H, Hkv, Nq, Nk, D):
     # the weights are 1 / ties of each row, exact before the sum's rounding and the division
     tol = (Nk + 8) * 2.0 ** -23 * (mag + np.abs(want))
     assert (np.abs(got - want) <= tol).all(), np.abs(got - want).max()
+    lens, mask = r.integers(0, Nk + 1, B), (r.random((B, Nk)) < 0.5).astype(np.uint8)
+    got = run(hip, t, q, k, v, lens, mask, out="f32", layout="tokens", scale=1.0)
+    want, mag = mx4.cross_attention(qv, kv, vv, lens, mask, scale=1.0)
+    assert (np.abs(got - want) <= (Nk + 8) * 2.0 ** -23 * (mag + np.abs(want))).all()
 
 
 @pytest.mark.gpu

@@ -6,7 +6,7 @@ import pytest
 
 from conftest import randn, rng
 from oracle import mx4
-from test_mx4 import run_linear
+from test_mx4 import CODE, cast, np_type, run_linear, values
 
 
 # ---- CPU ----
@@ -83,3 +83,59 @@ def test_gate_limits(hip, M):
     got = run_linear(hip, "aria_hip_glu_mx4_dev", np.zeros((M, K), np.float32), "f32", K, q, s, b, M, K, N, "f32")
     want = np.array([44.0, 52.25, 1.5e38, np.inf, 0, 0, np.nan, np.nan, 0])
     assert np.allclose(got, want[None], rtol=2.0 ** -21, atol=0, equal_nan=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N", [(700, 512, 256), (17, 2048, 96), (344, 4096, 1024), (2592, 1024, 1030)])
+@pytest.mark.parametrize("xt,yt,bias", [("f32", "f32", True), ("bf16", "f16", False)])
+def test_quantised_apart_gives_the_same_bits(hip, M, K, N, xt, yt, bias):
+    """Where the linear takes two launches, quantising first and multiplying the packed operands is the same to the bit."""
+    from aria_amd.device import DeviceArray as DA, sync
+    L = hip.lib()
+    r = rng(M + N)
+    x, _ = cast(randn(r, (M, K)), xt)
+    q, s = mx4.quant(randn(r, (N, K)))
+    b = randn(r, N) if bias else None
+    want = run_linear(hip, "aria_hip_linear_mx4_dev", x, xt, K, q, s, b, M, K, N, yt)
+    dx, dq, ds = DA.from_host(x), DA.from_host(q), DA.from_host(s)
+    db = DA.from_host(b) if bias else None
+    xq, xs, dy = DA((M, K // 2), np.uint8), DA((M, K // 32), np.uint8), DA((M, N), np_type(yt))
+    hip.check(L.aria_hip_mx4_quant_dev(xq.p, xs.p, dx.p, CODE[xt], M, K, K, None))
+    hip.check(L.aria_hip_gemm_mx4_dev(dy.p, CODE[yt], xq.p, xs.p, dq.p, ds.p, db.p if bias else None, M, K, N, None))
+    sync()
+    assert np.array_equal(values(dy.to_host(), yt), want)
+
+
+@pytest.mark.gpu
+def test_rows_of_several_launches(hip):
+    """More rows than one launch of the quantiser takes (268435392 at K up to 32): the border between two launches, both
+    ends, and what lies behind the last row."""
+    from aria_amd.device import DeviceArray as DA, sync
+    L = hip.lib()
+    border, period = 268435392, 4096
+    rows = border + 70001
+    x = np.resize(np.ldexp(randn(rng(1), period), np.arange(period) % 20 - 10).astype(np.float16), rows)
+    want_q, want_s = mx4.quant(x[:period, None].astype(np.float32))
+    dx, dq, ds = DA.from_host(x), DA((rows + 8, 16), np.uint8), DA(rows + 8, np.uint8)
+    fill = np.full(128, 0xAB, np.uint8)
+    L.aria_cuda_memcpy_h2d(dq.p + 16 * rows, fill.ctypes.data, 128)
+    L.aria_cuda_memcpy_h2d(ds.p + rows, fill.ctypes.data, 8)
+    print(f"[gpu] mx4 quant rows {rows}", flush=True)
+    hip.check(L.aria_hip_mx4_quant_dev(dq.p, ds.p, dx.p, CODE["f16"], rows, 1, 1, None))
+    dy = DA(rows + 8, np.float16)
+    L.aria_cuda_memcpy_h2d(dy.p + 2 * rows, fill.ctypes.data, 16)
+    hip.check(L.aria_hip_mx4_dequant_dev(dy.p, CODE["f16"], dq.p, ds.p, rows, 1, None))
+    sync()
+
+    def part(d, first, n, size, dtype):
+        out = np.empty((n, size // np.dtype(dtype).itemsize), dtype)
+        L.aria_cuda_memcpy_d2h(out.ctypes.data, d.p + first * size, n * size)
+        return out
+    v = mx4.dequant(want_q, want_s, 1).astype(np.float16)
+    for first, n in ((0, 5000), (border - 5000, 10000), (rows - 5000, 5000)):
+        at = np.arange(first, first + n) % period
+        assert np.array_equal(part(dq, first, n, 16, np.uint8), want_q[at])
+        assert np.array_equal(part(ds, first, n, 1, np.uint8), want_s[at])
+        assert np.array_equal(part(dy, first, n, 2, np.float16), v[at])
+    assert (part(dq, rows, 8, 16, np.uint8) == 0xAB).all() and (part(ds, rows, 8, 1, np.uint8) == 0xAB).all()
+    assert (part(dy, rows, 8, 2, np.uint16) == 0xABAB).all()
