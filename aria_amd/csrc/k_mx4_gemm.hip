@@ -33,7 +33,8 @@ __device__ __forceinline__ uint4 mx_scale_end(const uint8_t *row, int b, int nb)
 }
 
 /* V results of one row from column n on: four fp32 or eight 16-bit values. Non-temporal: they are not read here, and in
- * the L2s they would take the operands' place (2592 x 1024 x 4096 to fp32 18.3 us, 15.1 so; 8192 x 1024 x 8192 108 and 82) */
+ * the L2s they would take the operands' place (2592 x 1024 -> 4096 to bf16 13.4 us, 14.6 else; to fp32 15.0 and 15.8; 8192 x
+ * 1024 -> 8192, 57 to bf16 and 69 to fp32, within 3 % either way) */
 template <int V>
 __device__ __forceinline__ void mx_store_row(const MxArgs &a, int m, int n, const float (&v)[V]) {
     const size_t at = (size_t)m * a.N + n;
@@ -86,13 +87,17 @@ __device__ __forceinline__ void wave_order() {
  * WK groups of WM x WN waves; a group's waves share LDS stages and take one of WK parts of K; a wave owns
  * FM x FN blocks of 32 x 32 outputs (GLU: the first half of its FN are value rows, the second half
  * the gate rows of the same columns). Chunks of 256 K (128 bytes of every row) move to LDS by DMA, NST stages;
- * chunk c of a row sits at c ^ ((row >> 1) & 7), so that fragment reads (32 rows x 16 bytes per lane half) are
- * free of bank conflicts. With two stages the next chunk moves under the current one's products; with one, the CU's other
+ * chunk c of a row sits at c ^ ((row >> 1) & 7), so that each eight lanes of a fragment read (32 rows x 16 bytes per lane half)
+ * meet every bank once. (The conflicts that are counted, a third of the LDS' active cycles at 8192 x 4096 x 8192, are 8 % in the
+ * form that reads the same fragments but no scales from LDS: they come from the scale dwords, 16 bytes apart, and
+ * the output's staging.) With two stages the next chunk moves under the current one's products; with one, the CU's other
  * workgroups fill the wait.
  * Barriers (none where a group is one wave) follow the wait for this wave's transfers and fragment reads, so behind one the
  * chunk is whole and, with two stages, the other stage free.
- * What bounds it: at 8192 x 4096 x 8192 the matrix pipes' power (the fp4 MFMA from registers reaches 6.6 - 6.9
- * PFLOP/s on random codes, 8.9 on zeros; the chunk loop 4.4, the launch with its prologue and output 3.4);
+ * What bounds it: at 8192 x 4096 x 8192 waiting: the matrix pipes are busy in 41 - 43 % of the launch's cycles, with one workgroup a
+ * CU whose waves all wait for their transfers and meet at every chunk (the fp4 MFMA from registers reaches 6.6 - 6.9
+ * PFLOP/s on random codes, 8.9 on zeros; the chunk loop 4.4, the launch with its prologue and output 3.6). Power shows
+ * in the clock, 1.9 - 2.0 GHz of 2.4 in that launch;
  * at a few rounds of tiles the latency of a tile's first chunk and of its output.
  */
 template <int FM, int FN, int WM, int WN, int WK, int NST, bool GLU>
@@ -585,7 +590,10 @@ static hipError_t launch(MxArgs a, hipStream_t s) {
 
 /* Which tile: the least estimated time, in us, over one launch. A configuration takes at least the latency of one tile, and where
  * there are many tiles the time that all CUs need for them; both grow with the chunks of K, the large tiles' also
- * with the bytes of output. Fitted to M = 17 .. 8192, N = 1024 .. 8192, K = 256 .. 8192 (within 25 % there, mostly 10 %).
+ * with the bytes of output. Fitted to M = 17 .. 8192, N = 1024 .. 8192, K = 256 .. 8192. Over 720 shapes there (both outputs' sizes,
+ * gated and not) the estimate of the form that is taken is 7 % off in the median, 21 % or less in nine of ten, 36 % at most, and the
+ * form within 5 % of the best one in 641, 10 % in 694, 26 % at most (1.5 % in the mean). A form far from being taken can be
+ * misjudged by much more (t64 by 50 %, t256 by 160 %).
  *  t32, t64: 32 x 32 (GLU: 32 x 64) and 64 x 64, K split over four one-wave groups, several workgroups to a CU;
  *  t128a, t128b: 128 x 128 in one stage, three workgroups to a CU, and in two stages, two to a CU, for long K and few tiles;
  *  t256: 256 x 256 in rounds of one to a CU.

@@ -93,7 +93,12 @@ __host__ __device__ constexpr int xa_part(int DP) { return 32 * DP + 96; }
  * QW > 1 there are two stages, the next tile moving under the current one's products. With QW = 1 a wave works by itself,
  * without barriers, is bound by the keys' bytes, and has one stage, so that two workgroups fit a CU (16 x 4 key heads x up to
  * 8192 keys of 128: 56 us with two stages and one workgroup, 45 with one and two, the join included); the next tile's keys
- * then move while this one's values are added, its values while the scores are made (45 to 42).
+ * then move while this one's values are added, its values while the scores are made (45 to 42). That overlap needs a call without a
+ * mask: the compiler waits for a mask byte with everything that is on its way, the next tile's transfers included (the
+ * same sequences, their keys in the last-level cache: 35.5 us with a mask that keeps 7 of 8 keys, 31.8 without).
+ * Widths other than 64 and 128 are padded to the next of the two, and their chunks past D are looked at in every transfer: 4 x 16 x
+ * 4096 rows x 2048 keys of 72 or 96 take 313 and 316 us, of 128 273, of 32 144 and of 64 148; one row over 16 x 4 x 8192
+ * keys of 72 46 us, of 96 50, of 128 46.
  * What bounds it: with many rows the VALU, 69 % busy beside the MFMAs' 46 % at 4 x 16 x 4096 rows x 2048 keys of 64 (0.88
  * PFLOP/s; an exponential, a fused multiply-add, half a maximum, half a conversion and half a dot product per score);
  * with a single row the keys' bytes (4.9 TB/s without the join); at a few tiles a wave the latency of one tile, about 1 us. */
@@ -513,8 +518,12 @@ __global__ __launch_bounds__(64) void k_xattn_join(XaArgs x) {
  *    fill, each reading the keys for itself (16 heads x 172 rows x 257 keys of 64: 6.2 us, 8.5 with qw 4; x 710 rows x 1024 keys: 25.2 and 14.5);
  *  qw 4, ks 2: up to a workgroup per CU, and up to 700 of them over long keys of 64 (2 x 16 x 710 rows x 257 keys: 8.9 us, 9.5 with
  *    one slice; 2 x 16 x 1296 x 1296: 29.1 and 31.4, of 128 54.2 and 49.4);
- *  qw 4, ks 1; and qw 8 where four rounds of 256 rows fill the CUs (4 x 16 x 4096 x 2048 of 64: 166 us with 4, 158 with 8; of 128,
- *    where 8 waves' registers fill the CU: 164 and 168). */
+ *  qw 4, ks 1; and qw 8, width 64, from four rounds of 256 rows on: it gains 3 - 7 % from two rounds on (2 x 16 x 4096 x 2048
+ *    82.5 and 77.8 us, 4 x 16 x 4096 x 2048 158 and 152, 8 x 16 x 3000 x 257 47.5 and 46.0) and loses below (1296 rows of 64 heads,
+ *    1.5 rounds, x 2048: 62.6 and 69.9); of 128, where 8 waves' registers fill the CU: 164 and 168.
+ * Over 444 shapes (8 to 128 heads in all, 40 to 4096 rows, 64 to 2048 keys, widths 64 and 128) the form taken is within 5 % of
+ * the best in 348 and 4 % behind in the mean. It is furthest behind at 64 to 128 blocks of 128 rows over 1300 keys and more, where
+ * single waves' slices would be faster (8 heads x 1296 x 2048: 23.1 us, 15.1 with qw 1). */
 struct XaPlan { int qw, ks, DP, nrb, T, ns, per; };
 static XaPlan xa_plan(const aria_k_xattn *a) {
     XaPlan p;

@@ -272,7 +272,8 @@ int aria_hip_cross_attention_f16(float *out, const float *q, const float *k, con
  * overlap no input. */
 int aria_hip_mx4_quant_dev(uint8_t *dq, uint8_t *dscale, const void *dx, int xtype, int rows, int K, int64_t ldx,
                            void *stream);
-/* y [rows, K] from packed rows, rounded to ytype (fp32 holds every value) */
+/* y [rows, K] from packed rows, rounded to ytype. fp32 holds every value of a pack made here; in one
+ * from elsewhere byte 253 with codes 4 and 6 and byte 254 with 2 and above lie past it: Inf. */
 int aria_hip_mx4_dequant_dev(void *dy, int ytype, const uint8_t *dq, const uint8_t *dscale, int rows, int K,
                              void *stream);
 /* dy[m,n] = sum_k x[m,k] w[n,k] (+ db[n]; db NULL = none) on packed activations [M, K] and weights
