@@ -39,6 +39,49 @@ class CrossAttention(C.Structure):
 
 _X = C.POINTER(CrossAttention)
 
+
+def _strides(*names):
+    return [(f"{n}_{axis}", _i64) for n in names for axis in ("batch", "token", "head")]
+
+
+class RotaryScaling(C.Structure):
+    """aria_hip_rotary_scaling of include/aria_hip.h: the frequencies of rotary positions."""
+    _fields_ = [("rot", _i), ("kind", _i)] + [(n, C.c_double) for n in ("base", "factor", "trained", "low", "high", "gain")]
+
+
+class Rotary(C.Structure):
+    """aria_hip_rotary of include/aria_hip.h: queries and keys rotated by table."""
+    _fields_ = ([(n, _P) for n in ("q", "k", "q_out", "k_out", "cos", "sin", "pos", "first")] + [("pos_stride", _i64)] +
+                [(n, _i) for n in ("type", "B", "N", "Hq", "Hk", "D", "rot", "npos", "interleaved", "inverse")] +
+                _strides("q", "k", "qo", "ko"))
+
+
+class KVCache(C.Structure):
+    """aria_hip_kv of include/aria_hip.h: keys and values as e4m3 rows."""
+    _fields_ = ([(n, _P) for n in ("k", "v", "k_scale", "v_scale")] +
+                [(n, _i64) for n in ("batch", "head", "token", "s_batch", "s_head")] +
+                [(n, _i) for n in ("B", "Hkv", "D", "cap")])
+
+
+class KVWrite(C.Structure):
+    """aria_hip_kv_write of include/aria_hip.h."""
+    _fields_ = ([("cache", KVCache)] + [(n, _P) for n in ("k", "v", "q", "q_out", "cos", "sin", "pos", "first", "count")] +
+                [("pos_stride", _i64)] + [(n, _i) for n in ("type", "N", "Hq", "rot", "npos", "interleaved")] +
+                _strides("k", "v", "q", "qo"))
+
+
+class KVRead(C.Structure):
+    """aria_hip_kv_read of include/aria_hip.h."""
+    _fields_ = ([("cache", KVCache)] + [(n, _P) for n in ("k", "v", "first", "count")] + [("type", _i), ("N", _i)] +
+                _strides("k", "v"))
+
+
+class PrefixAttention(C.Structure):
+    """aria_hip_prefix_attn of include/aria_hip.h: one attention over shared prefixes and own keys."""
+    _fields_ = ([("q", _P), ("out", _P), ("prefix", KVCache), ("own", KVCache)] +
+                [(n, _P) for n in ("prefix_len", "own_len", "first")] +
+                [(n, _i) for n in ("type", "out_f32", "B", "H", "Nq")] + [("scale", _f)] + _strides("q", "o"))
+
 # name -> (restype, argtypes); every symbol declared in include/aria_gpu.h and include/aria_hip.h
 SIGNATURES = {
     # include/aria_gpu.h
@@ -120,6 +163,12 @@ SIGNATURES = {
     "aria_hip_attention_f16": (_i, [_P, _P, _P, _P, _i, _i, _i, _i, _i]),
     "aria_hip_cross_attention_ws_bytes": (_sz, [_X]),
     "aria_hip_cross_attention_dev": (_i, [_X, _P, _P]),
+    "aria_hip_rotary_table_dev": (_i, [_P, _P, C.POINTER(RotaryScaling), _i64, _i, _P]),
+    "aria_hip_rotary_dev": (_i, [C.POINTER(Rotary), _P]),
+    "aria_hip_kv_write_dev": (_i, [C.POINTER(KVWrite), _P]),
+    "aria_hip_kv_read_dev": (_i, [C.POINTER(KVRead), _P]),
+    "aria_hip_prefix_attention_ws_bytes": (_sz, [C.POINTER(PrefixAttention)]),
+    "aria_hip_prefix_attention_dev": (_i, [C.POINTER(PrefixAttention), _P, _P]),
     "aria_hip_mx4_quant_dev": (_i, [_P, _P, _P, _i, _i, _i, _i64, _P]),
     "aria_hip_mx4_dequant_dev": (_i, [_P, _i, _P, _P, _i, _i, _P]),
     "aria_hip_gemm_mx4_dev": (_i, [_P, _i, _P, _P, _P, _P, _P, _i, _i, _i, _P]),

@@ -680,6 +680,136 @@ int aria_hip_cross_attention_dev(const aria_hip_cross_attn *a, void *dws, void *
     return 0;
 }
 
+/* rotary positions, the 8-bit cache (k_states.hip) and attention over shared prefixes (k_pattn.hip). Arguments are checked
+ * before the device is looked for. */
+#define ST_TOKENS (1 << 30)
+#define ST_HEADS (1 << 16)
+static int st_aligned(const void *p, int type) { return ((uintptr_t)p & mx4_el_mask(type)) == 0; }
+
+int aria_hip_rotary_table_dev(float *dcos, float *dsin, const aria_hip_rotary_scaling *a, int64_t first, int n,
+                              void *stream) {
+    REQ(a && n >= 0 && first >= 0 && first + n <= (1 << 24) + 1);
+    REQ(a->rot >= 2 && a->rot <= 256 && a->rot % 2 == 0 && a->kind >= 0 && a->kind <= 3);
+    REQ(a->base > 1.0 && isfinite(a->base) && isfinite(a->gain));
+    REQ(a->kind == 0 || (a->factor > 0.0 && isfinite(a->factor)));
+    REQ(a->kind != 2 || a->rot >= 4);
+    REQ(a->kind != 3 || (a->trained > 0.0 && isfinite(a->trained) && isfinite(a->low) && isfinite(a->high) && a->high > a->low));
+    REQ(n == 0 || (dcos && dsin));
+    REQ((((uintptr_t)dcos | (uintptr_t)dsin) & 3u) == 0);
+    const double pi2 = 6.283185307179586476925;
+    double turns[128], base = a->base;
+    if (a->kind == 2) base *= pow(a->factor, (double)a->rot / (a->rot - 2));
+    for (int i = 0; i < a->rot / 2; i++) {
+        double f = pow(base, -2.0 * i / a->rot);
+        if (a->kind == 1) f /= a->factor;
+        if (a->kind == 3) {
+            double w = (a->trained * f / pi2 - a->low) / (a->high - a->low);
+            w = w < 0.0 ? 0.0 : w > 1.0 ? 1.0 : w;
+            f *= w + (1.0 - w) / a->factor;
+        }
+        turns[i] = f / pi2;
+        REQ(isfinite(turns[i]) && turns[i] <= 0x1p20);   /* whole turns and a fraction fit 64 bits at any position */
+    }
+    if (n == 0) return 0;
+    ENSURE();
+    KCK(aria_k_rotary_table(dcos, dsin, turns, a->rot, a->gain, first, n, pick(stream)), "k_rotary_table");
+    return 0;
+}
+
+int aria_hip_rotary_dev(const aria_hip_rotary *a, void *stream) {
+    REQ(a && MX4_TYPE(a->type) && a->B >= 0 && a->N >= 0 && (int64_t)a->B * a->N <= ST_TOKENS);
+    REQ(a->D >= 2 && a->D <= 256 && a->D % 2 == 0 && a->rot >= 0 && a->rot <= a->D && a->rot % 2 == 0 && a->npos >= 0);
+    REQ(a->Hq >= 0 && a->Hq <= ST_HEADS && a->Hk >= 0 && a->Hk <= ST_HEADS);
+    REQ(!a->q == !a->q_out && !a->k == !a->k_out);
+    REQ(st_aligned(a->q, a->type) && st_aligned(a->q_out, a->type) && st_aligned(a->k, a->type) && st_aligned(a->k_out, a->type));
+    REQ((((uintptr_t)a->cos | (uintptr_t)a->sin | (uintptr_t)a->pos | (uintptr_t)a->first) & 3u) == 0);
+    REQ((a->q_batch | a->q_token | a->q_head | a->k_batch | a->k_token | a->k_head | a->qo_batch | a->qo_token | a->qo_head |
+         a->ko_batch | a->ko_token | a->ko_head | a->pos_stride) >= 0);
+    if (a->B == 0 || a->N == 0) return 0;
+    REQ((a->q || a->Hq == 0) && a->rot >= 0 && (a->rot == 0 || a->npos == 0 || (a->cos && a->sin)));
+    ENSURE();
+    KCK(aria_k_rotary(a, pick(stream)), "k_rotary");
+    return 0;
+}
+
+/* sizes and strides of a cache; pointers where it holds slots */
+static int kv_check(const aria_hip_kv *c, int widest) {
+    REQ(c->B >= 0 && c->B <= ST_HEADS && c->Hkv > 0 && c->Hkv <= ST_HEADS && c->cap >= 0 && c->cap <= ST_TOKENS);
+    REQ(c->D >= 16 && c->D <= widest && c->D % 16 == 0);
+    REQ(c->B == 0 || c->cap == 0 || (c->k && c->v && c->k_scale && c->v_scale));
+    REQ((((uintptr_t)c->k | (uintptr_t)c->v) & 15u) == 0);
+    REQ((c->batch | c->head | c->token | c->s_batch | c->s_head) >= 0 && ((c->batch | c->head | c->token) & 15) == 0);
+    return 0;
+}
+int aria_hip_kv_write_dev(const aria_hip_kv_write *a, void *stream) {
+    REQ(a);
+    const aria_hip_kv *c = &a->cache;
+    const int r = kv_check(c, 256);
+    if (r) return r;
+    REQ(MX4_TYPE(a->type) && a->N >= 0 && (int64_t)c->B * a->N <= ST_TOKENS);
+    REQ(a->rot >= 0 && a->rot <= c->D && a->rot % 2 == 0 && a->npos >= 0 && a->Hq >= 0 && a->Hq <= ST_HEADS);
+    REQ(!a->q == !a->q_out && (a->q || a->Hq == 0) && !a->cos == !a->sin && (a->cos || a->rot == 0 || a->npos == 0));
+    REQ(st_aligned(a->k, a->type) && st_aligned(a->v, a->type) && st_aligned(a->q, a->type) && st_aligned(a->q_out, a->type));
+    REQ((((uintptr_t)a->cos | (uintptr_t)a->sin | (uintptr_t)a->pos | (uintptr_t)a->first | (uintptr_t)a->count) & 3u) == 0);
+    REQ((a->k_batch | a->k_token | a->k_head | a->v_batch | a->v_token | a->v_head | a->q_batch | a->q_token | a->q_head |
+         a->qo_batch | a->qo_token | a->qo_head | a->pos_stride) >= 0);
+    if (c->B == 0 || a->N == 0) return 0;
+    REQ(a->k && a->v);
+    ENSURE();
+    KCK(aria_k_kv_write(a, pick(stream)), "k_kv_write");
+    return 0;
+}
+int aria_hip_kv_read_dev(const aria_hip_kv_read *a, void *stream) {
+    REQ(a);
+    const aria_hip_kv *c = &a->cache;
+    const int r = kv_check(c, 256);
+    if (r) return r;
+    REQ(MX4_TYPE(a->type) && a->N >= 0 && (int64_t)c->B * a->N <= ST_TOKENS);
+    REQ(st_aligned(a->k, a->type) && st_aligned(a->v, a->type));
+    REQ((((uintptr_t)a->first | (uintptr_t)a->count) & 3u) == 0);
+    REQ((a->k_batch | a->k_token | a->k_head | a->v_batch | a->v_token | a->v_head) >= 0);
+    if (c->B == 0 || a->N == 0 || c->cap == 0 || (!a->k && !a->v)) return 0;
+    ENSURE();
+    KCK(aria_k_kv_read(a, pick(stream)), "k_kv_read");
+    return 0;
+}
+
+static int pattn_check_sizes(const aria_hip_prefix_attn *a) {
+    REQ(a);
+    const aria_hip_kv *p = &a->prefix, *o = &a->own;
+    REQ(a->B >= 0 && a->H > 0 && a->Nq >= 0 && (int64_t)a->B * a->H <= (1 << 20));
+    REQ((int64_t)a->B * a->H * a->Nq <= (1 << 30));
+    REQ(o->Hkv > 0 && p->Hkv == o->Hkv && a->H % o->Hkv == 0 && p->D == o->D && o->D >= 16 && o->D <= 128 && o->D % 16 == 0);
+    REQ(o->B == a->B && p->B >= 1 && a->B % p->B == 0);
+    REQ(p->cap >= 0 && p->cap <= ST_TOKENS && o->cap >= 0 && o->cap <= ST_TOKENS);
+    return 0;
+}
+static int pattn_check(const aria_hip_prefix_attn *a) {
+    int r = pattn_check_sizes(a);
+    if (r || (r = kv_check(&a->prefix, 128)) || (r = kv_check(&a->own, 128))) return r;
+    REQ(a->type == 1 || a->type == 2);
+    REQ(a->B == 0 || a->Nq == 0 || (a->q && a->out));
+    REQ((((uintptr_t)a->q | (uintptr_t)a->out) & 15u) == 0);
+    REQ((((uintptr_t)a->prefix_len | (uintptr_t)a->own_len | (uintptr_t)a->first) & 3u) == 0);
+    const int64_t st = a->q_batch | a->q_head | a->q_token | a->o_batch | a->o_head | a->o_token;
+    REQ(st >= 0 && st % 8 == 0);
+    REQ(a->scale > 0.0f && a->scale <= 0x1p127f);   /* times log2 e still finite */
+    return 0;
+}
+size_t aria_hip_prefix_attention_ws_bytes(const aria_hip_prefix_attn *a) {
+    if (pattn_check_sizes(a) || a->B == 0 || a->Nq == 0) return 0;
+    return aria_k_pattn_ws_bytes(a);
+}
+int aria_hip_prefix_attention_dev(const aria_hip_prefix_attn *a, void *dws, void *stream) {
+    const int r = pattn_check(a);
+    if (r) return r;
+    if (a->B == 0 || a->Nq == 0) return 0;
+    REQ(((uintptr_t)dws & 255u) == 0 && (dws || aria_k_pattn_ws_bytes(a) == 0));
+    ENSURE();
+    KCK(aria_k_pattn_run(a, dws, pick(stream)), "k_pattn");
+    return 0;
+}
+
 /* ------------------------------------------------------------------------- */
 /* host-pointer forms (aria_hip.h) - one synchronous staged call each        */
 /* ------------------------------------------------------------------------- */

@@ -269,6 +269,17 @@ typedef aria_hip_cross_attn aria_k_xattn;
 size_t aria_k_xattn_ws_bytes(const aria_k_xattn *a);
 hipError_t aria_k_xattn_run(const aria_k_xattn *a, void *ws, hipStream_t s);
 
+/* Rotary positions and the 8-bit cache (k_states.hip), attention over shared prefixes (k_pattn.hip): the
+ * public descriptions as the kernels take them. turns [rot/2]: each pair's frequency over 2 pi; ws holds
+ * aria_k_pattn_ws_bytes bytes. */
+hipError_t aria_k_rotary_table(float *cos_t, float *sin_t, const double *turns, int rot, double gain, int64_t first,
+                               int n, hipStream_t s);
+hipError_t aria_k_rotary(const aria_hip_rotary *a, hipStream_t s);
+hipError_t aria_k_kv_write(const aria_hip_kv_write *a, hipStream_t s);
+hipError_t aria_k_kv_read(const aria_hip_kv_read *a, hipStream_t s);
+size_t aria_k_pattn_ws_bytes(const aria_hip_prefix_attn *a);
+hipError_t aria_k_pattn_run(const aria_hip_prefix_attn *a, void *ws, hipStream_t s);
+
 #ifdef __cplusplus
 }
 #endif

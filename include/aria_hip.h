@@ -299,6 +299,117 @@ int aria_hip_linear_mx4(float *y, const float *x, const uint8_t *q, const uint8_
 int aria_hip_glu_mx4(float *y, const float *x, const uint8_t *q, const uint8_t *scale, const float *b, int M, int K,
                      int inner);
 
+/* ---- rotary positions by table, a cache of keys and values in 8 bits, attention over shared prefixes
+ *      (no counterpart in the reference, whose rotary embedding takes positions 0 .. N-1 in fp32,
+ *      src/aria_ops.h:122-126, and whose attention takes one set of keys, src/aria_ops.h:135) ----
+ * Element types are aria_dtype's values: 0 fp32, 1 fp16, 2 bf16. Strides count elements (bytes in a
+ * cache), are not negative, and those of inputs may be 0 (broadcast); rows of outputs lie apart from
+ * each other and, unless stated, from every input. Pointers and strides of states need only their
+ * element's alignment. Heads at most 2^16 each, B * N at most 2^30, D at most 256. */
+
+/* Frequencies of the rotated pairs i = 0 .. rot/2 - 1, f_i = base^(-2i/rot), for contexts longer than
+ * the trained one. kind 0: f_i; 1 (linear): f_i / factor; 2 (base): base * factor^(rot/(rot-2)) in
+ * base's place, which leaves f_0 and divides the last by factor; 3 (by turns): with t = trained * f_i / 2 pi
+ * turns over the trained length and w = (t - low) / (high - low) held to 0 .. 1, f_i (w + (1 - w) / factor).
+ * gain multiplies both tables. rot even, 2 .. 256 (kind 2: from 4); base > 1; factor > 0 (kinds 1 - 3);
+ * trained > 0, high > low (kind 3); all finite. */
+typedef struct {
+    int rot, kind;
+    double base, factor, trained, low, high, gain;
+} aria_hip_rotary_scaling;
+/* dcos, dsin [n, rot/2] fp32 for positions first .. first + n - 1 (not negative, at most 2^24): the angle in 64
+ * bits, so that far positions keep fp32's precision. 4-byte aligned. */
+int aria_hip_rotary_table_dev(float *dcos, float *dsin, const aria_hip_rotary_scaling *a, int64_t first, int n,
+                              void *stream);
+
+/* Rotates the first rot dims of every head of q [B, N, Hq, D] and, where k is given, of k [B, N, Hk, D]
+ * into q_out and k_out; dims from rot on are copied. Pairs are (i, i + rot/2), or (2i, 2i + 1) where
+ * interleaved: (a, b) -> (a c - b s, b c + a s), and by the other sign of s where inverse (the adjoint: a
+ * gradient's way back). c, s = row p of cos, sin [npos, rot/2], p the token's position: pos[b *
+ * pos_stride + t], or without pos first[b] + t (first NULL: t). Rows of a position outside 0 .. npos - 1
+ * (padding) are left as they are. Products and sums in fp32 (fp32 states: in 64 bits), rounded once.
+ * An output may be its own input with the same strides. D even, rot even, 0 .. D. */
+typedef struct {
+    const void *q, *k;
+    void *q_out, *k_out;
+    const float *cos, *sin;
+    const int32_t *pos, *first;
+    int64_t pos_stride;
+    int type, B, N, Hq, Hk, D, rot, npos, interleaved, inverse;
+    int64_t q_batch, q_token, q_head, k_batch, k_token, k_head;
+    int64_t qo_batch, qo_token, qo_head, ko_batch, ko_token, ko_head;
+} aria_hip_rotary;
+int aria_hip_rotary_dev(const aria_hip_rotary *a, void *stream);
+
+/* A cache of keys and values: slot t of head h of sequence b is a row of D codes at k (v) + b * batch +
+ * h * head + t * token bytes and a scale byte at k_scale (v_scale) + b * s_batch + h * s_head + t. Codes are
+ * e4m3 (sign, 4 bits of exponent with bias 7, 3 of mantissa, largest 448, no infinity); the row stands
+ * for code * 2^(byte - 127). byte: the smallest, at least 1, for which the row's largest magnitude is at
+ * most 448 * 2^(byte - 127); codes to nearest, ties to even. A row that holds an Inf or a NaN gets byte
+ * 255 and codes 0x7F: it stands for NaN. (Of a pack from elsewhere: a byte of 0 and NaN codes under another
+ * byte than 255 are not supported.) D: a multiple of 16 up to 256. k and v 16-byte aligned, batch, head and token
+ * multiples of 16; B and Hkv at most 2^16, cap at most 2^30. */
+typedef struct {
+    uint8_t *k, *v, *k_scale, *v_scale;
+    int64_t batch, head, token, s_batch, s_head;
+    int B, Hkv, D, cap;
+} aria_hip_kv;
+/* Writes tokens t < count[b] (count NULL: N; held to 0 .. N) of k, v [B, N, Hkv, D] to slots first[b] + t (first
+ * NULL: t); slots outside 0 .. cap - 1 are skipped. Where cos is given (rot > 0), keys are rotated before,
+ * as in aria_hip_rotary, by position pos[b * pos_stride + t], or the slot without pos; the rotated key is rounded to fp32,
+ * then to its code. A token whose position lies outside the table is not written. Queries q [B, N, Hq, D] of the same
+ * tokens (q NULL: none), rotated likewise, go to q_out in their own type, whatever their slot; q_out may be q.
+ * Two calls in flight must not write the same slot. */
+typedef struct {
+    aria_hip_kv cache;
+    const void *k, *v, *q;
+    void *q_out;
+    const float *cos, *sin;
+    const int32_t *pos, *first, *count;
+    int64_t pos_stride;
+    int type, N, Hq, rot, npos, interleaved;
+    int64_t k_batch, k_token, k_head, v_batch, v_token, v_head;
+    int64_t q_batch, q_token, q_head, qo_batch, qo_token, qo_head;
+} aria_hip_kv_write;
+int aria_hip_kv_write_dev(const aria_hip_kv_write *a, void *stream);
+/* Slots first[b] + t, t < count[b], as values in k, v [B, N, Hkv, D] (either NULL: not read), rounded to type
+ * and held to its finite range (NaN stays); rows of other t and of slots outside 0 .. cap - 1 are left as they are. */
+typedef struct {
+    aria_hip_kv cache;
+    void *k, *v;
+    const int32_t *first, *count;
+    int type, N;
+    int64_t k_batch, k_token, k_head, v_batch, v_token, v_head;
+} aria_hip_kv_read;
+int aria_hip_kv_read_dev(const aria_hip_kv_read *a, void *stream);
+
+/* Attention for a batch whose sequences share prefixes: q [B, H, Nq, D] fp16 or bf16 -> out [B, Nq, H, D]
+ * (out_f32: fp32). Sequence b sees prefix b / (B / prefix.B), of prefix.B that divide B, and sequence b of own;
+ * H / Hkv consecutive query heads read one head of both.
+ *   out[b,t,h] = sum_j p_j v_j, p = softmax over the keys j that it sees of scale * q . k_j:
+ * the prefix's slots below prefix_len (per prefix; NULL: cap), and own slots below own_len (per sequence; NULL:
+ * cap) that, where first is given, are at most first[b] + t (causal: query t stands at slot first[b] + t).
+ * Lengths are taken as held to 0 .. cap; a cache of cap 0 is absent (no pointers). Both descriptions give B, Hkv and D.
+ * A row that sees no key is zero. What the slots that a row does not see hold does not reach it (byte 255 included). A key
+ * or a value of byte 255 that it sees makes the whole row NaN.
+ * Cached values are rounded to q's type (exact in bf16; fp16 below 65520 and above 2^-24 steps), probabilities too; sums
+ * and softmax statistics are fp32. D up to 128; scale positive, at most 2^127; B * H at most 2^20, B * H * Nq at
+ * most 2^30. q and out 16-byte aligned, strides multiples of 8.
+ * Many sequences' rows together read a prefix once. dws: aria_hip_prefix_attention_ws_bytes(a) bytes (0: may be
+ * NULL), 256-byte aligned, not shared by calls that may run at the same time; the number goes by B, H, Nq and both
+ * caches' B, Hkv, D and cap alone. */
+typedef struct {
+    const void *q;
+    void *out;
+    aria_hip_kv prefix, own;
+    const int32_t *prefix_len, *own_len, *first;
+    int type, out_f32, B, H, Nq;
+    float scale;
+    int64_t q_batch, q_token, q_head, o_batch, o_token, o_head;
+} aria_hip_prefix_attn;
+size_t aria_hip_prefix_attention_ws_bytes(const aria_hip_prefix_attn *a);
+int aria_hip_prefix_attention_dev(const aria_hip_prefix_attn *a, void *dws, void *stream);
+
 /* Host-pointer forms with the reference's signatures (src/aria_quant.h:43-45, 64-65):
  * allocate, copy in, run, copy out, free; synchronous. Return 0 or an error. */
 int aria_hip_q8_quant(int8_t *q, float *scale, const float *W, int N, int K);
