@@ -787,6 +787,7 @@ static int pattn_check_sizes(const aria_hip_prefix_attn *a) {
 static int pattn_check(const aria_hip_prefix_attn *a) {
     int r = pattn_check_sizes(a);
     if (r || (r = kv_check(&a->prefix, 128)) || (r = kv_check(&a->own, 128))) return r;
+    REQ(a->prefix.token < (1 << 24) && a->own.token < (1 << 24));   /* lane offsets within a tile are 32 bits wide */
     REQ(a->type == 1 || a->type == 2);
     REQ(a->B == 0 || a->Nq == 0 || (a->q && a->out));
     REQ((((uintptr_t)a->q | (uintptr_t)a->out) & 15u) == 0);

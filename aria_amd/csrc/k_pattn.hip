@@ -12,7 +12,7 @@
  * 2^(scale_log2 s - ref) with a lazy reference, P rounded to the 16-bit type. Codes become 16-bit values on their way to LDS: a
  * lane loads 16 codes and their row's byte, converts them with the row's power of two (one instruction per two
  * values) and stores two 16-byte chunks where the swizzle wants them; the next tile's codes are on their way meanwhile.
- * Slots that no row sees become zeros there, and their scores -inf. A key or value row of byte 255 (NaN) is staged
+ * The scores of slots that a row does not see become -inf. A key or value row of byte 255 (NaN) is staged
  * as a key of NaNs and a value of zeros: a row that sees it gets a NaN weight, one that does not (a later token's slot) is not
  * touched by it.
  */
@@ -21,8 +21,8 @@
 
 #include <algorithm>
 
-/* 16-byte source of chunks that hold no slot or no dim */
-__device__ const uint4 pa_zero = {0, 0, 0, 0};
+typedef float pa_f32x2_t __attribute__((ext_vector_type(2)));
+#define PA_AHEAD 6           /* key fragments on their way to a score product */
 
 template <typename T> struct Pc;
 template <> struct Pc<_Float16> {
@@ -32,11 +32,23 @@ template <> struct Pc<__bf16> {
     template <bool HI> static __device__ __forceinline__ Xa<__bf16>::v2 cvt(unsigned u, float s) { return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(u, s, HI); }
 };
 
-/* one kind of workgroup: `sets` sets of R rows (a prefix's, or a sequence's), nrb row blocks to each and key head, ns splits of
- * `per` key tiles */
+/* Division by a number that the host knows, of 0 .. 2^31 - 1: by a product (the compiler's own takes some thirty
+ * instructions, and a launch fetches every one of them first) */
+struct PaDiv {
+    unsigned d, mul, sh;
+    PaDiv(int n = 1) : d(n), mul(0), sh(0) {
+        while ((1ull << (sh + 1)) < d) sh++;        /* 2^(sh + 1) >= d > 2^sh, d > 1 */
+        if (d > 1) mul = (unsigned)(((1ull << (32 + sh)) + d - 1) / d);
+    }
+    __device__ __forceinline__ unsigned of(unsigned n) const { return d == 1 ? n : __umulhi(n, mul) >> sh; }
+};
+
+/* One kind of workgroup: `sets` sets of R rows (a prefix's, or a sequence's), nrb row blocks to each and key head, ns splits of
+ * `per` key tiles. Form 0, 1, 2: a row block of 32, 64 or 128 rows, whose keys 4, 2 or 1 slices of waves share out */
 struct PaJobs {
-    int sets, R, nrb, ns, per, jobs;
-    int use_prefix, use_own;
+    int sets, R, nrb, ns, per, jobs, form;
+    int use_prefix, use_own, tp;                    /* tp: tiles of a prefix's capacity */
+    PaDiv dnrb, dns, dper;
     size_t part;             /* floats in front of its partial results */
 };
 struct PaArgs {
@@ -44,20 +56,25 @@ struct PaArgs {
     int G, Bp;               /* query heads per key head; sequences per prefix */
     int kinds, group;        /* one kind of workgroup or two; the first takes the rows of a prefix's sequences together */
     PaJobs j[2];
-    int jobs;
+    PaDiv dhkv, dseq, dg, dbp;                      /* Hkv, rows of a sequence and key head, G, Bp */
     float scale_log2;
     float *part;
 };
 
 /* keys of a tile */
-__host__ __device__ constexpr int pa_tile(int DP, int QW) { return DP == 64 || QW > 1 ? 64 : 32; }
+__host__ __device__ constexpr int pa_tile(int DP, int form) { return DP == 64 || form == 2 ? 64 : 32; }
 /* floats of a row's partial result: sums, reference, weights' sum, remainder of the reference */
 __host__ __device__ constexpr int pa_row(int DP) { return DP + 4; }
+/* LDS bytes of a form: the stages of every slice, later the output rows and each wave's 32 references, sums and remainders */
+__host__ __device__ constexpr int pa_lds(int DP, int form) {
+    const int ks = 4 >> form, st = (form ? 2 : 1) * ks * 2 * pa_tile(DP, form) * DP * 2, epi = form == 2 ? 0 : 4 * 32 * (DP + 4) * 4 + 4 * 96 * 4;
+    return st > epi ? st : epi;
+}
 
-template <typename T, int DP, int QW, int KS>
-__global__ __launch_bounds__(64 * QW * KS) void k_pattn(PaArgs x) {
-    constexpr int KT = pa_tile(DP, QW);
-    constexpr int NW = QW * KS;
+template <typename T, int DP, int FORM>
+__device__ __forceinline__ void pa_work(const PaArgs &x, int kind, int job, uint8_t *smem) {
+    constexpr int QW = 1 << FORM, KS = 4 >> FORM, NW = 4;
+    constexpr int KT = pa_tile(DP, FORM);
     constexpr int NST = QW > 1 ? 2 : 1;             /* LDS stages */
     constexpr int CPR = DP / 8;                     /* 16-byte chunks of values per key row */
     constexpr int C16 = DP / 16;                    /* 16-byte chunks of codes per key row */
@@ -66,8 +83,6 @@ __global__ __launch_bounds__(64 * QW * KS) void k_pattn(PaArgs x) {
     constexpr int ES = DP + 4;                      /* floats per staged output row */
     constexpr int KB = KT / 32, DT = DP / 32, DS = DP / 16;
     constexpr int STAGE = 2 * TB * KS;              /* K and V of every slice */
-    constexpr int EPI = NW * 32 * ES * 4 + NW * 96 * 4;
-    __shared__ __attribute__((aligned(16))) uint8_t smem[NST * STAGE > EPI ? NST * STAGE : EPI];
     typedef typename Xa<T>::v8 v8;
     typedef typename Xa<T>::v2 v2;
     const aria_hip_prefix_attn &a = x.a;
@@ -77,21 +92,62 @@ __global__ __launch_bounds__(64 * QW * KS) void k_pattn(PaArgs x) {
     const int wid = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int qw = wid % QW, ks = wid / QW;
 
-    int job = xcd_tile(blockIdx.x, x.jobs);
-    if (job >= x.jobs) return;
-    const int kind = job >= x.j[0].jobs;
-    if (kind) job -= x.j[0].jobs;
     const PaJobs &J = x.j[kind];
-    const int rb = job % J.nrb, split = job / J.nrb % J.ns, sh = job / J.nrb / J.ns, hk = sh % Hkv, set = sh / Hkv;
-    /* a set is a prefix's rows (kind 0 of 2: several sequences), or a sequence's */
+    unsigned rest = x.j[kind].dnrb.of(job), next;
+    const int rb = job - rest * J.nrb;
+    const int split = rest - (next = J.dns.of(rest)) * J.ns, set = x.dhkv.of(next), hk = next - set * Hkv, sh = next;
+    /* a set is a prefix's rows (several sequences), or a sequence's */
     const bool group = x.group && kind == 0;
-    const int per_seq = a.Nq * x.G;                 /* rows of one sequence and key head */
-    const int pf = group ? set : set / x.Bp;
+    const int pf = group ? set : x.dbp.of(set);
+
+    /* codes of a tile on their way. Slots behind the capacity repeat its last one and chunks past D the last chunk: the
+     * former are not seen, the latter's dims meet zeros of q or are not stored */
+    typedef __attribute__((address_space(1))) const uint8_t gu8;
+    typedef __attribute__((address_space(4))) const int ci32;
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    u32x4 kc[NC], vc[NC];
+    unsigned kb[NC], vb[NC];
+    const uint8_t *kp, *vp, *se, *sv;
+    unsigned tb;                                    /* bytes from slot to slot (below 2^24) */
+    int left;                                       /* slots from the tile's first to the capacity */
+    bool at_own;
+    auto seek = [&](bool own, int i) __attribute__((always_inline)) {
+        const aria_hip_kv &c = own ? a.own : a.prefix;
+        const long long b = own ? set : pf, at = b * c.batch + hk * c.head + (long long)i * KT * c.token;
+        const long long sat = b * c.s_batch + hk * c.s_head + (long long)i * KT;
+        kp = c.k + at;
+        vp = c.v + at;
+        se = c.k_scale + sat;
+        sv = c.v_scale + sat;
+        tb = (unsigned)c.token;
+        left = c.cap - i * KT;
+        at_own = own;
+    };
+    auto load = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < NC; j++) {
+            const int p = 64 * (QW * j + qw) + lane;
+            const unsigned r = min(p / C16, left - 1), off = r * tb + 16 * min(p % C16, D / 16 - 1);
+            kc[j] = *(__attribute__((address_space(1))) const u32x4 *)((gu8 *)kp + off);
+            vc[j] = *(__attribute__((address_space(1))) const u32x4 *)((gu8 *)vp + off);
+            kb[j] = ((gu8 *)se)[r];
+            vb[j] = ((gu8 *)sv)[r];
+        }
+    };
+    /* A split has J.per of the tiles, of which its slices take every KS-th. The first tile goes out before the lengths are here:
+     * it is the one that full caches would have */
+    const int w0 = split * J.per, i0 = w0 + ks, g_own = i0 >= J.tp, g_tile = g_own ? i0 - J.tp : i0;
+    const bool guess = !g_own || (J.use_own && g_tile * KT < a.own.cap);
+    if (guess) {
+        seek(g_own, g_tile);
+        load();
+    }
+
     auto where = [&](int row, int &b, int &tok, int &hd) __attribute__((always_inline)) {
-        const int r = group ? row % per_seq : row;
-        b = group ? set * x.Bp + row / per_seq : set;
-        tok = r / x.G;
-        hd = hk * x.G + r % x.G;
+        const int s = group ? x.dseq.of(row) : 0, r = row - s * (int)x.dseq.d;
+        b = group ? set * x.Bp + s : set;
+        tok = x.dg.of(r);
+        hd = hk * x.G + r - tok * x.G;
     };
     const int row0 = rb * 32 * QW + qw * 32;        /* the wave's first row; rows past R repeat the last */
     int qb, tok, hd;
@@ -112,48 +168,39 @@ __global__ __launch_bounds__(64 * QW * KS) void k_pattn(PaArgs x) {
     /* the slots that rows see: n0 of the prefix, and of the own part n1 (causal: lim of this lane's row, lim_lo of the
      * wave's first, lim_hi of the block's last) */
     int n0 = 0, n1 = 0, lim = 0, lim_lo = 0, lim_hi = 0;
-    if (J.use_prefix) n0 = a.prefix_len ? min(max(a.prefix_len[pf], 0), a.prefix.cap) : a.prefix.cap;
+    if (J.use_prefix) n0 = a.prefix_len ? min(max(((ci32 *)a.prefix_len)[pf], 0), a.prefix.cap) : a.prefix.cap;
     if (J.use_own) {
-        n1 = a.own_len ? min(max(a.own_len[set], 0), a.own.cap) : a.own.cap;
+        n1 = a.own_len ? min(max(((ci32 *)a.own_len)[set], 0), a.own.cap) : a.own.cap;
         lim = lim_lo = lim_hi = n1;
         if (a.first) {
-            const long long f = (long long)a.first[set] + 1;
+            const long long f = (long long)((ci32 *)a.first)[set] + 1;
             auto at = [&](int t) __attribute__((always_inline)) { return (int)min(max(f + t, 0ll), (long long)n1); };
             lim = at(tok);
-            lim_lo = at(min(row0, J.R - 1) / x.G);
-            lim_hi = at((min((rb + 1) * 32 * QW, J.R) - 1) / x.G);
+            lim_lo = at(x.dg.of(min(row0, J.R - 1)));
+            lim_hi = at(x.dg.of(min((rb + 1) * 32 * QW, J.R) - 1));
         }
     }
-    /* key tiles: nt0 of the prefix, then the own ones. A split has J.per of them, and a set with few of them fewer splits */
+    /* key tiles: nt0 of the prefix, then the own ones; a set with few of them has fewer splits */
     const int nt0 = (n0 + KT - 1) / KT, nt = nt0 + (lim_hi + KT - 1) / KT;
-    const int w0 = split * J.per;
     if (split > 0 && w0 >= nt0 + (n1 + KT - 1) / KT) return;      /* uniform per workgroup, before any barrier */
-    const int w1 = max(w0, min(w0 + J.per, nt));
-    const int sp = (w1 - w0 + KS - 1) / KS;
-    const int t0 = min(w0 + ks * sp, w1), t1 = min(t0 + sp, w1);
-
-    /* codes of a tile on their way */
-    uint4 kc[NC], vc[NC];
-    unsigned kb[NC], vb[NC];
-    auto load = [&](int i) __attribute__((always_inline)) {
-        const bool own = i >= nt0;
-        const aria_hip_kv &c = own ? a.own : a.prefix;
-        const long long b = own ? set : pf;
-        const int base = (own ? i - nt0 : i) * KT, left = (own ? n1 : n0) - base;
-        const uint8_t *k = c.k + b * c.batch + hk * c.head + base * c.token, *v = c.v + b * c.batch + hk * c.head + base * c.token;
-        const uint8_t *se = c.k_scale + b * c.s_batch + hk * c.s_head + base, *sv = c.v_scale + b * c.s_batch + hk * c.s_head + base;
-#pragma unroll
-        for (int j = 0; j < NC; j++) {
-            const int p = 64 * (QW * j + qw) + lane, r = p / C16, cc = p % C16;
-            const bool ok = r < left && 16 * cc < D;
-            const long long off = r * c.token + 16 * cc;
-            kc[j] = *reinterpret_cast<const uint4 *>(ok ? k + off : (const uint8_t *)&pa_zero);
-            vc[j] = *reinterpret_cast<const uint4 *>(ok ? v + off : (const uint8_t *)&pa_zero);
-            kb[j] = *(ok ? se + r : (const uint8_t *)&pa_zero);
-            vb[j] = *(ok ? sv + r : (const uint8_t *)&pa_zero);
+    const int w1 = min(w0 + J.per, nt);
+    if (i0 < w1 && !(guess && (g_own ? i0 >= nt0 && i0 - nt0 == g_tile : i0 < nt0))) {
+        seek(i0 >= nt0, i0 >= nt0 ? i0 - nt0 : i0);
+        load();
+    }
+    /* behind load(): on to the slice's next tile, i */
+    auto move = [&](int i) __attribute__((always_inline)) {
+        if (!at_own && i >= nt0) {
+            seek(true, i - nt0);
+        } else {
+            kp += (unsigned long long)tb * (KT * KS);
+            vp += (unsigned long long)tb * (KT * KS);
+            se += KT * KS;
+            sv += KT * KS;
+            left -= KT * KS;
         }
     };
-    auto put = [&](uint8_t *to, const uint4 &u, unsigned byte, int at0, int at1) __attribute__((always_inline)) {
+    auto put = [&](uint8_t *to, const u32x4 &u, unsigned byte, int at0, int at1) __attribute__((always_inline)) {
         const float s = __builtin_bit_cast(float, byte << 23);
         const v2 c0 = Pc<T>::template cvt<false>(u.x, s), c1 = Pc<T>::template cvt<true>(u.x, s);
         const v2 c2 = Pc<T>::template cvt<false>(u.y, s), c3 = Pc<T>::template cvt<true>(u.y, s);
@@ -162,22 +209,47 @@ __global__ __launch_bounds__(64 * QW * KS) void k_pattn(PaArgs x) {
         *reinterpret_cast<v8 *>(to + at0) = v8{c0[0], c0[1], c1[0], c1[1], c2[0], c2[1], c3[0], c3[1]};
         *reinterpret_cast<v8 *>(to + at1) = v8{c4[0], c4[1], c5[0], c5[1], c6[0], c6[1], c7[0], c7[1]};
     };
-    auto store = [&](int buf) __attribute__((always_inline)) {
-        uint8_t *K = smem + buf * STAGE + ks * 2 * TB, *V = K + TB;
+    /* rows of tile i that stand for NaN or lie behind its last slot */
+    auto fix = [&](int i) __attribute__((always_inline)) {
+        const int valid = i < nt0 ? n0 - i * KT : n1 - (i - nt0) * KT;
+        bool bad[NC], any = false;
 #pragma unroll
         for (int j = 0; j < NC; j++) {
-            const bool bad = kb[j] == 255u || vb[j] == 255u;
-            if (__builtin_expect(__ballot(bad) != 0, 0)) {
-                kc[j] = bad ? make_uint4(0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu) : kc[j];
-                vc[j] = bad ? make_uint4(0, 0, 0, 0) : vc[j];
-                kb[j] = bad ? 127u : kb[j];
-                vb[j] = bad ? 127u : vb[j];
-            }
-            const int p = 64 * (QW * j + qw) + lane, r = p / C16, cp = 2 * (p % C16);
-            const int zk = DP == 64 ? (r >> 1) & 7 : r & 15, zv = DP == 64 ? ((r >> 1) & 1) << 2 : (r & 3) << 2;
-            put(K, kc[j], kb[j], (r * CPR + (cp ^ zk)) * 16, (r * CPR + ((cp + 1) ^ zk)) * 16);
-            put(V, vc[j], vb[j], (r * CPR + (cp ^ zv)) * 16, (r * CPR + ((cp + 1) ^ zv)) * 16);
+            bad[j] = kb[j] == 255u || vb[j] == 255u || (64 * (QW * j + qw) + lane) / C16 >= valid;
+            any |= bad[j];
         }
+        if (__builtin_expect(__ballot(any) != 0, 0)) {
+#pragma unroll
+            for (int j = 0; j < NC; j++) {
+                kc[j] = bad[j] ? u32x4{0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu} : kc[j];
+                vc[j] = bad[j] ? u32x4{0, 0, 0, 0} : vc[j];
+                kb[j] = bad[j] ? 127u : kb[j];
+                vb[j] = bad[j] ? 127u : vb[j];
+            }
+        }
+    };
+    auto put_k = [&](int buf) __attribute__((always_inline)) {
+        uint8_t *K = smem + buf * STAGE + ks * 2 * TB;
+#pragma unroll
+        for (int j = 0; j < NC; j++) {
+            const int p = 64 * (QW * j + qw) + lane, r = p / C16, cp = 2 * (p % C16);
+            const int z = DP == 64 ? (r >> 1) & 7 : r & 15;
+            put(K, kc[j], kb[j], (r * CPR + (cp ^ z)) * 16, (r * CPR + ((cp + 1) ^ z)) * 16);
+        }
+    };
+    auto put_v = [&](int buf, const u32x4 (&c)[NC], const unsigned (&byte)[NC]) __attribute__((always_inline)) {
+        uint8_t *V = smem + buf * STAGE + ks * 2 * TB + TB;
+#pragma unroll
+        for (int j = 0; j < NC; j++) {
+            const int p = 64 * (QW * j + qw) + lane, r = p / C16, cp = 2 * (p % C16);
+            const int z = DP == 64 ? ((r >> 1) & 1) << 2 : (r & 3) << 2;
+            put(V, c[j], byte[j], (r * CPR + (cp ^ z)) * 16, (r * CPR + ((cp + 1) ^ z)) * 16);
+        }
+    };
+    auto store = [&](int buf, int i) __attribute__((always_inline)) {
+        fix(i);
+        put_k(buf);
+        put_v(buf, vc, vb);
     };
 
     xa_f32x16_t o[DT];
@@ -205,7 +277,7 @@ __global__ __launch_bounds__(64 * QW * KS) void k_pattn(PaArgs x) {
         }
     }
 
-    auto scores = [&](int buf, int i, xa_f32x16_t (&s)[KB]) __attribute__((always_inline)) {
+    auto scores = [&](int buf, xa_f32x16_t (&s)[KB]) __attribute__((always_inline)) {
         const uint8_t *K = smem + buf * STAGE + ks * 2 * TB;
 #pragma unroll
         for (int kb = 0; kb < KB; kb++)
@@ -216,6 +288,17 @@ __global__ __launch_bounds__(64 * QW * KS) void k_pattn(PaArgs x) {
 #pragma unroll
             for (int kb = 0; kb < KB; kb++)
                 s[kb] = Xa<T>::mfma(*reinterpret_cast<const v8 *>(K + koff[i] + kb * 32 * CPR * 16), qf[i], s[kb]);
+        /* fragments PA_AHEAD products ahead */
+        constexpr int N = DS * KB, AH = PA_AHEAD < N ? PA_AHEAD : N;
+        __builtin_amdgcn_sched_group_barrier(0x100, AH, 0);
+#pragma unroll
+        for (int i = 0; i < N - AH; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, AH, 0);
+    };
+    auto hide = [&](int i, xa_f32x16_t (&s)[KB]) __attribute__((always_inline)) {
         /* slots that a row of the wave does not see: the last tile of a part, the tiles that a causal limit crosses */
         const bool own = i >= nt0;
         const int base = (own ? i - nt0 : i) * KT;
@@ -272,45 +355,57 @@ __global__ __launch_bounds__(64 * QW * KS) void k_pattn(PaArgs x) {
                     const xa_i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((xa_lds_i16x4_t *)(p + 8 * CPR * 16));
                     vf[d] = __builtin_bit_cast(v8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
                 }
-                v8 p;
+                v2 p2[4];
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    p[i] = (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * h + i], sc, -rr));
+                for (int i = 0; i < 4; i++)
+                    p2[i] = __builtin_convertvector((pa_f32x2_t{__builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * h + 2 * i], sc, -rr)),
+                                                          __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * h + 2 * i + 1], sc, -rr))}), v2);
+                const v8 p = __builtin_shufflevector(__builtin_shufflevector(p2[0], p2[1], 0, 1, 2, 3), __builtin_shufflevector(p2[2], p2[3], 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
                 for (int d = 0; d < DT; d++) o[d] = Xa<T>::mfma(vf[d], p, o[d]);
 #pragma unroll
-                for (int i = 0; i < 4; i++) l = Xa<T>::dot2(v2{p[2 * i], p[2 * i + 1]}, one2, l);
+                for (int i = 0; i < 4; i++) l = Xa<T>::dot2(p2[i], one2, l);
             }
     };
     auto tile = [&](int buf, int i) __attribute__((always_inline)) {
+        if (row0 >= J.R) return;                    /* the last row block's waves without rows: they only fetch */
         xa_f32x16_t s[KB];
-        scores(buf, i, s);
+        scores(buf, s);
+        hide(i, s);
         move_ref(s);
         add(buf, s);
     };
 
+    /* the rows of q are here: this use tells the compiler, which else would wait for them, and with them for the next
+     * tile's codes, at every tile's first product */
+    auto have_q = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < DS; i++) asm volatile("" : "+v"(qf[i]));
+    };
+    have_q();
     if constexpr (NST == 2) {
-        if (t0 < t1) {
-            load(t0);
-            store(0);
-            if (t0 + 1 < t1) load(t0 + 1);
+        if (i0 < w1) {
+            store(0, i0);
+            move(i0 + KS);
+            if (i0 + KS < w1) load();
         }
         __syncthreads();
-        for (int i = t0; i < t0 + sp; i++) {        /* every slice meets as often; its tiles end at t1 */
-            const int buf = (i - t0) & 1;
-            if (i + 1 < t1) {
-                store(buf ^ 1);
-                if (i + 2 < t1) load(i + 2);
+        for (int n = 0, i = i0; n < w1 - w0; n += KS, i += KS) {    /* every slice meets as often; its tiles end at w1 */
+            const int buf = n / KS & 1;
+            if (i + KS < w1) {
+                store(buf ^ 1, i + KS);
+                move(i + 2 * KS);
+                if (i + 2 * KS < w1) load();
             }
-            if (i < t1) tile(buf, i);
+            if (i < w1) tile(buf, i);
             __syncthreads();
         }
     } else {
         /* one wave's tiles: its LDS accesses are in order */
-        if (t0 < t1) load(t0);
-        for (int i = t0; i < t1; i++) {
-            store(0);
-            if (i + 1 < t1) load(i + 1);
+        for (int i = i0; i < w1; i += KS) {
+            store(0, i);
+            move(i + KS);
+            if (i + KS < w1) load();
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
             tile(0, i);
@@ -320,8 +415,35 @@ __global__ __launch_bounds__(64 * QW * KS) void k_pattn(PaArgs x) {
         __syncthreads();                            /* slices still reading their stages */
     }
 
-    /* join: lanes l and l ^ 32 hold half of a row's sum each */
+    /* lanes l and l ^ 32 hold half of a row's sum each */
     l += xor32_f32(l, lane);
+    if constexpr (KS == 1) {
+        /* from the accumulators: through LDS, in whole rows, this took 2 us more */
+        if (row0 + l32 < J.R) {
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            float *P = x.part + J.part + ((size_t)(sh * J.ns + split) * J.R + row0 + l32) * pa_row(DP);
+            const long long at = qb * a.o_batch + hd * a.o_head + tok * a.o_token;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int c = 32 * d + 8 * r + 4 * g;
+                    const float y[4] = {o[d][4 * r], o[d][4 * r + 1], o[d][4 * r + 2], o[d][4 * r + 3]};
+                    if (x.part) {
+                        *reinterpret_cast<float4 *>(P + c) = make_float4(y[0], y[1], y[2], y[3]);
+                    } else if (c < D) {
+                        if (a.out_f32) {
+                            *reinterpret_cast<float4 *>((float *)a.out + at + c) = make_float4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+                        } else {
+                            typedef T v4 __attribute__((ext_vector_type(4)));
+                            *reinterpret_cast<v4 *>((T *)a.out + at + c) = v4{(T)(y[0] * inv), (T)(y[1] * inv), (T)(y[2] * inv), (T)(y[3] * inv)};
+                        }
+                    }
+                }
+            if (x.part && g == 0) *reinterpret_cast<float4 *>(P + DP) = make_float4(ref, l, lo, 0.0f);
+        }
+        return;
+    }
     float *E = (float *)smem + wid * 32 * ES;
     float *ML = (float *)smem + NW * 32 * ES;       /* per wave 32 references, 32 sums, 32 remainders of the references */
 #pragma unroll
@@ -335,9 +457,9 @@ __global__ __launch_bounds__(64 * QW * KS) void k_pattn(PaArgs x) {
 
     /* a group of CPR lanes finishes one row, 8 dims per lane; the KS waves of a block of rows take them in turn */
     constexpr int RPW = 64 / CPR;                    /* rows per wave at once */
-    const int c8 = 8 * (lane % CPR);
+    const int c8 = 8 * (lane % CPR), rows = min(32, J.R - row0);
 #pragma unroll 1
-    for (int i = ks; i < 32 / RPW; i += KS) {
+    for (int i = ks; i * RPW < rows; i += KS) {
         const int q = i * RPW + lane / CPR;          /* row within the block */
         float v[8], m[KS], c[KS];
 #pragma unroll
@@ -362,10 +484,9 @@ __global__ __launch_bounds__(64 * QW * KS) void k_pattn(PaArgs x) {
 #pragma unroll
             for (int j = 0; j < 8; j++) v[j] = __builtin_fmaf(f, e[j], v[j]);
         }
-        const int orow = rb * 32 * QW + qw * 32 + q;
-        if (orow >= J.R || c8 >= D) continue;
+        if (q >= rows || c8 >= D) continue;
         if (x.part) {
-            float *P = x.part + J.part + ((size_t)(sh * J.ns + split) * J.R + orow) * pa_row(DP);
+            float *P = x.part + J.part + ((size_t)(sh * J.ns + split) * J.R + row0 + q) * pa_row(DP);
             *reinterpret_cast<float4 *>(P + c8) = make_float4(v[0], v[1], v[2], v[3]);
             *reinterpret_cast<float4 *>(P + c8 + 4) = make_float4(v[4], v[5], v[6], v[7]);
             if (c8 == 0) *reinterpret_cast<float4 *>(P + DP) = make_float4(rm, rs, rl, 0.0f);
@@ -373,7 +494,7 @@ __global__ __launch_bounds__(64 * QW * KS) void k_pattn(PaArgs x) {
         }
         const float inv = rs == 0.0f ? 0.0f : 1.0f / rs;
         int b, t, h;
-        where(orow, b, t, h);
+        where(row0 + q, b, t, h);
         const long long at = b * a.o_batch + h * a.o_head + t * a.o_token + c8;
         if (a.out_f32) {
             float *y = (float *)a.out + at;
@@ -388,113 +509,270 @@ __global__ __launch_bounds__(64 * QW * KS) void k_pattn(PaArgs x) {
     }
 }
 
-/* Joins the partial results of one row: those of the prefix's splits, then those of the own part's. A group of DP / 8 lanes per
- * 8 dims, the wave's 64 / (DP / 8) groups take the splits in turn and add up through lane exchanges */
-template <typename T, int DP>
-__global__ __launch_bounds__(64) void k_pattn_join(PaArgs x, int KT) {
-    constexpr int CPR = DP / 8, NG = 64 / CPR;
+/* One dword of every 64 bytes of a kernel's arguments, all on their way together: the compiler loads arguments where it first
+ * needs them, and each line that is not in the scalar cache yet costs 0.4 us there */
+template <typename A>
+__device__ __forceinline__ void pa_fetch(const A &x) {
+    const int *p = (const int *)&x;
+    int v = 0;
+#pragma unroll
+    for (unsigned i = 0; i < (sizeof(A) + 63) / 64; i++) v |= p[16 * i];
+    asm volatile("" : : "s"(v));
+}
+
+/* FORMS: the forms that the launch's kinds have, a bit to each */
+template <typename T, int DP, int FORMS>
+__global__ __launch_bounds__(256) void k_pattn(PaArgs x) {
+    constexpr int l0 = FORMS & 1 ? pa_lds(DP, 0) : 0, l1 = FORMS & 2 ? pa_lds(DP, 1) : 0, l2 = FORMS & 4 ? pa_lds(DP, 2) : 0;
+    __shared__ __attribute__((aligned(16))) uint8_t smem[l0 > l1 ? (l0 > l2 ? l0 : l2) : l1 > l2 ? l1 : l2];
+    pa_fetch(x);
+    /* each kind spreads over all XCDs by itself, neighbouring jobs (which read the same keys) to one */
+    const int first = (x.j[0].jobs + 7) & ~7, kind = (int)blockIdx.x >= first;
+    const int job = xcd_tile(blockIdx.x - (kind ? first : 0), x.j[kind].jobs);
+    if (job >= x.j[kind].jobs) return;
+    const int form = x.j[kind].form;
+    if constexpr ((FORMS & 1) != 0) if (form == 0) pa_work<T, DP, 0>(x, kind, job, smem);
+    if constexpr ((FORMS & 2) != 0) if (form == 1) pa_work<T, DP, 1>(x, kind, job, smem);
+    if constexpr ((FORMS & 4) != 0) if (form == 2) pa_work<T, DP, 2>(x, kind, job, smem);
+}
+
+/* Joins the partial results of a row: those of the prefix's splits, then those of the own part's. WR waves to a row: first
+ * each thread takes a split's reference and sum, then groups of DP / 8 lanes, 8 dims to a lane, take the splits' sums in turn */
+template <typename T, int DP, int WR>
+__global__ __launch_bounds__(256) void k_pattn_join(PaArgs x) {
+    constexpr int CPR = DP / 8, TR = 64 * WR, NG = TR / CPR, RB = 4 / WR, MOST = 512;
+    constexpr int FIRST = 2;                                   /* a group's splits that are on their way before the factors are known */
+    __shared__ float fac[RB][MOST], red[RB][WR][4];
+    __shared__ __attribute__((aligned(16))) float acc[RB][WR][DP];
+    pa_fetch(x);
     const aria_hip_prefix_attn &a = x.a;
-    const int per_seq = a.Nq * x.G;
-    for (int i = blockIdx.x; i < a.B * a.H * a.Nq; i += gridDim.x) {
-        const int hk = i / per_seq % a.own.Hkv, b = i / per_seq / a.own.Hkv, row = i % per_seq;
-        const int lane = threadIdx.x, grp = lane / CPR, c8 = 8 * (lane % CPR), D = a.own.D;
-        const int pf = b / x.Bp;
+    const int per_seq = a.Nq * x.G, rows = a.B * a.H * a.Nq;
+    const int sub = threadIdx.x / TR, tr = threadIdx.x % TR, wv = tr / 64, lane = threadIdx.x & 63;
+    const int grp = tr / CPR, c8 = 8 * (tr % CPR), D = a.own.D;
+    for (int i0 = blockIdx.x * RB; i0 < rows; i0 += gridDim.x * RB) {
+        const int i = min(i0 + sub, rows - 1);
+        const int bh = x.dseq.of(i), row = i - bh * per_seq, b = x.dhkv.of(bh), hk = bh - b * a.own.Hkv, pf = x.dbp.of(b);
         const int n0 = a.prefix_len ? min(max(a.prefix_len[pf], 0), a.prefix.cap) : a.prefix.cap;
         const int n1 = a.own_len ? min(max(a.own_len[b], 0), a.own.cap) : a.own.cap;
-        const int nt0 = (n0 + KT - 1) / KT, nt1 = (n1 + KT - 1) / KT;
-        auto splits = [&](const PaJobs &J, int nt) { return max(1, (nt + J.per - 1) / J.per); };   /* those that hold keys */
-        const int s0 = splits(x.j[0], x.group ? nt0 : nt0 + nt1), s1 = x.kinds == 2 ? splits(x.j[1], nt1) : 0;
-        const int set0 = x.group ? pf : b, row_0 = x.group ? (b - pf * x.Bp) * per_seq + row : row;
-        auto at = [&](int s) __attribute__((always_inline)) -> const float * {
-            if (s < s0) return x.part + x.j[0].part + ((size_t)((set0 * a.own.Hkv + hk) * x.j[0].ns + s) * x.j[0].R + row_0) * pa_row(DP);
-            return x.part + x.j[1].part + ((size_t)((b * a.own.Hkv + hk) * x.j[1].ns + s - s0) * x.j[1].R + row) * pa_row(DP);
+        auto splits = [&](int kind, bool p, bool o) __attribute__((always_inline)) {   /* those that hold keys */
+            const PaJobs &J = x.j[kind];
+            const int KT = pa_tile(DP, J.form), nt = (p ? (n0 + KT - 1) / KT : 0) + (o ? (n1 + KT - 1) / KT : 0);
+            return max(1u, J.dper.of(nt + J.per - 1));
         };
-        const int ns = s0 + s1;
-        float m = XA_MIN, ml = -INFINITY;                          /* the largest reference and its largest remainder */
-        for (int s = lane; s < ns; s += 64) {
-            const float *p = at(s) + DP;
-            ml = p[0] > m ? p[2] : p[0] == m ? fmaxf(ml, p[2]) : ml;
-            m = fmaxf(m, p[0]);
+        const int s0 = splits(0, true, !x.group), s1 = x.kinds == 2 ? (int)splits(1, false, true) : 0, ns = s0 + s1;
+        const int set0 = x.group ? pf : b, row_0 = x.group ? (b - pf * x.Bp) * per_seq + row : row;
+        const float *p0 = x.part + x.j[0].part + ((size_t)(set0 * a.own.Hkv + hk) * x.j[0].ns * x.j[0].R + row_0) * pa_row(DP);
+        const float *p1 = x.part + x.j[1].part + ((size_t)(b * a.own.Hkv + hk) * x.j[1].ns * x.j[1].R + row) * pa_row(DP);
+        const size_t st0 = (size_t)x.j[0].R * pa_row(DP), st1 = (size_t)x.j[1].R * pa_row(DP);
+        auto at = [&](int s) __attribute__((always_inline)) { return s < s0 ? p0 + s * st0 : p1 + (s - s0) * st1; };
+        float4 u[FIRST], w[FIRST];
+#pragma unroll
+        for (int j = 0; j < FIRST; j++) {
+            const float *p = at(min(grp + j * NG, ns - 1)) + c8;
+            u[j] = *reinterpret_cast<const float4 *>(p);
+            w[j] = *reinterpret_cast<const float4 *>(p + 4);
         }
-        const float ma = grp_max<64>(m);
-        ml = grp_max<64>(m == ma ? ml : -INFINITY);
-        m = ma;
-        float rs = 0.0f, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (c8 < D)
-#pragma unroll 4
-            for (int s = grp; s < ns; s += NG) {
-                const float *p = at(s);
-                const float f = __builtin_amdgcn_exp2f((p[DP] - m) + (p[DP + 2] - ml));
-                rs = __builtin_fmaf(f, p[DP + 1], rs);
-                const float4 u = *reinterpret_cast<const float4 *>(p + c8), w = *reinterpret_cast<const float4 *>(p + c8 + 4);
-                const float e[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+        float4 h = make_float4(XA_MIN, 0.0f, -INFINITY, 0.0f);  /* reference, sum, remainder of this thread's split */
+        if (tr < ns) h = *reinterpret_cast<const float4 *>(at(tr) + DP);
+        float m = h.x, ml = h.z;                               /* the largest reference and its largest remainder */
+        for (int s = tr + TR; s < ns; s += TR) {
+            const float4 g = *reinterpret_cast<const float4 *>(at(s) + DP);
+            ml = g.x > m ? g.z : g.x == m ? fmaxf(ml, g.z) : ml;
+            m = fmaxf(m, g.x);
+        }
+        const float mw = grp_max<64>(m), lw = grp_max<64>(m == mw ? ml : -INFINITY);
+        m = mw;
+        ml = lw;
+        if constexpr (WR > 1) {
+            if (lane == 0) { red[sub][wv][0] = m; red[sub][wv][1] = ml; }
+            __syncthreads();
 #pragma unroll
-                for (int j = 0; j < 8; j++) v[j] = __builtin_fmaf(f, e[j], v[j]);
+            for (int k = 0; k < WR; k++) {
+                const float mk = red[sub][k][0], lk = red[sub][k][1];
+                ml = mk > m ? lk : mk == m ? fmaxf(ml, lk) : ml;
+                m = fmaxf(m, mk);
             }
+        }
+        float rs = 0.0f;
+        for (int s = tr; s < ns; s += TR) {
+            const float4 g = s == tr ? h : *reinterpret_cast<const float4 *>(at(s) + DP);
+            const float f = __builtin_amdgcn_exp2f((g.x - m) + (g.z - ml));
+            fac[sub][s] = f;
+            rs = __builtin_fmaf(f, g.y, rs);
+        }
+        rs = grp_sum<64>(rs);
+        if constexpr (WR > 1) {
+            if (lane == 0) red[sub][wv][2] = rs;
+        }
+        __syncthreads();
+        if constexpr (WR > 1) {
+            rs = 0.0f;
 #pragma unroll
-        for (int k = CPR; k < 64; k *= 2) {
-            rs += __shfl_xor(rs, k, 64);
+            for (int k = 0; k < WR; k++) rs += red[sub][k][2];
+        }
+        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        auto more = [&](float f, const float4 &u, const float4 &w) __attribute__((always_inline)) {
+            const float e[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = __builtin_fmaf(f, e[j], v[j]);
+        };
+#pragma unroll
+        for (int j = 0; j < FIRST; j++)
+            if (grp + j * NG < ns) more(fac[sub][grp + j * NG], u[j], w[j]);
+#pragma unroll 4
+        for (int s = grp + FIRST * NG; s < ns; s += NG) {
+            const float *p = at(s) + c8;
+            more(fac[sub][s], *reinterpret_cast<const float4 *>(p), *reinterpret_cast<const float4 *>(p + 4));
+        }
+#pragma unroll
+        for (int k = CPR; k < 64; k *= 2)
 #pragma unroll
             for (int j = 0; j < 8; j++) v[j] += __shfl_xor(v[j], k, 64);
-        }
-        if (grp != 0 || c8 >= D) continue;
-        const float inv = rs == 0.0f ? 0.0f : 1.0f / rs;
-        const long long out = b * a.o_batch + (hk * x.G + row % x.G) * a.o_head + (row / x.G) * a.o_token + c8;
+        if constexpr (WR > 1) {
+            if (lane < CPR) {
+                *reinterpret_cast<float4 *>(&acc[sub][wv][c8]) = make_float4(v[0], v[1], v[2], v[3]);
+                *reinterpret_cast<float4 *>(&acc[sub][wv][c8 + 4]) = make_float4(v[4], v[5], v[6], v[7]);
+            }
+            __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            if (a.out_f32) ((float *)a.out)[out + j] = v[j] * inv;
-            else ((T *)a.out)[out + j] = (T)(v[j] * inv);
+            for (int k = 0; k < WR; k++)
+                if (k != wv)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) v[j] += acc[sub][k][c8 + j];
         }
+        if (grp == 0 && c8 < D && i0 + sub < rows) {
+            const float inv = rs == 0.0f ? 0.0f : 1.0f / rs;
+            const int t = x.dg.of(row);
+            const long long out = b * a.o_batch + (hk * x.G + row - t * x.G) * a.o_head + t * a.o_token + c8;
+            if (a.out_f32) {
+                float *y = (float *)a.out + out;
+                *reinterpret_cast<float4 *>(y) = make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+                *reinterpret_cast<float4 *>(y + 4) = make_float4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
+            } else {
+                typename Xa<T>::v8 y;
+#pragma unroll
+                for (int j = 0; j < 8; j++) y[j] = (T)(v[j] * inv);
+                *reinterpret_cast<typename Xa<T>::v8 *>((T *)a.out + out) = y;
+            }
+        }
+        __syncthreads();                                       /* fac and acc serve the next rows */
     }
 }
 
-/* How a call runs */
-struct PaPlan { int qw, ks, DP, join; };
+/* How a call runs: whether the rows of a prefix's sequences share its tiles, each kind's form and number of splits, by an
+ * estimate of the launches' time. */
+#define PA_SPLITS 256        /* of one kind at most: the join holds a factor of each in LDS */
+struct PaPlan {
+    int DP, join;
+};
 static PaPlan pa_plan(const aria_hip_prefix_attn *a, PaArgs &x) {
+    const int Hkv = a->own.Hkv, P = a->prefix.B, np = a->prefix.cap, no = a->own.cap;
     PaPlan p;
-    const int Hkv = a->own.Hkv, P = a->prefix.B;
+    p.DP = a->own.D <= 64 ? 64 : 128;
     x.G = a->H / Hkv;
     x.Bp = a->B / P;
-    p.DP = a->own.D <= 64 ? 64 : 128;
-    const int R = a->Nq * x.G;
-    const bool has_p = a->prefix.cap > 0, has_o = a->own.cap > 0;
-    const bool share = has_p && x.Bp > 1 && R < 128;
-    const long long rows = share ? (long long)R * x.Bp : R, sets = share ? P : a->B;
-    p.qw = rows <= 32 || sets * Hkv * ((rows + 127) / 128) < 64 ? 1 : 4;
-    p.ks = p.qw == 1 ? 4 : 1;
-    const int KT = pa_tile(p.DP, p.qw), br = 32 * p.qw;
-    auto tiles = [&](int cap) { return (cap + KT - 1) / KT; };
-    auto set_up = [&](PaJobs &J, int sets, long long R, int nt, int up, int uo, size_t part) {
-        J.sets = sets;
-        J.R = (int)R;
-        J.nrb = (int)((R + br - 1) / br);
-        J.use_prefix = up;
-        J.use_own = uo;
-        J.part = part;
-        /* at least 256 keys to a workgroup, and two workgroups to a CU */
-        const long long wg = (long long)sets * Hkv * J.nrb;
-        J.ns = p.qw == 1 ? (int)std::max<long long>(1, std::min<long long>((long long)nt * KT / 256, 512 / wg)) : 1;
-        J.per = std::max(1, (nt + J.ns - 1) / J.ns);
-        J.jobs = (int)(wg * J.ns);
-        return part + (size_t)sets * Hkv * J.ns * R * pa_row(p.DP);
+    const long long R = (long long)a->Nq * x.G;
+    /* us for 1024 keys of a workgroup that has its CU alone, of one of two, and of one of as many as a CU holds, and that number:
+     * of forms 0, 1 and 2 at widths 64 and 128 */
+    static const double alone[2][3] = {{5.2, 9.5, 17.0}, {10.0, 17.0, 25.0}}, paired[2][3] = {{8.6, 14.7, 25.3}, {15.0, 25.4, 38.4}};
+    static const double full[2][3] = {{8.6, 14.7, 33.0}, {15.0, 25.4, 38.4}};
+    static const int hold[2][3] = {{2, 2, 3}, {2, 2, 2}};
+    const int wide = p.DP == 128;
+    const double begin = 2.5;                                 /* us of a workgroup beside its tiles */
+    struct Kind {
+        long long sets, R, wg;
+        int n0, n1, form, nt, ns, per;
     };
-    x.group = share;
-    if (share) {
-        const size_t n = set_up(x.j[0], P, rows, tiles(a->prefix.cap), 1, 0, 0);
-        x.kinds = 1;
-        x.j[1] = PaJobs{};
-        if (has_o) {
-            x.kinds = 2;
-            set_up(x.j[1], a->B, R, tiles(a->own.cap), 0, 1, n);
+    auto kind = [&](long long sets, long long R, int n0, int n1, int form) {
+        const int br = 32 << form, KT = pa_tile(p.DP, form);
+        Kind k{sets, R, sets * Hkv * ((R + br - 1) / br), n0, n1, form, (n0 + KT - 1) / KT + (n1 + KT - 1) / KT, 1, 1};
+        return k;
+    };
+    auto split = [&](Kind &k, long long ns) {
+        k.ns = (int)std::max<long long>(1, std::min<long long>(ns, std::min(PA_SPLITS, k.nt)));
+        k.per = std::max(1, (k.nt + k.ns - 1) / k.ns);
+        k.ns = std::max(1, (k.nt + k.per - 1) / k.per);
+    };
+    auto estimate = [&](const Kind *k, int kinds) {
+        long long jobs = 0;
+        double all = 0, longest = 0, bytes = 0;
+        for (int i = 0; i < kinds; i++) jobs += k[i].wg * k[i].ns;
+        for (int i = 0; i < kinds; i++) {
+            const double keys = (double)k[i].per * pa_tile(p.DP, k[i].form) / 1024;
+            all += (double)k[i].wg * k[i].ns * (begin + keys * full[wide][k[i].form]) / (256 * hold[wide][k[i].form]);
+            longest = std::max(longest, begin + keys * (jobs <= 256 ? alone : jobs <= 512 ? paired : full)[wide][k[i].form]);
+            bytes += (double)k[i].sets * Hkv * k[i].ns * k[i].R * pa_row(p.DP) * sizeof(float);
         }
-        p.join = x.kinds == 2 || x.j[0].ns > 1;
-    } else {
-        x.kinds = 1;
-        set_up(x.j[0], a->B, R, (has_p ? tiles(a->prefix.cap) : 0) + (has_o ? tiles(a->own.cap) : 0), has_p, has_o, 0);
-        x.j[1] = PaJobs{};
-        p.join = x.j[0].ns > 1;
+        if (jobs > 768 && jobs < 3000) all += 0.25 * longest;  /* the last round is not full */
+        const double t = std::max(all, longest);
+        return kinds == 2 || k[0].ns > 1 ? t + 4.0 + bytes / 1.6e6 : t;
+    };
+    double best = 1e30;
+    Kind got[2];
+    int got_kinds = 1, got_group = 0;
+    auto attempt = [&](Kind *k, int kinds, int group) {
+        const double t = estimate(k, kinds);
+        if (t < best) {
+            best = t;
+            got[0] = k[0];
+            if (kinds == 2) got[1] = k[1];
+            got_kinds = kinds;
+            got_group = group;
+        }
+    };
+    for (int group = 0; group < (np > 0 && x.Bp > 1 ? 2 : 1); group++) {
+        const int kinds = group && no > 0 ? 2 : 1;
+        for (int form = 0; form < 3; form++) {
+            Kind k[2];
+            k[0] = group ? kind(P, R * x.Bp, np, 0, form) : kind(a->B, R, np, no, form);
+            if (form && k[0].R <= 16 << form) continue;       /* half of the block idle */
+            for (int j = 0; j < (kinds == 2 ? 3 : 1); j++) {
+                if (kinds == 2) {
+                    k[1] = kind(a->B, R, 0, no, R <= 32 ? 0 : R <= 64 ? 1 : 2);
+                    split(k[1], j == 0 ? 1 : j == 1 ? (k[1].nt + 7) / 8 : (k[1].nt + 3) / 4);
+                    if (j && k[1].ns == 1) break;
+                }
+                const long long others = kinds == 2 ? k[1].wg * k[1].ns : 0;
+                const long long room[4] = {0, 256 - others, 512 - others, 512};
+                int last = 0;
+                for (int i = 0; i < 4; i++) {
+                    split(k[0], room[i] / k[0].wg);
+                    if (k[0].ns != last) attempt(k, kinds, group);
+                    last = k[0].ns;
+                }
+                split(k[0], (k[0].nt + 3) / 4);
+                if (k[0].wg * k[0].ns < 256) attempt(k, kinds, group);
+            }
+        }
     }
-    x.jobs = x.j[0].jobs + x.j[1].jobs;
+    x.dhkv = PaDiv(Hkv);
+    x.dseq = PaDiv((int)R);
+    x.dg = PaDiv(x.G);
+    x.dbp = PaDiv(x.Bp);
+    x.group = got_group;
+    x.kinds = got_kinds;
+    x.j[0] = x.j[1] = PaJobs{};
+    size_t part = 0;
+    for (int i = 0; i < got_kinds; i++) {
+        const Kind &k = got[i];
+        PaJobs &J = x.j[i];
+        J.sets = (int)k.sets;
+        J.R = (int)k.R;
+        J.nrb = (int)(k.wg / (k.sets * Hkv));
+        J.form = k.form;
+        J.ns = k.ns;
+        J.per = k.per;
+        J.jobs = (int)(k.wg * k.ns);
+        J.use_prefix = k.n0 > 0;
+        J.use_own = k.n1 > 0;
+        J.tp = (k.n0 + pa_tile(p.DP, k.form) - 1) / pa_tile(p.DP, k.form);
+        J.dnrb = PaDiv(J.nrb);
+        J.dns = PaDiv(J.ns);
+        J.dper = PaDiv(J.per);
+        J.part = part;
+        part += (size_t)k.sets * Hkv * k.ns * k.R * pa_row(p.DP);
+    }
+    p.join = got_kinds == 2 || got[0].ns > 1;
     return p;
 }
 
@@ -502,27 +780,27 @@ extern "C" size_t aria_k_pattn_ws_bytes(const aria_hip_prefix_attn *a) {
     PaArgs x{};
     const PaPlan p = pa_plan(a, x);
     size_t n = 0;
-    for (int i = 0; i < 2; i++) n += (size_t)x.j[i].sets * a->own.Hkv * x.j[i].ns * x.j[i].R * pa_row(p.DP);
+    for (int i = 0; i < x.kinds; i++) n += (size_t)x.j[i].sets * a->own.Hkv * x.j[i].ns * x.j[i].R * pa_row(p.DP);
     return p.join ? n * sizeof(float) : 0;
 }
 
-template <typename T>
-static hipError_t pa_launch(const PaPlan &p, const PaArgs &x, hipStream_t s) {
-    const dim3 grid((unsigned)((x.jobs + 7) / 8 * 8));
-    if (p.qw == 1) {
-        if (p.DP == 64) hipLaunchKernelGGL((k_pattn<T, 64, 1, 4>), grid, dim3(256), 0, s, x);
-        else hipLaunchKernelGGL((k_pattn<T, 128, 1, 4>), grid, dim3(256), 0, s, x);
-    } else {
-        if (p.DP == 64) hipLaunchKernelGGL((k_pattn<T, 64, 4, 1>), grid, dim3(256), 0, s, x);
-        else hipLaunchKernelGGL((k_pattn<T, 128, 4, 1>), grid, dim3(256), 0, s, x);
+template <typename T, int DP>
+static void pa_launch(const PaPlan &p, const PaArgs &x, hipStream_t s) {
+    const dim3 grid((unsigned)(((x.j[0].jobs + 7) & ~7) + ((x.j[1].jobs + 7) & ~7)));
+    switch (1 << x.j[0].form | (x.kinds == 2 ? 1 << x.j[1].form : 0)) {
+    case 1: hipLaunchKernelGGL((k_pattn<T, DP, 1>), grid, dim3(256), 0, s, x); break;
+    case 2: hipLaunchKernelGGL((k_pattn<T, DP, 2>), grid, dim3(256), 0, s, x); break;
+    case 3: hipLaunchKernelGGL((k_pattn<T, DP, 3>), grid, dim3(256), 0, s, x); break;
+    case 4: hipLaunchKernelGGL((k_pattn<T, DP, 4>), grid, dim3(256), 0, s, x); break;
+    case 5: hipLaunchKernelGGL((k_pattn<T, DP, 5>), grid, dim3(256), 0, s, x); break;
+    case 6: hipLaunchKernelGGL((k_pattn<T, DP, 6>), grid, dim3(256), 0, s, x); break;
     }
-    if (p.join) {
-        const dim3 rows((unsigned)std::min(x.a.B * x.a.H * x.a.Nq, 1 << 20));
-        const int KT = pa_tile(p.DP, p.qw);
-        if (p.DP == 64) hipLaunchKernelGGL((k_pattn_join<T, 64>), rows, dim3(64), 0, s, x, KT);
-        else hipLaunchKernelGGL((k_pattn_join<T, 128>), rows, dim3(64), 0, s, x, KT);
-    }
-    return hipGetLastError();
+    if (!p.join) return;
+    const int rows = x.a.B * x.a.H * x.a.Nq;
+    if (x.j[0].ns + x.j[1].ns > 16)
+        hipLaunchKernelGGL((k_pattn_join<T, DP, 4>), dim3(std::min(rows, 1 << 20)), dim3(256), 0, s, x);
+    else
+        hipLaunchKernelGGL((k_pattn_join<T, DP, 1>), dim3(std::min((rows + 3) / 4, 1 << 20)), dim3(256), 0, s, x);
 }
 
 extern "C" hipError_t aria_k_pattn_run(const aria_hip_prefix_attn *a, void *ws, hipStream_t s) {
@@ -532,5 +810,9 @@ extern "C" hipError_t aria_k_pattn_run(const aria_hip_prefix_attn *a, void *ws, 
     const PaPlan p = pa_plan(a, x);
     x.scale_log2 = a->scale * ARIA_LOG2E;
     x.part = p.join ? (float *)ws : nullptr;
-    return a->type == 1 ? pa_launch<_Float16>(p, x, s) : pa_launch<__bf16>(p, x, s);
+    if (a->type == 1 && p.DP == 64) pa_launch<_Float16, 64>(p, x, s);
+    else if (a->type == 1) pa_launch<_Float16, 128>(p, x, s);
+    else if (p.DP == 64) pa_launch<__bf16, 64>(p, x, s);
+    else pa_launch<__bf16, 128>(p, x, s);
+    return hipGetLastError();
 }

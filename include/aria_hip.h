@@ -394,7 +394,7 @@ int aria_hip_kv_read_dev(const aria_hip_kv_read *a, void *stream);
  * or a value of byte 255 that it sees makes the whole row NaN.
  * Cached values are rounded to q's type (exact in bf16; fp16 below 65520 and above 2^-24 steps), probabilities too; sums
  * and softmax statistics are fp32. D up to 128; scale positive, at most 2^127; B * H at most 2^20, B * H * Nq at
- * most 2^30. q and out 16-byte aligned, strides multiples of 8.
+ * most 2^30; a cache's token stride below 2^24. q and out 16-byte aligned, strides multiples of 8.
  * Many sequences' rows together read a prefix once. dws: aria_hip_prefix_attention_ws_bytes(a) bytes (0: may be
  * NULL), 256-byte aligned, not shared by calls that may run at the same time; the number goes by B, H, Nq and both
  * caches' B, Hkv, D and cap alone. */
