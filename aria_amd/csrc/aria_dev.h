@@ -231,6 +231,28 @@ __device__ __forceinline__ void dma16_s(const void *base, unsigned off, uint32_t
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(m), "v"(off), "s"(b) : "memory");
 }
 
+/* Division by a number that the host knows, of 0 .. 2^31 - 1: by a product (the compiler's own takes some thirty
+ * instructions, and a launch fetches every one of them first) */
+struct HostDiv {
+    unsigned d, mul, sh;
+    HostDiv(int n = 1) : d(n), mul(0), sh(0) {
+        while ((1ull << (sh + 1)) < d) sh++;        /* 2^(sh + 1) >= d > 2^sh, d > 1 */
+        if (d > 1) mul = (unsigned)(((1ull << (32 + sh)) + d - 1) / d);
+    }
+    __device__ __forceinline__ unsigned of(unsigned n) const { return d == 1 ? n : __umulhi(n, mul) >> sh; }
+};
+
+/* One dword of every 64 bytes of a kernel's arguments, all on their way together: the compiler loads arguments where it first
+ * needs them, and each line that is not in the scalar cache yet costs 0.4 us there */
+template <typename A>
+__device__ __forceinline__ void fetch_args(const A &x) {
+    const int *p = (const int *)&x;
+    int v = 0;
+#pragma unroll
+    for (unsigned i = 0; i < (sizeof(A) + 63) / 64; i++) v |= p[16 * i];
+    asm volatile("" : : "s"(v));
+}
+
 template <int I>
 using IC = std::integral_constant<int, I>;
 /* f(IC<0>{}), ..., f(IC<N-1>{}) */

@@ -32,23 +32,12 @@ template <> struct Pc<__bf16> {
     template <bool HI> static __device__ __forceinline__ Xa<__bf16>::v2 cvt(unsigned u, float s) { return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(u, s, HI); }
 };
 
-/* Division by a number that the host knows, of 0 .. 2^31 - 1: by a product (the compiler's own takes some thirty
- * instructions, and a launch fetches every one of them first) */
-struct PaDiv {
-    unsigned d, mul, sh;
-    PaDiv(int n = 1) : d(n), mul(0), sh(0) {
-        while ((1ull << (sh + 1)) < d) sh++;        /* 2^(sh + 1) >= d > 2^sh, d > 1 */
-        if (d > 1) mul = (unsigned)(((1ull << (32 + sh)) + d - 1) / d);
-    }
-    __device__ __forceinline__ unsigned of(unsigned n) const { return d == 1 ? n : __umulhi(n, mul) >> sh; }
-};
-
 /* One kind of workgroup: `sets` sets of R rows (a prefix's, or a sequence's), nrb row blocks to each and key head, ns splits of
  * `per` key tiles. Form 0, 1, 2: a row block of 32, 64 or 128 rows, whose keys 4, 2 or 1 slices of waves share out */
 struct PaJobs {
     int sets, R, nrb, ns, per, jobs, form;
     int use_prefix, use_own, tp;                    /* tp: tiles of a prefix's capacity */
-    PaDiv dnrb, dns, dper;
+    HostDiv dnrb, dns, dper;
     size_t part;             /* floats in front of its partial results */
 };
 struct PaArgs {
@@ -56,7 +45,7 @@ struct PaArgs {
     int G, Bp;               /* query heads per key head; sequences per prefix */
     int kinds, group;        /* one kind of workgroup or two; the first takes the rows of a prefix's sequences together */
     PaJobs j[2];
-    PaDiv dhkv, dseq, dg, dbp;                      /* Hkv, rows of a sequence and key head, G, Bp */
+    HostDiv dhkv, dseq, dg, dbp;                      /* Hkv, rows of a sequence and key head, G, Bp */
     float scale_log2;
     float *part;
 };
@@ -509,23 +498,12 @@ __device__ __forceinline__ void pa_work(const PaArgs &x, int kind, int job, uint
     }
 }
 
-/* One dword of every 64 bytes of a kernel's arguments, all on their way together: the compiler loads arguments where it first
- * needs them, and each line that is not in the scalar cache yet costs 0.4 us there */
-template <typename A>
-__device__ __forceinline__ void pa_fetch(const A &x) {
-    const int *p = (const int *)&x;
-    int v = 0;
-#pragma unroll
-    for (unsigned i = 0; i < (sizeof(A) + 63) / 64; i++) v |= p[16 * i];
-    asm volatile("" : : "s"(v));
-}
-
 /* FORMS: the forms that the launch's kinds have, a bit to each */
 template <typename T, int DP, int FORMS>
 __global__ __launch_bounds__(256) void k_pattn(PaArgs x) {
     constexpr int l0 = FORMS & 1 ? pa_lds(DP, 0) : 0, l1 = FORMS & 2 ? pa_lds(DP, 1) : 0, l2 = FORMS & 4 ? pa_lds(DP, 2) : 0;
     __shared__ __attribute__((aligned(16))) uint8_t smem[l0 > l1 ? (l0 > l2 ? l0 : l2) : l1 > l2 ? l1 : l2];
-    pa_fetch(x);
+    fetch_args(x);
     /* each kind spreads over all XCDs by itself, neighbouring jobs (which read the same keys) to one */
     const int first = (x.j[0].jobs + 7) & ~7, kind = (int)blockIdx.x >= first;
     const int job = xcd_tile(blockIdx.x - (kind ? first : 0), x.j[kind].jobs);
@@ -544,7 +522,7 @@ __global__ __launch_bounds__(256) void k_pattn_join(PaArgs x) {
     constexpr int FIRST = 2;                                   /* a group's splits that are on their way before the factors are known */
     __shared__ float fac[RB][MOST], red[RB][WR][4];
     __shared__ __attribute__((aligned(16))) float acc[RB][WR][DP];
-    pa_fetch(x);
+    fetch_args(x);
     const aria_hip_prefix_attn &a = x.a;
     const int per_seq = a.Nq * x.G, rows = a.B * a.H * a.Nq;
     const int sub = threadIdx.x / TR, tr = threadIdx.x % TR, wv = tr / 64, lane = threadIdx.x & 63;
@@ -745,10 +723,10 @@ static PaPlan pa_plan(const aria_hip_prefix_attn *a, PaArgs &x) {
             }
         }
     }
-    x.dhkv = PaDiv(Hkv);
-    x.dseq = PaDiv((int)R);
-    x.dg = PaDiv(x.G);
-    x.dbp = PaDiv(x.Bp);
+    x.dhkv = HostDiv(Hkv);
+    x.dseq = HostDiv((int)R);
+    x.dg = HostDiv(x.G);
+    x.dbp = HostDiv(x.Bp);
     x.group = got_group;
     x.kinds = got_kinds;
     x.j[0] = x.j[1] = PaJobs{};
@@ -766,9 +744,9 @@ static PaPlan pa_plan(const aria_hip_prefix_attn *a, PaArgs &x) {
         J.use_prefix = k.n0 > 0;
         J.use_own = k.n1 > 0;
         J.tp = (k.n0 + pa_tile(p.DP, k.form) - 1) / pa_tile(p.DP, k.form);
-        J.dnrb = PaDiv(J.nrb);
-        J.dns = PaDiv(J.ns);
-        J.dper = PaDiv(J.per);
+        J.dnrb = HostDiv(J.nrb);
+        J.dns = HostDiv(J.ns);
+        J.dper = HostDiv(J.per);
         J.part = part;
         part += (size_t)k.sets * Hkv * k.ns * k.R * pa_row(p.DP);
     }

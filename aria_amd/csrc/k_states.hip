@@ -62,28 +62,6 @@ extern "C" hipError_t aria_k_rotary_table(float *cos_t, float *sin_t, const doub
 
 /* ---- rotation and the cache ---- */
 
-/* elements off .. off + n - 1 of p (n at most 8, the others read as zero) as eight elements; p + off has its element's
- * alignment only */
-template <typename T>
-__device__ __forceinline__ void ld8(const T *p, int n, T (&f)[8]) {
-    if (n >= 8) {
-        __builtin_memcpy(f, p, sizeof f);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) f[i] = i < n ? p[i] : (T)0.0f;
-    }
-}
-template <typename T>
-__device__ __forceinline__ void st8(T *p, int n, const T (&f)[8]) {
-    if (n >= 8) {
-        __builtin_memcpy(p, f, sizeof f);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (i < n) p[i] = f[i];
-    }
-}
-
 /* the larger of two magnitudes as bits: an Inf or a NaN is above every finite value */
 struct OpMaxBits {
     __device__ __forceinline__ float operator()(float a, float b) const {
@@ -111,136 +89,273 @@ struct StArgs {
     int B, N, D, rot, npos, cap, inverse;
     int nsec, chunks;        /* sections, and groups of HG heads in all of them */
     int64_t blocks;          /* workgroups' shares: one, or every ST_GRID-th, to each */
-    int lr;                  /* lanes that hold rotated pairs */
+    HostDiv dn, dchunks;
 };
 
-/* A group of LPR lanes takes HG heads of one token. Lane l < lr holds the pairs 8 l .. 8 l + 7, the others 16 plain
- * dims each, as two runs of eight: a at ia, b at ib. The products and the sum of a rotation are fp32 where the result is rounded
- * to 16 bits; where it is an fp32 number (fp32 states, keys before they are quantised) they are 64 bits wide, so that it is
- * the rounded exact value and a code does not depend on the order of two roundings. */
+/* a and b of a pair, rotated. The products and the sum are fp32 where the result is rounded to 16 bits; where it is an fp32
+ * number (fp32 states, keys before they are quantised) they are 64 bits wide, so that it is the rounded exact value and a code
+ * does not hang on the order of two roundings */
+template <bool WIDE>
+__device__ __forceinline__ void st_turn(float &a, float &b, float c, float s) {
+    const float u = a, w = b;
+    if constexpr (WIDE) {
+        a = (float)__builtin_fma((double)u, (double)c, -((double)w * (double)s));
+        b = (float)__builtin_fma((double)w, (double)c, (double)u * (double)s);
+    } else {
+        a = __builtin_fmaf(u, c, -(w * s));
+        b = __builtin_fmaf(w, c, u * s);
+    }
+}
+/* the byte of a row from the bits of its largest magnitude; 448 = 1.75 * 2^8 */
+__device__ __forceinline__ unsigned st_byte(unsigned bits) {
+    const unsigned e = bits >> 23;
+    return e == 255u ? 255u : (unsigned)max(1, (int)e - 8 + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0));
+}
+/* 2^(127 - byte) */
+__device__ __forceinline__ float st_inverse(unsigned byte) { return __builtin_bit_cast(float, (254u - min(byte, 253u)) << 23); }
+
+/* where a share's token lies; false: it is none, or not to be written */
+struct StTok {
+    int b, t;
+    int64_t slot, p;
+};
+__device__ __forceinline__ bool st_token(const StArgs &x, const StSec &s, unsigned tok, StTok &k) {
+    if (tok >= (unsigned)x.B * x.N) return false;
+    k.b = x.dn.of(tok);
+    k.t = tok - k.b * x.N;
+    if (x.count && k.t >= x.count[k.b]) return false;
+    k.slot = (x.first ? (int64_t)x.first[k.b] : 0) + k.t;
+    k.p = x.pos ? (int64_t)x.pos[k.b * x.pos_stride + k.t] : k.slot;
+    if (x.rot && (k.p < 0 || k.p >= x.npos)) return false;
+    return !(s.scale && (k.slot < 0 || k.slot >= x.cap));
+}
+
+/* Whole chunks of eight: D a multiple of 8, rot of 8 (interleaved) or 16. A group of LPR lanes takes HG heads of one token, 16
+ * dims of each to a lane as two chunks: interleaved the chunks 2 l and 2 l + 1, else those of the pairs 8 l .. 8 l + 7, and
+ * behind the rotated dims two plain ones. Every load of the HG rows is on its way before the first is used; chunks and heads
+ * past the last repeat it and are not stored. */
 template <int TY, bool INTER, int LPR, int HG>
 __global__ __launch_bounds__(256) void k_states(StArgs x) {
     using T = typename StT<TY>::type;
-    const int l = threadIdx.x % LPR;
-    auto work = [&](int64_t blk) __attribute__((always_inline)) {
-        int chunk = (int)(blk % x.chunks);
-        const unsigned tok = (unsigned)(blk / x.chunks) * (256 / LPR) + threadIdx.x / LPR;   /* B N is at most 2^30 */
-        int si = 0;
+    typedef T v8 __attribute__((ext_vector_type(8), aligned(alignof(T))));
+    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+    typedef unsigned u2 __attribute__((ext_vector_type(2), aligned(8)));
+    fetch_args(x);
+    const int l = threadIdx.x % LPR, rh = x.rot / 2, nc = x.D / 8;
+    /* the lane's chunks, and whether their pairs are rotated */
+    int ca, cb;
+    bool ra, rb;
+    if (INTER) {
+        ca = 2 * l;
+        cb = ca + 1;
+        ra = 8 * ca < x.rot;
+        rb = 8 * cb < x.rot;
+    } else {
+        const int lr = rh / 8;
+        ra = rb = l < lr;
+        ca = ra ? l : 2 * l;                         /* rot / 8 + 2 (l - lr) = 2 l */
+        cb = ra ? l + lr : 2 * l + 1;
+    }
+    const bool ha = ca < nc, hb = cb < nc;
+    const int ia = 8 * min(ca, nc - 1), ib = 8 * min(cb, nc - 1);
+    const int ta = min(8 * l, max(rh - 4, 0)), tb = min(8 * l + 4, max(rh - 4, 0));      /* their tables' columns */
+
+    for (int64_t blk = blockIdx.x; blk < x.blocks; blk += gridDim.x) {
+        const unsigned tb_ = x.blocks <= 0x7FFFFFFF ? x.dchunks.of((unsigned)blk) : (unsigned)(blk / x.chunks);
+        int chunk = (int)(blk - (int64_t)tb_ * x.chunks), si = 0;
         while (si + 1 < x.nsec && chunk >= x.sec[si].chunks) chunk -= x.sec[si++].chunks;
         const StSec &s = x.sec[si];
-        if (tok >= (unsigned)x.B * x.N) return;
-        const int b = (int)(tok / (unsigned)x.N), t = (int)(tok % (unsigned)x.N);
-        if (x.count && t >= x.count[b]) return;
-        const int64_t slot = (x.first ? (int64_t)x.first[b] : 0) + t;
-        const int64_t p = x.pos ? (int64_t)x.pos[b * x.pos_stride + t] : slot;
-        if (x.rot && (p < 0 || p >= x.npos)) return;
-        if (s.scale && (slot < 0 || slot >= x.cap)) return;
-
-        const int rh = x.rot / 2;
-        const bool turn = l < x.lr && s.rotate;      /* this lane's pairs are rotated */
-        int ia, ib, na, nb, np;                      /* runs, their lengths, pairs */
-        if (l < x.lr) {
-            if (INTER) {
-                ia = 16 * l;
-                ib = ia + 8;
-                na = min(8, x.rot - ia);
-                nb = max(0, min(8, x.rot - ib));
-                np = (na + nb) / 2;
-            } else {
-                ia = 8 * l;
-                ib = rh + ia;
-                na = nb = np = min(8, rh - ia);
-            }
-        } else {
-            ia = x.rot + 16 * (l - x.lr);
-            ib = ia + 8;
-            na = max(0, min(8, x.D - ia));
-            nb = max(0, min(8, x.D - ib));
-            np = 0;
-        }
+        StTok k;
+        if (!st_token(x, s, tb_ * (256 / LPR) + threadIdx.x / LPR, k)) continue;
         const int h0 = chunk * HG, hn = min(HG, s.heads - h0);
-        T fa[HG][8], fb[HG][8];
-        const T *src = (const T *)s.src + b * s.sb + t * s.st + h0 * s.sh;
+        v8 fa[HG], fb[HG];
+        const T *src = (const T *)s.src + k.b * s.sb + k.t * s.st + h0 * s.sh;
 #pragma unroll
         for (int h = 0; h < HG; h++) {
-            if (h < hn) {
-                ld8(src + h * s.sh + ia, na, fa[h]);
-                ld8(src + h * s.sh + ib, nb, fb[h]);
+            const T *r = src + min(h, hn - 1) * s.sh;
+            fa[h] = *reinterpret_cast<const v8 *>(r + ia);
+            fb[h] = *reinterpret_cast<const v8 *>(r + ib);
+        }
+        f4 c[2], sn[2];
+        const bool turn = s.rotate;                  /* uniform */
+        if (turn) {
+            const float *ct = x.cos_t + k.p * rh, *st = x.sin_t + k.p * rh;
+            c[0] = *reinterpret_cast<const f4 *>(ct + ta);
+            c[1] = *reinterpret_cast<const f4 *>(ct + tb);
+            sn[0] = *reinterpret_cast<const f4 *>(st + ta);
+            sn[1] = *reinterpret_cast<const f4 *>(st + tb);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                c[0][i] = ra ? c[0][i] : 1.0f;       /* plain dims: by one and zero */
+                c[1][i] = rb ? c[1][i] : 1.0f;
+                sn[0][i] = ra ? (x.inverse ? -sn[0][i] : sn[0][i]) : 0.0f;
+                sn[1][i] = rb ? (x.inverse ? -sn[1][i] : sn[1][i]) : 0.0f;
             }
         }
-        float c[8], sn[8];
-        if (turn) {
-            ld8(x.cos_t + p * rh + 8 * l, np, c);
-            ld8(x.sin_t + p * rh + 8 * l, np, sn);
+        auto rows = [&](auto TURN, auto CACHE) __attribute__((always_inline)) {
+            constexpr bool turned = decltype(TURN)::value != 0, cache = decltype(CACHE)::value != 0;
 #pragma unroll
-            for (int i = 0; i < 8; i++) sn[i] = x.inverse ? -sn[i] : sn[i];
+            for (int h = 0; h < HG; h++) {
+                float v[16];                         /* chunk a, then chunk b */
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    v[i] = (float)fa[h][i];
+                    v[8 + i] = (float)fb[h][i];
+                }
+                if constexpr (turned) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int ja = INTER ? 2 * i : i, jb = INTER ? 2 * i + 1 : 8 + i;
+                        st_turn<TY == 0 || cache>(v[ja], v[jb], c[i / 4][i % 4], sn[i / 4][i % 4]);
+                    }
+                    if (!(ra && rb)) {               /* plain dims as they came: 0 times an Inf is none of theirs */
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            v[i] = ra ? v[i] : (float)fa[h][i];
+                            v[8 + i] = rb ? v[8 + i] : (float)fb[h][i];
+                        }
+                    }
+                }
+                if constexpr (!cache) {
+                    if (h >= hn) break;
+                    T *d = (T *)s.dst + k.b * s.db + k.t * s.dt + (h0 + h) * s.dh;
+                    v8 y;
+                    if (ha) {
+#pragma unroll
+                        for (int i = 0; i < 8; i++) y[i] = (T)v[i];
+                        *reinterpret_cast<v8 *>(d + ia) = y;
+                    }
+                    if (hb) {
+#pragma unroll
+                        for (int i = 0; i < 8; i++) y[i] = (T)v[8 + i];
+                        *reinterpret_cast<v8 *>(d + ib) = y;
+                    }
+                } else {
+                    float m = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 16; i++) m = OpMaxBits()(m, fabsf(v[i]));
+                    m = grp_reduce<LPR>(m, OpMaxBits());     /* repeated chunks change nothing */
+                    const unsigned byte = st_byte(__builtin_bit_cast(unsigned, m));
+                    const float r = st_inverse(byte);
+                    unsigned w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        int u = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i] * r, v[4 * i + 1] * r, 0, false);
+                        u = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i + 2] * r, v[4 * i + 3] * r, u, true);
+                        w[i] = byte == 255u ? 0x7F7F7F7Fu : (unsigned)u;
+                    }
+                    if (h >= hn) break;
+                    uint8_t *d = (uint8_t *)s.dst + k.b * s.db + k.slot * s.dt + (h0 + h) * s.dh;
+                    if (ha) *reinterpret_cast<u2 *>(d + ia) = u2{w[0], w[1]};
+                    if (hb) *reinterpret_cast<u2 *>(d + ib) = u2{w[2], w[3]};
+                    if (l == 0) s.scale[k.b * s.cb + (h0 + h) * s.ch + k.slot] = (uint8_t)byte;
+                }
+            }
+        };
+        if (s.scale) {
+            if (turn) rows(IC<1>{}, IC<1>{});
+            else rows(IC<0>{}, IC<1>{});
+        } else {
+            if (turn) rows(IC<1>{}, IC<0>{});
+            else rows(IC<0>{}, IC<0>{});
+        }
+    }
+}
+
+/* Any even D and rot: a wave takes HG heads of one token, a pair of dims to a lane (two, where D is over 128); pair p is
+ * (p, p + rot/2) or (2p, 2p + 1) and, behind the rotated ones, (2p, 2p + 1). */
+template <int TY, bool INTER, int HG>
+__global__ __launch_bounds__(256) void k_states_any(StArgs x) {
+    using T = typename StT<TY>::type;
+    constexpr int PL = 2;
+    fetch_args(x);
+    const int lane = threadIdx.x & 63, rh = x.rot / 2, np = x.D / 2;
+    int ia[PL], ib[PL], col[PL];
+    bool turns[PL], have[PL];
+#pragma unroll
+    for (int i = 0; i < PL; i++) {
+        const int p = min(lane + 64 * i, np - 1);
+        have[i] = lane + 64 * i < np;
+        turns[i] = p < rh;
+        ia[i] = !INTER && turns[i] ? p : 2 * p;
+        ib[i] = !INTER && turns[i] ? p + rh : 2 * p + 1;
+        col[i] = min(p, max(rh - 1, 0));
+    }
+    const bool two = np > 64;
+    for (int64_t blk = blockIdx.x; blk < x.blocks; blk += gridDim.x) {
+        const unsigned tb = x.blocks <= 0x7FFFFFFF ? x.dchunks.of((unsigned)blk) : (unsigned)(blk / x.chunks);
+        int chunk = (int)(blk - (int64_t)tb * x.chunks), si = 0;
+        while (si + 1 < x.nsec && chunk >= x.sec[si].chunks) chunk -= x.sec[si++].chunks;
+        const StSec &s = x.sec[si];
+        StTok k;
+        if (!st_token(x, s, tb * 4 + threadIdx.x / 64, k)) continue;
+        const int h0 = chunk * HG, hn = min(HG, s.heads - h0);
+        T fa[HG][PL], fb[HG][PL];
+        const T *src = (const T *)s.src + k.b * s.sb + k.t * s.st + h0 * s.sh;
+#pragma unroll
+        for (int h = 0; h < HG; h++) {
+            const T *r = src + min(h, hn - 1) * s.sh;
+#pragma unroll
+            for (int i = 0; i < PL; i++) {
+                if (i && !two) break;
+                fa[h][i] = r[ia[i]];
+                fb[h][i] = r[ib[i]];
+            }
+        }
+        float c[PL] = {1.0f, 1.0f}, sn[PL] = {0.0f, 0.0f};
+        if (s.rotate) {
+#pragma unroll
+            for (int i = 0; i < PL; i++) {
+                if (i && !two) break;
+                c[i] = x.cos_t[k.p * rh + col[i]];
+                sn[i] = x.sin_t[k.p * rh + col[i]];
+                sn[i] = x.inverse ? -sn[i] : sn[i];
+            }
         }
 #pragma unroll
         for (int h = 0; h < HG; h++) {
             if (h >= hn) break;
-            float v[16];                             /* run a, then run b */
+            float a[PL], b[PL], m = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                v[i] = (float)fa[h][i];
-                v[8 + i] = (float)fb[h][i];
-            }
-            if (turn) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int ja = INTER ? 2 * i : i, jb = INTER ? 2 * i + 1 : 8 + i;
-                    const float u = v[ja], w = v[jb];
-                    if (TY == 0 || s.scale) {        /* uniform */
-                        v[ja] = (float)__builtin_fma((double)u, (double)c[i], -((double)w * (double)sn[i]));
-                        v[jb] = (float)__builtin_fma((double)w, (double)c[i], (double)u * (double)sn[i]);
-                    } else {
-                        v[ja] = __builtin_fmaf(u, c[i], -(w * sn[i]));
-                        v[jb] = __builtin_fmaf(w, c[i], u * sn[i]);
-                    }
+            for (int i = 0; i < PL; i++) {
+                if (i && !two) break;
+                a[i] = (float)fa[h][i];
+                b[i] = (float)fb[h][i];
+                if (s.rotate && turns[i]) {
+                    if (TY == 0 || s.scale) st_turn<true>(a[i], b[i], c[i], sn[i]);
+                    else st_turn<false>(a[i], b[i], c[i], sn[i]);
                 }
+                m = OpMaxBits()(m, OpMaxBits()(fabsf(a[i]), fabsf(b[i])));
             }
             if (!s.scale) {
-                T *d = (T *)s.dst + b * s.db + t * s.dt + (h0 + h) * s.dh;
-                T ya[8], yb[8];
+                T *d = (T *)s.dst + k.b * s.db + k.t * s.dt + (h0 + h) * s.dh;
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    ya[i] = (T)v[i];
-                    yb[i] = (T)v[8 + i];
-                }
-                st8(d + ia, na, ya);
-                st8(d + ib, nb, yb);
-            } else {
-                float m = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 16; i++) m = OpMaxBits()(m, fabsf(v[i]));
-                m = grp_reduce<LPR>(m, OpMaxBits());
-                const unsigned bits = __builtin_bit_cast(unsigned, m), e = bits >> 23;
-                /* 448 = 1.75 * 2^8 */
-                const unsigned byte = e == 255u ? 255u : (unsigned)max(1, (int)e - 8 + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0));
-                const float r = __builtin_bit_cast(float, (254u - min(byte, 253u)) << 23);
-                unsigned w[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    int u = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i] * r, v[4 * i + 1] * r, 0, false);
-                    u = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i + 2] * r, v[4 * i + 3] * r, u, true);
-                    w[i] = byte == 255u ? 0x7F7F7F7Fu : (unsigned)u;
-                }
-                uint8_t *d = (uint8_t *)s.dst + b * s.db + slot * s.dt + (h0 + h) * s.dh;
-                uint8_t wa[8], wb[8];
-                __builtin_memcpy(wa, w, 8);
-                __builtin_memcpy(wb, w + 2, 8);
-                st8(d + ia, na, wa);
-                st8(d + ib, nb, wb);
-                if (l == 0) s.scale[b * s.cb + (h0 + h) * s.ch + slot] = (uint8_t)byte;
+                for (int i = 0; i < PL; i++)
+                    if (have[i]) {
+                        d[ia[i]] = (T)a[i];
+                        d[ib[i]] = (T)b[i];
+                    }
+                continue;
             }
+            m = grp_reduce<64>(m, OpMaxBits());
+            const unsigned byte = st_byte(__builtin_bit_cast(unsigned, m));
+            const float r = st_inverse(byte);
+            uint8_t *d = (uint8_t *)s.dst + k.b * s.db + k.slot * s.dt + (h0 + h) * s.dh;
+#pragma unroll
+            for (int i = 0; i < PL; i++)
+                if (have[i]) {
+                    const unsigned w = byte == 255u ? 0x7F7Fu : (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(a[i] * r, b[i] * r, 0, false);
+                    d[ia[i]] = (uint8_t)w;
+                    d[ib[i]] = (uint8_t)(w >> 8);
+                }
+            if (lane == 0) s.scale[k.b * s.cb + (h0 + h) * s.ch + k.slot] = (uint8_t)byte;
         }
-    };
-    for (int64_t blk = blockIdx.x; blk < x.blocks; blk += gridDim.x) work(blk);
+    }
 }
 
-template <int TY, bool INTER, int LPR>
-static void st_launch(StArgs &x, hipStream_t s) {
-    const int64_t blocks = ((int64_t)x.B * x.N + 256 / LPR - 1) / (256 / LPR);
-    /* four heads to a group where that still fills the CUs */
+/* shares of `per` tokens; four heads to a group where that still fills the CUs */
+static bool st_shares(StArgs &x, int per) {
+    const int64_t blocks = ((int64_t)x.B * x.N + per - 1) / per;
     int64_t four = 0, one = 0;
     for (int i = 0; i < x.nsec; i++) {
         four += (x.sec[i].heads + 3) / 4;
@@ -250,30 +365,36 @@ static void st_launch(StArgs &x, hipStream_t s) {
     for (int i = 0; i < x.nsec; i++) x.sec[i].chunks = hg4 ? (x.sec[i].heads + 3) / 4 : x.sec[i].heads;
     x.chunks = (int)(hg4 ? four : one);
     x.blocks = blocks * x.chunks;
+    x.dn = HostDiv(x.N);
+    x.dchunks = HostDiv(x.chunks);
+    return hg4;
+}
+template <int TY, bool INTER, int LPR>
+static void st_launch(StArgs &x, hipStream_t s) {
+    const bool hg4 = st_shares(x, 256 / LPR);
     const dim3 grid((unsigned)std::min<int64_t>(x.blocks, ST_GRID));
     if (hg4) hipLaunchKernelGGL((k_states<TY, INTER, LPR, 4>), grid, dim3(256), 0, s, x);
     else hipLaunchKernelGGL((k_states<TY, INTER, LPR, 1>), grid, dim3(256), 0, s, x);
 }
 template <int TY, bool INTER>
-static void st_lanes(StArgs &x, int lanes, hipStream_t s) {
-    if (lanes <= 4) st_launch<TY, INTER, 4>(x, s);
-    else if (lanes <= 8) st_launch<TY, INTER, 8>(x, s);
-    else if (lanes <= 16) st_launch<TY, INTER, 16>(x, s);
-    else st_launch<TY, INTER, 32>(x, s);
-}
-template <int TY>
-static void st_pairs(StArgs &x, int interleaved, hipStream_t s) {
-    const int rh = x.rot / 2;
-    x.lr = interleaved ? (x.rot + 15) / 16 : (rh + 7) / 8;
-    const int lanes = x.lr + (x.D - x.rot + 15) / 16;     /* at most 17: D 256 with few dims rotated */
-    if (interleaved) st_lanes<TY, true>(x, lanes, s);
-    else st_lanes<TY, false>(x, lanes, s);
+static void st_pairs(StArgs &x, hipStream_t s) {
+    if (x.D % 8 == 0 && x.rot % (INTER ? 8 : 16) == 0) {
+        const int lanes = (x.D + 15) / 16;
+        if (lanes <= 4) st_launch<TY, INTER, 4>(x, s);
+        else if (lanes <= 8) st_launch<TY, INTER, 8>(x, s);
+        else st_launch<TY, INTER, 16>(x, s);
+        return;
+    }
+    const bool hg4 = st_shares(x, 4);
+    const dim3 grid((unsigned)std::min<int64_t>(x.blocks, ST_GRID));
+    if (hg4) hipLaunchKernelGGL((k_states_any<TY, INTER, 4>), grid, dim3(256), 0, s, x);
+    else hipLaunchKernelGGL((k_states_any<TY, INTER, 1>), grid, dim3(256), 0, s, x);
 }
 static hipError_t st_run(StArgs &x, int type, int interleaved, hipStream_t s) {
     if (x.B <= 0 || x.N <= 0 || x.nsec == 0) return hipSuccess;
-    if (type == 0) st_pairs<0>(x, interleaved, s);
-    else if (type == 1) st_pairs<1>(x, interleaved, s);
-    else st_pairs<2>(x, interleaved, s);
+    if (type == 0) interleaved ? st_pairs<0, true>(x, s) : st_pairs<0, false>(x, s);
+    else if (type == 1) interleaved ? st_pairs<1, true>(x, s) : st_pairs<1, false>(x, s);
+    else interleaved ? st_pairs<2, true>(x, s) : st_pairs<2, false>(x, s);
     return hipGetLastError();
 }
 
