@@ -23,40 +23,78 @@ template <> struct StT<2> { using type = __bf16; };
 
 /* ---- tables ---- */
 
+#define TAB_EACH 4           /* positions of a thread */
 struct TabArgs {
     float *c, *s;
-    int64_t first;
-    int n, rh;
+    int64_t first, threads;
+    int n, rh, groups;       /* positions, pairs, groups of V pairs */
+    HostDiv dgroups;
     float gain;
     double turns[128];
 };
 
-/* The angle in turns, t = p f / 2 pi, loses its whole turns in 64 bits; what is left, at most half a turn, is an fp32 number
- * of half turns to a relative 2^-24. */
+/* cos and sin of a turns' fraction. The nearest quarter leaves t in 64 bits, exactly; of what is left, at most an eighth, the
+ * Taylor series to x^10 and x^9 (the next terms are below 2.4e-8 and 1.8e-9), 2 pi in two parts */
+__device__ __forceinline__ void tab_cos_sin(double t, float &c, float &s) {
+    const double r = t - __builtin_rint(t), q = __builtin_rint(4.0 * r);
+    const float x = (float)__builtin_fma(q, -0.25, r), z = x * x;
+    const int k = (int)q;
+    const float ps = __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, 42.0586939f, -76.7058598f), 81.6052493f), -41.3417022f), -1.7484556e-07f);
+    const float a = __builtin_fmaf(x, 6.28318531f, x * ps);
+    const float pc = __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, -26.4262568f, 60.2446414f), -85.4568172f), 64.939394f), -19.7392088f);
+    const float b = __builtin_fmaf(z, pc, 1.0f);
+    const float u = k & 1 ? b : a, v = k & 1 ? a : b;
+    s = k & 2 ? -u : u;
+    c = (k + 1) & 2 ? -v : v;
+}
+
+/* A thread makes V neighbouring pairs of TAB_EACH positions, whose frequencies it loads once */
+template <int V>
 __global__ __launch_bounds__(256) void k_rotary_table(TabArgs a) {
+    typedef float fv __attribute__((ext_vector_type(V), aligned(4)));
+    fetch_args(a);
     const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (at >= (int64_t)a.n * a.rh) return;
-    const int p = (int)(at / a.rh), i = (int)(at % a.rh);
-    const double t = (double)(a.first + p) * a.turns[i];
-    float c, s;
-    s = sinpif(2.0f * (float)(t - __builtin_rint(t)));
-    c = cospif(2.0f * (float)(t - __builtin_rint(t)));
-    a.c[at] = c * a.gain;
-    a.s[at] = s * a.gain;
+    if (at >= a.threads) return;
+    const unsigned row = a.dgroups.of((unsigned)at), g = (unsigned)at - row * a.groups, rows = (unsigned)(a.n + TAB_EACH - 1) / TAB_EACH;
+    double f[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) f[i] = a.turns[V * g + i];
+#pragma unroll
+    for (int j = 0; j < TAB_EACH; j++) {
+        const unsigned n = row + j * rows;                   /* neighbouring threads write neighbouring positions */
+        if (n >= (unsigned)a.n) break;
+        const double p = (double)(a.first + n);
+        fv c, s;
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            float u, w;
+            tab_cos_sin(p * f[i], u, w);
+            c[i] = u * a.gain;
+            s[i] = w * a.gain;
+        }
+        const int64_t o = (int64_t)n * a.rh + V * g;
+        *reinterpret_cast<fv *>(a.c + o) = c;
+        *reinterpret_cast<fv *>(a.s + o) = s;
+    }
 }
 
 extern "C" hipError_t aria_k_rotary_table(float *cos_t, float *sin_t, const double *turns, int rot, double gain,
                                           int64_t first, int n, hipStream_t s) {
-    TabArgs a;
+    TabArgs a{};
     a.c = cos_t;
     a.s = sin_t;
     a.first = first;
     a.n = n;
     a.rh = rot / 2;
     a.gain = (float)gain;
-    for (int i = 0; i < 128; i++) a.turns[i] = i < rot / 2 ? turns[i] : 0.0;
-    const int64_t blocks = ((int64_t)n * a.rh + 255) / 256;
-    hipLaunchKernelGGL(k_rotary_table, dim3((unsigned)blocks), dim3(256), 0, s, a);
+    for (int i = 0; i < rot / 2; i++) a.turns[i] = turns[i];
+    const int V = a.rh % 4 == 0 ? 4 : 1;
+    a.groups = a.rh / V;
+    a.dgroups = HostDiv(a.groups);
+    a.threads = (int64_t)((n + TAB_EACH - 1) / TAB_EACH) * a.groups;      /* below 2^30: n is at most 2^24 + 1 */
+    const dim3 grid((unsigned)((a.threads + 255) / 256));
+    if (V == 4) hipLaunchKernelGGL((k_rotary_table<4>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_rotary_table<1>), grid, dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
@@ -95,16 +133,15 @@ struct StArgs {
 /* a and b of a pair, rotated. The products and the sum are fp32 where the result is rounded to 16 bits; where it is an fp32
  * number (fp32 states, keys before they are quantised) they are 64 bits wide, so that it is the rounded exact value and a code
  * does not hang on the order of two roundings */
-template <bool WIDE>
 __device__ __forceinline__ void st_turn(float &a, float &b, float c, float s) {
     const float u = a, w = b;
-    if constexpr (WIDE) {
-        a = (float)__builtin_fma((double)u, (double)c, -((double)w * (double)s));
-        b = (float)__builtin_fma((double)w, (double)c, (double)u * (double)s);
-    } else {
-        a = __builtin_fmaf(u, c, -(w * s));
-        b = __builtin_fmaf(w, c, u * s);
-    }
+    a = __builtin_fmaf(u, c, -(w * s));
+    b = __builtin_fmaf(w, c, u * s);
+}
+__device__ __forceinline__ void st_turn(float &a, float &b, double c, double s) {
+    const double u = a, w = b;
+    a = (float)__builtin_fma(u, c, -(w * s));
+    b = (float)__builtin_fma(w, c, u * s);
 }
 /* the byte of a row from the bits of its largest magnitude; 448 = 1.75 * 2^8 */
 __device__ __forceinline__ unsigned st_byte(unsigned bits) {
@@ -194,6 +231,14 @@ __global__ __launch_bounds__(256) void k_states(StArgs x) {
         }
         auto rows = [&](auto TURN, auto CACHE) __attribute__((always_inline)) {
             constexpr bool turned = decltype(TURN)::value != 0, cache = decltype(CACHE)::value != 0;
+            using W = std::conditional_t<TY == 0 || cache, double, float>;
+            W cw[8], sw[8];
+            if constexpr (turned)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    cw[i] = c[i / 4][i % 4];
+                    sw[i] = sn[i / 4][i % 4];
+                }
 #pragma unroll
             for (int h = 0; h < HG; h++) {
                 float v[16];                         /* chunk a, then chunk b */
@@ -206,7 +251,7 @@ __global__ __launch_bounds__(256) void k_states(StArgs x) {
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
                         const int ja = INTER ? 2 * i : i, jb = INTER ? 2 * i + 1 : 8 + i;
-                        st_turn<TY == 0 || cache>(v[ja], v[jb], c[i / 4][i % 4], sn[i / 4][i % 4]);
+                        st_turn(v[ja], v[jb], cw[i], sw[i]);
                     }
                     if (!(ra && rb)) {               /* plain dims as they came: 0 times an Inf is none of theirs */
 #pragma unroll
@@ -322,8 +367,8 @@ __global__ __launch_bounds__(256) void k_states_any(StArgs x) {
                 a[i] = (float)fa[h][i];
                 b[i] = (float)fb[h][i];
                 if (s.rotate && turns[i]) {
-                    if (TY == 0 || s.scale) st_turn<true>(a[i], b[i], c[i], sn[i]);
-                    else st_turn<false>(a[i], b[i], c[i], sn[i]);
+                    if (TY == 0 || s.scale) st_turn(a[i], b[i], (double)c[i], (double)sn[i]);
+                    else st_turn(a[i], b[i], c[i], sn[i]);
                 }
                 m = OpMaxBits()(m, OpMaxBits()(fabsf(a[i]), fabsf(b[i])));
             }
