@@ -51,26 +51,28 @@ struct PaArgs {
 };
 
 /* keys of a tile */
-__host__ __device__ constexpr int pa_tile(int DP, int form) { return DP == 64 || form == 2 ? 64 : 32; }
+__host__ __device__ constexpr int pa_tile(int DV, int form) { return DV <= 64 || form == 2 ? 64 : 32; }
 /* floats of a row's partial result: sums, reference, weights' sum, remainder of the reference */
-__host__ __device__ constexpr int pa_row(int DP) { return DP + 4; }
+__host__ __device__ constexpr int pa_row(int DV) { return DV + 4; }
 /* LDS bytes of a form: the stages of every slice, later the output rows and each wave's 32 references, sums and remainders */
-__host__ __device__ constexpr int pa_lds(int DP, int form) {
-    const int ks = 4 >> form, st = (form ? 2 : 1) * ks * 2 * pa_tile(DP, form) * DP * 2, epi = form == 2 ? 0 : 4 * 32 * (DP + 4) * 4 + 4 * 96 * 4;
+__host__ __device__ constexpr int pa_lds(int DV, int form) {
+    const int ks = 4 >> form, st = (form ? 2 : 1) * ks * 2 * pa_tile(DV, form) * (DV <= 64 ? 64 : 128) * 2;
+    const int epi = form == 2 ? 0 : 4 * 32 * (DV + 4) * 4 + 4 * 96 * 4;
     return st > epi ? st : epi;
 }
 
-template <typename T, int DP, int FORM>
+/* DV: the width as products see it, 32, 64, 96 or 128; a row in LDS has 64 or 128 dims (DP) */
+template <typename T, int DV, int FORM>
 __device__ __forceinline__ void pa_work(const PaArgs &x, int kind, int job, uint8_t *smem) {
     constexpr int QW = 1 << FORM, KS = 4 >> FORM, NW = 4;
-    constexpr int KT = pa_tile(DP, FORM);
+    constexpr int DP = DV <= 64 ? 64 : 128, KT = pa_tile(DV, FORM);
     constexpr int NST = QW > 1 ? 2 : 1;             /* LDS stages */
     constexpr int CPR = DP / 8;                     /* 16-byte chunks of values per key row */
     constexpr int C16 = DP / 16;                    /* 16-byte chunks of codes per key row */
     constexpr int NC = KT * C16 / (64 * QW);        /* code chunks per lane, tile and operand */
     constexpr int TB = KT * DP * 2;                 /* bytes of a tile of values */
-    constexpr int ES = DP + 4;                      /* floats per staged output row */
-    constexpr int KB = KT / 32, DT = DP / 32, DS = DP / 16;
+    constexpr int ES = DV + 4;                      /* floats per staged output row */
+    constexpr int KB = KT / 32, DT = DV / 32, DS = DV / 16;
     constexpr int STAGE = 2 * TB * KS;              /* K and V of every slice */
     typedef typename Xa<T>::v8 v8;
     typedef typename Xa<T>::v2 v2;
@@ -381,12 +383,12 @@ __device__ __forceinline__ void pa_work(const PaArgs &x, int kind, int job, uint
         __syncthreads();
         for (int n = 0, i = i0; n < w1 - w0; n += KS, i += KS) {    /* every slice meets as often; its tiles end at w1 */
             const int buf = n / KS & 1;
+            if (i < w1) tile(buf, i);
             if (i + KS < w1) {
                 store(buf ^ 1, i + KS);
                 move(i + 2 * KS);
                 if (i + 2 * KS < w1) load();
             }
-            if (i < w1) tile(buf, i);
             __syncthreads();
         }
     } else {
@@ -410,7 +412,7 @@ __device__ __forceinline__ void pa_work(const PaArgs &x, int kind, int job, uint
         /* from the accumulators: through LDS, in whole rows, this took 2 us more */
         if (row0 + l32 < J.R) {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            float *P = x.part + J.part + ((size_t)(sh * J.ns + split) * J.R + row0 + l32) * pa_row(DP);
+            float *P = x.part + J.part + ((size_t)(sh * J.ns + split) * J.R + row0 + l32) * pa_row(DV);
             const long long at = qb * a.o_batch + hd * a.o_head + tok * a.o_token;
 #pragma unroll
             for (int d = 0; d < DT; d++)
@@ -429,7 +431,7 @@ __device__ __forceinline__ void pa_work(const PaArgs &x, int kind, int job, uint
                         }
                     }
                 }
-            if (x.part && g == 0) *reinterpret_cast<float4 *>(P + DP) = make_float4(ref, l, lo, 0.0f);
+            if (x.part && g == 0) *reinterpret_cast<float4 *>(P + DV) = make_float4(ref, l, lo, 0.0f);
         }
         return;
     }
@@ -469,16 +471,16 @@ __device__ __forceinline__ void pa_work(const PaArgs &x, int kind, int job, uint
         for (int w = 0; w < KS; w++) {
             const float f = __builtin_amdgcn_exp2f((m[w] - rm) + (c[w] - rl));
             rs = __builtin_fmaf(f, ML[(w * QW + qw) * 96 + 32 + q], rs);
-            const float *e = (const float *)smem + ((w * QW + qw) * 32 + q) * ES + c8;
+            const float *e = (const float *)smem + ((w * QW + qw) * 32 + q) * ES + min(c8, DV - 8);
 #pragma unroll
             for (int j = 0; j < 8; j++) v[j] = __builtin_fmaf(f, e[j], v[j]);
         }
         if (q >= rows || c8 >= D) continue;
         if (x.part) {
-            float *P = x.part + J.part + ((size_t)(sh * J.ns + split) * J.R + row0 + q) * pa_row(DP);
+            float *P = x.part + J.part + ((size_t)(sh * J.ns + split) * J.R + row0 + q) * pa_row(DV);
             *reinterpret_cast<float4 *>(P + c8) = make_float4(v[0], v[1], v[2], v[3]);
             *reinterpret_cast<float4 *>(P + c8 + 4) = make_float4(v[4], v[5], v[6], v[7]);
-            if (c8 == 0) *reinterpret_cast<float4 *>(P + DP) = make_float4(rm, rs, rl, 0.0f);
+            if (c8 == 0) *reinterpret_cast<float4 *>(P + DV) = make_float4(rm, rs, rl, 0.0f);
             continue;
         }
         const float inv = rs == 0.0f ? 0.0f : 1.0f / rs;
@@ -499,9 +501,9 @@ __device__ __forceinline__ void pa_work(const PaArgs &x, int kind, int job, uint
 }
 
 /* FORMS: the forms that the launch's kinds have, a bit to each */
-template <typename T, int DP, int FORMS>
+template <typename T, int DV, int FORMS>
 __global__ __launch_bounds__(256) void k_pattn(PaArgs x) {
-    constexpr int l0 = FORMS & 1 ? pa_lds(DP, 0) : 0, l1 = FORMS & 2 ? pa_lds(DP, 1) : 0, l2 = FORMS & 4 ? pa_lds(DP, 2) : 0;
+    constexpr int l0 = FORMS & 1 ? pa_lds(DV, 0) : 0, l1 = FORMS & 2 ? pa_lds(DV, 1) : 0, l2 = FORMS & 4 ? pa_lds(DV, 2) : 0;
     __shared__ __attribute__((aligned(16))) uint8_t smem[l0 > l1 ? (l0 > l2 ? l0 : l2) : l1 > l2 ? l1 : l2];
     fetch_args(x);
     /* each kind spreads over all XCDs by itself, neighbouring jobs (which read the same keys) to one */
@@ -509,19 +511,19 @@ __global__ __launch_bounds__(256) void k_pattn(PaArgs x) {
     const int job = xcd_tile(blockIdx.x - (kind ? first : 0), x.j[kind].jobs);
     if (job >= x.j[kind].jobs) return;
     const int form = x.j[kind].form;
-    if constexpr ((FORMS & 1) != 0) if (form == 0) pa_work<T, DP, 0>(x, kind, job, smem);
-    if constexpr ((FORMS & 2) != 0) if (form == 1) pa_work<T, DP, 1>(x, kind, job, smem);
-    if constexpr ((FORMS & 4) != 0) if (form == 2) pa_work<T, DP, 2>(x, kind, job, smem);
+    if constexpr ((FORMS & 1) != 0) if (form == 0) pa_work<T, DV, 0>(x, kind, job, smem);
+    if constexpr ((FORMS & 2) != 0) if (form == 1) pa_work<T, DV, 1>(x, kind, job, smem);
+    if constexpr ((FORMS & 4) != 0) if (form == 2) pa_work<T, DV, 2>(x, kind, job, smem);
 }
 
 /* Joins the partial results of a row: those of the prefix's splits, then those of the own part's. WR waves to a row: first
- * each thread takes a split's reference and sum, then groups of DP / 8 lanes, 8 dims to a lane, take the splits' sums in turn */
-template <typename T, int DP, int WR>
+ * each thread takes a split's reference and sum, then groups of 8 or 16 lanes, 8 dims to a lane, take the splits' sums in turn */
+template <typename T, int DV, int WR>
 __global__ __launch_bounds__(256) void k_pattn_join(PaArgs x) {
-    constexpr int CPR = DP / 8, TR = 64 * WR, NG = TR / CPR, RB = 4 / WR, MOST = 512;
+    constexpr int CPR = DV <= 64 ? 8 : 16, TR = 64 * WR, NG = TR / CPR, RB = 4 / WR, MOST = 512;
     constexpr int FIRST = 2;                                   /* a group's splits that are on their way before the factors are known */
     __shared__ float fac[RB][MOST], red[RB][WR][4];
-    __shared__ __attribute__((aligned(16))) float acc[RB][WR][DP];
+    __shared__ __attribute__((aligned(16))) float acc[RB][WR][8 * CPR];
     fetch_args(x);
     const aria_hip_prefix_attn &a = x.a;
     const int per_seq = a.Nq * x.G, rows = a.B * a.H * a.Nq;
@@ -534,27 +536,27 @@ __global__ __launch_bounds__(256) void k_pattn_join(PaArgs x) {
         const int n1 = a.own_len ? min(max(a.own_len[b], 0), a.own.cap) : a.own.cap;
         auto splits = [&](int kind, bool p, bool o) __attribute__((always_inline)) {   /* those that hold keys */
             const PaJobs &J = x.j[kind];
-            const int KT = pa_tile(DP, J.form), nt = (p ? (n0 + KT - 1) / KT : 0) + (o ? (n1 + KT - 1) / KT : 0);
+            const int KT = pa_tile(DV, J.form), nt = (p ? (n0 + KT - 1) / KT : 0) + (o ? (n1 + KT - 1) / KT : 0);
             return max(1u, J.dper.of(nt + J.per - 1));
         };
         const int s0 = splits(0, true, !x.group), s1 = x.kinds == 2 ? (int)splits(1, false, true) : 0, ns = s0 + s1;
         const int set0 = x.group ? pf : b, row_0 = x.group ? (b - pf * x.Bp) * per_seq + row : row;
-        const float *p0 = x.part + x.j[0].part + ((size_t)(set0 * a.own.Hkv + hk) * x.j[0].ns * x.j[0].R + row_0) * pa_row(DP);
-        const float *p1 = x.part + x.j[1].part + ((size_t)(b * a.own.Hkv + hk) * x.j[1].ns * x.j[1].R + row) * pa_row(DP);
-        const size_t st0 = (size_t)x.j[0].R * pa_row(DP), st1 = (size_t)x.j[1].R * pa_row(DP);
+        const float *p0 = x.part + x.j[0].part + ((size_t)(set0 * a.own.Hkv + hk) * x.j[0].ns * x.j[0].R + row_0) * pa_row(DV);
+        const float *p1 = x.part + x.j[1].part + ((size_t)(b * a.own.Hkv + hk) * x.j[1].ns * x.j[1].R + row) * pa_row(DV);
+        const size_t st0 = (size_t)x.j[0].R * pa_row(DV), st1 = (size_t)x.j[1].R * pa_row(DV);
         auto at = [&](int s) __attribute__((always_inline)) { return s < s0 ? p0 + s * st0 : p1 + (s - s0) * st1; };
         float4 u[FIRST], w[FIRST];
 #pragma unroll
         for (int j = 0; j < FIRST; j++) {
-            const float *p = at(min(grp + j * NG, ns - 1)) + c8;
+            const float *p = at(min(grp + j * NG, ns - 1)) + min(c8, DV - 8);
             u[j] = *reinterpret_cast<const float4 *>(p);
             w[j] = *reinterpret_cast<const float4 *>(p + 4);
         }
         float4 h = make_float4(XA_MIN, 0.0f, -INFINITY, 0.0f);  /* reference, sum, remainder of this thread's split */
-        if (tr < ns) h = *reinterpret_cast<const float4 *>(at(tr) + DP);
+        if (tr < ns) h = *reinterpret_cast<const float4 *>(at(tr) + DV);
         float m = h.x, ml = h.z;                               /* the largest reference and its largest remainder */
         for (int s = tr + TR; s < ns; s += TR) {
-            const float4 g = *reinterpret_cast<const float4 *>(at(s) + DP);
+            const float4 g = *reinterpret_cast<const float4 *>(at(s) + DV);
             ml = g.x > m ? g.z : g.x == m ? fmaxf(ml, g.z) : ml;
             m = fmaxf(m, g.x);
         }
@@ -573,7 +575,7 @@ __global__ __launch_bounds__(256) void k_pattn_join(PaArgs x) {
         }
         float rs = 0.0f;
         for (int s = tr; s < ns; s += TR) {
-            const float4 g = s == tr ? h : *reinterpret_cast<const float4 *>(at(s) + DP);
+            const float4 g = s == tr ? h : *reinterpret_cast<const float4 *>(at(s) + DV);
             const float f = __builtin_amdgcn_exp2f((g.x - m) + (g.z - ml));
             fac[sub][s] = f;
             rs = __builtin_fmaf(f, g.y, rs);
@@ -599,7 +601,7 @@ __global__ __launch_bounds__(256) void k_pattn_join(PaArgs x) {
             if (grp + j * NG < ns) more(fac[sub][grp + j * NG], u[j], w[j]);
 #pragma unroll 4
         for (int s = grp + FIRST * NG; s < ns; s += NG) {
-            const float *p = at(s) + c8;
+            const float *p = at(s) + min(c8, DV - 8);
             more(fac[sub][s], *reinterpret_cast<const float4 *>(p), *reinterpret_cast<const float4 *>(p + 4));
         }
 #pragma unroll
@@ -641,12 +643,12 @@ __global__ __launch_bounds__(256) void k_pattn_join(PaArgs x) {
  * estimate of the launches' time. */
 #define PA_SPLITS 256        /* of one kind at most: the join holds a factor of each in LDS */
 struct PaPlan {
-    int DP, join;
+    int DV, join;
 };
 static PaPlan pa_plan(const aria_hip_prefix_attn *a, PaArgs &x) {
     const int Hkv = a->own.Hkv, P = a->prefix.B, np = a->prefix.cap, no = a->own.cap;
     PaPlan p;
-    p.DP = a->own.D <= 64 ? 64 : 128;
+    p.DV = (a->own.D + 31) / 32 * 32;
     x.G = a->H / Hkv;
     x.Bp = a->B / P;
     const long long R = (long long)a->Nq * x.G;
@@ -655,14 +657,14 @@ static PaPlan pa_plan(const aria_hip_prefix_attn *a, PaArgs &x) {
     static const double alone[2][3] = {{5.2, 9.5, 17.0}, {10.0, 17.0, 25.0}}, paired[2][3] = {{8.6, 14.7, 25.3}, {15.0, 25.4, 38.4}};
     static const double full[2][3] = {{8.6, 14.7, 33.0}, {15.0, 25.4, 38.4}};
     static const int hold[2][3] = {{2, 2, 3}, {2, 2, 2}};
-    const int wide = p.DP == 128;
+    const int wide = p.DV > 64;
     const double begin = 2.5;                                 /* us of a workgroup beside its tiles */
     struct Kind {
         long long sets, R, wg;
         int n0, n1, form, nt, ns, per;
     };
     auto kind = [&](long long sets, long long R, int n0, int n1, int form) {
-        const int br = 32 << form, KT = pa_tile(p.DP, form);
+        const int br = 32 << form, KT = pa_tile(p.DV, form);
         Kind k{sets, R, sets * Hkv * ((R + br - 1) / br), n0, n1, form, (n0 + KT - 1) / KT + (n1 + KT - 1) / KT, 1, 1};
         return k;
     };
@@ -676,10 +678,10 @@ static PaPlan pa_plan(const aria_hip_prefix_attn *a, PaArgs &x) {
         double all = 0, longest = 0, bytes = 0;
         for (int i = 0; i < kinds; i++) jobs += k[i].wg * k[i].ns;
         for (int i = 0; i < kinds; i++) {
-            const double keys = (double)k[i].per * pa_tile(p.DP, k[i].form) / 1024;
+            const double keys = (double)k[i].per * pa_tile(p.DV, k[i].form) / 1024;
             all += (double)k[i].wg * k[i].ns * (begin + keys * full[wide][k[i].form]) / (256 * hold[wide][k[i].form]);
             longest = std::max(longest, begin + keys * (jobs <= 256 ? alone : jobs <= 512 ? paired : full)[wide][k[i].form]);
-            bytes += (double)k[i].sets * Hkv * k[i].ns * k[i].R * pa_row(p.DP) * sizeof(float);
+            bytes += (double)k[i].sets * Hkv * k[i].ns * k[i].R * pa_row(p.DV) * sizeof(float);
         }
         if (jobs > 768 && jobs < 3000) all += 0.25 * longest;  /* the last round is not full */
         const double t = std::max(all, longest);
@@ -743,12 +745,12 @@ static PaPlan pa_plan(const aria_hip_prefix_attn *a, PaArgs &x) {
         J.jobs = (int)(k.wg * k.ns);
         J.use_prefix = k.n0 > 0;
         J.use_own = k.n1 > 0;
-        J.tp = (k.n0 + pa_tile(p.DP, k.form) - 1) / pa_tile(p.DP, k.form);
+        J.tp = (k.n0 + pa_tile(p.DV, k.form) - 1) / pa_tile(p.DV, k.form);
         J.dnrb = HostDiv(J.nrb);
         J.dns = HostDiv(J.ns);
         J.dper = HostDiv(J.per);
         J.part = part;
-        part += (size_t)k.sets * Hkv * k.ns * k.R * pa_row(p.DP);
+        part += (size_t)k.sets * Hkv * k.ns * k.R * pa_row(p.DV);
     }
     p.join = got_kinds == 2 || got[0].ns > 1;
     return p;
@@ -758,27 +760,35 @@ extern "C" size_t aria_k_pattn_ws_bytes(const aria_hip_prefix_attn *a) {
     PaArgs x{};
     const PaPlan p = pa_plan(a, x);
     size_t n = 0;
-    for (int i = 0; i < x.kinds; i++) n += (size_t)x.j[i].sets * a->own.Hkv * x.j[i].ns * x.j[i].R * pa_row(p.DP);
+    for (int i = 0; i < x.kinds; i++) n += (size_t)x.j[i].sets * a->own.Hkv * x.j[i].ns * x.j[i].R * pa_row(p.DV);
     return p.join ? n * sizeof(float) : 0;
 }
 
-template <typename T, int DP>
+template <typename T, int DV>
 static void pa_launch(const PaPlan &p, const PaArgs &x, hipStream_t s) {
     const dim3 grid((unsigned)(((x.j[0].jobs + 7) & ~7) + ((x.j[1].jobs + 7) & ~7)));
     switch (1 << x.j[0].form | (x.kinds == 2 ? 1 << x.j[1].form : 0)) {
-    case 1: hipLaunchKernelGGL((k_pattn<T, DP, 1>), grid, dim3(256), 0, s, x); break;
-    case 2: hipLaunchKernelGGL((k_pattn<T, DP, 2>), grid, dim3(256), 0, s, x); break;
-    case 3: hipLaunchKernelGGL((k_pattn<T, DP, 3>), grid, dim3(256), 0, s, x); break;
-    case 4: hipLaunchKernelGGL((k_pattn<T, DP, 4>), grid, dim3(256), 0, s, x); break;
-    case 5: hipLaunchKernelGGL((k_pattn<T, DP, 5>), grid, dim3(256), 0, s, x); break;
-    case 6: hipLaunchKernelGGL((k_pattn<T, DP, 6>), grid, dim3(256), 0, s, x); break;
+    case 1: hipLaunchKernelGGL((k_pattn<T, DV, 1>), grid, dim3(256), 0, s, x); break;
+    case 2: hipLaunchKernelGGL((k_pattn<T, DV, 2>), grid, dim3(256), 0, s, x); break;
+    case 3: hipLaunchKernelGGL((k_pattn<T, DV, 3>), grid, dim3(256), 0, s, x); break;
+    case 4: hipLaunchKernelGGL((k_pattn<T, DV, 4>), grid, dim3(256), 0, s, x); break;
+    case 5: hipLaunchKernelGGL((k_pattn<T, DV, 5>), grid, dim3(256), 0, s, x); break;
+    case 6: hipLaunchKernelGGL((k_pattn<T, DV, 6>), grid, dim3(256), 0, s, x); break;
     }
     if (!p.join) return;
     const int rows = x.a.B * x.a.H * x.a.Nq;
     if (x.j[0].ns + x.j[1].ns > 16)
-        hipLaunchKernelGGL((k_pattn_join<T, DP, 4>), dim3(std::min(rows, 1 << 20)), dim3(256), 0, s, x);
+        hipLaunchKernelGGL((k_pattn_join<T, DV, 4>), dim3(std::min(rows, 1 << 20)), dim3(256), 0, s, x);
     else
-        hipLaunchKernelGGL((k_pattn_join<T, DP, 1>), dim3(std::min((rows + 3) / 4, 1 << 20)), dim3(256), 0, s, x);
+        hipLaunchKernelGGL((k_pattn_join<T, DV, 1>), dim3(std::min((rows + 3) / 4, 1 << 20)), dim3(256), 0, s, x);
+}
+
+template <typename T>
+static void pa_width(const PaPlan &p, const PaArgs &x, hipStream_t s) {
+    if (p.DV == 32) pa_launch<T, 32>(p, x, s);
+    else if (p.DV == 64) pa_launch<T, 64>(p, x, s);
+    else if (p.DV == 96) pa_launch<T, 96>(p, x, s);
+    else pa_launch<T, 128>(p, x, s);
 }
 
 extern "C" hipError_t aria_k_pattn_run(const aria_hip_prefix_attn *a, void *ws, hipStream_t s) {
@@ -788,9 +798,7 @@ extern "C" hipError_t aria_k_pattn_run(const aria_hip_prefix_attn *a, void *ws, 
     const PaPlan p = pa_plan(a, x);
     x.scale_log2 = a->scale * ARIA_LOG2E;
     x.part = p.join ? (float *)ws : nullptr;
-    if (a->type == 1 && p.DP == 64) pa_launch<_Float16, 64>(p, x, s);
-    else if (a->type == 1) pa_launch<_Float16, 128>(p, x, s);
-    else if (p.DP == 64) pa_launch<__bf16, 64>(p, x, s);
-    else pa_launch<__bf16, 128>(p, x, s);
+    if (a->type == 1) pa_width<_Float16>(p, x, s);
+    else pa_width<__bf16>(p, x, s);
     return hipGetLastError();
 }
