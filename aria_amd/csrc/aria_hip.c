@@ -726,7 +726,7 @@ int aria_hip_rotary_dev(const aria_hip_rotary *a, void *stream) {
     REQ((a->q_batch | a->q_token | a->q_head | a->k_batch | a->k_token | a->k_head | a->qo_batch | a->qo_token | a->qo_head |
          a->ko_batch | a->ko_token | a->ko_head | a->pos_stride) >= 0);
     if (a->B == 0 || a->N == 0) return 0;
-    REQ((a->q || a->Hq == 0) && a->rot >= 0 && (a->rot == 0 || a->npos == 0 || (a->cos && a->sin)));
+    REQ((a->q || a->Hq == 0) && (a->rot == 0 || (a->cos && a->sin)));
     ENSURE();
     KCK(aria_k_rotary(a, pick(stream)), "k_rotary");
     return 0;
@@ -748,7 +748,7 @@ int aria_hip_kv_write_dev(const aria_hip_kv_write *a, void *stream) {
     if (r) return r;
     REQ(MX4_TYPE(a->type) && a->N >= 0 && (int64_t)c->B * a->N <= ST_TOKENS);
     REQ(a->rot >= 0 && a->rot <= c->D && a->rot % 2 == 0 && a->npos >= 0 && a->Hq >= 0 && a->Hq <= ST_HEADS);
-    REQ(!a->q == !a->q_out && (a->q || a->Hq == 0) && !a->cos == !a->sin && (a->cos || a->rot == 0 || a->npos == 0));
+    REQ(!a->q == !a->q_out && (a->q || a->Hq == 0) && (a->rot == 0 || (a->cos && a->sin)));
     REQ(st_aligned(a->k, a->type) && st_aligned(a->v, a->type) && st_aligned(a->q, a->type) && st_aligned(a->q_out, a->type));
     REQ((((uintptr_t)a->cos | (uintptr_t)a->sin | (uintptr_t)a->pos | (uintptr_t)a->first | (uintptr_t)a->count) & 3u) == 0);
     REQ((a->k_batch | a->k_token | a->k_head | a->v_batch | a->v_token | a->v_head | a->q_batch | a->q_token | a->q_head |

@@ -480,7 +480,7 @@ extern "C" hipError_t aria_k_kv_write(const aria_hip_kv_write *a, hipStream_t s)
     x.B = c.B;
     x.N = a->N;
     x.D = c.D;
-    x.rot = a->cos ? a->rot : 0;
+    x.rot = a->rot;
     x.npos = a->npos;
     x.cap = c.cap;
     if (c.cap > 0) {

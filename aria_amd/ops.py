@@ -378,3 +378,170 @@ def cross_attention(q, k, v, kv_len=None, mask=None):
     check(lib().aria_hip_cross_attention_f16(_p(out), _p(q), _p(k), _p(v), _p(kv_len), _p(mask), B, H, Hkv, Nq, Nk, D),
           "aria_hip_cross_attention_f16")
     return out
+
+
+# ---- rotary positions by table, e4m3 rows, attention over shared prefixes (include/aria_hip.h; no counterpart in the
+# reference) ----
+
+SCALINGS = {"none": 0, "linear": 1, "base": 2, "turns": 3}
+
+
+def _strides(desc, name, N, heads, D):
+    """packed [B, N, heads, D]"""
+    for axis, n in (("batch", N * heads * D), ("token", heads * D), ("head", D)):
+        setattr(desc, f"{name}_{axis}", n)
+
+
+class _Device:
+    """The device arrays of one call."""
+
+    def __enter__(self):
+        self.held = []
+        return self
+
+    def __exit__(self, *exc):
+        for a in self.held:
+            a.free()
+
+    def put(self, a, dtype=np.float32):
+        from .device import DeviceArray
+        if a is None:
+            return None
+        self.held.append(DeviceArray.from_host(np.ascontiguousarray(a, dtype)))
+        return self.held[-1]
+
+    def new(self, shape, dtype=np.float32):
+        from .device import DeviceArray
+        self.held.append(DeviceArray(shape, dtype))
+        return self.held[-1]
+
+    def cache(self, B, heads, slots, D):
+        from .cache import Cache
+        c = Cache(B, heads, slots, D)
+        self.held.append(c)
+        return c
+
+
+def _d(a):
+    return None if a is None else a.p
+
+
+def _call(fn, *args):
+    check(getattr(lib(), fn)(*args), fn)
+    check(lib().aria_hip_stream_sync(None), fn)
+
+
+def rotary_tables(n, rot, first=0, base=10000.0, scaling="none", factor=1.0, trained=1.0, low=0.0, high=1.0, gain=1.0):
+    """cos, sin [n, rot/2] of positions first .. first + n - 1."""
+    from . import RotaryScaling
+    a = RotaryScaling(rot=rot, kind=SCALINGS[scaling], base=base, factor=factor, trained=trained, low=low, high=high, gain=gain)
+    with _Device() as dev:
+        c, s = (dev.new((max(n, 0), max(rot, 0) // 2)) for _ in range(2))
+        _call("aria_hip_rotary_table_dev", c.p, s.p, a, first, n, None)
+        return c.to_host(), s.to_host()
+
+
+def _positions(pos, first, B, N):
+    if pos is not None and np.shape(pos) != (B, N):
+        raise ValueError(f"pos holds a position for each token, [{B}, {N}]: got {np.shape(pos)}")
+    if first is not None and np.shape(first) != (B,):
+        raise ValueError(f"first holds a position for each sequence, [{B}]: got {np.shape(first)}")
+
+
+def rotary(q, cos, sin, k=None, pos=None, first=None, interleaved=False, inverse=False):
+    """q [B, N, H, D] (and k [B, N, Hk, D]) rotated by rows of cos, sin [npos, rot/2]; tokens whose position lies outside
+    the tables come back as they are."""
+    from . import Rotary
+    q = _f32(q); k = _f32(k); cos = _f32(cos); sin = _f32(sin)
+    B, N, H, D = q.shape
+    if cos.shape != sin.shape or cos.ndim != 2:
+        raise ValueError(f"cos and sin are [positions, rot / 2]: got {cos.shape} and {sin.shape}")
+    if k is not None and (k.shape[:2] != (B, N) or k.shape[3] != D):
+        raise ValueError(f"k is [{B}, {N}, heads, {D}]: got {k.shape}")
+    _positions(pos, first, B, N)
+    with _Device() as dev:
+        dq, dk = dev.put(q), dev.put(k)
+        a = Rotary(q=dq.p, q_out=dq.p, k=_d(dk), k_out=_d(dk), cos=dev.put(cos).p, sin=dev.put(sin).p, pos=_d(dev.put(pos, np.int32)),
+                   first=_d(dev.put(first, np.int32)), pos_stride=N, type=0, B=B, N=N, Hq=H, Hk=0 if k is None else k.shape[2], D=D,
+                   rot=2 * cos.shape[1], npos=cos.shape[0], interleaved=interleaved, inverse=inverse)
+        for n in ("q", "qo"):
+            _strides(a, n, N, H, D)
+        for n in ("k", "ko"):
+            _strides(a, n, N, a.Hk, D)
+        _call("aria_hip_rotary_dev", a, None)
+        return dq.to_host() if k is None else (dq.to_host(), dk.to_host())
+
+
+def _write(dev, c, k, v, N):
+    from . import KVWrite
+    a = KVWrite(cache=c.desc, k=k.p, v=v.p, type=0, N=N)
+    for n in ("k", "v"):
+        _strides(a, n, N, c.heads, c.D)
+    _call("aria_hip_kv_write_dev", a, None)
+
+
+def e4m3_rows(x):
+    """x [..., D] as rows of the cache: codes u8 [..., D] and scale bytes u8 [...]."""
+    x = _f32(x)
+    D = x.shape[-1]
+    n = x.size // D if D else 0
+    with _Device() as dev:
+        c, d = dev.cache(1, 1, n, D), dev.put(x)
+        _write(dev, c, d, d, n)
+        return c.codes[0].to_host().reshape(x.shape), c.scales[0].to_host().reshape(x.shape[:-1])
+
+
+def e4m3_values(codes, scales):
+    """The values of such rows, fp32."""
+    from . import KVRead
+    codes = np.ascontiguousarray(codes, np.uint8); scales = np.ascontiguousarray(scales, np.uint8)
+    if scales.shape != codes.shape[:-1]:
+        raise ValueError(f"one scale byte for each row of codes: got {codes.shape} and {scales.shape}")
+    D, n = codes.shape[-1], scales.size
+    with _Device() as dev:
+        c, y = dev.cache(1, 1, n, D), dev.new((n, D))
+        c.codes[0].upload(codes.reshape(1, 1, n, D))
+        c.scales[0].upload(scales.reshape(1, 1, n))
+        a = KVRead(cache=c.desc, k=y.p, type=0, N=n)
+        _strides(a, "k", n, 1, D)
+        _call("aria_hip_kv_read_dev", a, None)
+        return y.to_host().reshape(codes.shape)
+
+
+def prefix_attention(q, prefix_k, prefix_v, k=None, v=None, prefix_len=None, own_len=None, first=None, scale=None):
+    """q [B, Nq, H, D] (rounded to fp16) over prefixes [P, n, Hkv, D] (sequence b reads prefix b // (B / P)) and own keys and values
+    [B, m, Hkv, D], both cached as e4m3 rows in the call; first [B]: query t of sequence b sees own keys up to first[b] + t
+    -> [B, Nq, H, D] fp32."""
+    from . import PrefixAttention
+    q = _f32(q)
+    B, Nq, H, D = q.shape
+    pk = _f32(prefix_k); pv = _f32(prefix_v)
+    P, n, Hkv = pk.shape[:3]
+    k = np.zeros((B, 0, Hkv, D), np.float32) if k is None else _f32(k)
+    v = np.zeros((B, 0, Hkv, D), np.float32) if v is None else _f32(v)
+    m = k.shape[1]
+    if pk.shape != (P, n, Hkv, D) or pv.shape != pk.shape or k.shape != (B, m, Hkv, D) or v.shape != k.shape:
+        raise ValueError(f"keys and values are [prefixes, n, heads, {D}] and [{B}, m, heads, {D}]: got {pk.shape}, {pv.shape}, "
+                         f"{k.shape} and {v.shape}")
+    lens = []
+    for x, rows, cap in ((prefix_len, P, n), (own_len, B, m), (first, B, None)):
+        if x is not None:
+            x = np.asarray(x)
+            if x.shape != (rows,):
+                raise ValueError(f"a length (or a first slot) for each of {rows}: got {x.shape}")
+            x = np.clip(x, -2 ** 31, 2 ** 31 - 1) if cap is None else np.clip(x, 0, cap)   # before 32 bits: 2^32 is not 0
+        lens.append(x)
+    with _Device() as dev:
+        cp, co = dev.cache(P, Hkv, n, D), dev.cache(B, Hkv, m, D)
+        for c, a, b, N in ((cp, pk, pv, n), (co, k, v, m)):
+            if N:
+                _write(dev, c, dev.put(a), dev.put(b), N)
+        dq, out = dev.put(q, np.float16), dev.new((B, Nq, H, D))
+        a = PrefixAttention(q=dq.p, out=out.p, prefix=cp.desc, own=co.desc, type=1, out_f32=1, B=B, H=H, Nq=Nq,
+                            scale=1.0 / np.sqrt(D) if scale is None else scale)
+        a.prefix_len, a.own_len, a.first = (_d(dev.put(x, np.int32)) for x in lens)
+        for s in ("q", "o"):
+            _strides(a, s, Nq, H, D)
+        ws = dev.new(max(1, lib().aria_hip_prefix_attention_ws_bytes(a)), np.uint8)
+        _call("aria_hip_prefix_attention_dev", a, ws.p, None)
+        return out.to_host()

@@ -355,7 +355,7 @@ typedef struct {
     int B, Hkv, D, cap;
 } aria_hip_kv;
 /* Writes tokens t < count[b] (count NULL: N; held to 0 .. N) of k, v [B, N, Hkv, D] to slots first[b] + t (first
- * NULL: t); slots outside 0 .. cap - 1 are skipped. Where cos is given (rot > 0), keys are rotated before,
+ * NULL: t); slots outside 0 .. cap - 1 are skipped. Where rot > 0 keys are rotated before,
  * as in aria_hip_rotary, by position pos[b * pos_stride + t], or the slot without pos; the rotated key is rounded to fp32,
  * then to its code. A token whose position lies outside the table is not written. Queries q [B, N, Hq, D] of the same
  * tokens (q NULL: none), rotated likewise, go to q_out in their own type, whatever their slot; q_out may be q.

@@ -302,3 +302,76 @@ def test_steps_of_a_batch(hip):
         told = np.arange(N)[None] < count[:, None]
         assert (np.abs(got - want) <= tol)[told].all()
         held = held + count
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Nq", [1, 40])
+def test_offsets_past_32_bits(hip, Nq):
+    """Sequences, heads and slots that lie further apart than 2^32 bytes: written, read and attended."""
+    from aria_amd.device import DeviceArray as DA, sync
+    L = hip.lib()
+    r = rng(Nq)
+    B, H, Hkv, D, n = 2, 2, 2, 64, 70
+    token, head, batch = 1 << 23, 1 << 30, (1 << 32) + (1 << 31) + 4096
+    size = batch + head + (n - 1) * token + D
+    code, byte = [DA((size,), np.uint8) for _ in range(2)], [DA((B * Hkv * n,), np.uint8) for _ in range(2)]
+    c = hip.KVCache(k=code[0].p, v=code[1].p, k_scale=byte[0].p, v_scale=byte[1].p, B=B, Hkv=Hkv, D=D, cap=n, batch=batch, head=head,
+                    token=token, s_batch=Hkv * n, s_head=n)
+    x = [cast(randn(r, (B, n, Hkv, D)), "bf16") for _ in range(2)]
+    dx = [dev(a[0], a[0].dtype) for a in x]
+    w = hip.KVWrite(cache=c, k=dx[0].p, v=dx[1].p, type=2, N=n)
+    back_ = [DA((B, n, Hkv, D)) for _ in range(2)]
+    a = hip.KVRead(cache=c, k=back_[0].p, v=back_[1].p, type=0, N=n)
+    for s in "kv":
+        for d in (w, a):
+            for axis, st in (("batch", n * Hkv * D), ("token", Hkv * D), ("head", D)):
+                setattr(d, f"{s}_{axis}", st)
+    hip.check(L.aria_hip_kv_write_dev(w, None))
+    hip.check(L.aria_hip_kv_read_dev(a, None))
+    sync()
+    held = [states.values(*states.rows(v)) for _, v in x]
+    assert all(np.array_equal(b.to_host(), h) for b, h in zip(back_, held))
+    q, qv = cast(randn(r, (B, H, Nq, D)), "bf16")
+    none = hip.KVCache(B=B, Hkv=Hkv, D=D)
+
+    class As:
+        def __init__(self, c):
+            self.c = c
+    pv = [h.transpose(0, 2, 1, 3) for h in held]
+    no = [np.zeros((B, Hkv, 0, D))] * 2
+    for prefix, own, p, o in ((c, none, pv, no), (none, c, no, pv)):
+        got = run(hip, "bf16", q, As(prefix), As(own))
+        want, mag = states.attention(qv, p, o)
+        assert (np.abs(got - want) <= tolerance(want, mag, qv, pv[0], pv[1], "bf16", "bf16", 1 / np.sqrt(D), n)).all()
+    for d in code:
+        d.free()
+
+
+@pytest.mark.gpu
+def test_two_streams_and_repeats(hip):
+    """Calls in flight on two streams with a workspace each, and the same call again: the same bits."""
+    from aria_amd.device import DeviceArray as DA
+    L = hip.lib()
+    r = rng(21)
+    jobs = []
+    for B, Pn, H, Hkv, Nq, n, m, D in ((16, 1, 8, 2, 2, 900, 60, 64), (6, 2, 4, 4, 50, 300, 90, 128)):
+        cp, co = fill(hip, r, Pn, Hkv, n, D)[0], fill(hip, r, B, Hkv, m, D)[0]
+        q = cast(randn(r, (B, H, Nq, D)), "f16")[0]
+        a = describe(hip, "f16", B, H, Nq, D, cp.c, co.c)
+        dq, do = DA.from_host(q), DA((B, Nq, H, D), np.float16)
+        a.q, a.out = dq.p, do.p
+        jobs.append((a, do, DA(max(1, int(L.aria_hip_prefix_attention_ws_bytes(a))), np.uint8), (cp, co, dq)))
+    want = []
+    for a, do, ws, _ in jobs:
+        hip.check(L.aria_hip_prefix_attention_dev(a, ws.p, None))
+        hip.check(L.aria_hip_stream_sync(None))
+        want.append(do.to_host())
+        do.upload(np.zeros(do.shape, do.dtype))
+    st = [L.aria_hip_stream_create() for _ in jobs]
+    for _ in range(5):
+        for s, (a, _, ws, _) in zip(st, jobs):
+            hip.check(L.aria_hip_prefix_attention_dev(a, ws.p, s))
+    for s, (_, do, _, _), w in zip(st, jobs, want):
+        hip.check(L.aria_hip_stream_sync(s))
+        assert do.to_host().tobytes() == w.tobytes()
+        L.aria_hip_stream_destroy(s)
