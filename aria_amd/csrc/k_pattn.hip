@@ -675,16 +675,21 @@ static PaPlan pa_plan(const aria_hip_prefix_attn *a, PaArgs &x) {
     };
     auto estimate = [&](const Kind *k, int kinds) {
         long long jobs = 0;
-        double all = 0, longest = 0, bytes = 0;
-        for (int i = 0; i < kinds; i++) jobs += k[i].wg * k[i].ns;
+        int slots = 768;
+        double all = 0, longest = 0, shortest = 1e30, bytes = 0;
+        for (int i = 0; i < kinds; i++) {
+            jobs += k[i].wg * k[i].ns;
+            slots = std::min(slots, 256 * hold[wide][k[i].form]);
+        }
         for (int i = 0; i < kinds; i++) {
             const double keys = (double)k[i].per * pa_tile(p.DV, k[i].form) / 1024;
             all += (double)k[i].wg * k[i].ns * (begin + keys * full[wide][k[i].form]) / (256 * hold[wide][k[i].form]);
             longest = std::max(longest, begin + keys * (jobs <= 256 ? alone : jobs <= 512 ? paired : full)[wide][k[i].form]);
+            shortest = std::min(shortest, begin + keys * alone[wide][k[i].form]);
             bytes += (double)k[i].sets * Hkv * k[i].ns * k[i].R * pa_row(p.DV) * sizeof(float);
         }
-        if (jobs > 768 && jobs < 3000) all += 0.25 * longest;  /* the last round is not full */
-        const double t = std::max(all, longest);
+        /* what does not fit the CUs at once begins when something ends, and the last round is not full */
+        const double t = jobs > slots ? std::max(all + 0.25 * longest, longest + shortest) : std::max(all, longest);
         return kinds == 2 || k[0].ns > 1 ? t + 4.0 + bytes / 1.6e6 : t;
     };
     double best = 1e30;
