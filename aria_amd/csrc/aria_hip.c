@@ -688,7 +688,7 @@ static int st_aligned(const void *p, int type) { return ((uintptr_t)p & mx4_el_m
 
 int aria_hip_rotary_table_dev(float *dcos, float *dsin, const aria_hip_rotary_scaling *a, int64_t first, int n,
                               void *stream) {
-    REQ(a && n >= 0 && first >= 0 && first + n <= (1 << 24) + 1);
+    REQ(a && n >= 0 && first >= 0 && first <= (1 << 24) && first + n <= (1 << 24) + 1);
     REQ(a->rot >= 2 && a->rot <= 256 && a->rot % 2 == 0 && a->kind >= 0 && a->kind <= 3);
     REQ(a->base > 1.0 && isfinite(a->base) && isfinite(a->gain));
     REQ(a->kind == 0 || (a->factor > 0.0 && isfinite(a->factor)));
@@ -697,10 +697,13 @@ int aria_hip_rotary_table_dev(float *dcos, float *dsin, const aria_hip_rotary_sc
     REQ(n == 0 || (dcos && dsin));
     REQ((((uintptr_t)dcos | (uintptr_t)dsin) & 3u) == 0);
     const double pi2 = 6.283185307179586476925;
-    double turns[128], base = a->base;
-    if (a->kind == 2) base *= pow(a->factor, (double)a->rot / (a->rot - 2));
-    for (int i = 0; i < a->rot / 2; i++) {
-        double f = pow(base, -2.0 * i / a->rot);
+    double turns[128];
+    /* powers of one ratio in 64-bit significands: 128 roundings of 2^-64 stay below a double's */
+    long double base = a->base, power = 1.0L;
+    if (a->kind == 2) base *= powl(a->factor, (long double)a->rot / (a->rot - 2));
+    const long double ratio = powl(base, -2.0L / a->rot);
+    for (int i = 0; i < a->rot / 2; i++, power *= ratio) {
+        double f = (double)power;
         if (a->kind == 1) f /= a->factor;
         if (a->kind == 3) {
             double w = (a->trained * f / pi2 - a->low) / (a->high - a->low);

@@ -317,7 +317,7 @@ typedef struct {
     int rot, kind;
     double base, factor, trained, low, high, gain;
 } aria_hip_rotary_scaling;
-/* dcos, dsin [n, rot/2] fp32 for positions first .. first + n - 1 (not negative, at most 2^24): the angle in 64
+/* dcos, dsin [n, rot/2] fp32 for positions first .. first + n - 1 (first and all of them 0 .. 2^24): the angle in 64
  * bits, so that far positions keep fp32's precision. 4-byte aligned. */
 int aria_hip_rotary_table_dev(float *dcos, float *dsin, const aria_hip_rotary_scaling *a, int64_t first, int n,
                               void *stream);

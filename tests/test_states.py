@@ -111,6 +111,16 @@ def test_refusals_table():
     assert call(n=0, c=None, s=None) == 0
 
 
+def test_refusal_of_a_far_first():
+    """A first position near the end of 64 bits is refused, not added to."""
+    import aria_amd
+    L = aria_amd.lib()
+    a = aria_amd.RotaryScaling(rot=64, kind=0, base=10000.0, factor=2.0, trained=4096.0, low=1.0, high=32.0, gain=1.0)
+    for first in ((1 << 63) - 1, (1 << 63) - 4, -(1 << 63), (1 << 24) + 1):
+        assert L.aria_hip_rotary_table_dev(P, P, a, first, 4, None) == -1
+        assert "invalid argument" in aria_amd.last_error()
+
+
 def test_refusals_rotary():
     import aria_amd
     L = aria_amd.lib()
