@@ -7,9 +7,14 @@
  * brings the row's largest magnitude to 448 or less: a power of two scales exactly, so a code is the value rounded
  * once, and e4m3's own exponent makes a finer scale unnecessary.
  *
- * All of it is bound by bytes (or, for single tokens, by the launch): a group of lanes holds one row in registers
- * from load to store, the row's maximum goes through lane exchanges, and a group takes several heads of one token, so that
- * table rows are read once for them and more loads are in flight.
+ * All of it is bound by bytes, or, for single tokens, by the launch: a group of lanes holds one row in registers
+ * from load to store, the row's maximum goes through lane exchanges, and a group takes four heads of one token where that still
+ * fills the CUs, so that table rows are read once for them and more loads are in flight. 4 x 8192 tokens of 20 heads of 128 rotated
+ * in bf16 (353 MB): 72 us, 4.9 TB/s, what a copy of 1 GiB reaches (83 with two heads, 76 with eight, 128 where odd widths branch in
+ * the same kernel). Lanes load and store 16 bytes beside their neighbours': 32 bytes to a lane in two pieces took 106 us for 8 x 4096 tokens of 10 interleaved
+ * heads of 128 in fp32 (407 MB), now 76, and 177 for 4 x 8192 tokens of 8 heads of 128 from fp32 to the cache and back (609 MB), now
+ * 147, the most of it in reading. 4 x 16384 tokens of 8 heads written and read back in bf16 (804 MB with the codes): 172 us, of which the keys'
+ * rotation in 64 bits costs 9. One token of 64 sequences: two launches of 3 us.
  */
 #include "aria_dev.h"
 #include "aria_hip_kernels.h"
@@ -48,7 +53,8 @@ __device__ __forceinline__ void tab_cos_sin(double t, float &c, float &s) {
     c = (k + 1) & 2 ? -v : v;
 }
 
-/* A thread makes V neighbouring pairs of TAB_EACH positions, whose frequencies it loads once */
+/* A thread makes V neighbouring pairs of TAB_EACH positions, whose frequencies it loads once: 131072 x 64 pairs (67 MB) in 13.6 us,
+ * the rate of its stores (20 us with the device library's functions of half turns, a pair to a thread) */
 template <int V>
 __global__ __launch_bounds__(256) void k_rotary_table(TabArgs a) {
     typedef float fv __attribute__((ext_vector_type(V), aligned(4)));
@@ -167,35 +173,39 @@ __device__ __forceinline__ bool st_token(const StArgs &x, const StSec &s, unsign
     return !(s.scale && (k.slot < 0 || k.slot >= x.cap));
 }
 
-/* Whole chunks of eight: D a multiple of 8, rot of 8 (interleaved) or 16. A group of LPR lanes takes HG heads of one token, 16
- * dims of each to a lane as two chunks: interleaved the chunks 2 l and 2 l + 1, else those of the pairs 8 l .. 8 l + 7, and
- * behind the rotated dims two plain ones. Every load of the HG rows is on its way before the first is used; chunks and heads
- * past the last repeat it and are not stored. */
+/* Whole chunks of 16 bytes, CW elements: D and rot multiples of CW (interleaved), rot of 2 CW (halves). A group of LPR lanes takes
+ * HG heads of one token, two chunks of each to a lane, so that neighbouring lanes' chunks are neighbours: interleaved the chunks l and
+ * l + (half of them), else those of the pairs CW l .. CW l + CW - 1, and behind the rotated dims two plain ones. Every load of the
+ * HG rows is on its way before the first is used; chunks and heads past the last repeat it and are not stored. */
 template <int TY, bool INTER, int LPR, int HG>
 __global__ __launch_bounds__(256) void k_states(StArgs x) {
     using T = typename StT<TY>::type;
-    typedef T v8 __attribute__((ext_vector_type(8), aligned(alignof(T))));
-    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
-    typedef unsigned u2 __attribute__((ext_vector_type(2), aligned(8)));
+    constexpr int CW = 16 / sizeof(T), CH = CW / 2;
+    typedef T vc __attribute__((ext_vector_type(CW), aligned(alignof(T))));
+    typedef float fh __attribute__((ext_vector_type(CH), aligned(4)));
     fetch_args(x);
-    const int l = threadIdx.x % LPR, rh = x.rot / 2, nc = x.D / 8;
+    const int l = threadIdx.x % LPR, rh = x.rot / 2, nc = x.D / CW;
     /* the lane's chunks, and whether their pairs are rotated */
     int ca, cb;
-    bool ra, rb;
+    bool ra, rb, ha;
     if (INTER) {
-        ca = 2 * l;
-        cb = ca + 1;
-        ra = 8 * ca < x.rot;
-        rb = 8 * cb < x.rot;
+        const int half = (nc + 1) / 2;
+        ca = l;
+        cb = l + half;
+        ha = l < half;
+        ra = CW * ca < x.rot;
+        rb = CW * cb < x.rot;
     } else {
-        const int lr = rh / 8;
+        const int lr = rh / CW, half = (nc - 2 * lr + 1) / 2;
         ra = rb = l < lr;
-        ca = ra ? l : 2 * l;                         /* rot / 8 + 2 (l - lr) = 2 l */
-        cb = ra ? l + lr : 2 * l + 1;
+        ca = ra ? l : l + lr;
+        cb = ra ? l + lr : ca + half;
+        ha = l < lr + half;
     }
-    const bool ha = ca < nc, hb = cb < nc;
-    const int ia = 8 * min(ca, nc - 1), ib = 8 * min(cb, nc - 1);
-    const int ta = min(8 * l, max(rh - 4, 0)), tb = min(8 * l + 4, max(rh - 4, 0));      /* their tables' columns */
+    const bool hb = ha && cb < nc;
+    const int ia = CW * min(ca, nc - 1), ib = CW * min(cb, nc - 1);
+    /* their tables' columns */
+    const int ta = min(INTER ? CH * ca : CW * l, max(rh - CH, 0)), tb = min(INTER ? CH * cb : CW * l + CH, max(rh - CH, 0));
 
     for (int64_t blk = blockIdx.x; blk < x.blocks; blk += gridDim.x) {
         const unsigned tb_ = x.blocks <= 0x7FFFFFFF ? x.dchunks.of((unsigned)blk) : (unsigned)(blk / x.chunks);
@@ -205,24 +215,24 @@ __global__ __launch_bounds__(256) void k_states(StArgs x) {
         StTok k;
         if (!st_token(x, s, tb_ * (256 / LPR) + threadIdx.x / LPR, k)) continue;
         const int h0 = chunk * HG, hn = min(HG, s.heads - h0);
-        v8 fa[HG], fb[HG];
+        vc fa[HG], fb[HG];
         const T *src = (const T *)s.src + k.b * s.sb + k.t * s.st + h0 * s.sh;
 #pragma unroll
         for (int h = 0; h < HG; h++) {
             const T *r = src + min(h, hn - 1) * s.sh;
-            fa[h] = *reinterpret_cast<const v8 *>(r + ia);
-            fb[h] = *reinterpret_cast<const v8 *>(r + ib);
+            fa[h] = *reinterpret_cast<const vc *>(r + ia);
+            fb[h] = *reinterpret_cast<const vc *>(r + ib);
         }
-        f4 c[2], sn[2];
+        fh c[2], sn[2];
         const bool turn = s.rotate;                  /* uniform */
         if (turn) {
             const float *ct = x.cos_t + k.p * rh, *st = x.sin_t + k.p * rh;
-            c[0] = *reinterpret_cast<const f4 *>(ct + ta);
-            c[1] = *reinterpret_cast<const f4 *>(ct + tb);
-            sn[0] = *reinterpret_cast<const f4 *>(st + ta);
-            sn[1] = *reinterpret_cast<const f4 *>(st + tb);
+            c[0] = *reinterpret_cast<const fh *>(ct + ta);
+            c[1] = *reinterpret_cast<const fh *>(ct + tb);
+            sn[0] = *reinterpret_cast<const fh *>(st + ta);
+            sn[1] = *reinterpret_cast<const fh *>(st + tb);
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
+            for (int i = 0; i < CH; i++) {
                 c[0][i] = ra ? c[0][i] : 1.0f;       /* plain dims: by one and zero */
                 c[1][i] = rb ? c[1][i] : 1.0f;
                 sn[0][i] = ra ? (x.inverse ? -sn[0][i] : sn[0][i]) : 0.0f;
@@ -232,67 +242,67 @@ __global__ __launch_bounds__(256) void k_states(StArgs x) {
         auto rows = [&](auto TURN, auto CACHE) __attribute__((always_inline)) {
             constexpr bool turned = decltype(TURN)::value != 0, cache = decltype(CACHE)::value != 0;
             using W = std::conditional_t<TY == 0 || cache, double, float>;
-            W cw[8], sw[8];
+            W cw[CW], sw[CW];
             if constexpr (turned)
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    cw[i] = c[i / 4][i % 4];
-                    sw[i] = sn[i / 4][i % 4];
+                for (int i = 0; i < CW; i++) {
+                    cw[i] = c[i / CH][i % CH];
+                    sw[i] = sn[i / CH][i % CH];
                 }
 #pragma unroll
             for (int h = 0; h < HG; h++) {
-                float v[16];                         /* chunk a, then chunk b */
+                float v[2 * CW];                         /* chunk a, then chunk b */
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
+                for (int i = 0; i < CW; i++) {
                     v[i] = (float)fa[h][i];
-                    v[8 + i] = (float)fb[h][i];
+                    v[CW + i] = (float)fb[h][i];
                 }
                 if constexpr (turned) {
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const int ja = INTER ? 2 * i : i, jb = INTER ? 2 * i + 1 : 8 + i;
+                    for (int i = 0; i < CW; i++) {
+                        const int ja = INTER ? 2 * i : i, jb = INTER ? 2 * i + 1 : CW + i;
                         st_turn(v[ja], v[jb], cw[i], sw[i]);
                     }
                     if (!(ra && rb)) {               /* plain dims as they came: 0 times an Inf is none of theirs */
 #pragma unroll
-                        for (int i = 0; i < 8; i++) {
+                        for (int i = 0; i < CW; i++) {
                             v[i] = ra ? v[i] : (float)fa[h][i];
-                            v[8 + i] = rb ? v[8 + i] : (float)fb[h][i];
+                            v[CW + i] = rb ? v[CW + i] : (float)fb[h][i];
                         }
                     }
                 }
                 if constexpr (!cache) {
                     if (h >= hn) break;
                     T *d = (T *)s.dst + k.b * s.db + k.t * s.dt + (h0 + h) * s.dh;
-                    v8 y;
+                    vc y;
                     if (ha) {
 #pragma unroll
-                        for (int i = 0; i < 8; i++) y[i] = (T)v[i];
-                        *reinterpret_cast<v8 *>(d + ia) = y;
+                        for (int i = 0; i < CW; i++) y[i] = (T)v[i];
+                        *reinterpret_cast<vc *>(d + ia) = y;
                     }
                     if (hb) {
 #pragma unroll
-                        for (int i = 0; i < 8; i++) y[i] = (T)v[8 + i];
-                        *reinterpret_cast<v8 *>(d + ib) = y;
+                        for (int i = 0; i < CW; i++) y[i] = (T)v[CW + i];
+                        *reinterpret_cast<vc *>(d + ib) = y;
                     }
                 } else {
                     float m = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 16; i++) m = OpMaxBits()(m, fabsf(v[i]));
+                    for (int i = 0; i < 2 * CW; i++) m = OpMaxBits()(m, fabsf(v[i]));
                     m = grp_reduce<LPR>(m, OpMaxBits());     /* repeated chunks change nothing */
                     const unsigned byte = st_byte(__builtin_bit_cast(unsigned, m));
                     const float r = st_inverse(byte);
-                    unsigned w[4];
+                    unsigned w[CH];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
+                    for (int i = 0; i < CH; i++) {
                         int u = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i] * r, v[4 * i + 1] * r, 0, false);
                         u = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i + 2] * r, v[4 * i + 3] * r, u, true);
                         w[i] = byte == 255u ? 0x7F7F7F7Fu : (unsigned)u;
                     }
                     if (h >= hn) break;
                     uint8_t *d = (uint8_t *)s.dst + k.b * s.db + k.slot * s.dt + (h0 + h) * s.dh;
-                    if (ha) *reinterpret_cast<u2 *>(d + ia) = u2{w[0], w[1]};
-                    if (hb) *reinterpret_cast<u2 *>(d + ib) = u2{w[2], w[3]};
+                    if (ha) __builtin_memcpy(__builtin_assume_aligned(d + ia, CW), w, CW);
+                    if (hb) __builtin_memcpy(__builtin_assume_aligned(d + ib, CW), w + CW / 4, CW);
                     if (l == 0) s.scale[k.b * s.cb + (h0 + h) * s.ch + k.slot] = (uint8_t)byte;
                 }
             }
@@ -398,15 +408,18 @@ __global__ __launch_bounds__(256) void k_states_any(StArgs x) {
     }
 }
 
-/* shares of `per` tokens; four heads to a group where that still fills the CUs */
-static bool st_shares(StArgs &x, int per) {
+/* shares of `per` tokens; four heads to a group where that makes `enough` workgroups to fill the CUs. Whole chunks: 1024 (thresholds of
+ * 256 and 512 cost some shapes of 500 to 1000 workgroups up to 12 %, 2048 gained one 15 % and lost others 4 %). A wave to a row: 320, since starting
+ * four times the workgroups costs more (rotated heads of 128: 192 groups of four 3.41 us with one head and 3.54 with four, 384
+ * 4.28 and 3.78, 1536 10.2 and 6.0) */
+static bool st_shares(StArgs &x, int per, int enough) {
     const int64_t blocks = ((int64_t)x.B * x.N + per - 1) / per;
     int64_t four = 0, one = 0;
     for (int i = 0; i < x.nsec; i++) {
         four += (x.sec[i].heads + 3) / 4;
         one += x.sec[i].heads;
     }
-    const bool hg4 = blocks * four >= 1024;
+    const bool hg4 = blocks * four >= enough;
     for (int i = 0; i < x.nsec; i++) x.sec[i].chunks = hg4 ? (x.sec[i].heads + 3) / 4 : x.sec[i].heads;
     x.chunks = (int)(hg4 ? four : one);
     x.blocks = blocks * x.chunks;
@@ -416,21 +429,23 @@ static bool st_shares(StArgs &x, int per) {
 }
 template <int TY, bool INTER, int LPR>
 static void st_launch(StArgs &x, hipStream_t s) {
-    const bool hg4 = st_shares(x, 256 / LPR);
+    const bool hg4 = st_shares(x, 256 / LPR, 1024);
     const dim3 grid((unsigned)std::min<int64_t>(x.blocks, ST_GRID));
     if (hg4) hipLaunchKernelGGL((k_states<TY, INTER, LPR, 4>), grid, dim3(256), 0, s, x);
     else hipLaunchKernelGGL((k_states<TY, INTER, LPR, 1>), grid, dim3(256), 0, s, x);
 }
 template <int TY, bool INTER>
 static void st_pairs(StArgs &x, hipStream_t s) {
-    if (x.D % 8 == 0 && x.rot % (INTER ? 8 : 16) == 0) {
-        const int lanes = (x.D + 15) / 16;
+    constexpr int CW = TY == 0 ? 4 : 8;
+    if (x.D % CW == 0 && x.rot % (INTER ? CW : 2 * CW) == 0) {
+        const int lanes = (x.D + 2 * CW - 1) / (2 * CW);
         if (lanes <= 4) st_launch<TY, INTER, 4>(x, s);
         else if (lanes <= 8) st_launch<TY, INTER, 8>(x, s);
-        else st_launch<TY, INTER, 16>(x, s);
+        else if (TY || lanes <= 16) st_launch<TY, INTER, 16>(x, s);
+        else if constexpr (TY == 0) st_launch<TY, INTER, 32>(x, s);
         return;
     }
-    const bool hg4 = st_shares(x, 4);
+    const bool hg4 = st_shares(x, 4, 320);
     const dim3 grid((unsigned)std::min<int64_t>(x.blocks, ST_GRID));
     if (hg4) hipLaunchKernelGGL((k_states_any<TY, INTER, 4>), grid, dim3(256), 0, s, x);
     else hipLaunchKernelGGL((k_states_any<TY, INTER, 1>), grid, dim3(256), 0, s, x);
@@ -510,6 +525,9 @@ struct RdArgs {
 template <int TY, int LPR, int HG>
 __global__ __launch_bounds__(256) void k_kv_read(RdArgs x) {
     using T = typename StT<TY>::type;
+    constexpr int CW = 16 / sizeof(T);
+    typedef T vc __attribute__((ext_vector_type(CW), aligned(alignof(T))));
+    typedef unsigned uc __attribute__((ext_vector_type(CW / 4), aligned(CW)));
     const aria_hip_kv_read &a = x.a;
     const aria_hip_kv &c = a.cache;
     constexpr float most = TY == 0 ? 3.40282347e38f : TY == 1 ? 65504.0f : 3.38953139e38f;
@@ -523,40 +541,45 @@ __global__ __launch_bounds__(256) void k_kv_read(RdArgs x) {
         const unsigned tok = (unsigned)(blk / per) * (256 / LPR) + threadIdx.x / LPR;
         const bool is_v = x.two ? chunk >= x.chunks : a.k == nullptr;
         if (x.two && is_v) chunk -= x.chunks;
-        if (tok >= (unsigned)c.B * a.N || 16 * l >= c.D) return;
+        if (tok >= (unsigned)c.B * a.N || CW * l >= c.D / 2) return;
         const int b = (int)(tok / (unsigned)a.N), t = (int)(tok % (unsigned)a.N);
         if (a.count && t >= a.count[b]) return;
         const int64_t slot = (a.first ? (int64_t)a.first[b] : 0) + t;
         if (slot < 0 || slot >= c.cap) return;
         const int h0 = chunk * HG, hn = min(HG, c.Hkv - h0);
-        const uint8_t *src = (is_v ? c.v : c.k) + b * c.batch + slot * c.token + h0 * c.head + 16 * l;
+        const uint8_t *src = (is_v ? c.v : c.k) + b * c.batch + slot * c.token + h0 * c.head + CW * l;
         const uint8_t *sp = (is_v ? c.v_scale : c.k_scale) + b * c.s_batch + h0 * c.s_head + slot;
-        T *dst = is_v ? (T *)a.v + b * a.v_batch + t * a.v_token + h0 * a.v_head + 16 * l
-                      : (T *)a.k + b * a.k_batch + t * a.k_token + h0 * a.k_head + 16 * l;
+        T *dst = is_v ? (T *)a.v + b * a.v_batch + t * a.v_token + h0 * a.v_head + CW * l
+                      : (T *)a.k + b * a.k_batch + t * a.k_token + h0 * a.k_head + CW * l;
         const int64_t dh = is_v ? a.v_head : a.k_head;
-        uint4 u[HG];
+        const int other = c.D / 2;
+        uc u[HG][2];
         unsigned e[HG];
 #pragma unroll
         for (int h = 0; h < HG; h++)
             if (h < hn) {
-                u[h] = *reinterpret_cast<const uint4 *>(src + h * c.head);
+                u[h][0] = *reinterpret_cast<const uc *>(src + h * c.head);
+                u[h][1] = *reinterpret_cast<const uc *>(src + h * c.head + other);
                 e[h] = sp[h * c.s_head];
             }
 #pragma unroll
         for (int h = 0; h < HG; h++) {
             if (h >= hn) break;
             const float f = __builtin_bit_cast(float, e[h] << 23);
-            const unsigned w[4] = {u[h].x, u[h].y, u[h].z, u[h].w};
-            T y[16];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const auto p = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], false), q = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], true);
-                y[4 * i] = held(p[0] * f);
-                y[4 * i + 1] = held(p[1] * f);
-                y[4 * i + 2] = held(q[0] * f);
-                y[4 * i + 3] = held(q[1] * f);
+            for (int j = 0; j < 2; j++) {
+                vc y;
+#pragma unroll
+                for (int i = 0; i < CW / 4; i++) {
+                    const unsigned w = u[h][j][i];
+                    const auto p = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), q = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+                    y[4 * i] = held(p[0] * f);
+                    y[4 * i + 1] = held(p[1] * f);
+                    y[4 * i + 2] = held(q[0] * f);
+                    y[4 * i + 3] = held(q[1] * f);
+                }
+                *reinterpret_cast<vc *>(dst + h * dh + j * other) = y;
             }
-            __builtin_memcpy(dst + h * dh, y, sizeof y);
         }
     };
     for (int64_t blk = blockIdx.x; blk < x.blocks; blk += gridDim.x) work(blk);
@@ -575,10 +598,11 @@ static void rd_launch(RdArgs &x, hipStream_t s) {
 }
 template <int TY>
 static void rd_lanes(RdArgs &x, hipStream_t s) {
-    const int lanes = x.a.cache.D / 16;
+    const int lanes = x.a.cache.D / (TY == 0 ? 8 : 16);
     if (lanes <= 4) rd_launch<TY, 4>(x, s);
     else if (lanes <= 8) rd_launch<TY, 8>(x, s);
-    else rd_launch<TY, 16>(x, s);
+    else if (TY || lanes <= 16) rd_launch<TY, 16>(x, s);
+    else if constexpr (TY == 0) rd_launch<TY, 32>(x, s);
 }
 
 extern "C" hipError_t aria_k_kv_read(const aria_hip_kv_read *a, hipStream_t s) {

@@ -264,6 +264,16 @@ def test_rotary(hip, t, inter, B, N, H, Hk, D, rot, layout, pad):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("D,rot", [(4, 4), (8, 8), (12, 4), (24, 8), (24, 16), (36, 20), (36, 32), (40, 40), (132, 128), (136, 96), (232, 16),
+                                   (256, 256), (256, 0)])
+def test_rotary_odd_chunks(hip, t, inter, D, rot):
+    """Odd numbers of 16-byte chunks, one chunk, more lanes than chunks, and the widest rows."""
+    test_rotary(hip, t, inter, 2, 9, 5, 3, D, rot, "tokens", 3)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("inter", [False, True])
 @pytest.mark.parametrize("D,rot", [(64, 32), (80, 74), (128, 128)])
 def test_rotary_in_place_and_back(hip, inter, D, rot):
