@@ -3,18 +3,30 @@
  * rows (gfx950): o = sum_j p_j v_j, p = softmax over the keys j that a row sees of scale * q . k_j. A row that
  * sees no key is zero.
  *
- * A row is a (sequence, token, query head of the group) triple. Two forms: where a sequence's own rows fill a
- * workgroup (or nothing is shared), a workgroup walks through the prefix's key tiles and then through the own ones. Else the rows
- * of all sequences of a prefix go over its keys together, the rows of each sequence over its own keys, and a second kernel joins
- * what they found: the prefix is read, converted and multiplied once for all of them.
+ * A row is a (sequence, token, query head of the group) triple. Where it pays, the rows of all sequences of a prefix go over its
+ * keys together, the rows of each sequence over its own keys in the same launch, and a second kernel joins what they found: the prefix
+ * is read, converted and multiplied once for all of them. Else a workgroup walks through the prefix's key tiles and then through the
+ * own ones. Either way the keys may be split over workgroups, to be joined too.
  *
  * The arithmetic is that of k_xattn.hip: S^T = K Q^T and O^T = V^T P^T with v_mfma_f32_32x32x16, scores in registers, weights
- * 2^(scale_log2 s - ref) with a lazy reference, P rounded to the 16-bit type. Codes become 16-bit values on their way to LDS: a
- * lane loads 16 codes and their row's byte, converts them with the row's power of two (one instruction per two
- * values) and stores two 16-byte chunks where the swizzle wants them; the next tile's codes are on their way meanwhile.
+ * 2^(scale_log2 s - ref) with a lazy reference, P rounded to the 16-bit type (half a step of it per weight; the row sum adds the rounded
+ * values). Codes become 16-bit values on their way to LDS: a lane loads 16 codes and their row's byte, converts them with
+ * the row's power of two (one instruction per two values, exact in bf16) and stores two 16-byte chunks where the swizzle wants
+ * them; the next tile's codes are on their way meanwhile. Converted once, a tile serves up to 128 rows.
  * The scores of slots that a row does not see become -inf. A key or value row of byte 255 (NaN) is staged
  * as a key of NaNs and a value of zeros: a row that sees it gets a NaN weight, one that does not (a later token's slot) is not
- * touched by it.
+ * touched by it. So are slots behind a length, whose scores are -inf for every row.
+ *
+ * What bounds it (us of a call among others):
+ *  - many rows: the chain of one tile, which two waves a SIMD do not hide. 8 sequences of 512 tokens, 4 heads to each of 4 key heads of
+ *    128, over 8192 + up to 1024 keys: 306, 0.96 PFLOP/s; matrix pipe, VALU and LDS are busy 38 % each, 29 % of the waves' cycles are waits
+ *    and barriers. No gain there from the scores of the next 32 keys beside this step's softmax (311), more workgroups of 32-key tiles
+ *    (331), other orders (317); the next tile's scores need 329 registers (470).
+ *    4 sequences of 1296 tokens, 16 heads of 64, over 2048 + 1296 keys: 102, 0.70 PFLOP/s; 704 workgroups are 2.75 a CU, where three
+ *    run at once, and end together only on some of them (CUs busy 83 %).
+ *  - few rows over many keys: their bytes (8 tokens over 131072 shared keys, 135 MB: 27 in the kernel and 6 in the join).
+ *  - little of both: the launch and the latency of a tile. 172 tokens over 257 keys of 64: 10.5; in the kernel the arguments are there after
+ *    0.3 us, the lengths after 1.7, the first tile in LDS after 2.4 and done after 3.3.
  */
 #include "xattn_dev.h"
 #include "aria_hip_kernels.h"
@@ -33,7 +45,8 @@ template <> struct Pc<__bf16> {
 };
 
 /* One kind of workgroup: `sets` sets of R rows (a prefix's, or a sequence's), nrb row blocks to each and key head, ns splits of
- * `per` key tiles. Form 0, 1, 2: a row block of 32, 64 or 128 rows, whose keys 4, 2 or 1 slices of waves share out */
+ * `per` key tiles. Form 0, 1, 2: a row block of 32, 64 or 128 rows, whose keys 4, 2 or 1 slices of waves share out. Form 0 has one LDS
+ * stage to a wave and no barriers in its loop, the others two stages */
 struct PaJobs {
     int sets, R, nrb, ns, per, jobs, form;
     int use_prefix, use_own, tp;                    /* tp: tiles of a prefix's capacity */
@@ -640,7 +653,11 @@ __global__ __launch_bounds__(256) void k_pattn_join(PaArgs x) {
 }
 
 /* How a call runs: whether the rows of a prefix's sequences share its tiles, each kind's form and number of splits, by an
- * estimate of the launches' time. */
+ * estimate of the launches' time, whose constants were measured (a workgroup's time for 1024 keys, alone on its CU, one of two and
+ * one of as many as fit; 2.5 us for the rest of it; 4 us and 1.6 TB/s for what is joined). One token of 32 sequences over 8192
+ * shared and 512 own keys takes 18 us with the prefix's rows together and 38 with each sequence's alone; 1296 tokens of 4 sequences
+ * over 2048 + 1296 keys 105 us alone and 144 together; 14 x 58 tokens over 2 x 75761 keys 317 together and 541 alone (128 rows), 428 (64), 495
+ * (32). Over 40 drawn shapes the form taken is within 8 % of the best of the forced ones, and 1 % behind in the mean. */
 #define PA_SPLITS 256        /* of one kind at most: the join holds a factor of each in LDS */
 struct PaPlan {
     int DV, join;
@@ -653,11 +670,12 @@ static PaPlan pa_plan(const aria_hip_prefix_attn *a, PaArgs &x) {
     x.Bp = a->B / P;
     const long long R = (long long)a->Nq * x.G;
     /* us for 1024 keys of a workgroup that has its CU alone, of one of two, and of one of as many as a CU holds, and that number:
-     * of forms 0, 1 and 2 at widths 64 and 128 */
-    static const double alone[2][3] = {{5.2, 9.5, 17.0}, {10.0, 17.0, 25.0}}, paired[2][3] = {{8.6, 14.7, 25.3}, {15.0, 25.4, 38.4}};
-    static const double full[2][3] = {{8.6, 14.7, 33.0}, {15.0, 25.4, 38.4}};
-    static const int hold[2][3] = {{2, 2, 3}, {2, 2, 2}};
-    const int wide = p.DV > 64;
+     * of forms 0, 1 and 2 at widths 32, 64, 96 and 128 */
+    static const double alone[4][3] = {{5.2, 9.5, 15.5}, {5.2, 9.5, 17.0}, {9.9, 17.8, 22.5}, {10.0, 17.0, 25.0}};
+    static const double paired[4][3] = {{7.4, 12.7, 21.0}, {8.6, 14.7, 25.3}, {14.5, 24.3, 33.2}, {15.0, 25.4, 38.4}};
+    static const double full[4][3] = {{7.4, 12.7, 28.0}, {8.6, 14.7, 33.0}, {14.5, 24.3, 33.2}, {15.0, 25.4, 38.4}};
+    static const int hold[4][3] = {{2, 2, 3}, {2, 2, 3}, {2, 2, 2}, {2, 2, 2}};
+    const int wide = p.DV / 32 - 1;
     const double begin = 2.5;                                 /* us of a workgroup beside its tiles */
     struct Kind {
         long long sets, R, wg;
