@@ -12,7 +12,7 @@
  * fills the CUs, so that table rows are read once for them and more loads are in flight. 4 x 8192 tokens of 20 heads of 128 rotated
  * in bf16 (353 MB): 72 us, 4.9 TB/s, what a copy of 1 GiB reaches (83 with two heads, 76 with eight, 128 where odd widths branch in
  * the same kernel). Lanes load and store 16 bytes beside their neighbours': 32 bytes to a lane in two pieces took 106 us for 8 x 4096 tokens of 10 interleaved
- * heads of 128 in fp32 (407 MB), now 76, and 177 for 4 x 8192 tokens of 8 heads of 128 from fp32 to the cache and back (609 MB), now
+ * heads of 128 in fp32 (407 MB), now 76, and 177 for 4 x 8192 tokens of 8 heads of 128 from fp32 to the cache and back (671 MB with the codes), now
  * 147, the most of it in reading. 4 x 16384 tokens of 8 heads written and read back in bf16 (804 MB with the codes): 172 us, of which the keys'
  * rotation in 64 bits costs 9. One token of 64 sequences: two launches of 3 us.
  */
