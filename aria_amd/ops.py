@@ -441,11 +441,17 @@ def rotary_tables(n, rot, first=0, base=10000.0, scaling="none", factor=1.0, tra
         return c.to_host(), s.to_host()
 
 
+def _int32(x):
+    """held to 32 bits, so that 2^32 does not become 0"""
+    return None if x is None else np.clip(np.asarray(x), -2 ** 31, 2 ** 31 - 1)
+
+
 def _positions(pos, first, B, N):
     if pos is not None and np.shape(pos) != (B, N):
         raise ValueError(f"pos holds a position for each token, [{B}, {N}]: got {np.shape(pos)}")
     if first is not None and np.shape(first) != (B,):
         raise ValueError(f"first holds a position for each sequence, [{B}]: got {np.shape(first)}")
+    return _int32(pos), _int32(first)
 
 
 def rotary(q, cos, sin, k=None, pos=None, first=None, interleaved=False, inverse=False):
@@ -458,7 +464,7 @@ def rotary(q, cos, sin, k=None, pos=None, first=None, interleaved=False, inverse
         raise ValueError(f"cos and sin are [positions, rot / 2]: got {cos.shape} and {sin.shape}")
     if k is not None and (k.shape[:2] != (B, N) or k.shape[3] != D):
         raise ValueError(f"k is [{B}, {N}, heads, {D}]: got {k.shape}")
-    _positions(pos, first, B, N)
+    pos, first = _positions(pos, first, B, N)
     with _Device() as dev:
         dq, dk = dev.put(q), dev.put(k)
         a = Rotary(q=dq.p, q_out=dq.p, k=_d(dk), k_out=_d(dk), cos=dev.put(cos).p, sin=dev.put(sin).p, pos=_d(dev.put(pos, np.int32)),
@@ -529,7 +535,7 @@ def prefix_attention(q, prefix_k, prefix_v, k=None, v=None, prefix_len=None, own
             x = np.asarray(x)
             if x.shape != (rows,):
                 raise ValueError(f"a length (or a first slot) for each of {rows}: got {x.shape}")
-            x = np.clip(x, -2 ** 31, 2 ** 31 - 1) if cap is None else np.clip(x, 0, cap)   # before 32 bits: 2^32 is not 0
+            x = _int32(x) if cap is None else np.clip(x, 0, cap)   # before 32 bits
         lens.append(x)
     with _Device() as dev:
         cp, co = dev.cache(P, Hkv, n, D), dev.cache(B, Hkv, m, D)

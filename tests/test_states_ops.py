@@ -55,6 +55,40 @@ def test_rotary(hip):
 
 
 @pytest.mark.gpu
+def test_far_positions_are_outside(hip):
+    """A position of 2^32 or -2^40 is outside the table like any other, and does not come back into it as 32 bits."""
+    from aria_amd import ops
+    cos, sin = ops.rotary_tables(8, 32)
+    q = randn(rng(4), (3, 2, 4, 64))
+    pos = np.array([[2 ** 32 + 5, 3], [-2 ** 40, 2 ** 63 - 1], [7, 2 ** 31]])
+    got = ops.rotary(q, cos, sin, pos=pos)
+    want = q.copy()
+    for b, t in ((0, 1), (2, 0)):
+        want[b, t], _ = states.rotate(q[b, t], cos[pos[b, t]], sin[pos[b, t]], False)
+    assert np.abs(got - want).max() <= 2.0 ** -24 * np.abs(want).max()
+    got = ops.rotary(q, cos, sin, first=[2 ** 32, -2 ** 32, 6])
+    want = q.copy()
+    for t in (0, 1):
+        want[2, t], _ = states.rotate(q[2, t], cos[6 + t], sin[6 + t], False)
+    assert np.abs(got - want).max() <= 2.0 ** -24 * np.abs(want).max()
+
+
+@pytest.mark.gpu
+def test_nothing_to_do(hip):
+    from aria_amd import ops
+    z = np.zeros
+    cos, sin = ops.rotary_tables(0, 32)
+    assert cos.shape == sin.shape == (0, 16)
+    assert ops.rotary(z((2, 0, 4, 64)), z((4, 16)), z((4, 16))).shape == (2, 0, 4, 64)
+    x = randn(rng(5), (1, 3, 4, 64))
+    assert np.array_equal(ops.rotary(x, cos, sin), x), "every position is outside an empty table"
+    code, byte = ops.e4m3_rows(z((0, 32)))
+    assert code.shape == (0, 32) and byte.shape == (0,) and ops.e4m3_values(code, byte).shape == (0, 32)
+    assert ops.prefix_attention(z((2, 0, 4, 64)), z((1, 5, 2, 64)), z((1, 5, 2, 64))).shape == (2, 0, 4, 64)
+    assert not ops.prefix_attention(x, z((1, 0, 2, 64)), z((1, 0, 2, 64))).any(), "rows that see no key are zero"
+
+
+@pytest.mark.gpu
 def test_rows(hip):
     import aria_amd
     from aria_amd import ops
