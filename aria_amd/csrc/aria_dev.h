@@ -76,9 +76,9 @@ struct OpMin {
 
 template <int G, typename Op>
 __device__ __forceinline__ float grp_reduce(float v, Op op) {
-    static_assert(G == 4 || G == 8 || G == 16 || G == 32 || G == 64, "group size");
+    static_assert(G == 2 || G == 4 || G == 8 || G == 16 || G == 32 || G == 64, "group size");
     v = op(v, dpp_f32<DPP_QUAD_XOR1>(v));
-    v = op(v, dpp_f32<DPP_QUAD_XOR2>(v));
+    if (G >= 4) v = op(v, dpp_f32<DPP_QUAD_XOR2>(v));
     if (G >= 8) v = op(v, dpp_f32<DPP_ROW_HALF_MIRROR>(v));
     if (G >= 16) v = op(v, dpp_f32<DPP_ROW_MIRROR>(v));
     if (G == 32) v = op(v, __shfl_xor(v, 16, ARIA_WAVE));

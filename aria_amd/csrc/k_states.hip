@@ -408,30 +408,35 @@ __global__ __launch_bounds__(256) void k_states_any(StArgs x) {
     }
 }
 
-/* shares of `per` tokens; four heads to a group where that makes `enough` workgroups to fill the CUs. Whole chunks: 1024 (thresholds of
- * 256 and 512 cost some shapes of 500 to 1000 workgroups up to 12 %, 2048 gained one 15 % and lost others 4 %). A wave to a row: 320, since starting
- * four times the workgroups costs more (rotated heads of 128: 192 groups of four 3.41 us with one head and 3.54 with four, 384
- * 4.28 and 3.78, 1536 10.2 and 6.0) */
-static bool st_shares(StArgs &x, int per, int enough) {
+/* shares of `per` tokens, and how many heads a group takes: four, or two where no section has more (two heads of 32 in groups of
+ * four: 80 us, 59 x 9154 tokens in fp16; of two: 50), where that makes `enough` workgroups to fill the CUs; else one. Whole
+ * chunks: 1024 (thresholds of 256 and 512 cost some shapes of 500 to 1000 workgroups up to 12 %, 2048 gained one 15 % and lost others 4 %). A wave to a
+ * row: 320, since starting four times the workgroups costs more (rotated heads of 128: 192 groups of four 3.41 us with one head and
+ * 3.54 with four, 384 4.28 and 3.78, 1536 10.2 and 6.0) */
+static int st_shares(StArgs &x, int per, int enough) {
     const int64_t blocks = ((int64_t)x.B * x.N + per - 1) / per;
-    int64_t four = 0, one = 0;
-    for (int i = 0; i < x.nsec; i++) {
-        four += (x.sec[i].heads + 3) / 4;
-        one += x.sec[i].heads;
-    }
-    const bool hg4 = blocks * four >= enough;
-    for (int i = 0; i < x.nsec; i++) x.sec[i].chunks = hg4 ? (x.sec[i].heads + 3) / 4 : x.sec[i].heads;
-    x.chunks = (int)(hg4 ? four : one);
+    int most = 0;
+    for (int i = 0; i < x.nsec; i++) most = std::max(most, x.sec[i].heads);
+    auto chunks = [&](int hg) {
+        int64_t n = 0;
+        for (int i = 0; i < x.nsec; i++) n += (x.sec[i].heads + hg - 1) / hg;
+        return n;
+    };
+    int hg = most > 2 ? 4 : most;
+    if (blocks * chunks(hg) < enough) hg = 1;
+    for (int i = 0; i < x.nsec; i++) x.sec[i].chunks = (x.sec[i].heads + hg - 1) / hg;
+    x.chunks = (int)chunks(hg);
     x.blocks = blocks * x.chunks;
     x.dn = HostDiv(x.N);
     x.dchunks = HostDiv(x.chunks);
-    return hg4;
+    return hg;
 }
 template <int TY, bool INTER, int LPR>
 static void st_launch(StArgs &x, hipStream_t s) {
-    const bool hg4 = st_shares(x, 256 / LPR, 1024);
+    const int hg = st_shares(x, 256 / LPR, 1024);
     const dim3 grid((unsigned)std::min<int64_t>(x.blocks, ST_GRID));
-    if (hg4) hipLaunchKernelGGL((k_states<TY, INTER, LPR, 4>), grid, dim3(256), 0, s, x);
+    if (hg == 4) hipLaunchKernelGGL((k_states<TY, INTER, LPR, 4>), grid, dim3(256), 0, s, x);
+    else if (hg == 2) hipLaunchKernelGGL((k_states<TY, INTER, LPR, 2>), grid, dim3(256), 0, s, x);
     else hipLaunchKernelGGL((k_states<TY, INTER, LPR, 1>), grid, dim3(256), 0, s, x);
 }
 template <int TY, bool INTER>
@@ -439,15 +444,17 @@ static void st_pairs(StArgs &x, hipStream_t s) {
     constexpr int CW = TY == 0 ? 4 : 8;
     if (x.D % CW == 0 && x.rot % (INTER ? CW : 2 * CW) == 0) {
         const int lanes = (x.D + 2 * CW - 1) / (2 * CW);
-        if (lanes <= 4) st_launch<TY, INTER, 4>(x, s);
+        if (lanes <= 2) st_launch<TY, INTER, 2>(x, s);
+        else if (lanes <= 4) st_launch<TY, INTER, 4>(x, s);
         else if (lanes <= 8) st_launch<TY, INTER, 8>(x, s);
         else if (TY || lanes <= 16) st_launch<TY, INTER, 16>(x, s);
         else if constexpr (TY == 0) st_launch<TY, INTER, 32>(x, s);
         return;
     }
-    const bool hg4 = st_shares(x, 4, 320);
+    const int hg = st_shares(x, 4, 320);
     const dim3 grid((unsigned)std::min<int64_t>(x.blocks, ST_GRID));
-    if (hg4) hipLaunchKernelGGL((k_states_any<TY, INTER, 4>), grid, dim3(256), 0, s, x);
+    if (hg == 4) hipLaunchKernelGGL((k_states_any<TY, INTER, 4>), grid, dim3(256), 0, s, x);
+    else if (hg == 2) hipLaunchKernelGGL((k_states_any<TY, INTER, 2>), grid, dim3(256), 0, s, x);
     else hipLaunchKernelGGL((k_states_any<TY, INTER, 1>), grid, dim3(256), 0, s, x);
 }
 static hipError_t st_run(StArgs &x, int type, int interleaved, hipStream_t s) {
@@ -599,7 +606,8 @@ static void rd_launch(RdArgs &x, hipStream_t s) {
 template <int TY>
 static void rd_lanes(RdArgs &x, hipStream_t s) {
     const int lanes = x.a.cache.D / (TY == 0 ? 8 : 16);
-    if (lanes <= 4) rd_launch<TY, 4>(x, s);
+    if (lanes <= 2) rd_launch<TY, 2>(x, s);
+    else if (lanes <= 4) rd_launch<TY, 4>(x, s);
     else if (lanes <= 8) rd_launch<TY, 8>(x, s);
     else if (TY || lanes <= 16) rd_launch<TY, 16>(x, s);
     else if constexpr (TY == 0) rd_launch<TY, 32>(x, s);
