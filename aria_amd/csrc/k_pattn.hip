@@ -657,7 +657,11 @@ __global__ __launch_bounds__(256) void k_pattn_join(PaArgs x) {
  * one of as many as fit; 2.5 us for the rest of it; 4 us and 1.6 TB/s for what is joined). One token of 32 sequences over 8192
  * shared and 512 own keys takes 18 us with the prefix's rows together and 38 with each sequence's alone; 1296 tokens of 4 sequences
  * over 2048 + 1296 keys 105 us alone and 144 together; 14 x 58 tokens over 2 x 75761 keys 317 together and 541 alone (128 rows), 428 (64), 495
- * (32). Over 40 drawn shapes the form taken is within 8 % of the best of the forced ones, and 1 % behind in the mean. */
+ * (32). Over 40 drawn shapes the form taken was within 8 % of
+ * the best of the forced ones, and 1 % behind in the mean. Splits may make up to 2304 workgroups, several to a place one after the
+ * other: their rounds even out, where 257 to 400 unsplit ones leave most CUs with one while others have two (24 x 348 tokens of 4
+ * heads of 32 over 21135 keys 392 -> 205 us). Such rounds are estimated less well, so they have to win by 8 %: of 750 drawn shapes 27
+ * took 5 to 48 % less for it and three 3 to 9 % more (without the 8 %, one took 21 % more). */
 #define PA_SPLITS 256        /* of one kind at most: the join holds a factor of each in LDS */
 struct PaPlan {
     int DV, join;
@@ -713,8 +717,8 @@ static PaPlan pa_plan(const aria_hip_prefix_attn *a, PaArgs &x) {
     double best = 1e30;
     Kind got[2];
     int got_kinds = 1, got_group = 0;
-    auto attempt = [&](Kind *k, int kinds, int group) {
-        const double t = estimate(k, kinds);
+    auto attempt = [&](Kind *k, int kinds, int group, double more = 1.0) {
+        const double t = more * estimate(k, kinds);
         if (t < best) {
             best = t;
             got[0] = k[0];
@@ -736,11 +740,11 @@ static PaPlan pa_plan(const aria_hip_prefix_attn *a, PaArgs &x) {
                     if (j && k[1].ns == 1) break;
                 }
                 const long long others = kinds == 2 ? k[1].wg * k[1].ns : 0;
-                const long long room[4] = {0, 256 - others, 512 - others, 512};
+                const long long room[8] = {0, 256 - others, 512 - others, 512, 768 - others, 1024 - others, 1536 - others, 2304 - others};
                 int last = 0;
-                for (int i = 0; i < 4; i++) {
+                for (int i = 0; i < 8; i++) {
                     split(k[0], room[i] / k[0].wg);
-                    if (k[0].ns != last) attempt(k, kinds, group);
+                    if (k[0].ns != last) attempt(k, kinds, group, i < 4 ? 1.0 : 1.08);
                     last = k[0].ns;
                 }
                 split(k[0], (k[0].nt + 3) / 4);

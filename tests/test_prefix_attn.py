@@ -144,6 +144,29 @@ SHAPES = [
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B,Pn,H,Hkv,Nq,n,m,D", [(6, 1, 8, 8, 710, 8716, 250, 64), (11, 1, 8, 4, 388, 9001, 0, 64),
+                                                 (6, 2, 8, 4, 134, 16001, 291, 32), (3, 1, 32, 8, 437, 5001, 700, 128)])
+def test_splits_in_several_rounds(hip, B, Pn, H, Hkv, Nq, n, m, D):
+    """Many rows over long keys: more workgroups than the CUs hold at once, whose results are joined."""
+    r = rng(B * Nq + n)
+    print(f"[gpu] prefix attention f16 B {B}/{Pn} H {H}/{Hkv} Nq {Nq} keys {n} + {m} D {D}", flush=True)
+    q, qv = cast(randn(r, (B, H, Nq, D)), "f16")
+    cp, pv = fill(hip, r, Pn, Hkv, n, D)
+    co, ov = fill(hip, r, B, Hkv, m, D)
+    pl, ol = np.full(Pn, n - 5), r.integers(0, m + 1, B)
+    first = ol - Nq // 2
+    got = run(hip, "f16", q, cp, co, pl, ol, first, "f32")
+    G = H // Hkv
+    for b, h in ((0, 0), (B - 1, H - 1)):        # two heads of them all
+        p, k = b * Pn // B, h // G
+        one = [x[p:p + 1, k:k + 1] for x in pv], [x[b:b + 1, k:k + 1] for x in ov]
+        want, mag = states.attention(qv[b:b + 1, h:h + 1], *one, pl[p:p + 1], ol[b:b + 1], first[b:b + 1])
+        kk, vv = (np.concatenate((one[0][i].ravel(), one[1][i].ravel())) for i in range(2))
+        tol = tolerance(want, mag, qv[b:b + 1, h:h + 1], kk, vv, "f16", "f32", 1 / np.sqrt(D), n + m)
+        assert (np.abs(got[b:b + 1, :, h:h + 1] - want) <= tol).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("t", ["f16", "bf16"])
 @pytest.mark.parametrize("shape", SHAPES)
 def test_shapes(hip, t, shape):
