@@ -409,8 +409,9 @@ __global__ __launch_bounds__(256) void k_states_any(StArgs x) {
 }
 
 /* shares of `per` tokens, and how many heads a group takes: four, or two where no section has more (two heads of 32 in groups of
- * four: 80 us, 59 x 9154 tokens in fp16; of two: 50), where that makes `enough` workgroups to fill the CUs; else one. Whole
- * chunks: 1024 (thresholds of 256 and 512 cost some shapes of 500 to 1000 workgroups up to 12 %, 2048 gained one 15 % and lost others 4 %). A wave to a
+ * four: 80 us, 59 x 9154 tokens in fp16; of two: 50), where that makes `enough` workgroups to fill the CUs; else two, else one
+ * (3 x 1037 tokens of 8 heads of 80 in fp32, written and read back: 12.2 us with one head in both kernels, 10.2 with two). Whole chunks: 1024
+ * (thresholds of 256 and 512 cost some shapes of 500 to 1000 workgroups up to 12 %, 2048 gained one 15 % and lost others 4 %). A wave to a
  * row: 320, since starting four times the workgroups costs more (rotated heads of 128: 192 groups of four 3.41 us with one head and
  * 3.54 with four, 384 4.28 and 3.78, 1536 10.2 and 6.0) */
 static int st_shares(StArgs &x, int per, int enough) {
@@ -423,7 +424,8 @@ static int st_shares(StArgs &x, int per, int enough) {
         return n;
     };
     int hg = most > 2 ? 4 : most;
-    if (blocks * chunks(hg) < enough) hg = 1;
+    if (hg == 4 && blocks * chunks(4) < enough) hg = 2;
+    if (hg == 2 && blocks * chunks(2) < enough) hg = 1;
     for (int i = 0; i < x.nsec; i++) x.sec[i].chunks = (x.sec[i].heads + hg - 1) / hg;
     x.chunks = (int)chunks(hg);
     x.blocks = blocks * x.chunks;
@@ -595,12 +597,14 @@ __global__ __launch_bounds__(256) void k_kv_read(RdArgs x) {
 template <int TY, int LPR>
 static void rd_launch(RdArgs &x, hipStream_t s) {
     const int64_t blocks = ((int64_t)x.a.cache.B * x.a.N + 256 / LPR - 1) / (256 / LPR);
-    const int ops = x.two ? 2 : 1, four = (x.a.cache.Hkv + 3) / 4;
-    const bool hg4 = blocks * four * ops >= 1024;
-    x.chunks = hg4 ? four : x.a.cache.Hkv;
+    const int ops = x.two ? 2 : 1, heads = x.a.cache.Hkv;
+    /* as in st_shares() */
+    const int hg = blocks * ((heads + 3) / 4) * ops >= 1024 ? 4 : blocks * ((heads + 1) / 2) * ops >= 1024 ? 2 : 1;
+    x.chunks = (heads + hg - 1) / hg;
     x.blocks = blocks * x.chunks * ops;
     const dim3 grid((unsigned)std::min<int64_t>(x.blocks, ST_GRID));
-    if (hg4) hipLaunchKernelGGL((k_kv_read<TY, LPR, 4>), grid, dim3(256), 0, s, x);
+    if (hg == 4) hipLaunchKernelGGL((k_kv_read<TY, LPR, 4>), grid, dim3(256), 0, s, x);
+    else if (hg == 2) hipLaunchKernelGGL((k_kv_read<TY, LPR, 2>), grid, dim3(256), 0, s, x);
     else hipLaunchKernelGGL((k_kv_read<TY, LPR, 1>), grid, dim3(256), 0, s, x);
 }
 template <int TY>
