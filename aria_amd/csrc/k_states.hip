@@ -409,11 +409,12 @@ __global__ __launch_bounds__(256) void k_states_any(StArgs x) {
 }
 
 /* shares of `per` tokens, and how many heads a group takes: four, or two where no section has more (two heads of 32 in groups of
- * four: 80 us, 59 x 9154 tokens in fp16; of two: 50), where that makes `enough` workgroups to fill the CUs; else two, else one
- * (3 x 1037 tokens of 8 heads of 80 in fp32, written and read back: 12.2 us with one head in both kernels, 10.2 with two). Whole chunks: 1024
- * (thresholds of 256 and 512 cost some shapes of 500 to 1000 workgroups up to 12 %, 2048 gained one 15 % and lost others 4 %). A wave to a
- * row: 320, since starting four times the workgroups costs more (rotated heads of 128: 192 groups of four 3.41 us with one head and
- * 3.54 with four, 384 4.28 and 3.78, 1536 10.2 and 6.0) */
+ * four: 80 us, 59 x 9154 tokens in fp16; of two: 50), where that makes `enough` workgroups to fill the CUs; else two, where that makes
+ * half as many (2 x 1296 tokens of 16 heads of 64, written and read back: 12.1 us with one head, 11.2 with two; 26 x 373 tokens of 20 heads
+ * of 32 rotated 8.1 and 6.5; of 366 shapes the worst lost 7 %); else one. Whole chunks: 1024 (thresholds of 256 and 512 for four heads cost
+ * some shapes of 500 to 1000 workgroups up to 12 %, 2048 gained one 15 % and lost others 4 %). A wave to a row: 320, since starting four
+ * times the workgroups costs more (rotated heads of 128: 192 groups of four 3.41 us with one head and 3.54 with four, 384 4.28 and
+ * 3.78, 1536 10.2 and 6.0) */
 static int st_shares(StArgs &x, int per, int enough) {
     const int64_t blocks = ((int64_t)x.B * x.N + per - 1) / per;
     int most = 0;
@@ -425,7 +426,7 @@ static int st_shares(StArgs &x, int per, int enough) {
     };
     int hg = most > 2 ? 4 : most;
     if (hg == 4 && blocks * chunks(4) < enough) hg = 2;
-    if (hg == 2 && blocks * chunks(2) < enough) hg = 1;
+    if (hg == 2 && blocks * chunks(2) < enough / 2) hg = 1;
     for (int i = 0; i < x.nsec; i++) x.sec[i].chunks = (x.sec[i].heads + hg - 1) / hg;
     x.chunks = (int)chunks(hg);
     x.blocks = blocks * x.chunks;
@@ -599,7 +600,7 @@ static void rd_launch(RdArgs &x, hipStream_t s) {
     const int64_t blocks = ((int64_t)x.a.cache.B * x.a.N + 256 / LPR - 1) / (256 / LPR);
     const int ops = x.two ? 2 : 1, heads = x.a.cache.Hkv;
     /* as in st_shares() */
-    const int hg = blocks * ((heads + 3) / 4) * ops >= 1024 ? 4 : blocks * ((heads + 1) / 2) * ops >= 1024 ? 2 : 1;
+    const int hg = blocks * ((heads + 3) / 4) * ops >= 1024 ? 4 : blocks * ((heads + 1) / 2) * ops >= 512 ? 2 : 1;
     x.chunks = (heads + hg - 1) / hg;
     x.blocks = blocks * x.chunks * ops;
     const dim3 grid((unsigned)std::min<int64_t>(x.blocks, ST_GRID));
