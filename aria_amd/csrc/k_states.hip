@@ -176,7 +176,8 @@ __device__ __forceinline__ bool st_token(const StArgs &x, const StSec &s, unsign
 /* Whole chunks of 16 bytes, CW elements: D and rot multiples of CW (interleaved), rot of 2 CW (halves). A group of LPR lanes takes
  * HG heads of one token, two chunks of each to a lane, so that neighbouring lanes' chunks are neighbours: interleaved the chunks l and
  * l + (half of them), else those of the pairs CW l .. CW l + CW - 1, and behind the rotated dims two plain ones. Every load of the
- * HG rows is on its way before the first is used; chunks and heads past the last repeat it and are not stored. */
+ * HG rows is on its way before the first is used; chunks and heads past the last repeat it, are not stored and do not count in a row's
+ * maximum. */
 template <int TY, bool INTER, int LPR, int HG>
 __global__ __launch_bounds__(256) void k_states(StArgs x) {
     using T = typename StT<TY>::type;
@@ -286,10 +287,14 @@ __global__ __launch_bounds__(256) void k_states(StArgs x) {
                         *reinterpret_cast<vc *>(d + ib) = y;
                     }
                 } else {
-                    float m = 0.0f;
+                    float ma = 0.0f, mb = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 2 * CW; i++) m = OpMaxBits()(m, fabsf(v[i]));
-                    m = grp_reduce<LPR>(m, OpMaxBits());     /* repeated chunks change nothing */
+                    for (int i = 0; i < CW; i++) {
+                        ma = OpMaxBits()(ma, fabsf(v[i]));
+                        mb = OpMaxBits()(mb, fabsf(v[CW + i]));
+                    }
+                    /* a repeated chunk does not count: it is not rotated as its owner's is */
+                    const float m = grp_reduce<LPR>(OpMaxBits()(ha ? ma : 0.0f, hb ? mb : 0.0f), OpMaxBits());
                     const unsigned byte = st_byte(__builtin_bit_cast(unsigned, m));
                     const float r = st_inverse(byte);
                     unsigned w[CH];
