@@ -15,7 +15,8 @@
  * them; the next tile's codes are on their way meanwhile. Converted once, a tile serves up to 128 rows.
  * The scores of slots that a row does not see become -inf. A key or value row of byte 255 (NaN) is staged
  * as a key of NaNs and a value of zeros: a row that sees it gets a NaN weight, one that does not (a later token's slot) is not
- * touched by it. So are slots behind a length, whose scores are -inf for every row.
+ * touched by it. So are slots behind a length, whose scores are -inf for every row. A row whose byte lets codes pass the type's largest number
+ * (65504 in fp16 is 65536 as a code) is held to it: an infinity would reach the rows that do not see it as 0 times itself.
  *
  * What bounds it (us of a call among others):
  *  - many rows: the chain of one tile, which two waves a SIMD do not hide. 8 sequences of 512 tokens, 4 heads to each of 4 key heads of
@@ -36,11 +37,17 @@
 typedef float pa_f32x2_t __attribute__((ext_vector_type(2)));
 #define PA_AHEAD 6           /* key fragments on their way to a score product */
 
+/* cvt: two codes of a dword times their row's power of two. LARGE: the first byte under which a code may lie past the type's largest
+ * number MOST (448 * 2^7 and 448 * 2^119 do not) */
 template <typename T> struct Pc;
 template <> struct Pc<_Float16> {
+    static constexpr unsigned LARGE = 135;
+    static constexpr float MOST = 65504.0f;
     template <bool HI> static __device__ __forceinline__ Xa<_Float16>::v2 cvt(unsigned u, float s) { return __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(u, s, HI); }
 };
 template <> struct Pc<__bf16> {
+    static constexpr unsigned LARGE = 247;
+    static constexpr float MOST = 3.38953139e38f;
     template <bool HI> static __device__ __forceinline__ Xa<__bf16>::v2 cvt(unsigned u, float s) { return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(u, s, HI); }
 };
 
@@ -204,8 +211,25 @@ __device__ __forceinline__ void pa_work(const PaArgs &x, int kind, int job, uint
             left -= KT * KS;
         }
     };
-    auto put = [&](uint8_t *to, const u32x4 &u, unsigned byte, int at0, int at1) __attribute__((always_inline)) {
+    auto put = [&](auto HELD, uint8_t *to, const u32x4 &u, unsigned byte, int at0, int at1) __attribute__((always_inline)) {
         const float s = __builtin_bit_cast(float, byte << 23);
+        if constexpr (decltype(HELD)::value != 0) {
+            T y[16];
+            auto held = [&](float v) __attribute__((always_inline)) {
+                return (T)__builtin_elementwise_minimum(__builtin_elementwise_maximum(v * s, -Pc<T>::MOST), Pc<T>::MOST);
+            };
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const auto p = __builtin_amdgcn_cvt_pk_f32_fp8((int)u[i], false), q = __builtin_amdgcn_cvt_pk_f32_fp8((int)u[i], true);
+                y[4 * i] = held(p[0]);
+                y[4 * i + 1] = held(p[1]);
+                y[4 * i + 2] = held(q[0]);
+                y[4 * i + 3] = held(q[1]);
+            }
+            __builtin_memcpy(__builtin_assume_aligned(to + at0, 16), y, 16);
+            __builtin_memcpy(__builtin_assume_aligned(to + at1, 16), y + 8, 16);
+            return;
+        }
         const v2 c0 = Pc<T>::template cvt<false>(u.x, s), c1 = Pc<T>::template cvt<true>(u.x, s);
         const v2 c2 = Pc<T>::template cvt<false>(u.y, s), c3 = Pc<T>::template cvt<true>(u.y, s);
         const v2 c4 = Pc<T>::template cvt<false>(u.z, s), c5 = Pc<T>::template cvt<true>(u.z, s);
@@ -213,47 +237,53 @@ __device__ __forceinline__ void pa_work(const PaArgs &x, int kind, int job, uint
         *reinterpret_cast<v8 *>(to + at0) = v8{c0[0], c0[1], c1[0], c1[1], c2[0], c2[1], c3[0], c3[1]};
         *reinterpret_cast<v8 *>(to + at1) = v8{c4[0], c4[1], c5[0], c5[1], c6[0], c6[1], c7[0], c7[1]};
     };
-    /* rows of tile i that stand for NaN or lie behind its last slot */
+    /* rows of tile i that stand for NaN or lie behind its last slot; whether others may hold more than the type does */
     auto fix = [&](int i) __attribute__((always_inline)) {
         const int valid = i < nt0 ? n0 - i * KT : n1 - (i - nt0) * KT;
-        bool bad[NC], any = false;
+        bool any = false;
 #pragma unroll
-        for (int j = 0; j < NC; j++) {
-            bad[j] = kb[j] == 255u || vb[j] == 255u || (64 * (QW * j + qw) + lane) / C16 >= valid;
-            any |= bad[j];
-        }
+        for (int j = 0; j < NC; j++) any |= max(kb[j], vb[j]) >= Pc<T>::LARGE || (64 * (QW * j + qw) + lane) / C16 >= valid;
+        bool large = false;
         if (__builtin_expect(__ballot(any) != 0, 0)) {
 #pragma unroll
             for (int j = 0; j < NC; j++) {
-                kc[j] = bad[j] ? u32x4{0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu} : kc[j];
-                vc[j] = bad[j] ? u32x4{0, 0, 0, 0} : vc[j];
-                kb[j] = bad[j] ? 127u : kb[j];
-                vb[j] = bad[j] ? 127u : vb[j];
+                const bool bad = kb[j] == 255u || vb[j] == 255u || (64 * (QW * j + qw) + lane) / C16 >= valid;
+                kc[j] = bad ? u32x4{0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu} : kc[j];
+                vc[j] = bad ? u32x4{0, 0, 0, 0} : vc[j];
+                kb[j] = bad ? 127u : kb[j];
+                vb[j] = bad ? 127u : vb[j];
+                large |= max(kb[j], vb[j]) >= Pc<T>::LARGE;
             }
+            large = __ballot(large) != 0;
         }
+        return large;
     };
-    auto put_k = [&](int buf) __attribute__((always_inline)) {
+    auto put_k = [&](auto HELD, int buf) __attribute__((always_inline)) {
         uint8_t *K = smem + buf * STAGE + ks * 2 * TB;
 #pragma unroll
         for (int j = 0; j < NC; j++) {
             const int p = 64 * (QW * j + qw) + lane, r = p / C16, cp = 2 * (p % C16);
             const int z = DP == 64 ? (r >> 1) & 7 : r & 15;
-            put(K, kc[j], kb[j], (r * CPR + (cp ^ z)) * 16, (r * CPR + ((cp + 1) ^ z)) * 16);
+            put(HELD, K, kc[j], kb[j], (r * CPR + (cp ^ z)) * 16, (r * CPR + ((cp + 1) ^ z)) * 16);
         }
     };
-    auto put_v = [&](int buf, const u32x4 (&c)[NC], const unsigned (&byte)[NC]) __attribute__((always_inline)) {
+    auto put_v = [&](auto HELD, int buf) __attribute__((always_inline)) {
         uint8_t *V = smem + buf * STAGE + ks * 2 * TB + TB;
 #pragma unroll
         for (int j = 0; j < NC; j++) {
             const int p = 64 * (QW * j + qw) + lane, r = p / C16, cp = 2 * (p % C16);
             const int z = DP == 64 ? ((r >> 1) & 1) << 2 : (r & 3) << 2;
-            put(V, c[j], byte[j], (r * CPR + (cp ^ z)) * 16, (r * CPR + ((cp + 1) ^ z)) * 16);
+            put(HELD, V, vc[j], vb[j], (r * CPR + (cp ^ z)) * 16, (r * CPR + ((cp + 1) ^ z)) * 16);
         }
     };
     auto store = [&](int buf, int i) __attribute__((always_inline)) {
-        fix(i);
-        put_k(buf);
-        put_v(buf, vc, vb);
+        const bool large = fix(i);
+        put_k(IC<0>{}, buf);
+        put_v(IC<0>{}, buf);
+        if (__builtin_expect(large, 0)) {           /* once more: the fast path keeps its straight line */
+            put_k(IC<1>{}, buf);
+            put_v(IC<1>{}, buf);
+        }
     };
 
     xa_f32x16_t o[DT];
