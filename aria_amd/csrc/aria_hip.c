@@ -696,22 +696,24 @@ int aria_hip_rotary_table_dev(float *dcos, float *dsin, const aria_hip_rotary_sc
     REQ(a->kind != 3 || (a->trained > 0.0 && isfinite(a->trained) && isfinite(a->low) && isfinite(a->high) && a->high > a->low));
     REQ(n == 0 || (dcos && dsin));
     REQ((((uintptr_t)dcos | (uintptr_t)dsin) & 3u) == 0);
-    const double pi2 = 6.283185307179586476925;
+    const long double pi2 = 6.283185307179586476925286766559L;
     double turns[128];
-    /* powers of one ratio in 64-bit significands: 128 roundings of 2^-64 stay below a double's */
+    /* powers of one ratio in 64-bit significands: 128 roundings of 2^-64 of at most 16 turns are 2^-53, 2^-29 turns at position 2^24.
+     * Positions are whole numbers, so whole turns from one to the next change nothing: without them at most half a turn remains,
+     * which a double holds to 2^-55 */
     long double base = a->base, power = 1.0L;
     if (a->kind == 2) base *= powl(a->factor, (long double)a->rot / (a->rot - 2));
     const long double ratio = powl(base, -2.0L / a->rot);
     for (int i = 0; i < a->rot / 2; i++, power *= ratio) {
-        double f = (double)power;
-        if (a->kind == 1) f /= a->factor;
+        long double t = power / pi2;
+        if (a->kind == 1) t /= a->factor;
         if (a->kind == 3) {
-            double w = (a->trained * f / pi2 - a->low) / (a->high - a->low);
-            w = w < 0.0 ? 0.0 : w > 1.0 ? 1.0 : w;
-            f *= w + (1.0 - w) / a->factor;
+            long double w = (a->trained * t - a->low) / ((long double)a->high - a->low);
+            w = w < 0.0L ? 0.0L : w > 1.0L ? 1.0L : w;
+            t *= w + (1.0L - w) / a->factor;
         }
-        turns[i] = f / pi2;
-        REQ(isfinite(turns[i]) && turns[i] <= 0x1p20);   /* whole turns and a fraction fit 64 bits at any position */
+        REQ(t <= 16.0L);
+        turns[i] = (double)(t - rintl(t));
     }
     if (n == 0) return 0;
     ENSURE();
