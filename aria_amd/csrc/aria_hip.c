@@ -690,7 +690,7 @@ int aria_hip_rotary_table_dev(float *dcos, float *dsin, const aria_hip_rotary_sc
                               void *stream) {
     REQ(a && n >= 0 && first >= 0 && first <= (1 << 24) && first + n <= (1 << 24) + 1);
     REQ(a->rot >= 2 && a->rot <= 256 && a->rot % 2 == 0 && a->kind >= 0 && a->kind <= 3);
-    REQ(a->base > 1.0 && isfinite(a->base) && isfinite(a->gain));
+    REQ(a->base > 1.0 && isfinite(a->base) && isfinite((float)a->gain));
     REQ(a->kind == 0 || (a->factor > 0.0 && isfinite(a->factor)));
     REQ(a->kind != 2 || a->rot >= 4);
     REQ(a->kind != 3 || (a->trained > 0.0 && isfinite(a->trained) && isfinite(a->low) && isfinite(a->high) && a->high > a->low));

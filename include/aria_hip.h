@@ -312,7 +312,7 @@ int aria_hip_glu_mx4(float *y, const float *x, const uint8_t *q, const uint8_t *
  * base's place, which leaves f_0 and divides the last by factor; 3 (by turns): with t = trained * f_i / 2 pi
  * turns over the trained length and w = (t - low) / (high - low) held to 0 .. 1, f_i (w + (1 - w) / factor).
  * gain multiplies both tables. rot even, 2 .. 256 (kind 2: from 4); base > 1; factor > 0 (kinds 1 - 3);
- * trained > 0, high > low (kind 3); all finite. No pair may make more than 16 turns from one position to the
+ * trained > 0, high > low (kind 3); all finite, gain in fp32 too. No pair may make more than 16 turns from one position to the
  * next (kinds 1 and 3: factor from 0.01 on). */
 typedef struct {
     int rot, kind;

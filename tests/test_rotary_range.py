@@ -24,6 +24,15 @@ def test_more_than_16_turns_a_position():
     assert aria_amd.lib().aria_hip_rotary_table_dev(P, P, scaling(kind=1, factor=0.01), 0, 0, None) == 0
 
 
+@pytest.mark.parametrize("gain", [1e39, -3.5e38, 1e300])
+def test_gain_beyond_fp32(gain):
+    """It would be infinite in the tables' type, and 0 times it not a number."""
+    import aria_amd
+    assert aria_amd.lib().aria_hip_rotary_table_dev(P, P, scaling(gain=gain), 0, 4, None) == -1
+    assert "invalid argument" in aria_amd.last_error()
+    assert aria_amd.lib().aria_hip_rotary_table_dev(P, P, scaling(gain=gain * 1e-300), 0, 0, None) == 0
+
+
 # ---- GPU ----
 
 @pytest.mark.gpu
