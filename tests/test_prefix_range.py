@@ -69,6 +69,30 @@ def test_beyond_the_type(hip, t, big, shape):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("B,Nq,m,D", [(1, 8, 40, 64), (3, 40, 90, 128), (2, 150, 170, 96)])
+def test_beside_a_row_that_is_nan(hip, t, B, Nq, m, D):
+    """A large value, a row of byte 255 and a large key in one tile, slot by slot: each reaches the rows behind it alone."""
+    r = rng(Nq)
+    q = randn(r, (B, 2, Nq, D))
+    q[..., D - 3] = 0
+    q, _ = cast(q, t)
+    cp, co = fill(hip, r, 1, 1, 20, D)[0], fill(hip, r, B, 1, m, D)[0]
+    first, slot = np.full(B, m - Nq), m - Nq // 2
+    clean = run(hip, t, q, cp, co, first=first, out="f32")
+    place(co, 1, 0, slot, D - 3, 0.25 * LARGEST[t] if t == "bf16" else 2.0 * LARGEST[t])
+    for i in range(2):
+        code, byte = (x.copy() for x in co.get(i))
+        code[0, slot + 1], byte[0, slot + 1] = 0x7F, 255
+        co.put(i, code, byte)
+    place(co, 0, 0, slot + 2, D - 3, -LARGEST[t])
+    got = run(hip, t, q, cp, co, first=first, out="f32")
+    last = first[0] + np.arange(Nq)          # the last slot that a token sees
+    assert np.array_equal(got[1:], clean[1:]) and np.array_equal(got[0, last < slot], clean[0, last < slot])
+    assert not np.isnan(got[0, last == slot]).any() and np.isnan(got[0, last > slot]).all()
+
+
+@pytest.mark.gpu
 def test_finite_states_stay_finite(hip):
     """Host arrays whose values fp16 does not reach."""
     from aria_amd import ops
