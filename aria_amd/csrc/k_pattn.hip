@@ -20,13 +20,13 @@
  *
  * What bounds it (us of a call among others):
  *  - many rows: the chain of one tile, which two waves a SIMD do not hide. 8 sequences of 512 tokens, 4 heads to each of 4 key heads of
- *    128, over 8192 + up to 1024 keys: 306, 0.96 PFLOP/s; matrix pipe, VALU and LDS are busy 38 % each, 29 % of the waves' cycles are waits
- *    and barriers. No gain there from the scores of the next 32 keys beside this step's softmax (311), more workgroups of 32-key tiles
+ *    128, over 8192 + up to 1024 keys: 309, 0.95 PFLOP/s; matrix pipe, VALU and LDS are busy 38 % each, 29 % of the waves' cycles are waits
+ *    and barriers. No gain there (306 that day) from the scores of the next 32 keys beside this step's softmax (311), more workgroups of 32-key tiles
  *    (331), other orders (317); the next tile's scores need 329 registers (470).
- *    4 sequences of 1296 tokens, 16 heads of 64, over 2048 + 1296 keys: 102, 0.70 PFLOP/s; 704 workgroups are 2.75 a CU, where three
+ *    4 sequences of 1296 tokens, 16 heads of 64, over 2048 + 1296 keys: 104, 0.68 PFLOP/s; 704 workgroups are 2.75 a CU, where three
  *    run at once, and end together only on some of them (CUs busy 83 %).
  *  - few rows over many keys: their bytes (8 tokens over 131072 shared keys, 135 MB: 27 in the kernel and 6 in the join).
- *  - little of both: the launch and the latency of a tile. 172 tokens over 257 keys of 64: 10.5; in the kernel the arguments are there after
+ *  - little of both: the launch and the latency of a tile. 172 tokens over 257 keys of 64: 10.6; in the kernel the arguments are there after
  *    0.3 us, the lengths after 1.7, the first tile in LDS after 2.4 and done after 3.3.
  */
 #include "xattn_dev.h"
@@ -686,7 +686,7 @@ __global__ __launch_bounds__(256) void k_pattn_join(PaArgs x) {
  * estimate of the launches' time, whose constants were measured (a workgroup's time for 1024 keys, alone on its CU, one of two and
  * one of as many as fit; 2.5 us for the rest of it; 4 us and 1.6 TB/s for what is joined). One token of 32 sequences over 8192
  * shared and 512 own keys takes 18 us with the prefix's rows together and 38 with each sequence's alone; 1296 tokens of 4 sequences
- * over 2048 + 1296 keys 105 us alone and 144 together; 14 x 58 tokens over 2 x 75761 keys 317 together and 541 alone (128 rows), 428 (64), 495
+ * over 2048 + 1296 keys 104 us alone and 144 together; 14 x 58 tokens over 2 x 75761 keys 317 together and 541 alone (128 rows), 428 (64), 495
  * (32). Over 40 drawn shapes the form taken was within 8 % of
  * the best of the forced ones, and 1 % behind in the mean. Splits may make up to 2304 workgroups, several to a place one after the
  * other: their rounds even out, where 257 to 400 unsplit ones leave most CUs with one while others have two (24 x 348 tokens of 4

@@ -39,7 +39,7 @@ struct TabArgs {
 };
 
 /* cos and sin of a turns' fraction. The nearest quarter leaves t in 64 bits, exactly; of what is left, at most an eighth, the
- * Taylor series to x^10 and x^9 (the next terms are below 2.4e-8 and 1.8e-9), 2 pi in two parts */
+ * Taylor series to x^10 and x^9 (the next terms are below 1.2e-10 and 1.8e-9), 2 pi in two parts */
 __device__ __forceinline__ void tab_cos_sin(double t, float &c, float &s) {
     const double r = t - __builtin_rint(t), q = __builtin_rint(4.0 * r);
     const float x = (float)__builtin_fma(q, -0.25, r), z = x * x;
@@ -53,8 +53,8 @@ __device__ __forceinline__ void tab_cos_sin(double t, float &c, float &s) {
     c = (k + 1) & 2 ? -v : v;
 }
 
-/* A thread makes V neighbouring pairs of TAB_EACH positions, whose frequencies it loads once: 131072 x 64 pairs (67 MB) in 13.6 us,
- * the rate of its stores (20 us with the device library's functions of half turns, a pair to a thread) */
+/* A thread makes V neighbouring pairs of TAB_EACH positions, whose frequencies it loads once: 131072 x 64 pairs (67 MB) in 13.4 us,
+ * where a fill of as many bytes takes 11.4 (20 us with the device library's functions of half turns, a pair to a thread) */
 template <int V>
 __global__ __launch_bounds__(256) void k_rotary_table(TabArgs a) {
     typedef float fv __attribute__((ext_vector_type(V), aligned(4)));

@@ -516,7 +516,7 @@ def e4m3_values(codes, scales):
 
 def prefix_attention(q, prefix_k, prefix_v, k=None, v=None, prefix_len=None, own_len=None, first=None, scale=None):
     """q [B, Nq, H, D] (rounded to fp16) over prefixes [P, n, Hkv, D] (sequence b reads prefix b // (B / P)) and own keys and values
-    [B, m, Hkv, D], both cached as e4m3 rows in the call; first [B]: query t of sequence b sees own keys up to first[b] + t
+    [B, m, Hkv, D], both cached as e4m3 rows in the call and held to fp16's range; first [B]: query t of sequence b sees own keys up to first[b] + t
     -> [B, Nq, H, D] fp32."""
     from . import PrefixAttention
     q = _f32(q)

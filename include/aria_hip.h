@@ -394,11 +394,14 @@ int aria_hip_kv_read_dev(const aria_hip_kv_read *a, void *stream);
  * A row that sees no key is zero. What the slots that a row does not see hold does not reach it (byte 255 included). A key
  * or a value of byte 255 that it sees makes the whole row NaN.
  * Cached values are rounded to q's type (exact in bf16; fp16 above 2^-24 steps) and held to its finite range, as reading them is;
- * probabilities are rounded to it too; sums and softmax statistics are fp32. D up to 128; scale positive, at most 2^127; B * H at most 2^20, B * H * Nq at
- * most 2^30; a cache's token stride below 2^24. q and out 16-byte aligned, strides multiples of 8.
- * Many sequences' rows together read a prefix once. dws: aria_hip_prefix_attention_ws_bytes(a) bytes (0: may be
- * NULL), 256-byte aligned, not shared by calls that may run at the same time; the number goes by B, H, Nq and both
- * caches' B, Hkv, D and cap alone. */
+ * probabilities are rounded to it too, and in fp16 one below 2^-32 of its row's largest may count as zero. Sums and softmax
+ * statistics are fp32: scores times scale, and sums of values under weights of up to 2^15, have to stay within it. D up to
+ * 128; scale positive, at most 2^127; B * H at most 2^20, B * H * Nq at most 2^30; a cache's token stride below 2^24. q and out
+ * 16-byte aligned, strides multiples of 8. Many sequences' rows together read a prefix once.
+ * dws: aria_hip_prefix_attention_ws_bytes(a) bytes (0: may be NULL), 256-byte aligned, not shared by calls that may run at the
+ * same time; the number goes by B, H, Nq and both caches' B, Hkv, D and cap alone. It may fall where one of them grows
+ * (8 sequences of 300 tokens may need 60 MB and of 400 none): a workspace for several descriptions has the largest number of
+ * them all, not that of the largest description. */
 typedef struct {
     const void *q;
     void *out;
